@@ -16,6 +16,9 @@ from gelib_amd.SO3partArr import SO3partArr, SO3partArr_CGproductFn, SO3partArr_
 from gelib_amd.SO3vecArr import SO3vecArr, SO3vecArr_CGproductFn, SO3vecArr_DiagCGproductFn  # noqa: F401
 from gelib_amd.SO3weights import SO3weights, SO3linear, CGproduct_linear  # noqa: F401
 from gelib_amd.gather_map import gather_map  # noqa: F401
+from gelib_amd.group_norm_act import group_norm_act  # noqa: F401
+from gelib_amd.linear_act import linear_act  # noqa: F401
+from gelib_amd.AdamW import AdamW  # noqa: F401
 from gelib_amd.O3 import O3element, O3irrep, O3type, O3part, O3vec, O3vec_CGproductFn, O3vec_DiagCGproductFn  # noqa: F401
 
 

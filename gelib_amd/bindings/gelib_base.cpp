@@ -9,6 +9,7 @@
 #include <pybind11/stl.h>
 
 #include "gelib/GElib.hpp"
+#include "real_ops.h"
 
 namespace py = pybind11;
 using namespace GElib;
@@ -90,6 +91,8 @@ static std::vector<gelib_part_desc> parts_on_gpu(const std::vector<at::Tensor> &
 
 PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("version", []() { return std::string(_GELIB_VERSION); });
+
+  bind_real_ops(m);
 
   m.def("in_memory", [](const py::args &ts) {
     for (const py::handle t : ts) {

@@ -1,0 +1,314 @@
+// The operators on real channels (group norm with an activation, linear layer with its epilogue, AdamW) for gelib_base: tensors
+// are checked and results allocated here, one call of the C ABI does the rest on torch's current stream of the tensors' GPU.
+// (A step over hundreds of parameters, or a layer on a few rows, would spend longer in Python than on the GPU.)
+#include <torch/extension.h>
+#include <c10/hip/HIPStream.h>
+
+#include "real_ops.h"
+
+namespace py = pybind11;
+
+namespace {
+
+typedef std::optional<at::Tensor> Maybe;
+
+void done(int status) {
+  if (status == GELIB_HIP_OK) return;
+  std::string why = gelib_hip_strerror(status);
+  if (status == GELIB_HIP_ERR_RUNTIME) why += std::string(": ") + gelib_hip_last_runtime_error();
+  throw std::runtime_error("GElib error: " + why + " (status " + std::to_string(status) + ")");
+}
+
+int type_of(const at::Tensor &x) {
+  switch (x.scalar_type()) {
+    case at::kFloat: return GELIB_HIP_F32;
+    case at::kBFloat16: return GELIB_HIP_BF16;
+    case at::kHalf: return GELIB_HIP_F16;
+    default: throw py::type_error("GElib: float32, bfloat16 and float16 tensors are taken");
+  }
+}
+
+void like(const at::Tensor &t, const at::Tensor &x, const char *name) {
+  if (t.scalar_type() != x.scalar_type()) throw py::type_error(std::string("GElib: ") + name + " has another type than x");
+  if (t.device() != x.device()) throw py::value_error(std::string("GElib: ") + name + " is on another device than x");
+}
+
+void on_gpu(const at::Tensor &x) {
+  if (!x.is_cuda()) throw py::value_error("GElib: tensors must be on GPU: these operators have no host form in this build");
+}
+
+at::Tensor plain(const at::Tensor &t) { return t.resolve_neg().contiguous(); }
+
+void *ptr(const at::Tensor &t) { return t.defined() && t.numel() ? t.data_ptr() : nullptr; }
+
+struct OnDevice {
+  c10::OptionalDeviceGuard guard;
+  void *stream;
+  explicit OnDevice(const at::Tensor &x) : guard(x.device()), stream((void *)c10::hip::getCurrentHIPStream(x.device().index()).stream()) {}
+};
+
+at::Tensor workspace(uint64_t bytes, const at::Tensor &x) {
+  return bytes ? at::empty({(int64_t)bytes}, x.options().dtype(at::kByte)) : at::Tensor();
+}
+
+int act_of(const std::string &act) {
+  if (act == "none") return GELIB_HIP_ACT_NONE;
+  if (act == "relu") return GELIB_HIP_ACT_RELU;
+  if (act == "silu") return GELIB_HIP_ACT_SILU;
+  if (act == "gelu") return GELIB_HIP_ACT_GELU;
+  throw py::value_error("GElib: act is one of 'none', 'relu', 'silu', 'gelu'");
+}
+
+// ---- group norm ----
+
+// x as samples x positions x channels: the strides of its samples and positions, of x itself where its positions are evenly
+// spaced and its channels contiguous, else of a copy
+struct NormShape {
+  at::Tensor x;
+  int64_t N, S, xs, xp;
+  int C;
+};
+NormShape norm_shape(const at::Tensor &t) {
+  NormShape r;
+  r.x = t.resolve_neg();
+  const int64_t d = t.dim();
+  r.N = t.size(0), r.C = (int)t.size(d - 1), r.S = 1;
+  for (int64_t k = 1; k < d - 1; k++) r.S *= t.size(k);
+  bool even = t.stride(d - 1) == 1 || r.C == 1;
+  int64_t step = -1, inner = 1;   // position stride, positions of the dimensions already seen
+  for (int64_t k = d - 2; k >= 1 && even; k--) {
+    if (t.size(k) == 1) continue;
+    if (step < 0) step = r.x.stride(k);
+    else even = r.x.stride(k) == step * inner;
+    inner *= t.size(k);
+  }
+  if (!even || r.x.numel() == 0) {
+    r.x = r.x.contiguous();
+    step = r.C;
+  }
+  r.xp = step < 0 ? r.C : step;
+  r.xs = r.N > 1 ? r.x.stride(0) : r.S * r.C;
+  return r;
+}
+
+void norm_check(const at::Tensor &x, int64_t groups, const Maybe &w, const Maybe &b, const Maybe &lengths) {
+  on_gpu(x);
+  type_of(x);
+  if (x.dim() < 2) throw py::value_error("GElib: x has a batch dimension first and its channels last");
+  const int64_t C = x.size(-1);
+  if (groups < 1 || C < 1 || C % groups || C > 0x7fffffff) throw py::value_error("GElib: the number of groups divides the number of channels");
+  for (auto *t : {&w, &b})
+    if (*t) {
+      like(**t, x, t == &w ? "weight" : "bias");
+      if ((*t)->dim() != 1 || (*t)->size(0) != C) throw py::value_error("GElib: weight and bias have one value a channel");
+    }
+  if (lengths) {
+    if (lengths->scalar_type() != at::kInt) throw py::type_error("GElib: lengths are int32");
+    if (lengths->device() != x.device()) throw py::value_error("GElib: lengths are on another device than x");
+    if (lengths->dim() != 1 || lengths->size(0) != x.size(0)) throw py::value_error("GElib: one length a sample");
+  }
+}
+
+std::tuple<at::Tensor, at::Tensor, at::Tensor> norm_fwd(const at::Tensor &x, int64_t groups, const Maybe &w, const Maybe &b, double eps,
+                                                        const std::string &act, const Maybe &lengths, bool keep) {
+  norm_check(x, groups, w, b, lengths);
+  const int a = act_of(act);
+  if (!(eps >= 0)) throw py::value_error("GElib: eps is not below zero");
+  OnDevice on(x);
+  NormShape s = norm_shape(x);
+  at::Tensor W = w ? plain(*w) : at::Tensor(), B = b ? plain(*b) : at::Tensor(), L = lengths ? lengths->contiguous() : at::Tensor();
+  at::Tensor y = at::empty(x.sizes(), x.options().memory_format(at::MemoryFormat::Contiguous)), mean, rstd;
+  if (keep) mean = at::empty({s.N, groups}, x.options().dtype(at::kFloat)), rstd = at::empty_like(mean);
+  const uint64_t bytes = gelib_hip_group_norm_act_workspace_bytes(0, type_of(x), s.N, s.S, s.C, (int)groups);
+  at::Tensor ws = workspace(bytes, x);
+  done(gelib_hip_group_norm_act_fwd(ptr(y), (float *)ptr(mean), (float *)ptr(rstd), ptr(s.x), ptr(W), ptr(B), (int32_t *)ptr(L), type_of(x), s.N, s.S,
+                                    s.C, (int)groups, s.xs, s.xp, (float)eps, a, ptr(ws), bytes, on.stream));
+  return {y, mean, rstd};
+}
+
+std::tuple<Maybe, Maybe, Maybe> norm_bwd(const at::Tensor &gy_, const at::Tensor &mean, const at::Tensor &rstd, const at::Tensor &x, int64_t groups,
+                                         const Maybe &w, const Maybe &b, const std::string &act, const Maybe &lengths, bool need_x, bool need_w,
+                                         bool need_b) {
+  norm_check(x, groups, w, b, lengths);
+  OnDevice on(x);
+  NormShape s = norm_shape(x);
+  at::Tensor gy = plain(gy_), W = w ? plain(*w) : at::Tensor(), B = b ? plain(*b) : at::Tensor(), L = lengths ? lengths->contiguous() : at::Tensor();
+  like(gy, x, "the gradient");
+  if (gy.sizes() != x.sizes()) throw py::value_error("GElib: the gradient has another shape than x");
+  const auto packed = x.options().memory_format(at::MemoryFormat::Contiguous);
+  at::Tensor gx = need_x ? at::empty(x.sizes(), packed) : at::Tensor(), gw = need_w ? at::empty({s.C}, packed) : at::Tensor(),
+             gb = need_b ? at::empty({s.C}, packed) : at::Tensor();
+  const uint64_t bytes = gelib_hip_group_norm_act_workspace_bytes(1, type_of(x), s.N, s.S, s.C, (int)groups);
+  at::Tensor ws = workspace(bytes, x);
+  done(gelib_hip_group_norm_act_bwd(ptr(gx), ptr(gw), ptr(gb), ptr(gy), (float *)ptr(mean), (float *)ptr(rstd), ptr(s.x), ptr(W), ptr(B), (int32_t *)ptr(L),
+                                    type_of(x), s.N, s.S, s.C, (int)groups, s.xs, s.xp, act_of(act), ptr(ws), bytes, on.stream));
+  auto some = [](const at::Tensor &t) { return t.defined() ? Maybe(t) : Maybe(); };
+  return {some(gx), some(gw), some(gb)};
+}
+
+// ---- linear layer ----
+
+struct Rows {   // x as rows: itself where they are evenly spaced and contiguous, else a copy
+  at::Tensor x;
+  int64_t rows, stride;
+  int K;
+};
+Rows rows_of(const at::Tensor &t) {
+  Rows r;
+  r.x = t.resolve_neg();
+  const int64_t d = t.dim();
+  r.K = (int)t.size(d - 1), r.rows = 1;
+  bool even = t.stride(d - 1) == 1 || r.K == 1;
+  int64_t step = -1;
+  for (int64_t k = d - 2; k >= 0; k--) {
+    if (t.size(k) != 1 && even) {
+      if (step < 0) step = r.x.stride(k);
+      else even = r.x.stride(k) == step * r.rows;
+    }
+    r.rows *= t.size(k);
+  }
+  if (!even || r.x.numel() == 0) {
+    r.x = r.x.contiguous();
+    step = r.K;
+  }
+  r.stride = step < 0 ? r.K : step;
+  return r;
+}
+
+void linear_check(const at::Tensor &x, const at::Tensor &w) {
+  on_gpu(x);
+  type_of(x);
+  like(w, x, "w");
+  if (x.dim() < 1 || w.dim() != 2 || w.size(0) != x.size(-1)) throw py::value_error("GElib: x (..., n_in) and w (n_in, n_out) are needed");
+  if (w.size(0) > 0x7fffffff || w.size(1) > 0x7fffffff) throw py::value_error("GElib: too many channels");
+}
+
+std::tuple<at::Tensor, Maybe> linear_fwd(const at::Tensor &x, const at::Tensor &w, const Maybe &b, const Maybe &r, const std::string &act, bool keep) {
+  linear_check(x, w);
+  const int a = act_of(act);
+  std::vector<int64_t> shape(x.sizes().begin(), x.sizes().end());
+  shape.back() = w.size(1);
+  if (b) {
+    like(*b, x, "bias");
+    if (b->dim() != 1 || b->size(0) != w.size(1)) throw py::value_error("GElib: bias has one value a column of w");
+  }
+  if (r) {
+    like(*r, x, "residual");
+    if (r->sizes() != at::IntArrayRef(shape)) throw py::value_error("GElib: residual is shaped like the result");
+  }
+  OnDevice on(x);
+  Rows X = rows_of(x);
+  at::Tensor W = plain(w), B = b ? plain(*b) : at::Tensor(), R = r ? plain(*r) : at::Tensor();
+  const auto packed = x.options().memory_format(at::MemoryFormat::Contiguous);
+  at::Tensor y = at::empty(shape, packed), slope;
+  if (keep && a != GELIB_HIP_ACT_NONE) slope = at::empty(shape, packed.dtype(x.scalar_type() == at::kFloat ? at::kFloat : at::kHalf));
+  const int N = (int)w.size(1);
+  const uint64_t bytes = gelib_hip_linear_act_workspace_bytes(0, type_of(x), X.rows, X.K, N);
+  at::Tensor ws = workspace(bytes, x);
+  done(gelib_hip_linear_act_fwd(ptr(y), ptr(slope), ptr(X.x), ptr(W), ptr(B), ptr(R), type_of(x), X.rows, X.K, N, X.stride, a, ptr(ws), bytes, on.stream));
+  return {y, slope.defined() ? Maybe(slope) : Maybe()};
+}
+
+std::tuple<Maybe, Maybe, Maybe> linear_bwd(const at::Tensor &gy_, const Maybe &slope, const at::Tensor &x, const at::Tensor &w, bool need_x, bool need_w,
+                                           bool need_b) {
+  linear_check(x, w);
+  OnDevice on(x);
+  Rows X = rows_of(x);
+  at::Tensor gy = plain(gy_), W = plain(w);
+  like(gy, x, "the gradient");
+  const int N = (int)w.size(1);
+  if (gy.numel() != X.rows * N) throw py::value_error("GElib: the gradient has another shape than the result");
+  const auto packed = x.options().memory_format(at::MemoryFormat::Contiguous);
+  at::Tensor gx = need_x ? at::empty(x.sizes(), packed) : at::Tensor(), gw = need_w ? at::empty(w.sizes(), packed) : at::Tensor(),
+             gb = need_b ? at::empty({N}, packed) : at::Tensor();
+  const int what = (ptr(gx) ? 1 : 0) | (ptr(gw) ? 2 : 0) | (ptr(gb) ? 4 : 0) | (slope && slope->numel() ? 8 : 0);
+  const uint64_t bytes = gelib_hip_linear_act_workspace_bytes(what, type_of(x), X.rows, X.K, N);
+  at::Tensor ws = workspace(bytes, x);
+  done(gelib_hip_linear_act_bwd(ptr(gx), ptr(gw), ptr(gb), ptr(gy), slope ? ptr(*slope) : nullptr, ptr(X.x), ptr(W), type_of(x), X.rows, X.K, N, X.stride,
+                                ptr(ws), bytes, on.stream));
+  auto some = [](const at::Tensor &t) { return t.defined() ? Maybe(t) : Maybe(); };
+  return {some(gx), some(gw), some(gb)};
+}
+
+// ---- AdamW ----
+
+// The parameters of an optimizer that share hyperparameters: where their moments begin in its arrays and the steps each has taken
+// (one without a gradient takes none).
+struct AdamWGroup {
+  std::vector<at::Tensor> params;
+  std::vector<int64_t> first, steps;
+
+  AdamWGroup(std::vector<at::Tensor> p, std::vector<int64_t> f) : params(std::move(p)), first(std::move(f)), steps(params.size(), 0) {
+    if (first.size() != params.size()) throw py::value_error("GElib: one place a parameter");
+  }
+
+  void step(const at::Tensor &m, const at::Tensor &v, const Maybe &mt, const Maybe &vt, int bits, double lr, double beta1, double beta2, double eps,
+            double decay, uint64_t seed) {
+    struct Lists {
+      std::vector<void *> p;
+      std::vector<const void *> g;
+      std::vector<int64_t> n, first, step;
+    } lists[2];   // float32 and complex64, bfloat16
+    std::vector<at::Tensor> copies;   // of gradients that are not contiguous
+    std::vector<size_t> moved;
+    OnDevice on(m);
+    for (size_t k = 0; k < params.size(); k++) {
+      const at::Tensor &t = params[k], &grad = t.grad();
+      if (!grad.defined() || t.numel() == 0) continue;
+      const auto type = t.scalar_type();
+      const bool cplx = type == at::kComplexFloat;
+      if (!cplx && type != at::kFloat && type != at::kBFloat16) throw py::type_error("GElib: parameters are float32, bfloat16 or complex64");
+      if (grad.is_sparse() || grad.scalar_type() != type) throw py::type_error("GElib: a gradient is dense and has its parameter's type");
+      if (t.device() != m.device() || grad.device() != m.device()) throw py::value_error("GElib: parameters, gradients and moments are on one GPU");
+      if (!t.is_contiguous() || t.is_conj() || t.is_neg()) throw py::value_error("GElib: parameters are contiguous in memory");
+      if (grad.sizes() != t.sizes()) throw py::value_error("GElib: a gradient is shaped like its parameter");
+      const void *g = grad.data_ptr();
+      if (!grad.is_contiguous() || grad.is_conj() || grad.is_neg()) {
+        copies.push_back(grad.resolve_conj().resolve_neg().contiguous());
+        g = copies.back().data_ptr();
+      }
+      Lists &l = lists[type == at::kBFloat16];
+      l.p.push_back(t.data_ptr());
+      l.g.push_back(g);
+      l.n.push_back(t.numel() * (cplx ? 2 : 1));
+      l.first.push_back(first[k]);
+      l.step.push_back(steps[k] + 1);
+      moved.push_back(k);
+    }
+    for (int b = 0; b < 2; b++)
+      if (Lists &l = lists[b]; !l.p.empty())
+        done(gelib_hip_adamw_step((int)l.p.size(), l.p.data(), l.g.data(), l.n.data(), l.first.data(), l.step.data(), ptr(m), ptr(v),
+                                  mt ? (int16_t *)ptr(*mt) : nullptr, vt ? (int16_t *)ptr(*vt) : nullptr, b ? GELIB_HIP_BF16 : GELIB_HIP_F32, bits, lr,
+                                  beta1, beta2, eps, decay, seed, on.stream));
+    for (size_t k : moved) steps[k]++;
+  }
+};
+
+std::tuple<at::Tensor, at::Tensor> adamw_moments(const at::Tensor &m, const at::Tensor &v, const at::Tensor &mt, const at::Tensor &vt) {
+  OnDevice on(m);
+  at::Tensor a = at::empty(m.sizes(), m.options().dtype(at::kBFloat16)), b = at::empty_like(a);
+  done(gelib_hip_adamw_moments(ptr(a), ptr(b), ptr(m), ptr(v), (int16_t *)ptr(mt), (int16_t *)ptr(vt), m.numel(), on.stream));
+  return {a, b};
+}
+
+void adamw_set_moments(const at::Tensor &m, const at::Tensor &v, const at::Tensor &mt, const at::Tensor &vt, const at::Tensor &a, const at::Tensor &b) {
+  OnDevice on(m);
+  TORCH_CHECK(a.scalar_type() == at::kFloat && b.scalar_type() == at::kFloat && a.numel() == m.numel() && b.numel() == m.numel() && a.device() == m.device() &&
+              b.device() == m.device() && a.is_contiguous() && b.is_contiguous(), "GElib: moments are given as float32, one an element");
+  done(gelib_hip_adamw_set_moments(ptr(m), ptr(v), (int16_t *)ptr(mt), (int16_t *)ptr(vt), (float *)ptr(a), (float *)ptr(b), m.numel(), on.stream));
+}
+
+}  // namespace
+
+void bind_real_ops(py::module_ &m) {
+  m.def("group_norm_act_fwd", &norm_fwd);
+  m.def("group_norm_act_bwd", &norm_bwd);
+  m.def("linear_act_fwd", &linear_fwd);
+  m.def("linear_act_bwd", &linear_bwd);
+  py::class_<AdamWGroup>(m, "AdamWGroup", "Parameters of one AdamW step, with the places of their moments")
+      .def(py::init<std::vector<at::Tensor>, std::vector<int64_t>>())
+      .def("step", &AdamWGroup::step)
+      .def_readwrite("steps", &AdamWGroup::steps);
+  m.def("adamw_moments", &adamw_moments);
+  m.def("adamw_set_moments", &adamw_set_moments);
+}

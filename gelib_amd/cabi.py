@@ -26,6 +26,9 @@ SYMBOLS = [
     "gelib_hip_so3vec_cg_linear_bwd", "gelib_hip_so3vec_cg_linear_bwd_workspace_bytes",
     "gelib_hip_set_option", "gelib_hip_set_stream_workspace",
     "gelib_hip_last_path", "gelib_hip_last_streaming",
+    "gelib_hip_group_norm_act_fwd", "gelib_hip_group_norm_act_bwd", "gelib_hip_group_norm_act_workspace_bytes",
+    "gelib_hip_linear_act_fwd", "gelib_hip_linear_act_bwd", "gelib_hip_linear_act_workspace_bytes",
+    "gelib_hip_adamw_step", "gelib_hip_adamw_moments", "gelib_hip_adamw_set_moments",
     "gelib_hip_malloc", "gelib_hip_free", "gelib_hip_memcpy", "gelib_hip_memset", "gelib_hip_synchronize",
 ]
 

@@ -186,6 +186,17 @@ int check_range(const void *ptr, const int64_t dims[5], const int64_t strides[5]
   return GELIB_HIP_OK;
 }
 
+}  // namespace
+
+int check_memory(const void *ptr, int64_t bytes) {
+  const int64_t d[5] = {bytes, 1, 1, 1, 1}, st[5] = {1, 0, 0, 0, 0};
+  return check_range(ptr, d, st, 1);
+}
+
+void set_last_path(PathId path) { t_last_path = path; }
+
+namespace {
+
 int check_pointer(const gelib_part_desc *d) { return check_range(d->ptr, d->dims, d->strides, sizeof(float2)); }
 
 PartDev to_dev(const gelib_part_desc *d, const long long E[3], long long own[3]) {

@@ -32,13 +32,17 @@ struct PartOp {
   bool diag;
 };
 
-enum PathId { kPathNone = 0, kPathGeneric = 1, kPathUnrolled = 2, kPathStaged = 3, kPathDiag6 = 4, kPathOnePair = 5, kPathLinear = 6 };
+enum PathId { kPathNone = 0, kPathGeneric = 1, kPathUnrolled = 2, kPathStaged = 3, kPathDiag6 = 4, kPathOnePair = 5, kPathLinear = 6, kPathReal = 7 };
 
 // ---- coefficient bank (cg_bank.cpp) ----
 double cg_coeff(int l1, int l2, int l, int m1, int m2);
 void cg_matrix_host(int l1, int l2, int l, float *out);
 // Device copy of one (2l1+1)x(2l2+1) table on the current device; cached for the life of the process.
 int cg_matrix_device(int l1, int l2, int l, const float **dptr);
+
+// ---- checks of the C entry points (cabi.cpp) ----
+int check_memory(const void *ptr, int64_t bytes);   // bytes from ptr on are device memory of one allocation of the current GPU
+void set_last_path(PathId path);
 
 // ---- error plumbing ----
 int record_hip_error(hipError_t e, const char *what);

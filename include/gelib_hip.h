@@ -265,6 +265,64 @@ int gelib_hip_so3vec_cg_linear_bwd(const gelib_part_desc *xg, const gelib_part_d
 uint64_t gelib_hip_so3vec_cg_linear_bwd_workspace_bytes(int ng, const gelib_part_desc *g, int nx, const gelib_part_desc *x,
                                                         int ny, const gelib_part_desc *y, int64_t batch_chunk);
 
+/* ---- operators on real channels: the network on invariants behind the equivariant layers, and the step that trains it -------------
+ * No counterpart in the reference, whose users take them from torch.  Tensors hold float32, bfloat16 or float16 values
+ * (enum gelib_hip_dtype; one type per call), channels last and contiguous; sums, statistics and moments are float32.  act:
+ * enum gelib_hip_act (GELU with the error function).  Results overwrite; orders of summation do not depend on timing.
+ * workspace: device memory, 16-byte aligned, of at least what the size query says, rules as for the channel mixing above. */
+enum gelib_hip_dtype { GELIB_HIP_F32 = 0, GELIB_HIP_BF16 = 1, GELIB_HIP_F16 = 2 };
+enum gelib_hip_act { GELIB_HIP_ACT_NONE = 0, GELIB_HIP_ACT_RELU = 1, GELIB_HIP_ACT_SILU = 2, GELIB_HIP_ACT_GELU = 3 };
+
+/* Group norm with an activation.  x: samples x positions x channels at the given strides (elements); a group is
+ * channels / groups neighbouring channels over the first lengths[n] positions of sample n (lengths NULL: all of them; values
+ * are held to 0..positions).  xh = (x - mean) rstd with rstd = (var + eps)^-1/2, y = act(xh weight[c] + bias[c]) (NULL: 1
+ * and 0), packed; zero behind a length, where x is not read.  mean, rstd: float32 (samples, groups) for the backward pass, or
+ * both NULL. */
+int gelib_hip_group_norm_act_fwd(void *y, float *mean, float *rstd, const void *x, const void *weight, const void *bias,
+                                 const int32_t *lengths, int dtype, int64_t samples, int64_t positions, int channels, int groups,
+                                 int64_t x_sample_stride, int64_t x_position_stride, float eps, int act, void *workspace,
+                                 uint64_t workspace_bytes, void *stream);
+/* Its gradients, from the packed gradient gy of y: gx (packed), gw and gb (channels); any of them may be NULL. */
+int gelib_hip_group_norm_act_bwd(void *gx, void *gw, void *gb, const void *gy, const float *mean, const float *rstd, const void *x,
+                                 const void *weight, const void *bias, const int32_t *lengths, int dtype, int64_t samples,
+                                 int64_t positions, int channels, int groups, int64_t x_sample_stride, int64_t x_position_stride,
+                                 int act, void *workspace, uint64_t workspace_bytes, void *stream);
+uint64_t gelib_hip_group_norm_act_workspace_bytes(int backward, int dtype, int64_t samples, int64_t positions, int channels,
+                                                  int groups);
+
+/* Linear layer: z = x w + bias, y = act(z) + residual; x (rows, n_in) at a row stride, w (n_in, n_out) as the matrices of
+ * SO3weights, bias (n_out) and residual (rows, n_out) may be NULL; y packed.  slope (NULL: not wanted; not written where act is
+ * GELIB_HIP_ACT_NONE): act'(z) for the backward pass, (rows, n_out) float32 for float32 layers and float16 for the others. */
+int gelib_hip_linear_act_fwd(void *y, void *slope, const void *x, const void *w, const void *bias, const void *residual, int dtype,
+                             int64_t rows, int n_in, int n_out, int64_t x_row_stride, int act, void *workspace,
+                             uint64_t workspace_bytes, void *stream);
+/* With gz = gy slope (slope NULL: gy): gx = gz w^T, gw = x^T gz, gb = sum of gz over the rows, all packed; any may be NULL.  In
+ * 16-bit layers gz is rounded to the layer's type for the two products, not for gb.  The gradient of the residual is gy. */
+int gelib_hip_linear_act_bwd(void *gx, void *gw, void *gb, const void *gy, const void *slope, const void *x, const void *w, int dtype,
+                             int64_t rows, int n_in, int n_out, int64_t x_row_stride, void *workspace, uint64_t workspace_bytes,
+                             void *stream);
+/* backward: bits 1, 2 and 4 for gx, gw and gb, 8 for a slope; 0 for the forward call */
+uint64_t gelib_hip_linear_act_workspace_bytes(int backward, int dtype, int64_t rows, int n_in, int n_out);
+
+/* One AdamW step over ntensors parameters p[k] of n[k] elements with gradients g[k] of the same type (float32 or bfloat16; a
+ * complex tensor is twice as many floats):
+ *     m = beta1 m + (1 - beta1) g,  v = beta2 v + (1 - beta2) g^2,
+ *     p = p (1 - lr weight_decay) - lr / (1 - beta1^t) m / (sqrt(v / (1 - beta2^t)) + eps),  t = step[k], from 1 on.
+ * The moments of parameter k are elements first[k].. of the arrays m and v, first[k] a multiple of 256; runs do not overlap
+ * and their unused ends are zero.  state_bits 32: float32 arrays, m_top and v_top NULL.  state_bits 8: a byte an element, and
+ * m_top, v_top a 16-bit integer for every 256 elements: code c of v stands for the float whose bits are (c + top - 254) << 20
+ * (0: zero, 255: not finite), code c of m for (c % 128 + top - 126) << 20 with sign c / 128 (0: zero, 127: not finite).  These
+ * codes, and bfloat16 parameters, are rounded at random with bits that are a function of seed, step[k] and element alone. */
+int gelib_hip_adamw_step(int ntensors, void *const *p, const void *const *g, const int64_t *n, const int64_t *first,
+                         const int64_t *step, void *m, void *v, int16_t *m_top, int16_t *v_top, int dtype, int state_bits,
+                         double lr, double beta1, double beta2, double eps, double weight_decay, uint64_t seed, void *stream);
+/* What 8-bit moments stand for, as bfloat16 (exact); n, the elements of the arrays, is a multiple of 256. */
+int gelib_hip_adamw_moments(void *m_values, void *v_values, const void *m, const void *v, const int16_t *m_top, const int16_t *v_top,
+                            int64_t n, void *stream);
+/* The 8-bit moments nearest to float32 values (v not below zero); what moments() told comes back as it was. */
+int gelib_hip_adamw_set_moments(void *m, void *v, int16_t *m_top, int16_t *v_top, const float *m_values, const float *v_values,
+                                int64_t n, void *stream);
+
 /* ---- gather: sums of slices along the batch or a grid dimension ---------------------------------------------------------
  * A gather map is a list of (source, target) pairs with 0 <= source < n_in, 0 <= target < n_out (the arguments of
  * cnine::GatherMapB(sources, targets), python/bindings/gather_map_py.cpp:17-18).  create() checks the indices, sorts the
@@ -362,7 +420,7 @@ int gelib_hip_set_stream_workspace(void *stream, void *ptr, uint64_t bytes);
  * gelib_hip_last_path() tells which kernel family the last call of this thread used
  * (0 = none, 1 = generic, 2 = unrolled small-l kernels, 3 = staged any-l kernels, 4 = lane-per-channel Diag
  * kernels for operand l up to 6, 5 = single-pair kernels for large l, 6 = the product fused with the weight matrices, or
- * the matrices' gradients alone, straight from the operands).
+ * the matrices' gradients alone, straight from the operands, 7 = the operators on real channels).
  */
 int gelib_hip_set_option(const char *name, int value);
 int gelib_hip_last_path(void);
