@@ -1,0 +1,6 @@
+// The matrix products of linear layers of this type.
+#include "linear_gemm.h"
+
+namespace gelib_hip {
+template int launch_gemm<bhalf_t>(GemmForm, int, bool, const GemmArgs &, hipStream_t);
+}

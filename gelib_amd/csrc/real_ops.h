@@ -73,23 +73,42 @@ __device__ __forceinline__ T from_f(float v) { return (T)v; }   // round to near
 
 enum Act { kActNone = 0, kActRelu = 1, kActSilu = 2, kActGelu = 3 };
 
+// Phi(z), the normal distribution, given e = exp(-z^2 / 2): 1/2 erfc(|z| / sqrt 2) as e times a polynomial in 1 / (1 + p |z| / sqrt 2)
+// (Abramowitz & Stegun, Handbook of Mathematical Functions, 7.1.26: erf to 1.5e-7), reflected for z > 0.  The exponential serves
+// the density in gelu' too: value and slope together are 16 instructions, where the library's erff is 40 and exp comes on top.
+__device__ __forceinline__ float normal_cdf(float z, float e) {
+  const float t = __builtin_amdgcn_rcpf(1.f + 0.3275911f * 0.70710678118654752f * __builtin_fabsf(z));
+  const float tail = 0.5f * e * t * (0.254829592f + t * (-0.284496736f + t * (1.421413741f + t * (-1.453152027f + t * 1.061405429f))));
+  return z > 0.f ? 1.f - tail : tail;
+}
+
 // act(z) and act'(z).  exp and the reciprocal are the hardware's (1 ulp): the sums in front of them are the coarser part.
+// kActNone stands for relu too where a flag says so.
+template <int ACT>
+__device__ __forceinline__ void act_both(float z, float &value, float &slope, bool relu = false) {
+  if (ACT == kActSilu) {
+    const float s = __builtin_amdgcn_rcpf(1.f + __expf(-z));
+    value = z * s, slope = s * (1.f + z * (1.f - s));
+  } else if (ACT == kActGelu) {
+    const float e = __expf(-0.5f * z * z), cdf = normal_cdf(z, e);
+    value = z * cdf, slope = cdf + z * 0.39894228040143268f * e;
+  } else if (ACT == kActRelu || relu) {
+    value = z < 0.f ? 0.f : z, slope = z > 0.f ? 1.f : z == z ? 0.f : z;   // (a NaN stays one)
+  } else {
+    value = z, slope = 1.f;
+  }
+}
 template <int ACT>
 __device__ __forceinline__ float act_value(float z) {
-  if (ACT == kActRelu) return z < 0.f ? 0.f : z;   // (a NaN stays one)
-  if (ACT == kActSilu) return z * __builtin_amdgcn_rcpf(1.f + __expf(-z));
-  if (ACT == kActGelu) return 0.5f * z * (1.f + erff(z * 0.70710678118654752f));
-  return z;
+  float v, s;
+  act_both<ACT>(z, v, s);
+  return v;
 }
 template <int ACT>
 __device__ __forceinline__ float act_slope(float z) {
-  if (ACT == kActRelu) return z > 0.f ? 1.f : z == z ? 0.f : z;
-  if (ACT == kActSilu) {
-    const float s = __builtin_amdgcn_rcpf(1.f + __expf(-z));
-    return s * (1.f + z * (1.f - s));
-  }
-  if (ACT == kActGelu) return 0.5f * (1.f + erff(z * 0.70710678118654752f)) + z * 0.39894228040143268f * __expf(-0.5f * z * z);
-  return 1.f;
+  float v, s;
+  act_both<ACT>(z, v, s);
+  return s;
 }
 #endif
 
