@@ -62,7 +62,8 @@ int act_of(const std::string &act) {
 // ---- group norm ----
 
 // x as samples x positions x channels: the strides of its samples and positions, of x itself where its positions are evenly
-// spaced and its channels contiguous, else of a copy
+// spaced, its channels contiguous and its rows aligned as those of a packed tensor are (16 bytes where the number of channels
+// allows), else of a copy: reading and writing it once is less than narrow loads cost, and a result does not depend on the layout
 struct NormShape {
   at::Tensor x;
   int64_t N, S, xs, xp;
@@ -82,8 +83,10 @@ NormShape norm_shape(const at::Tensor &t) {
     else even = r.x.stride(k) == step * inner;
     inner *= t.size(k);
   }
+  const int64_t e = t.element_size(), width = r.C % (16 / e) == 0 ? 16 / e : r.C % 2 == 0 ? 2 : 1;
+  if (even) even = (step < 0 || step % width == 0) && (r.N == 1 || r.x.stride(0) % width == 0) && (uintptr_t)r.x.data_ptr() % (width * e) == 0;
   if (!even || r.x.numel() == 0) {
-    r.x = r.x.contiguous();
+    r.x = r.x.is_contiguous() ? r.x.clone() : r.x.contiguous();
     step = r.C;
   }
   r.xp = step < 0 ? r.C : step;
@@ -132,7 +135,9 @@ std::tuple<Maybe, Maybe, Maybe> norm_bwd(const at::Tensor &gy_, const at::Tensor
   norm_check(x, groups, w, b, lengths);
   OnDevice on(x);
   NormShape s = norm_shape(x);
-  at::Tensor gy = plain(gy_), W = w ? plain(*w) : at::Tensor(), B = b ? plain(*b) : at::Tensor(), L = lengths ? lengths->contiguous() : at::Tensor();
+  at::Tensor gy = plain(gy_);
+  if ((uintptr_t)gy.data_ptr() % 16) gy = gy.clone();
+  at::Tensor W = w ? plain(*w) : at::Tensor(), B = b ? plain(*b) : at::Tensor(), L = lengths ? lengths->contiguous() : at::Tensor();
   like(gy, x, "the gradient");
   if (gy.sizes() != x.sizes()) throw py::value_error("GElib: the gradient has another shape than x");
   const auto packed = x.options().memory_format(at::MemoryFormat::Contiguous);

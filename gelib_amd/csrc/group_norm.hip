@@ -1,8 +1,9 @@
-// Group norm with an activation, channels last: a group is C / G neighbouring channels over the positions of a sample that count,
-//     xh = (x - mean) rstd,  y = act(xh w + b);   gz = gy act'(z), q = gz w, gx = rstd (q - mean(q) - xh mean(q xh)),
-//     gw = sum gz xh, gb = sum gz over samples and positions.
-// Positions behind a sample's length are zero in y and gx and are never read.
-#include "real_ops.h"
+// Group norm with an activation (group_norm_impl.h): how a call's tensors are cut into blocks, and simple kernels for what those do
+// not take (one block cannot hold a row of the channels that a group and the loads' alignment ask for: groups of more than 512
+// loads, 4096 bfloat16 channels).
+#include <numeric>
+
+#include "group_norm_impl.h"
 
 namespace gelib_hip {
 
@@ -17,16 +18,12 @@ __device__ __forceinline__ float block_sum(float v, float *lds) {
   return (lds[0] + lds[1]) + (lds[2] + lds[3]);
 }
 
-__device__ __forceinline__ long long length_of(const NormArgs &a, long long n) {
-  return a.lengths ? (long long)max(0, (int)min((long long)a.lengths[n], a.S)) : a.S;
-}
-
 // a block per (sample, group)
 template <typename T, int ACT>
-__global__ void __launch_bounds__(256) norm_fwd_kernel(const NormArgs a) {
+__global__ void __launch_bounds__(256) norm_wide_fwd(const NormArgs a, long long base) {
   __shared__ float lds[4];
-  const long long n = blockIdx.x / a.G;
-  const int g = (int)(blockIdx.x % a.G), cg = a.C / a.G, c0 = g * cg;
+  const long long tile = base + blockIdx.x, n = tile / a.G;
+  const int g = (int)(tile % a.G), cg = a.C / a.G, c0 = g * cg;
   const long long len = length_of(a, n), cnt = len * cg;
   const T *x = (const T *)a.x + n * a.xs + c0;
   T *y = (T *)a.y + n * a.S * a.C + c0;
@@ -39,7 +36,7 @@ __global__ void __launch_bounds__(256) norm_fwd_kernel(const NormArgs a) {
     sum += d * d;
   }
   const float rstd = 1.f / sqrtf((cnt ? block_sum(sum, lds) / (float)cnt : 0.f) + a.eps);
-  if (a.mean && threadIdx.x == 0) a.mean[blockIdx.x] = mean, a.rstd[blockIdx.x] = rstd;
+  if (a.mean && threadIdx.x == 0) a.mean[tile] = mean, a.rstd[tile] = rstd;
   for (long long i = threadIdx.x; i < a.S * cg; i += 256) {
     const long long s = i / cg;
     const int c = (int)(i % cg);
@@ -53,14 +50,14 @@ __global__ void __launch_bounds__(256) norm_fwd_kernel(const NormArgs a) {
 }
 
 template <typename T, int ACT>
-__global__ void __launch_bounds__(256) norm_gx_kernel(const NormArgs a) {
+__global__ void __launch_bounds__(256) norm_wide_gx(const NormArgs a, long long base) {
   __shared__ float lds[4];
-  const long long n = blockIdx.x / a.G;
-  const int g = (int)(blockIdx.x % a.G), cg = a.C / a.G, c0 = g * cg;
+  const long long tile = base + blockIdx.x, n = tile / a.G;
+  const int g = (int)(tile % a.G), cg = a.C / a.G, c0 = g * cg;
   const long long len = length_of(a, n), cnt = len * cg;
   const T *x = (const T *)a.x + n * a.xs + c0, *gy = (const T *)a.gy + n * a.S * a.C + c0;
   T *gx = (T *)a.y + n * a.S * a.C + c0;
-  const float mean = a.mean[blockIdx.x], rstd = a.rstd[blockIdx.x];
+  const float mean = a.mean[tile], rstd = a.rstd[tile];
   auto at = [&](long long i, float &q, float &xh) {
     const long long s = i / cg;
     const int c = (int)(i % cg);
@@ -86,7 +83,7 @@ __global__ void __launch_bounds__(256) norm_gx_kernel(const NormArgs a) {
 
 // a block per channel
 template <typename T, int ACT>
-__global__ void __launch_bounds__(256) norm_gw_kernel(const NormArgs a) {
+__global__ void __launch_bounds__(256) norm_wide_gw(const NormArgs a) {
   __shared__ float lds[4];
   const int c = blockIdx.x, g = c / (a.C / a.G);
   const float w = a.w ? to_f(((const T *)a.w)[c]) : 1.f, b = a.b ? to_f(((const T *)a.b)[c]) : 0.f;
@@ -106,37 +103,128 @@ __global__ void __launch_bounds__(256) norm_gw_kernel(const NormArgs a) {
 }
 
 template <typename T, int ACT>
-int run(bool backward, const NormArgs &a, hipStream_t s) {
-  const long long tiles = a.S ? a.N * a.G : 0;
-  if (!tiles && !a.gw && !a.gb) return 0;
-  if (!backward) {
-    if (tiles) hipLaunchKernelGGL((norm_fwd_kernel<T, ACT>), dim3((unsigned)tiles), dim3(256), 0, s, a);
-  } else {
-    if (tiles && a.y) hipLaunchKernelGGL((norm_gx_kernel<T, ACT>), dim3((unsigned)tiles), dim3(256), 0, s, a);
-    if (a.gw || a.gb) hipLaunchKernelGGL((norm_gw_kernel<T, ACT>), dim3(a.C), dim3(256), 0, s, a);
+int run_wide(bool backward, const NormArgs &a, hipStream_t s) {
+  const long long tiles = a.N * a.G, most = 1LL << 23;   // blocks of a launch
+  for (long long t = 0; t < tiles; t += most) {
+    const dim3 grid((unsigned)std::min(most, tiles - t));
+    if (!backward) hipLaunchKernelGGL((norm_wide_fwd<T, ACT>), grid, dim3(256), 0, s, a, t);
+    else if (a.y) hipLaunchKernelGGL((norm_wide_gx<T, ACT>), grid, dim3(256), 0, s, a, t);
   }
+  if (backward && (a.gw || a.gb)) hipLaunchKernelGGL((norm_wide_gw<T, ACT>), dim3(a.C), dim3(256), 0, s, a);
   const hipError_t e = hipGetLastError();
   return e == hipSuccess ? 0 : record_hip_error(e, "group norm launch");
 }
 
 template <typename T>
-int run_act(bool backward, const NormArgs &a, hipStream_t s) {
+int run_wide_act(bool backward, const NormArgs &a, hipStream_t s) {
   switch (a.act) {
-    case kActRelu: return run<T, kActRelu>(backward, a, s);
-    case kActSilu: return run<T, kActSilu>(backward, a, s);
-    case kActGelu: return run<T, kActGelu>(backward, a, s);
+    case kActRelu: return run_wide<T, kActRelu>(backward, a, s);
+    case kActSilu: return run_wide<T, kActSilu>(backward, a, s);
+    case kActGelu: return run_wide<T, kActGelu>(backward, a, s);
   }
-  return run<T, kActNone>(backward, a, s);
+  return run_wide<T, kActNone>(backward, a, s);
+}
+
+// How a call is cut; false where one block cannot hold a row of the channels that belong together.
+bool plan_norm(bool backward, int V, int e, long long N, long long S, int C, int G, NormPlan *out) {
+  NormPlan p = {};
+  const int cg = C / G, Cq = V / std::gcd(V, cg) * cg, quanta = C / Cq;   // Cq: whole groups and whole loads
+  if (Cq / V > kNormMostT) return false;
+  p.V = V;
+  auto stripes_of = [&](int per) {   // stripes of about `per` quanta, as even as they can be
+    per = std::max(1, std::min(per, quanta));
+    p.stripes = (quanta + per - 1) / per;
+    p.Cw = (quanta + p.stripes - 1) / p.stripes * Cq;
+    p.stripes = (C + p.Cw - 1) / p.Cw;
+    p.TX = p.Cw / V;
+  };
+  stripes_of((128 / e + Cq - 1) / Cq);
+  const int down = std::max(1, kNormMostT / p.TX);
+  p.NS = 1;
+  if (S <= (long long)down * kNormMostR) {
+    p.TY = (int)std::min<long long>(S, down);
+    p.R = (int)((S + p.TY - 1) / p.TY);
+    // several small samples a block, as long as 512 blocks are left
+    p.NS = (int)std::max<long long>(1, std::min<long long>(256 / (p.TX * p.TY), N * p.stripes / 512));
+    const long long sets = (N + p.NS - 1) / p.NS;
+    // forward: a block a set; backward: about a thousand blocks walk over the sets, each with one row of sums for gw and gb
+    p.blocks = std::min<long long>(sets, backward ? std::max(1, 1024 / p.stripes) : 1 << 22);
+  } else {
+    stripes_of(256 * V / Cq);
+    p.TY = std::max(1, kNormMostT / p.TX);
+    int r = kNormMostR;
+    while (r > 1 && N * ((S + (long long)r * p.TY - 1) / ((long long)r * p.TY)) * p.stripes < 512) r /= 2;
+    p.rows = (long long)r * p.TY;
+    p.chunks = (S + p.rows - 1) / p.rows;
+    if (p.chunks > 1 << 22) return false;
+  }
+  p.T = (p.TX * p.TY * p.NS + 63) / 64 * 64;
+  *out = p;
+  return p.stripes <= 65535;
+}
+
+struct NormSpace {
+  size_t stats = 0, sums = 0, means = 0, total = 0;   // offsets of the last two in front of them
+};
+NormSpace space_of(bool backward, const NormPlan &p, long long N, int C, int G) {
+  auto up = [](size_t n) { return (n + 255) & ~(size_t)255; };
+  NormSpace r;
+  const size_t stats = p.R ? 0 : up((size_t)N * p.chunks * 8 * (backward ? C : G));
+  r.sums = stats;
+  const size_t sums = !backward ? 0 : up((size_t)(p.R ? p.blocks : N) * C * 8);
+  r.means = r.sums + sums;
+  r.total = r.means + (p.R ? 0 : up((size_t)N * G * 8));   // (forward: means and rstds of a call that keeps none)
+  return r;
+}
+
+// the widest load that every row of a call allows
+int load_width(const NormArgs &a, int e) {
+  const uintptr_t p = (uintptr_t)a.x | (uintptr_t)a.y | (uintptr_t)a.gy;
+  for (int V : {16 / e, 2})
+    if (a.C % V == 0 && a.xs % V == 0 && a.xp % V == 0 && p % (V * e) == 0) return V;
+  return 1;
+}
+
+template <typename T>
+int run_empty(const NormArgs &a, hipStream_t s) {
+  hipLaunchKernelGGL((norm_join<T>), dim3((2 * a.C + 31) / 32), dim3(256), 0, s, (const float *)nullptr, (T *)a.gw, (T *)a.gb, 0LL, a.C);
+  const hipError_t e = hipGetLastError();
+  return e == hipSuccess ? 0 : record_hip_error(e, "group norm launch");
 }
 
 }  // namespace
 
-size_t norm_workspace(bool, int, long long, long long, int, int) { return 0; }
+size_t norm_workspace(bool backward, int dtype, long long N, long long S, int C, int G) {
+  if (N == 0 || S == 0) return 0;
+  const int e = (int)dtype_bytes(dtype);
+  size_t most = 0;
+  for (int V : {16 / e, 2, 1}) {
+    NormPlan p;
+    if (C % V == 0 && plan_norm(backward, V, e, N, S, C, G, &p)) most = std::max(most, space_of(backward, p, N, C, G).total);
+  }
+  return most;
+}
 
 int launch_norm(bool backward, int dtype, const NormArgs &a, hipStream_t s) {
-  if (dtype == GELIB_HIP_F32) return run_act<float>(backward, a, s);
-  if (dtype == GELIB_HIP_BF16) return run_act<bhalf_t>(backward, a, s);
-  return run_act<half_t>(backward, a, s);
+  const bool sums = backward && (a.gw || a.gb);
+  if (a.N == 0 || a.S == 0) {
+    if (!sums) return 0;
+    return dtype == GELIB_HIP_F32 ? run_empty<float>(a, s) : dtype == GELIB_HIP_BF16 ? run_empty<bhalf_t>(a, s) : run_empty<half_t>(a, s);
+  }
+  if (backward && !sums && !a.y) return 0;
+  const int e = (int)dtype_bytes(dtype);
+  NormDev d = {};
+  d.a = a;
+  if (!plan_norm(backward, load_width(a, e), e, a.N, a.S, a.C, a.G, &d.p))
+    return dtype == GELIB_HIP_F32 ? run_wide_act<float>(backward, a, s) : dtype == GELIB_HIP_BF16 ? run_wide_act<bhalf_t>(backward, a, s) : run_wide_act<half_t>(backward, a, s);
+  const NormSpace sp = space_of(backward, d.p, a.N, a.C, a.G);
+  char *ws = (char *)a.ws;
+  if (!d.p.R) d.stats = (float *)ws;
+  if (sums || (backward && !d.p.R)) d.sums = (float *)(ws + sp.sums);
+  if (!d.p.R && backward) d.means = (float *)(ws + sp.means);
+  if (!d.p.R && !backward && !a.mean) d.a.mean = (float *)(ws + sp.means), d.a.rstd = d.a.mean + a.N * a.G;
+  return dtype == GELIB_HIP_F32 ? launch_norm_typed<float>(backward, d, s) : dtype == GELIB_HIP_BF16 ? launch_norm_typed<bhalf_t>(backward, d, s)
+                                                                                                     : launch_norm_typed<half_t>(backward, d, s);
 }
 
 }  // namespace gelib_hip

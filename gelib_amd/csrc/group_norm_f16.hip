@@ -1,0 +1,6 @@
+// Group norm of this type.
+#include "group_norm_impl.h"
+
+namespace gelib_hip {
+template int launch_norm_typed<half_t>(bool, const NormDev &, hipStream_t);
+}

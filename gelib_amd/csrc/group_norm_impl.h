@@ -1,0 +1,647 @@
+// Group norm with an activation, channels last: a group is C / G neighbouring channels over the positions of a sample that count,
+//     xh = (x - mean) rstd,  y = act(xh w + b);   gz = gy act'(z), q = gz w, gx = rstd (q - mean(q) - xh mean(q xh)),
+//     gw = sum gz xh, gb = sum gz over samples and positions.
+// Positions behind a sample's length are zero in y and gx and are never read.
+//
+// A block owns whole groups of one sample (or of several small ones): a stripe of Cw channels, at least 128 bytes of a row, by all
+// positions, TX threads of V channels (one load) side by side and TY of them down the positions.  Where a stripe fits a block's
+// registers (16 loads a thread, 512 threads: 128 KB) it is read once, and the statistics are formed around the mean from registers;
+// the backward pass keeps gz there too, in float32.  Larger samples are cut into chunks of positions: every chunk's mean and sum of
+// squares around it (backward: its channel sums), joined by the parallel form of the variance, then a second pass over x, which the
+// memory-side cache still holds up to its 256 MB.  What bounds either is HBM; sums go over channels first and groups after, so any
+// channels a group will do, and the channel sums are the gradients of w and b.
+// No atomics: sums have one order.
+#pragma once
+
+#include "real_ops.h"
+
+namespace gelib_hip {
+
+struct NormPlan {
+  int V, TX, TY, NS, R;       // channels a load; threads across and down; samples of a block; loads a thread holds (0: in chunks)
+  int Cw, stripes;            // channels of a block
+  int T;                      // threads
+  long long rows, chunks;     // positions of a chunk, chunks of a sample (in chunks)
+  long long blocks;           // along the samples (whole: they walk over the groups of NS samples)
+};
+
+struct NormDev {
+  NormArgs a;
+  NormPlan p;
+  float *stats;   // in chunks, forward: [n][chunk][G] mean and sum of squares; backward: [n][chunk][2][C]
+  float *sums;    // backward: [blocks or n][2][C] channel sums of gz xh and of gz
+  float *means;   // in chunks, backward: [n][G][2] mean of q and of q xh
+};
+
+template <typename T>
+int launch_norm_typed(bool backward, const NormDev &d, hipStream_t s);
+
+#ifdef __HIPCC__
+
+namespace {
+
+constexpr int kNormMostT = 512, kNormMostR = 16;
+
+template <typename T, int V>
+struct Pack {
+  T v[V];
+};
+template <typename T, int V>
+__device__ __forceinline__ Pack<T, V> load_pack(const T *p) {
+  Pack<T, V> r;
+  __builtin_memcpy(&r, __builtin_assume_aligned(p, V * sizeof(T)), sizeof(r));
+  return r;
+}
+template <typename T, int V>
+__device__ __forceinline__ void store_pack(T *p, const Pack<T, V> &r) { __builtin_memcpy(__builtin_assume_aligned(p, V * sizeof(T)), &r, sizeof(r)); }
+
+__device__ __forceinline__ long long length_of(const NormArgs &a, long long n) {
+  return a.lengths ? max(0LL, min((long long)a.lengths[n], a.S)) : a.S;
+}
+
+// Where a thread stands: its first channel in the stripe and in the row, its place down the positions
+struct Place {
+  int tx, ns, ty, col, c0, cw;   // col: first of its V columns among the block's NS * Cw; cw: channels of this stripe
+  bool on;
+};
+__device__ __forceinline__ Place place_of(const NormDev &d) {
+  Place w;
+  const int t = threadIdx.x, rest = t / d.p.TX;
+  w.tx = t - rest * d.p.TX;
+  w.ty = rest / d.p.NS;
+  w.ns = rest - w.ty * d.p.NS;
+  w.c0 = blockIdx.y * d.p.Cw;
+  w.cw = min(d.p.Cw, d.a.C - w.c0);
+  w.col = w.ns * d.p.Cw + w.tx * d.p.V;
+  w.on = w.ty < d.p.TY && w.tx * d.p.V < w.cw;
+  return w;
+}
+
+// Sums of v over the threads down the positions, one for every column, into out[column] (out and scratch: columns * TY floats and
+// columns * parts).  All threads take part.
+template <int V>
+__device__ __forceinline__ void column_sums(const NormDev &d, const Place &w, const float *v, float *lds, float *out) {
+  const int cols = d.p.NS * d.p.Cw, t = threadIdx.x;
+  __syncthreads();
+  if (w.ty < d.p.TY) {
+#pragma unroll
+    for (int i = 0; i < V; i++) lds[w.ty * cols + w.col + i] = v[i];
+  }
+  __syncthreads();
+  const int parts = max(1, min(d.p.TY, d.p.T / cols));
+  if (parts == 1) {
+    for (int c = t; c < cols; c += d.p.T) {
+      float s = 0.f;
+      for (int k = 0; k < d.p.TY; k++) s += lds[k * cols + c];
+      out[c] = s;
+    }
+    __syncthreads();
+    return;
+  }
+  const int c = t % cols, part = t / cols;
+  float s = 0.f;
+  if (part < parts) {
+    for (int k = part; k < d.p.TY; k += parts) s += lds[k * cols + c];
+  }
+  __syncthreads();
+  if (part < parts) lds[part * cols + c] = s;
+  __syncthreads();
+  if (t < cols) {
+    for (int k = 1; k < parts; k++) s += lds[k * cols + t];
+    out[t] = s;
+  }
+  __syncthreads();
+}
+
+// of[g] = f(sum over the columns of group g of in), for the NS * groups of the block; f(group, sum)
+template <typename F>
+__device__ __forceinline__ void group_sums(const NormDev &d, const Place &w, const float *in, F f) {
+  const int cg = d.a.C / d.a.G, gs = w.cw / cg, groups = d.p.NS * gs;
+  if (cg <= 16) {
+    for (int g = threadIdx.x; g < groups; g += d.p.T) {
+      const float *p = in + g / gs * d.p.Cw + g % gs * cg;
+      float s = 0.f;
+      for (int i = 0; i < cg; i++) s += p[i];
+      f(g, s);
+    }
+  } else {
+    const int waves = d.p.T / 64, lane = threadIdx.x % 64;
+    for (int g = threadIdx.x / 64; g < groups && (int)threadIdx.x / 64 < waves; g += waves) {
+      const float *p = in + g / gs * d.p.Cw + g % gs * cg;
+      float s = 0.f;
+      for (int i = lane; i < cg; i += 64) s += p[i];
+#pragma unroll
+      for (int m = 32; m >= 1; m >>= 1) s += __shfl_xor(s, m);
+      if (lane == 0) f(g, s);
+    }
+  }
+  __syncthreads();
+}
+
+template <typename T, int V>
+__device__ __forceinline__ void load_channels(const void *from, const Place &w, float otherwise, float *v) {
+#pragma unroll
+  for (int i = 0; i < V; i++) v[i] = from && w.on ? to_f(((const T *)from)[w.c0 + w.tx * V + i]) : otherwise;
+}
+// the group (of the block's NS * groups) of each of a thread's channels
+template <int V>
+__device__ __forceinline__ void groups_of(const NormDev &d, const Place &w, int *g) {
+  const int cg = d.a.C / d.a.G, gs = w.cw / cg;
+#pragma unroll
+  for (int i = 0; i < V; i++) g[i] = w.on ? w.ns * gs + (w.tx * V + i) / cg : 0;
+}
+
+extern __shared__ float norm_lds[];
+
+// Statistics of what the threads hold in xr (R loads each, those at positions below len count): mean and sum of squares around it of
+// every group of the block, in mean[] and square[].
+template <typename T, int V, int R>
+__device__ __forceinline__ void block_stats(const NormDev &d, const Place &w, const Pack<T, V> *xr, long long len, float *scratch, float *chan, float *mean,
+                                            float *square) {
+  float s[V] = {};
+  int g[V];
+  groups_of<V>(d, w, g);
+#pragma unroll
+  for (int r = 0; r < R; r++)
+    if (w.on && w.ty + (long long)r * d.p.TY < len) {
+#pragma unroll
+      for (int i = 0; i < V; i++) s[i] += to_f(xr[r].v[i]);
+    }
+  // (a sample's length: every group of it has the same count)
+  float *lens = square + d.p.NS * (d.p.Cw / (d.a.C / d.a.G));
+  if (w.tx == 0 && w.ty == 0) lens[w.ns] = (float)len;
+  column_sums<V>(d, w, s, scratch, chan);
+  const int cg = d.a.C / d.a.G, gs = w.cw / cg;
+  group_sums(d, w, chan, [&](int k, float sum) { mean[k] = lens[k / gs] > 0.f ? sum / (lens[k / gs] * (float)cg) : 0.f; });
+#pragma unroll
+  for (int i = 0; i < V; i++) s[i] = 0.f;
+  float mu[V];
+#pragma unroll
+  for (int i = 0; i < V; i++) mu[i] = mean[g[i]];
+#pragma unroll
+  for (int r = 0; r < R; r++)
+    if (w.on && w.ty + (long long)r * d.p.TY < len) {
+#pragma unroll
+      for (int i = 0; i < V; i++) {
+        const float e = to_f(xr[r].v[i]) - mu[i];
+        s[i] += e * e;
+      }
+    }
+  column_sums<V>(d, w, s, scratch, chan);
+  group_sums(d, w, chan, [&](int k, float sum) { square[k] = sum; });
+}
+
+// LDS of a block: partial column sums, two sets of column sums, two numbers a group, a length a sample
+inline size_t norm_lds_bytes(const NormPlan &p, int cg) {
+  const size_t cols = (size_t)p.NS * p.Cw;
+  return (cols * p.TY + 2 * cols + 2 * (size_t)p.NS * (p.Cw / cg) + p.NS) * 4;
+}
+struct Lds {
+  float *scratch, *chan, *chan2, *first, *second;
+};
+__device__ __forceinline__ Lds lds_of(const NormDev &d) {
+  const int cols = d.p.NS * d.p.Cw;
+  Lds l;
+  l.scratch = norm_lds, l.chan = l.scratch + cols * d.p.TY, l.chan2 = l.chan + cols, l.first = l.chan2 + cols;
+  l.second = l.first + d.p.NS * (d.p.Cw / (d.a.C / d.a.G));
+  return l;
+}
+
+template <typename T, int V, int ACT, int R>
+__global__ void __launch_bounds__(kNormMostT) norm_whole_fwd(const NormDev d) {
+  const Place w = place_of(d);
+  const Lds l = lds_of(d);
+  const NormArgs &a = d.a;
+  const int cg = a.C / a.G, gs = w.cw / cg;
+  float W[V], B[V];
+  int g[V];
+  load_channels<T, V>(a.w, w, 1.f, W);
+  load_channels<T, V>(a.b, w, 0.f, B);
+  groups_of<V>(d, w, g);
+  for (long long n0 = (long long)blockIdx.x * d.p.NS; n0 < a.N; n0 += (long long)gridDim.x * d.p.NS) {
+    const long long n = n0 + w.ns;
+    const bool on = w.on && n < a.N;
+    const long long len = n < a.N ? length_of(a, n) : 0;
+    const T *x = (const T *)a.x + n * a.xs + w.c0 + w.tx * V;
+    Pack<T, V> xr[R];
+#pragma unroll
+    for (int r = 0; r < R; r++) {
+      const long long s = w.ty + (long long)r * d.p.TY;
+      if (on && s < len) xr[r] = load_pack<T, V>(x + s * a.xp);
+    }
+    block_stats<T, V, R>(d, w, xr, len, l.scratch, l.chan, l.first, l.second);
+    float mu[V], k[V];
+#pragma unroll
+    for (int i = 0; i < V; i++) {
+      mu[i] = l.first[g[i]];
+      const float cnt = (float)len * (float)cg;
+      k[i] = 1.f / sqrtf((cnt > 0.f ? l.second[g[i]] / cnt : 0.f) + a.eps);
+      if (a.mean && on && w.ty == 0 && (w.tx * V + i) % cg == 0) {
+        const long long at = n * a.G + w.c0 / cg + g[i] - w.ns * gs;
+        a.mean[at] = mu[i], a.rstd[at] = k[i];
+      }
+      k[i] *= W[i];
+    }
+    T *y = (T *)a.y + n * a.S * a.C + w.c0 + w.tx * V;
+#pragma unroll
+    for (int r = 0; r < R; r++) {
+      const long long s = w.ty + (long long)r * d.p.TY;
+      if (!on || s >= a.S) continue;
+      Pack<T, V> o;
+#pragma unroll
+      for (int i = 0; i < V; i++) {
+        float v, e;
+        act_both<ACT>((to_f(xr[r].v[i]) - mu[i]) * k[i] + B[i], v, e, a.act == kActRelu);
+        o.v[i] = from_f<T>(s < len ? v : 0.f);
+      }
+      store_pack<T, V>(y + s * a.C, o);
+    }
+    __syncthreads();
+  }
+}
+
+// xh and gz of one load
+template <typename T, int V, int ACT>
+__device__ __forceinline__ void gz_of(const Pack<T, V> &x, const Pack<T, V> &gy, const float *mu, const float *k, const float *W, const float *B, bool relu,
+                                      float *xh, float *gz) {
+#pragma unroll
+  for (int i = 0; i < V; i++) {
+    float v, e;
+    xh[i] = (to_f(x.v[i]) - mu[i]) * k[i];
+    act_both<ACT>(xh[i] * W[i] + B[i], v, e, relu);
+    gz[i] = to_f(gy.v[i]) * e;
+  }
+}
+
+// adds the NS samples' column sums to a thread's running ones (channel threadIdx.x + j T of the stripe)
+template <int J>
+__device__ __forceinline__ void keep_sums(const NormDev &d, const Place &w, const float *chan, float *acc) {
+#pragma unroll
+  for (int j = 0; j < J; j++) {
+    const int c = threadIdx.x + j * d.p.T;
+    if (c < w.cw)
+      for (int k = 0; k < d.p.NS; k++) acc[j] += chan[k * d.p.Cw + c];
+  }
+}
+// sums of q = gz w and of q xh of the groups, divided by their count, from the column sums of gz and gz xh
+template <typename T>
+__device__ __forceinline__ void group_means(const NormDev &d, const Place &w, float *chan, float *chan2, const float *lens, float *m1, float *m2) {
+  const int cg = d.a.C / d.a.G, gs = w.cw / cg, cols = d.p.NS * d.p.Cw;
+  if (d.a.w) {
+    for (int c = threadIdx.x; c < cols; c += d.p.T)
+      if (c % d.p.Cw < w.cw) {
+        const float W = to_f(((const T *)d.a.w)[w.c0 + c % d.p.Cw]);
+        chan[c] *= W, chan2[c] *= W;
+      }
+    __syncthreads();
+  }
+  auto mean = [&](float *m) { return [=](int k, float sum) { m[k] = lens[k / gs] > 0.f ? sum / (lens[k / gs] * (float)cg) : 0.f; }; };
+  group_sums(d, w, chan, mean(m1));
+  group_sums(d, w, chan2, mean(m2));
+}
+
+template <typename T, int V, int ACT, int R>
+__global__ void __launch_bounds__(kNormMostT) norm_whole_bwd(const NormDev d) {
+  const Place w = place_of(d);
+  const Lds l = lds_of(d);
+  const NormArgs &a = d.a;
+  const int cg = a.C / a.G, gs = w.cw / cg;
+  float W[V], B[V], accw[V] = {}, accb[V] = {};
+  int g[V];
+  load_channels<T, V>(a.w, w, 1.f, W);
+  load_channels<T, V>(a.b, w, 0.f, B);
+  groups_of<V>(d, w, g);
+  float *lens = l.second + d.p.NS * (d.p.Cw / cg);
+  for (long long n0 = (long long)blockIdx.x * d.p.NS; n0 < a.N; n0 += (long long)gridDim.x * d.p.NS) {
+    const long long n = n0 + w.ns;
+    const bool on = w.on && n < a.N;
+    const long long len = n < a.N ? length_of(a, n) : 0;
+    const T *x = (const T *)a.x + n * a.xs + w.c0 + w.tx * V, *gy = (const T *)a.gy + n * a.S * a.C + w.c0 + w.tx * V;
+    Pack<T, V> xr[R], gr[R];
+    float mu[V], k[V], gz[R][V], s1[V] = {}, s2[V] = {};
+#pragma unroll
+    for (int r = 0; r < R; r++) {
+      const long long s = w.ty + (long long)r * d.p.TY;
+      if (on && s < len) xr[r] = load_pack<T, V>(x + s * a.xp), gr[r] = load_pack<T, V>(gy + s * a.C);
+    }
+#pragma unroll
+    for (int i = 0; i < V; i++) {
+      const long long at = n * a.G + w.c0 / cg + g[i] - w.ns * gs;
+      mu[i] = on ? a.mean[at] : 0.f, k[i] = on ? a.rstd[at] : 0.f;
+    }
+#pragma unroll
+    for (int r = 0; r < R; r++)
+      if (on && w.ty + (long long)r * d.p.TY < len) {
+        float xh[V];
+        gz_of<T, V, ACT>(xr[r], gr[r], mu, k, W, B, a.act == kActRelu, xh, gz[r]);
+#pragma unroll
+        for (int i = 0; i < V; i++) s1[i] += gz[r][i], s2[i] += gz[r][i] * xh[i];
+      }
+    if (w.tx == 0 && w.ty == 0) lens[w.ns] = (float)len;
+    column_sums<V>(d, w, s1, l.scratch, l.chan);
+    column_sums<V>(d, w, s2, l.scratch, l.chan2);
+    if (d.sums) {
+      keep_sums<V>(d, w, l.chan2, accw);
+      keep_sums<V>(d, w, l.chan, accb);
+      __syncthreads();
+    }
+    if (a.y) {
+      group_means<T>(d, w, l.chan, l.chan2, lens, l.first, l.second);
+      float m1[V], m2[V];
+#pragma unroll
+      for (int i = 0; i < V; i++) m1[i] = l.first[g[i]], m2[i] = l.second[g[i]];
+      T *gx = (T *)a.y + n * a.S * a.C + w.c0 + w.tx * V;
+#pragma unroll
+      for (int r = 0; r < R; r++) {
+        const long long s = w.ty + (long long)r * d.p.TY;
+        if (!on || s >= a.S) continue;
+        Pack<T, V> o;
+#pragma unroll
+        for (int i = 0; i < V; i++) {
+          const float xh = (to_f(xr[r].v[i]) - mu[i]) * k[i];
+          o.v[i] = from_f<T>(s < len ? k[i] * (gz[r][i] * W[i] - m1[i] - xh * m2[i]) : 0.f);
+        }
+        store_pack<T, V>(gx + s * a.C, o);
+      }
+    }
+    __syncthreads();
+  }
+  if (d.sums) {
+    float *to = d.sums + (long long)blockIdx.x * 2 * a.C + w.c0;
+#pragma unroll
+    for (int j = 0; j < V; j++) {
+      const int c = threadIdx.x + j * d.p.T;
+      if (c < w.cw) to[c] = accw[j], to[a.C + c] = accb[j];
+    }
+  }
+}
+
+// ---- samples in chunks ----
+
+// mean and sum of squares of a chunk's groups: block (chunk, stripe) of sample blockIdx.z
+template <typename T, int V>
+__global__ void __launch_bounds__(kNormMostT) norm_chunk_stats(const NormDev d, long long nbase) {
+  const Place w = place_of(d);
+  const Lds l = lds_of(d);
+  const NormArgs &a = d.a;
+  const int cg = a.C / a.G;
+  const long long n = nbase + blockIdx.z, s0 = blockIdx.x * d.p.rows, len = max(0LL, min(d.p.rows, length_of(a, n) - s0));
+  const T *x = (const T *)a.x + n * a.xs + s0 * a.xp + w.c0 + w.tx * V;
+  Pack<T, V> xr[kNormMostR];
+#pragma unroll
+  for (int r = 0; r < kNormMostR; r++) {
+    const long long s = w.ty + (long long)r * d.p.TY;
+    if (w.on && s < len) xr[r] = load_pack<T, V>(x + s * a.xp);
+  }
+  block_stats<T, V, kNormMostR>(d, w, xr, len, l.scratch, l.chan, l.first, l.second);
+  float *to = d.stats + ((n * d.p.chunks + blockIdx.x) * a.G + w.c0 / cg) * 2;
+  for (int k = threadIdx.x; k < w.cw / cg; k += d.p.T) to[2 * k] = l.first[k], to[2 * k + 1] = l.second[k];
+}
+
+// the chunks of a sample joined: a wave a group
+static __global__ void __launch_bounds__(256) norm_stats_join(const NormDev d) {
+  const NormArgs &a = d.a;
+  const long long at = (long long)blockIdx.x * 4 + threadIdx.x / 64, n = at / a.G;
+  const int g = (int)(at - n * a.G), lane = threadIdx.x % 64;
+  if (n >= a.N) return;
+  const long long len = length_of(a, n);
+  const float *p = d.stats + (n * d.p.chunks * a.G + g) * 2;
+  auto count = [&](long long k) { return (float)max(0LL, min(d.p.rows, len - k * d.p.rows)); };
+  auto all = [](float s) {
+#pragma unroll
+    for (int m = 32; m >= 1; m >>= 1) s += __shfl_xor(s, m);
+    return s;
+  };
+  // (means of chunks around the first one's: their sum is as exact as they are)
+  const float first = len ? p[0] : 0.f;
+  float s = 0.f, q = 0.f;
+  for (long long k = lane; k < d.p.chunks && k * d.p.rows < len; k += 64) s += count(k) * (p[k * a.G * 2] - first);
+  const float mean = first + (len ? all(s) / (float)len : 0.f);
+  for (long long k = lane; k < d.p.chunks && k * d.p.rows < len; k += 64) {
+    const float e = p[k * a.G * 2] - mean;
+    q += p[k * a.G * 2 + 1] + count(k) * (float)(a.C / a.G) * e * e;
+  }
+  q = all(q);
+  if (lane == 0) a.mean[at] = mean, a.rstd[at] = 1.f / sqrtf((len ? q / ((float)len * (float)(a.C / a.G)) : 0.f) + a.eps);
+}
+
+// second pass: y of a chunk
+template <typename T, int V, int ACT>
+__global__ void __launch_bounds__(kNormMostT) norm_apply_fwd(const NormDev d, long long nbase) {
+  const Place w = place_of(d);
+  if (!w.on) return;
+  const NormArgs &a = d.a;
+  const int cg = a.C / a.G;
+  const long long n = nbase + blockIdx.z, s0 = blockIdx.x * d.p.rows, len = length_of(a, n), end = min(s0 + d.p.rows, a.S);
+  float B[V], mu[V], k[V];
+  load_channels<T, V>(a.w, w, 1.f, k);
+  load_channels<T, V>(a.b, w, 0.f, B);
+#pragma unroll
+  for (int i = 0; i < V; i++) {
+    const long long at = n * a.G + (w.c0 + w.tx * V + i) / cg;
+    mu[i] = a.mean[at], k[i] *= a.rstd[at];
+  }
+  const T *x = (const T *)a.x + n * a.xs + w.c0 + w.tx * V;
+  T *y = (T *)a.y + n * a.S * a.C + w.c0 + w.tx * V;
+#pragma unroll 4
+  for (long long s = s0 + w.ty; s < end; s += d.p.TY) {
+    Pack<T, V> o;
+    if (s < len) {
+      o = load_pack<T, V>(x + s * a.xp);
+#pragma unroll
+      for (int i = 0; i < V; i++) {
+        float v, e;
+        act_both<ACT>((to_f(o.v[i]) - mu[i]) * k[i] + B[i], v, e, a.act == kActRelu);
+        o.v[i] = from_f<T>(v);
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < V; i++) o.v[i] = from_f<T>(0.f);
+    }
+    store_pack<T, V>(y + s * a.C, o);
+  }
+}
+
+// channel sums of gz and gz xh of a chunk
+template <typename T, int V, int ACT>
+__global__ void __launch_bounds__(kNormMostT) norm_chunk_sums(const NormDev d, long long nbase) {
+  const Place w = place_of(d);
+  const Lds l = lds_of(d);
+  const NormArgs &a = d.a;
+  const int cg = a.C / a.G;
+  const long long n = nbase + blockIdx.z, s0 = blockIdx.x * d.p.rows, end = min(s0 + d.p.rows, length_of(a, n));
+  float W[V], B[V], mu[V], k[V], s1[V] = {}, s2[V] = {};
+  load_channels<T, V>(a.w, w, 1.f, W);
+  load_channels<T, V>(a.b, w, 0.f, B);
+  if (w.on) {
+#pragma unroll
+    for (int i = 0; i < V; i++) {
+      const long long at = n * a.G + (w.c0 + w.tx * V + i) / cg;
+      mu[i] = a.mean[at], k[i] = a.rstd[at];
+    }
+    const T *x = (const T *)a.x + n * a.xs + w.c0 + w.tx * V, *gy = (const T *)a.gy + n * a.S * a.C + w.c0 + w.tx * V;
+#pragma unroll 4
+    for (long long s = s0 + w.ty; s < end; s += d.p.TY) {
+      float xh[V], gz[V];
+      gz_of<T, V, ACT>(load_pack<T, V>(x + s * a.xp), load_pack<T, V>(gy + s * a.C), mu, k, W, B, a.act == kActRelu, xh, gz);
+#pragma unroll
+      for (int i = 0; i < V; i++) s1[i] += gz[i], s2[i] += gz[i] * xh[i];
+    }
+  }
+  column_sums<V>(d, w, s1, l.scratch, l.chan);
+  column_sums<V>(d, w, s2, l.scratch, l.chan2);
+  float *to = d.stats + (n * d.p.chunks + blockIdx.x) * 2 * a.C + w.c0;
+  for (int c = threadIdx.x; c < w.cw; c += d.p.T) to[c] = l.chan2[c], to[a.C + c] = l.chan[c];
+}
+
+// the chunks of a sample joined: block (stripe) of sample blockIdx.z.  32 channels at a time by T / 32 runs of chunks.
+template <typename T>
+__global__ void __launch_bounds__(kNormMostT) norm_sums_join(const NormDev d, long long nbase) {
+  const Place w = place_of(d);
+  const Lds l = lds_of(d);
+  const NormArgs &a = d.a;
+  const int cg = a.C / a.G, gs = w.cw / cg, runs = d.p.T / 32, run = threadIdx.x / 32;
+  const long long n = nbase + blockIdx.z, len = length_of(a, n);
+  const long long chunks = (len + d.p.rows - 1) / d.p.rows;
+  __shared__ float part[kNormMostT / 32][2][33];
+  float *lens = l.second + d.p.Cw / cg;
+  if (threadIdx.x == 0) lens[0] = (float)len;
+  for (int base = 0; base < w.cw; base += 32) {
+    const int c = base + threadIdx.x % 32;
+    float s1 = 0.f, s2 = 0.f;
+    if (c < w.cw) {
+      const float *p = d.stats + n * d.p.chunks * 2 * a.C + w.c0 + c;
+#pragma unroll 4
+      for (long long k = run; k < chunks; k += runs) s2 += p[k * 2 * a.C], s1 += p[k * 2 * a.C + a.C];
+    }
+    part[run][0][threadIdx.x % 32] = s1, part[run][1][threadIdx.x % 32] = s2;
+    __syncthreads();
+    if (threadIdx.x < 64 && base + (int)threadIdx.x % 32 < w.cw) {
+      const int which = threadIdx.x / 32;
+      float s = 0.f;
+      for (int k = 0; k < runs; k++) s += part[k][which][threadIdx.x % 32];
+      (which ? l.chan2 : l.chan)[base + threadIdx.x % 32] = s;
+    }
+    __syncthreads();
+  }
+  float *to = d.sums + n * 2 * a.C + w.c0;
+  for (int c = threadIdx.x; c < w.cw; c += d.p.T) to[c] = l.chan2[c], to[a.C + c] = l.chan[c];
+  __syncthreads();
+  group_means<T>(d, w, l.chan, l.chan2, lens, l.first, l.second);
+  float *m = d.means + (n * a.G + w.c0 / cg) * 2;
+  for (int k = threadIdx.x; k < gs; k += d.p.T) m[2 * k] = l.first[k], m[2 * k + 1] = l.second[k];
+}
+
+template <typename T, int V, int ACT>
+__global__ void __launch_bounds__(kNormMostT) norm_apply_bwd(const NormDev d, long long nbase) {
+  const Place w = place_of(d);
+  if (!w.on) return;
+  const NormArgs &a = d.a;
+  const int cg = a.C / a.G;
+  const long long n = nbase + blockIdx.z, s0 = blockIdx.x * d.p.rows, len = length_of(a, n), end = min(s0 + d.p.rows, a.S);
+  float W[V], B[V], mu[V], k[V], m1[V], m2[V];
+  load_channels<T, V>(a.w, w, 1.f, W);
+  load_channels<T, V>(a.b, w, 0.f, B);
+#pragma unroll
+  for (int i = 0; i < V; i++) {
+    const long long at = n * a.G + (w.c0 + w.tx * V + i) / cg;
+    mu[i] = a.mean[at], k[i] = a.rstd[at], m1[i] = d.means[2 * at], m2[i] = d.means[2 * at + 1];
+  }
+  const T *x = (const T *)a.x + n * a.xs + w.c0 + w.tx * V, *gy = (const T *)a.gy + n * a.S * a.C + w.c0 + w.tx * V;
+  T *gx = (T *)a.y + n * a.S * a.C + w.c0 + w.tx * V;
+#pragma unroll 4
+  for (long long s = s0 + w.ty; s < end; s += d.p.TY) {
+    Pack<T, V> o;
+    if (s < len) {
+      float xh[V], gz[V];
+      gz_of<T, V, ACT>(load_pack<T, V>(x + s * a.xp), load_pack<T, V>(gy + s * a.C), mu, k, W, B, a.act == kActRelu, xh, gz);
+#pragma unroll
+      for (int i = 0; i < V; i++) o.v[i] = from_f<T>(k[i] * (gz[i] * W[i] - m1[i] - xh[i] * m2[i]));
+    } else {
+#pragma unroll
+      for (int i = 0; i < V; i++) o.v[i] = from_f<T>(0.f);
+    }
+    store_pack<T, V>(gx + s * a.C, o);
+  }
+}
+
+// gw and gb: sums of `rows` rows of [2][C]; 32 columns by 8 runs of rows a block
+template <typename T>
+__global__ void __launch_bounds__(256) norm_join(const float *sums, T *gw, T *gb, long long rows, int C) {
+  __shared__ float lds[8][32];
+  const long long c = (long long)blockIdx.x * 32 + threadIdx.x % 32;
+  const int run = threadIdx.x / 32;
+  float s = 0.f;
+  if (c < 2LL * C) {
+#pragma unroll 8
+    for (long long k = run; k < rows; k += 8) s += sums[k * 2 * C + c];
+  }
+  lds[run][threadIdx.x % 32] = s;
+  __syncthreads();
+  if (run == 0 && c < 2LL * C) {
+    for (int k = 1; k < 8; k++) s += lds[k][threadIdx.x];
+    if (c < C && gw) gw[c] = from_f<T>(s);
+    if (c >= C && gb) gb[c - C] = from_f<T>(s);
+  }
+}
+
+template <typename T, int V, int ACT>
+int run_norm(bool backward, const NormDev &d, hipStream_t s) {
+  const NormArgs &a = d.a;
+  const NormPlan &p = d.p;
+  const size_t lds = norm_lds_bytes(p, a.C / a.G);
+  const dim3 block(p.T);
+  if (p.R) {
+    const dim3 grid((unsigned)p.blocks, p.stripes);
+#define GELIB_NORM(R)                                                                                              \
+  do {                                                                                                             \
+    if (backward) hipLaunchKernelGGL((norm_whole_bwd<T, V, ACT, R>), grid, block, lds, s, d);                      \
+    else hipLaunchKernelGGL((norm_whole_fwd<T, V, ACT, R>), grid, block, lds, s, d);                               \
+  } while (0)
+    if (p.R == 1) GELIB_NORM(1);
+    else if (p.R <= 4) GELIB_NORM(4);
+    else GELIB_NORM(kNormMostR);
+#undef GELIB_NORM
+    if (backward && d.sums)
+      hipLaunchKernelGGL((norm_join<T>), dim3((2 * a.C + 31) / 32), dim3(256), 0, s, (const float *)d.sums, (T *)a.gw, (T *)a.gb, p.blocks, a.C);
+  } else {
+    const long long most = std::min(a.N, 32768LL);   // samples of a launch (its third dimension)
+    auto each = [&](auto kernel, unsigned chunks, size_t bytes) {
+      for (long long n = 0; n < a.N; n += most)
+        hipLaunchKernelGGL(kernel, dim3(chunks, p.stripes, (unsigned)std::min(most, a.N - n)), block, bytes, s, d, n);
+    };
+    if (!backward) {
+      each(norm_chunk_stats<T, V>, (unsigned)p.chunks, lds);
+      hipLaunchKernelGGL(norm_stats_join, dim3((unsigned)((a.N * a.G + 3) / 4)), dim3(256), 0, s, d);
+      each(norm_apply_fwd<T, V, ACT>, (unsigned)p.chunks, 0);
+    } else {
+      each(norm_chunk_sums<T, V, ACT>, (unsigned)p.chunks, lds);
+      each(norm_sums_join<T>, 1, lds);
+      if (a.y) each(norm_apply_bwd<T, V, ACT>, (unsigned)p.chunks, 0);
+      if (a.gw || a.gb)
+        hipLaunchKernelGGL((norm_join<T>), dim3((2 * a.C + 31) / 32), dim3(256), 0, s, (const float *)d.sums, (T *)a.gw, (T *)a.gb, a.N, a.C);
+    }
+  }
+  const hipError_t e = hipGetLastError();
+  return e == hipSuccess ? 0 : record_hip_error(e, "group norm launch");
+}
+
+template <typename T, int V>
+int run_norm_act(bool backward, const NormDev &d, hipStream_t s) {
+  if (d.a.act == kActSilu) return run_norm<T, V, kActSilu>(backward, d, s);
+  if (d.a.act == kActGelu) return run_norm<T, V, kActGelu>(backward, d, s);
+  return run_norm<T, V, kActNone>(backward, d, s);
+}
+
+}  // namespace
+
+template <typename T>
+int launch_norm_typed(bool backward, const NormDev &d, hipStream_t s) {
+  if (d.p.V == 16 / (int)sizeof(T)) return run_norm_act<T, 16 / sizeof(T)>(backward, d, s);
+  if (d.p.V == 2) return run_norm_act<T, 2>(backward, d, s);
+  return run_norm_act<T, 1>(backward, d, s);
+}
+
+#endif
+
+}  // namespace gelib_hip
