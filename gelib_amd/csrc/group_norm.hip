@@ -1,8 +1,6 @@
 // Group norm with an activation (group_norm_impl.h): how a call's tensors are cut into blocks, and simple kernels for what those do
-// not take (one block cannot hold a row of the channels that a group and the loads' alignment ask for: groups of more than 512
-// loads, 4096 bfloat16 channels).
-#include <numeric>
-
+// not take (one block cannot hold a row of the channels that a group and the loads' alignment ask for: groups of more than 256
+// loads, 2048 bfloat16 channels; 512 where samples are short).
 #include "group_norm_impl.h"
 
 namespace gelib_hip {
@@ -141,7 +139,7 @@ bool plan_norm(bool backward, int V, int e, long long N, long long S, int C, int
   stripes_of((128 / e + Cq - 1) / Cq);
   const int down = std::max(1, kNormMostT / p.TX);
   p.NS = 1;
-  if (S <= (long long)down * kNormMostR) {
+  if (S <= (long long)down * (backward ? kNormMostRBack : kNormMostR)) {
     p.TY = (int)std::min<long long>(S, down);
     p.R = (int)((S + p.TY - 1) / p.TY);
     // several small samples a block, as long as 512 blocks are left
@@ -150,8 +148,9 @@ bool plan_norm(bool backward, int V, int e, long long N, long long S, int C, int
     // forward: a block a set; backward: about a thousand blocks walk over the sets, each with one row of sums for gw and gb
     p.blocks = std::min<long long>(sets, backward ? std::max(1, 1024 / p.stripes) : 1 << 22);
   } else {
-    stripes_of(256 * V / Cq);
-    p.TY = std::max(1, kNormMostT / p.TX);
+    stripes_of(std::min(256, std::max(64, Cq / V)) * V / Cq);
+    p.TY = kNormChunkT / p.TX;
+    if (p.TY == 0) return false;
     int r = kNormMostR;
     while (r > 1 && N * ((S + (long long)r * p.TY - 1) / ((long long)r * p.TY)) * p.stripes < 512) r /= 2;
     p.rows = (long long)r * p.TY;

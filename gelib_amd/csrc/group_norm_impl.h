@@ -6,12 +6,14 @@
 // A block owns whole groups of one sample (or of several small ones): a stripe of Cw channels, at least 128 bytes of a row, by all
 // positions, TX threads of V channels (one load) side by side and TY of them down the positions.  Where a stripe fits a block's
 // registers (16 loads a thread, 512 threads: 128 KB) it is read once, and the statistics are formed around the mean from registers;
-// the backward pass keeps gz there too, in float32.  Larger samples are cut into chunks of positions: every chunk's mean and sum of
+// the backward pass forms gz twice from what it holds.  Larger samples are cut into chunks of positions: every chunk's mean and sum of
 // squares around it (backward: its channel sums), joined by the parallel form of the variance, then a second pass over x, which the
 // memory-side cache still holds up to its 256 MB.  What bounds either is HBM; sums go over channels first and groups after, so any
 // channels a group will do, and the channel sums are the gradients of w and b.
 // No atomics: sums have one order.
 #pragma once
+
+#include <numeric>
 
 #include "real_ops.h"
 
@@ -40,20 +42,55 @@ int launch_norm_typed(bool backward, const NormDev &d, hipStream_t s);
 
 namespace {
 
-constexpr int kNormMostT = 512, kNormMostR = 16;
+// Most threads of a block, and loads that a thread holds: more than 8 of x and 8 of gy beside the channels' numbers do not fit 256
+// registers.  Chunks take 256 threads, three to five blocks a compute unit, so that loads are under way while others reduce.
+constexpr int kNormMostT = 512, kNormMostR = 16, kNormMostRBack = 8, kNormChunkT = 256;
 
+template <typename T>
+struct Short { typedef T type; };
+template <>
+struct Short<float> { typedef half_t type; };   // (never converted to)
+
+// A load of V values as the 32-bit words that it is: values are unpacked where they are used, two instructions for two of them.
 template <typename T, int V>
 struct Pack {
-  T v[V];
+  static constexpr int N = (V * (int)sizeof(T) + 3) / 4;
+  unsigned w[N];
+  __device__ __forceinline__ float at(int i) const {
+    if (sizeof(T) == 4) return __uint_as_float(w[i]);
+    const unsigned h = w[i / 2];
+    if (__is_same(T, bhalf_t)) return __uint_as_float(i % 2 ? h & 0xffff0000u : h << 16);
+    return (float)__builtin_bit_cast(half_t, (unsigned short)(i % 2 ? h >> 16 : h));
+  }
+  __device__ __forceinline__ void set(const float *v) {
+#pragma unroll
+    for (int k = 0; k < N; k++) {
+      if (sizeof(T) == 4) w[k] = __float_as_uint(v[k]);
+      else w[k] = bits(v[2 * k]) | (V > 1 ? (unsigned)bits(v[2 * k + (V > 1)]) << 16 : 0u);
+    }
+  }
+  // Hides where the words come from: the compiler unpacks them again where they are used next, instead of keeping every value in a
+  // register of its own from one use to the other (16 loads of 8 values: 128 registers more, and 218 spilled)
+  __device__ __forceinline__ void forget() {
+#pragma unroll
+    for (int k = 0; k < N; k++) asm volatile("" : "+v"(w[k]));
+  }
+
+ private:
+  static __device__ __forceinline__ unsigned short bits(float v) { return __builtin_bit_cast(unsigned short, from_f<typename Short<T>::type>(v)); }
 };
 template <typename T, int V>
 __device__ __forceinline__ Pack<T, V> load_pack(const T *p) {
   Pack<T, V> r;
-  __builtin_memcpy(&r, __builtin_assume_aligned(p, V * sizeof(T)), sizeof(r));
+  if constexpr (V * sizeof(T) < 4) r.w[0] = *(const unsigned short *)p;
+  else __builtin_memcpy(r.w, __builtin_assume_aligned(p, V * sizeof(T)), V * sizeof(T));
   return r;
 }
 template <typename T, int V>
-__device__ __forceinline__ void store_pack(T *p, const Pack<T, V> &r) { __builtin_memcpy(__builtin_assume_aligned(p, V * sizeof(T)), &r, sizeof(r)); }
+__device__ __forceinline__ void store_pack(T *p, const Pack<T, V> &r) {
+  if constexpr (V * sizeof(T) < 4) *(unsigned short *)p = (unsigned short)r.w[0];
+  else __builtin_memcpy(__builtin_assume_aligned(p, V * sizeof(T)), r.w, V * sizeof(T));
+}
 
 __device__ __forceinline__ long long length_of(const NormArgs &a, long long n) {
   return a.lengths ? max(0LL, min((long long)a.lengths[n], a.S)) : a.S;
@@ -83,6 +120,14 @@ template <int V>
 __device__ __forceinline__ void column_sums(const NormDev &d, const Place &w, const float *v, float *lds, float *out) {
   const int cols = d.p.NS * d.p.Cw, t = threadIdx.x;
   __syncthreads();
+  if (d.p.TY == 1) {
+    if (w.ty == 0) {
+#pragma unroll
+      for (int i = 0; i < V; i++) out[w.col + i] = v[i];
+    }
+    __syncthreads();
+    return;
+  }
   if (w.ty < d.p.TY) {
 #pragma unroll
     for (int i = 0; i < V; i++) lds[w.ty * cols + w.col + i] = v[i];
@@ -156,7 +201,7 @@ extern __shared__ float norm_lds[];
 // Statistics of what the threads hold in xr (R loads each, those at positions below len count): mean and sum of squares around it of
 // every group of the block, in mean[] and square[].
 template <typename T, int V, int R>
-__device__ __forceinline__ void block_stats(const NormDev &d, const Place &w, const Pack<T, V> *xr, long long len, float *scratch, float *chan, float *mean,
+__device__ __forceinline__ void block_stats(const NormDev &d, const Place &w, Pack<T, V> *xr, long long len, float *scratch, float *chan, float *mean,
                                             float *square) {
   float s[V] = {};
   int g[V];
@@ -165,7 +210,7 @@ __device__ __forceinline__ void block_stats(const NormDev &d, const Place &w, co
   for (int r = 0; r < R; r++)
     if (w.on && w.ty + (long long)r * d.p.TY < len) {
 #pragma unroll
-      for (int i = 0; i < V; i++) s[i] += to_f(xr[r].v[i]);
+      for (int i = 0; i < V; i++) s[i] += xr[r].at(i);
     }
   // (a sample's length: every group of it has the same count)
   float *lens = square + d.p.NS * (d.p.Cw / (d.a.C / d.a.G));
@@ -175,6 +220,8 @@ __device__ __forceinline__ void block_stats(const NormDev &d, const Place &w, co
   group_sums(d, w, chan, [&](int k, float sum) { mean[k] = lens[k / gs] > 0.f ? sum / (lens[k / gs] * (float)cg) : 0.f; });
 #pragma unroll
   for (int i = 0; i < V; i++) s[i] = 0.f;
+#pragma unroll
+  for (int r = 0; r < R; r++) xr[r].forget();
   float mu[V];
 #pragma unroll
   for (int i = 0; i < V; i++) mu[i] = mean[g[i]];
@@ -183,7 +230,7 @@ __device__ __forceinline__ void block_stats(const NormDev &d, const Place &w, co
     if (w.on && w.ty + (long long)r * d.p.TY < len) {
 #pragma unroll
       for (int i = 0; i < V; i++) {
-        const float e = to_f(xr[r].v[i]) - mu[i];
+        const float e = xr[r].at(i) - mu[i];
         s[i] += e * e;
       }
     }
@@ -247,14 +294,16 @@ __global__ void __launch_bounds__(kNormMostT) norm_whole_fwd(const NormDev d) {
     for (int r = 0; r < R; r++) {
       const long long s = w.ty + (long long)r * d.p.TY;
       if (!on || s >= a.S) continue;
-      Pack<T, V> o;
+      float o[V];
+      xr[r].forget();
 #pragma unroll
       for (int i = 0; i < V; i++) {
         float v, e;
-        act_both<ACT>((to_f(xr[r].v[i]) - mu[i]) * k[i] + B[i], v, e, a.act == kActRelu);
-        o.v[i] = from_f<T>(s < len ? v : 0.f);
+        act_both<ACT>((xr[r].at(i) - mu[i]) * k[i] + B[i], v, e, a.act == kActRelu);
+        o[i] = s < len ? v : 0.f;
       }
-      store_pack<T, V>(y + s * a.C, o);
+      xr[r].set(o);
+      store_pack<T, V>(y + s * a.C, xr[r]);
     }
     __syncthreads();
   }
@@ -267,9 +316,9 @@ __device__ __forceinline__ void gz_of(const Pack<T, V> &x, const Pack<T, V> &gy,
 #pragma unroll
   for (int i = 0; i < V; i++) {
     float v, e;
-    xh[i] = (to_f(x.v[i]) - mu[i]) * k[i];
+    xh[i] = (x.at(i) - mu[i]) * k[i];
     act_both<ACT>(xh[i] * W[i] + B[i], v, e, relu);
-    gz[i] = to_f(gy.v[i]) * e;
+    gz[i] = gy.at(i) * e;
   }
 }
 
@@ -318,7 +367,7 @@ __global__ void __launch_bounds__(kNormMostT) norm_whole_bwd(const NormDev d) {
     const long long len = n < a.N ? length_of(a, n) : 0;
     const T *x = (const T *)a.x + n * a.xs + w.c0 + w.tx * V, *gy = (const T *)a.gy + n * a.S * a.C + w.c0 + w.tx * V;
     Pack<T, V> xr[R], gr[R];
-    float mu[V], k[V], gz[R][V], s1[V] = {}, s2[V] = {};
+    float mu[V], k[V], s1[V] = {}, s2[V] = {};
 #pragma unroll
     for (int r = 0; r < R; r++) {
       const long long s = w.ty + (long long)r * d.p.TY;
@@ -332,10 +381,10 @@ __global__ void __launch_bounds__(kNormMostT) norm_whole_bwd(const NormDev d) {
 #pragma unroll
     for (int r = 0; r < R; r++)
       if (on && w.ty + (long long)r * d.p.TY < len) {
-        float xh[V];
-        gz_of<T, V, ACT>(xr[r], gr[r], mu, k, W, B, a.act == kActRelu, xh, gz[r]);
+        float xh[V], gz[V];
+        gz_of<T, V, ACT>(xr[r], gr[r], mu, k, W, B, a.act == kActRelu, xh, gz);
 #pragma unroll
-        for (int i = 0; i < V; i++) s1[i] += gz[r][i], s2[i] += gz[r][i] * xh[i];
+        for (int i = 0; i < V; i++) s1[i] += gz[i], s2[i] += gz[i] * xh[i];
       }
     if (w.tx == 0 && w.ty == 0) lens[w.ns] = (float)len;
     column_sums<V>(d, w, s1, l.scratch, l.chan);
@@ -355,13 +404,14 @@ __global__ void __launch_bounds__(kNormMostT) norm_whole_bwd(const NormDev d) {
       for (int r = 0; r < R; r++) {
         const long long s = w.ty + (long long)r * d.p.TY;
         if (!on || s >= a.S) continue;
-        Pack<T, V> o;
+        // (gz once more, rather than in registers from above: 128 of them where a thread holds 16 loads)
+        float xh[V], gz[V], o[V];
+        xr[r].forget(), gr[r].forget();
+        gz_of<T, V, ACT>(xr[r], gr[r], mu, k, W, B, a.act == kActRelu, xh, gz);
 #pragma unroll
-        for (int i = 0; i < V; i++) {
-          const float xh = (to_f(xr[r].v[i]) - mu[i]) * k[i];
-          o.v[i] = from_f<T>(s < len ? k[i] * (gz[r][i] * W[i] - m1[i] - xh * m2[i]) : 0.f);
-        }
-        store_pack<T, V>(gx + s * a.C, o);
+        for (int i = 0; i < V; i++) o[i] = s < len ? k[i] * (gz[i] * W[i] - m1[i] - xh[i] * m2[i]) : 0.f;
+        xr[r].set(o);
+        store_pack<T, V>(gx + s * a.C, xr[r]);
       }
     }
     __syncthreads();
@@ -380,7 +430,7 @@ __global__ void __launch_bounds__(kNormMostT) norm_whole_bwd(const NormDev d) {
 
 // mean and sum of squares of a chunk's groups: block (chunk, stripe) of sample blockIdx.z
 template <typename T, int V>
-__global__ void __launch_bounds__(kNormMostT) norm_chunk_stats(const NormDev d, long long nbase) {
+__global__ void __launch_bounds__(kNormChunkT) norm_chunk_stats(const NormDev d, long long nbase) {
   const Place w = place_of(d);
   const Lds l = lds_of(d);
   const NormArgs &a = d.a;
@@ -427,7 +477,7 @@ static __global__ void __launch_bounds__(256) norm_stats_join(const NormDev d) {
 
 // second pass: y of a chunk
 template <typename T, int V, int ACT>
-__global__ void __launch_bounds__(kNormMostT) norm_apply_fwd(const NormDev d, long long nbase) {
+__global__ void __launch_bounds__(kNormChunkT) norm_apply_fwd(const NormDev d, long long nbase) {
   const Place w = place_of(d);
   if (!w.on) return;
   const NormArgs &a = d.a;
@@ -445,26 +495,24 @@ __global__ void __launch_bounds__(kNormMostT) norm_apply_fwd(const NormDev d, lo
   T *y = (T *)a.y + n * a.S * a.C + w.c0 + w.tx * V;
 #pragma unroll 4
   for (long long s = s0 + w.ty; s < end; s += d.p.TY) {
-    Pack<T, V> o;
+    Pack<T, V> p = {};
     if (s < len) {
-      o = load_pack<T, V>(x + s * a.xp);
+      float o[V];
+      p = load_pack<T, V>(x + s * a.xp);
 #pragma unroll
       for (int i = 0; i < V; i++) {
-        float v, e;
-        act_both<ACT>((to_f(o.v[i]) - mu[i]) * k[i] + B[i], v, e, a.act == kActRelu);
-        o.v[i] = from_f<T>(v);
+        float e;
+        act_both<ACT>((p.at(i) - mu[i]) * k[i] + B[i], o[i], e, a.act == kActRelu);
       }
-    } else {
-#pragma unroll
-      for (int i = 0; i < V; i++) o.v[i] = from_f<T>(0.f);
+      p.set(o);
     }
-    store_pack<T, V>(y + s * a.C, o);
+    store_pack<T, V>(y + s * a.C, p);
   }
 }
 
 // channel sums of gz and gz xh of a chunk
 template <typename T, int V, int ACT>
-__global__ void __launch_bounds__(kNormMostT) norm_chunk_sums(const NormDev d, long long nbase) {
+__global__ void __launch_bounds__(kNormChunkT) norm_chunk_sums(const NormDev d, long long nbase) {
   const Place w = place_of(d);
   const Lds l = lds_of(d);
   const NormArgs &a = d.a;
@@ -496,14 +544,14 @@ __global__ void __launch_bounds__(kNormMostT) norm_chunk_sums(const NormDev d, l
 
 // the chunks of a sample joined: block (stripe) of sample blockIdx.z.  32 channels at a time by T / 32 runs of chunks.
 template <typename T>
-__global__ void __launch_bounds__(kNormMostT) norm_sums_join(const NormDev d, long long nbase) {
+__global__ void __launch_bounds__(kNormChunkT) norm_sums_join(const NormDev d, long long nbase) {
   const Place w = place_of(d);
   const Lds l = lds_of(d);
   const NormArgs &a = d.a;
   const int cg = a.C / a.G, gs = w.cw / cg, runs = d.p.T / 32, run = threadIdx.x / 32;
   const long long n = nbase + blockIdx.z, len = length_of(a, n);
   const long long chunks = (len + d.p.rows - 1) / d.p.rows;
-  __shared__ float part[kNormMostT / 32][2][33];
+  __shared__ float part[kNormChunkT / 32][2][33];
   float *lens = l.second + d.p.Cw / cg;
   if (threadIdx.x == 0) lens[0] = (float)len;
   for (int base = 0; base < w.cw; base += 32) {
@@ -533,7 +581,7 @@ __global__ void __launch_bounds__(kNormMostT) norm_sums_join(const NormDev d, lo
 }
 
 template <typename T, int V, int ACT>
-__global__ void __launch_bounds__(kNormMostT) norm_apply_bwd(const NormDev d, long long nbase) {
+__global__ void __launch_bounds__(kNormChunkT) norm_apply_bwd(const NormDev d, long long nbase) {
   const Place w = place_of(d);
   if (!w.on) return;
   const NormArgs &a = d.a;
@@ -551,17 +599,15 @@ __global__ void __launch_bounds__(kNormMostT) norm_apply_bwd(const NormDev d, lo
   T *gx = (T *)a.y + n * a.S * a.C + w.c0 + w.tx * V;
 #pragma unroll 4
   for (long long s = s0 + w.ty; s < end; s += d.p.TY) {
-    Pack<T, V> o;
+    Pack<T, V> p = {};
     if (s < len) {
-      float xh[V], gz[V];
+      float xh[V], gz[V], o[V];
       gz_of<T, V, ACT>(load_pack<T, V>(x + s * a.xp), load_pack<T, V>(gy + s * a.C), mu, k, W, B, a.act == kActRelu, xh, gz);
 #pragma unroll
-      for (int i = 0; i < V; i++) o.v[i] = from_f<T>(k[i] * (gz[i] * W[i] - m1[i] - xh[i] * m2[i]));
-    } else {
-#pragma unroll
-      for (int i = 0; i < V; i++) o.v[i] = from_f<T>(0.f);
+      for (int i = 0; i < V; i++) o[i] = k[i] * (gz[i] * W[i] - m1[i] - xh[i] * m2[i]);
+      p.set(o);
     }
-    store_pack<T, V>(gx + s * a.C, o);
+    store_pack<T, V>(gx + s * a.C, p);
   }
 }
 
@@ -600,7 +646,8 @@ int run_norm(bool backward, const NormDev &d, hipStream_t s) {
   } while (0)
     if (p.R == 1) GELIB_NORM(1);
     else if (p.R <= 4) GELIB_NORM(4);
-    else GELIB_NORM(kNormMostR);
+    else if (p.R <= 8) GELIB_NORM(8);
+    else hipLaunchKernelGGL((norm_whole_fwd<T, V, ACT, kNormMostR>), grid, block, lds, s, d);
 #undef GELIB_NORM
     if (backward && d.sums)
       hipLaunchKernelGGL((norm_join<T>), dim3((2 * a.C + 31) / 32), dim3(256), 0, s, (const float *)d.sums, (T *)a.gw, (T *)a.gb, p.blocks, a.C);
@@ -616,7 +663,11 @@ int run_norm(bool backward, const NormDev &d, hipStream_t s) {
       each(norm_apply_fwd<T, V, ACT>, (unsigned)p.chunks, 0);
     } else {
       each(norm_chunk_sums<T, V, ACT>, (unsigned)p.chunks, lds);
-      each(norm_sums_join<T>, 1, lds);
+      NormDev j = d;   // (stripes of about 32 channels: their sums are short, blocks are wanted)
+      const int cg = a.C / a.G, Cq = V / std::gcd(V, cg) * cg;
+      j.p.Cw = std::min(p.Cw, std::max(1, 32 / Cq) * Cq), j.p.stripes = (a.C + j.p.Cw - 1) / j.p.Cw, j.p.TX = 1, j.p.TY = 1, j.p.T = kNormChunkT;
+      for (long long n = 0; n < a.N; n += most)
+        hipLaunchKernelGGL((norm_sums_join<T>), dim3(1, j.p.stripes, (unsigned)std::min(most, a.N - n)), dim3(kNormChunkT), norm_lds_bytes(j.p, cg), s, j, n);
       if (a.y) each(norm_apply_bwd<T, V, ACT>, (unsigned)p.chunks, 0);
       if (a.gw || a.gb)
         hipLaunchKernelGGL((norm_join<T>), dim3((2 * a.C + 31) / 32), dim3(256), 0, s, (const float *)d.sums, (T *)a.gw, (T *)a.gb, a.N, a.C);
