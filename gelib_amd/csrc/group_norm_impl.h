@@ -45,6 +45,7 @@ namespace {
 // Most threads of a block, and loads that a thread holds: more than 8 of x and 8 of gy beside the channels' numbers do not fit 256
 // registers.  Chunks take 256 threads, three to five blocks a compute unit, so that loads are under way while others reduce.
 constexpr int kNormMostT = 512, kNormMostR = 16, kNormMostRBack = 8, kNormChunkT = 256;
+constexpr int kNormBatch = 4;   // positions whose loads a thread has under way together in the passes over chunks
 
 template <typename T>
 struct Short { typedef T type; };
@@ -183,17 +184,32 @@ __device__ __forceinline__ void group_sums(const NormDev &d, const Place &w, con
   __syncthreads();
 }
 
+// a thread's channels of w or b: one load where the array is aligned for it
 template <typename T, int V>
 __device__ __forceinline__ void load_channels(const void *from, const Place &w, float otherwise, float *v) {
 #pragma unroll
-  for (int i = 0; i < V; i++) v[i] = from && w.on ? to_f(((const T *)from)[w.c0 + w.tx * V + i]) : otherwise;
+  for (int i = 0; i < V; i++) v[i] = otherwise;
+  if (!from) return;
+  const T *p = (const T *)from + w.c0 + (w.on ? w.tx * V : 0);
+  if ((uintptr_t)from % (V * sizeof(T)) == 0) {
+    const Pack<T, V> k = load_pack<T, V>(p);
+#pragma unroll
+    for (int i = 0; i < V; i++) v[i] = k.at(i);
+  } else {
+#pragma unroll
+    for (int i = 0; i < V; i++) v[i] = to_f(p[i]);
+  }
 }
-// the group (of the block's NS * groups) of each of a thread's channels
+// the group of each of a thread's channels, counted from the stripe's first (0 for threads without channels): one division
 template <int V>
 __device__ __forceinline__ void groups_of(const NormDev &d, const Place &w, int *g) {
-  const int cg = d.a.C / d.a.G, gs = w.cw / cg;
+  const int cg = d.a.C / d.a.G, first = w.on ? w.tx * V : 0;
+  int at = first / cg, left = cg - (first - at * cg);
 #pragma unroll
-  for (int i = 0; i < V; i++) g[i] = w.on ? w.ns * gs + (w.tx * V + i) / cg : 0;
+  for (int i = 0; i < V; i++) {
+    g[i] = at;
+    if (--left == 0) at++, left = cg;
+  }
 }
 
 extern __shared__ float norm_lds[];
@@ -201,11 +217,9 @@ extern __shared__ float norm_lds[];
 // Statistics of what the threads hold in xr (R loads each, those at positions below len count): mean and sum of squares around it of
 // every group of the block, in mean[] and square[].
 template <typename T, int V, int R>
-__device__ __forceinline__ void block_stats(const NormDev &d, const Place &w, Pack<T, V> *xr, long long len, float *scratch, float *chan, float *mean,
+__device__ __forceinline__ void block_stats(const NormDev &d, const Place &w, const int *g, Pack<T, V> *xr, long long len, float *scratch, float *chan, float *mean,
                                             float *square) {
   float s[V] = {};
-  int g[V];
-  groups_of<V>(d, w, g);
 #pragma unroll
   for (int r = 0; r < R; r++)
     if (w.on && w.ty + (long long)r * d.p.TY < len) {
@@ -224,7 +238,7 @@ __device__ __forceinline__ void block_stats(const NormDev &d, const Place &w, Pa
   for (int r = 0; r < R; r++) xr[r].forget();
   float mu[V];
 #pragma unroll
-  for (int i = 0; i < V; i++) mu[i] = mean[g[i]];
+  for (int i = 0; i < V; i++) mu[i] = mean[w.ns * gs + g[i]];
 #pragma unroll
   for (int r = 0; r < R; r++)
     if (w.on && w.ty + (long long)r * d.p.TY < len) {
@@ -276,15 +290,16 @@ __global__ void __launch_bounds__(kNormMostT) norm_whole_fwd(const NormDev d) {
       const long long s = w.ty + (long long)r * d.p.TY;
       if (on && s < len) xr[r] = load_pack<T, V>(x + s * a.xp);
     }
-    block_stats<T, V, R>(d, w, xr, len, l.scratch, l.chan, l.first, l.second);
+    block_stats<T, V, R>(d, w, g, xr, len, l.scratch, l.chan, l.first, l.second);
     float mu[V], k[V];
 #pragma unroll
     for (int i = 0; i < V; i++) {
-      mu[i] = l.first[g[i]];
+      const int at_g = w.ns * gs + g[i];
+      mu[i] = l.first[at_g];
       const float cnt = (float)len * (float)cg;
-      k[i] = 1.f / sqrtf((cnt > 0.f ? l.second[g[i]] / cnt : 0.f) + a.eps);
-      if (a.mean && on && w.ty == 0 && (w.tx * V + i) % cg == 0) {
-        const long long at = n * a.G + w.c0 / cg + g[i] - w.ns * gs;
+      k[i] = 1.f / sqrtf((cnt > 0.f ? l.second[at_g] / cnt : 0.f) + a.eps);
+      if (a.mean && on && w.ty == 0 && (i ? g[i] != g[i - 1] : w.tx * V == g[0] * cg)) {
+        const long long at = n * a.G + w.c0 / cg + g[i];
         a.mean[at] = mu[i], a.rstd[at] = k[i];
       }
       k[i] *= W[i];
@@ -375,7 +390,7 @@ __global__ void __launch_bounds__(kNormMostT) norm_whole_bwd(const NormDev d) {
     }
 #pragma unroll
     for (int i = 0; i < V; i++) {
-      const long long at = n * a.G + w.c0 / cg + g[i] - w.ns * gs;
+      const long long at = n * a.G + w.c0 / cg + g[i];
       mu[i] = on ? a.mean[at] : 0.f, k[i] = on ? a.rstd[at] : 0.f;
     }
 #pragma unroll
@@ -398,7 +413,7 @@ __global__ void __launch_bounds__(kNormMostT) norm_whole_bwd(const NormDev d) {
       group_means<T>(d, w, l.chan, l.chan2, lens, l.first, l.second);
       float m1[V], m2[V];
 #pragma unroll
-      for (int i = 0; i < V; i++) m1[i] = l.first[g[i]], m2[i] = l.second[g[i]];
+      for (int i = 0; i < V; i++) m1[i] = l.first[w.ns * gs + g[i]], m2[i] = l.second[w.ns * gs + g[i]];
       T *gx = (T *)a.y + n * a.S * a.C + w.c0 + w.tx * V;
 #pragma unroll
       for (int r = 0; r < R; r++) {
@@ -443,7 +458,9 @@ __global__ void __launch_bounds__(kNormChunkT) norm_chunk_stats(const NormDev d,
     const long long s = w.ty + (long long)r * d.p.TY;
     if (w.on && s < len) xr[r] = load_pack<T, V>(x + s * a.xp);
   }
-  block_stats<T, V, kNormMostR>(d, w, xr, len, l.scratch, l.chan, l.first, l.second);
+  int g[V];
+  groups_of<V>(d, w, g);
+  block_stats<T, V, kNormMostR>(d, w, g, xr, len, l.scratch, l.chan, l.first, l.second);
   float *to = d.stats + ((n * d.p.chunks + blockIdx.x) * a.G + w.c0 / cg) * 2;
   for (int k = threadIdx.x; k < w.cw / cg; k += d.p.T) to[2 * k] = l.first[k], to[2 * k + 1] = l.second[k];
 }
@@ -484,29 +501,36 @@ __global__ void __launch_bounds__(kNormChunkT) norm_apply_fwd(const NormDev d, l
   const int cg = a.C / a.G;
   const long long n = nbase + blockIdx.z, s0 = blockIdx.x * d.p.rows, len = length_of(a, n), end = min(s0 + d.p.rows, a.S);
   float B[V], mu[V], k[V];
+  int g[V];
   load_channels<T, V>(a.w, w, 1.f, k);
   load_channels<T, V>(a.b, w, 0.f, B);
+  groups_of<V>(d, w, g);
 #pragma unroll
   for (int i = 0; i < V; i++) {
-    const long long at = n * a.G + (w.c0 + w.tx * V + i) / cg;
+    const long long at = n * a.G + w.c0 / cg + g[i];
     mu[i] = a.mean[at], k[i] *= a.rstd[at];
   }
   const T *x = (const T *)a.x + n * a.xs + w.c0 + w.tx * V;
   T *y = (T *)a.y + n * a.S * a.C + w.c0 + w.tx * V;
-#pragma unroll 4
-  for (long long s = s0 + w.ty; s < end; s += d.p.TY) {
-    Pack<T, V> p = {};
-    if (s < len) {
-      float o[V];
-      p = load_pack<T, V>(x + s * a.xp);
+  for (long long s = s0 + w.ty; s < end; s += kNormBatch * d.p.TY) {
+    Pack<T, V> p[kNormBatch] = {};
 #pragma unroll
-      for (int i = 0; i < V; i++) {
-        float e;
-        act_both<ACT>((p.at(i) - mu[i]) * k[i] + B[i], o[i], e, a.act == kActRelu);
+    for (int u = 0; u < kNormBatch; u++)
+      if (s + u * d.p.TY < min(len, end)) p[u] = load_pack<T, V>(x + (s + u * d.p.TY) * a.xp);
+#pragma unroll
+    for (int u = 0; u < kNormBatch; u++) {
+      if (s + u * d.p.TY >= end) break;
+      if (s + u * d.p.TY < len) {
+        float o[V];
+#pragma unroll
+        for (int i = 0; i < V; i++) {
+          float e;
+          act_both<ACT>((p[u].at(i) - mu[i]) * k[i] + B[i], o[i], e, a.act == kActRelu);
+        }
+        p[u].set(o);
       }
-      p.set(o);
+      store_pack<T, V>(y + (s + u * d.p.TY) * a.C, p[u]);
     }
-    store_pack<T, V>(y + s * a.C, p);
   }
 }
 
@@ -519,21 +543,32 @@ __global__ void __launch_bounds__(kNormChunkT) norm_chunk_sums(const NormDev d, 
   const int cg = a.C / a.G;
   const long long n = nbase + blockIdx.z, s0 = blockIdx.x * d.p.rows, end = min(s0 + d.p.rows, length_of(a, n));
   float W[V], B[V], mu[V], k[V], s1[V] = {}, s2[V] = {};
+  int g[V];
   load_channels<T, V>(a.w, w, 1.f, W);
   load_channels<T, V>(a.b, w, 0.f, B);
+  groups_of<V>(d, w, g);
   if (w.on) {
 #pragma unroll
     for (int i = 0; i < V; i++) {
-      const long long at = n * a.G + (w.c0 + w.tx * V + i) / cg;
+      const long long at = n * a.G + w.c0 / cg + g[i];
       mu[i] = a.mean[at], k[i] = a.rstd[at];
     }
     const T *x = (const T *)a.x + n * a.xs + w.c0 + w.tx * V, *gy = (const T *)a.gy + n * a.S * a.C + w.c0 + w.tx * V;
-#pragma unroll 4
-    for (long long s = s0 + w.ty; s < end; s += d.p.TY) {
-      float xh[V], gz[V];
-      gz_of<T, V, ACT>(load_pack<T, V>(x + s * a.xp), load_pack<T, V>(gy + s * a.C), mu, k, W, B, a.act == kActRelu, xh, gz);
+    for (long long s = s0 + w.ty; s < end; s += kNormBatch * d.p.TY) {
+      Pack<T, V> p[kNormBatch], q[kNormBatch];
 #pragma unroll
-      for (int i = 0; i < V; i++) s1[i] += gz[i], s2[i] += gz[i] * xh[i];
+      for (int u = 0; u < kNormBatch; u++) {
+        const long long at = min(s + u * d.p.TY, end - 1);   // (the last ones repeat and are not added)
+        p[u] = load_pack<T, V>(x + at * a.xp), q[u] = load_pack<T, V>(gy + at * a.C);
+      }
+#pragma unroll
+      for (int u = 0; u < kNormBatch; u++) {
+        if (s + u * d.p.TY >= end) break;
+        float xh[V], gz[V];
+        gz_of<T, V, ACT>(p[u], q[u], mu, k, W, B, a.act == kActRelu, xh, gz);
+#pragma unroll
+        for (int i = 0; i < V; i++) s1[i] += gz[i], s2[i] += gz[i] * xh[i];
+      }
     }
   }
   column_sums<V>(d, w, s1, l.scratch, l.chan);
@@ -588,26 +623,36 @@ __global__ void __launch_bounds__(kNormChunkT) norm_apply_bwd(const NormDev d, l
   const int cg = a.C / a.G;
   const long long n = nbase + blockIdx.z, s0 = blockIdx.x * d.p.rows, len = length_of(a, n), end = min(s0 + d.p.rows, a.S);
   float W[V], B[V], mu[V], k[V], m1[V], m2[V];
+  int g[V];
   load_channels<T, V>(a.w, w, 1.f, W);
   load_channels<T, V>(a.b, w, 0.f, B);
+  groups_of<V>(d, w, g);
 #pragma unroll
   for (int i = 0; i < V; i++) {
-    const long long at = n * a.G + (w.c0 + w.tx * V + i) / cg;
+    const long long at = n * a.G + w.c0 / cg + g[i];
     mu[i] = a.mean[at], k[i] = a.rstd[at], m1[i] = d.means[2 * at], m2[i] = d.means[2 * at + 1];
   }
   const T *x = (const T *)a.x + n * a.xs + w.c0 + w.tx * V, *gy = (const T *)a.gy + n * a.S * a.C + w.c0 + w.tx * V;
   T *gx = (T *)a.y + n * a.S * a.C + w.c0 + w.tx * V;
-#pragma unroll 4
-  for (long long s = s0 + w.ty; s < end; s += d.p.TY) {
-    Pack<T, V> p = {};
-    if (s < len) {
-      float xh[V], gz[V], o[V];
-      gz_of<T, V, ACT>(load_pack<T, V>(x + s * a.xp), load_pack<T, V>(gy + s * a.C), mu, k, W, B, a.act == kActRelu, xh, gz);
+  for (long long s = s0 + w.ty; s < end; s += kNormBatch * d.p.TY) {
+    Pack<T, V> p[kNormBatch] = {}, q[kNormBatch] = {};
 #pragma unroll
-      for (int i = 0; i < V; i++) o[i] = k[i] * (gz[i] * W[i] - m1[i] - xh[i] * m2[i]);
-      p.set(o);
+    for (int u = 0; u < kNormBatch; u++) {
+      const long long at = s + u * d.p.TY;
+      if (at < min(len, end)) p[u] = load_pack<T, V>(x + at * a.xp), q[u] = load_pack<T, V>(gy + at * a.C);
     }
-    store_pack<T, V>(gx + s * a.C, p);
+#pragma unroll
+    for (int u = 0; u < kNormBatch; u++) {
+      if (s + u * d.p.TY >= end) break;
+      if (s + u * d.p.TY < len) {
+        float xh[V], gz[V], o[V];
+        gz_of<T, V, ACT>(p[u], q[u], mu, k, W, B, a.act == kActRelu, xh, gz);
+#pragma unroll
+        for (int i = 0; i < V; i++) o[i] = k[i] * (gz[i] * W[i] - m1[i] - xh[i] * m2[i]);
+        p[u].set(o);
+      }
+      store_pack<T, V>(gx + (s + u * d.p.TY) * a.C, p[u]);
+    }
   }
 }
 
