@@ -11,6 +11,8 @@ namespace py = pybind11;
 namespace {
 
 typedef std::optional<at::Tensor> Maybe;
+using torch::autograd::AutogradContext;
+using torch::autograd::variable_list;
 
 void done(int status) {
   if (status == GELIB_HIP_OK) return;
@@ -121,7 +123,10 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor> norm_fwd(const at::Tensor &x, int
   NormShape s = norm_shape(x);
   at::Tensor W = w ? plain(*w) : at::Tensor(), B = b ? plain(*b) : at::Tensor(), L = lengths ? lengths->contiguous() : at::Tensor();
   at::Tensor y = at::empty(x.sizes(), x.options().memory_format(at::MemoryFormat::Contiguous)), mean, rstd;
-  if (keep) mean = at::empty({s.N, groups}, x.options().dtype(at::kFloat)), rstd = at::empty_like(mean);
+  if (keep) {
+    const at::Tensor both = at::empty({2, s.N, groups}, x.options().dtype(at::kFloat));
+    mean = both[0], rstd = both[1];
+  }
   const uint64_t bytes = gelib_hip_group_norm_act_workspace_bytes(0, type_of(x), s.N, s.S, s.C, (int)groups);
   at::Tensor ws = workspace(bytes, x);
   done(gelib_hip_group_norm_act_fwd(ptr(y), (float *)ptr(mean), (float *)ptr(rstd), ptr(s.x), ptr(W), ptr(B), (int32_t *)ptr(L), type_of(x), s.N, s.S,
@@ -129,8 +134,8 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor> norm_fwd(const at::Tensor &x, int
   return {y, mean, rstd};
 }
 
-std::tuple<Maybe, Maybe, Maybe> norm_bwd(const at::Tensor &gy_, const at::Tensor &mean, const at::Tensor &rstd, const at::Tensor &x, int64_t groups,
-                                         const Maybe &w, const Maybe &b, const std::string &act, const Maybe &lengths, bool need_x, bool need_w,
+std::tuple<at::Tensor, at::Tensor, at::Tensor> norm_bwd(const at::Tensor &gy_, const at::Tensor &mean, const at::Tensor &rstd, const at::Tensor &x, int64_t groups,
+                                         const Maybe &w, const Maybe &b, int act, const Maybe &lengths, bool need_x, bool need_w,
                                          bool need_b) {
   norm_check(x, groups, w, b, lengths);
   OnDevice on(x);
@@ -146,9 +151,92 @@ std::tuple<Maybe, Maybe, Maybe> norm_bwd(const at::Tensor &gy_, const at::Tensor
   const uint64_t bytes = gelib_hip_group_norm_act_workspace_bytes(1, type_of(x), s.N, s.S, s.C, (int)groups);
   at::Tensor ws = workspace(bytes, x);
   done(gelib_hip_group_norm_act_bwd(ptr(gx), ptr(gw), ptr(gb), ptr(gy), (float *)ptr(mean), (float *)ptr(rstd), ptr(s.x), ptr(W), ptr(B), (int32_t *)ptr(L),
-                                    type_of(x), s.N, s.S, s.C, (int)groups, s.xs, s.xp, act_of(act), ptr(ws), bytes, on.stream));
-  auto some = [](const at::Tensor &t) { return t.defined() ? Maybe(t) : Maybe(); };
-  return {some(gx), some(gw), some(gb)};
+                                    type_of(x), s.N, s.S, s.C, (int)groups, s.xs, s.xp, act, ptr(ws), bytes, on.stream));
+  return {gx, gw, gb};
+}
+
+// The same from torch's own operations: for gradients of gradients.
+at::Tensor activated(const at::Tensor &z, int64_t act) {
+  return act == GELIB_HIP_ACT_RELU ? at::relu(z) : act == GELIB_HIP_ACT_SILU ? at::silu(z) : act == GELIB_HIP_ACT_GELU ? at::gelu(z) : z;
+}
+at::Tensor norm_from_torch(const at::Tensor &x, const at::Tensor &w, const at::Tensor &b, const at::Tensor &lengths, int64_t groups, double eps, int64_t act) {
+  const int64_t n = x.size(0), c = x.size(-1);
+  at::Tensor t = x.reshape({n, -1, groups, c / groups}).to(at::kFloat), live, count;
+  if (lengths.defined()) {
+    const at::Tensor held = lengths.clamp(0, t.size(1));
+    live = at::arange(t.size(1), held.options()).lt(held.unsqueeze(1)).view({n, -1, 1, 1});
+    count = (held.clamp_min(1) * t.size(3)).view({n, 1, 1, 1});
+    t = t.masked_fill(live.logical_not(), 0);
+  } else {
+    count = at::full({}, (double)t.size(1) * t.size(3), t.options());
+  }
+  at::Tensor d = t - t.sum({1, 3}, true) / count;
+  if (live.defined()) d = d.masked_fill(live.logical_not(), 0);
+  t = (d * (d.square().sum({1, 3}, true) / count + eps).rsqrt()).reshape(x.sizes());
+  if (w.defined()) t = t * w.to(at::kFloat);
+  if (b.defined()) t = t + b.to(at::kFloat);
+  t = activated(t, act);
+  if (live.defined()) t = t.reshape({n, -1, groups, c / groups}).masked_fill(live.logical_not(), 0).reshape(x.sizes());
+  return t.to(x.scalar_type());
+}
+
+// Gradients with a graph of their own of f(tensors) for those that need one.
+template <typename F>
+variable_list graph_grads(F f, const variable_list &tensors, const at::Tensor &g) {
+  at::AutoGradMode on(true);
+  variable_list views, wanted, grads(tensors.size());
+  for (const at::Tensor &t : tensors) {
+    views.push_back(t.defined() ? t.view_as(t) : t);   // (one tensor may stand in two places)
+    if (t.defined() && t.requires_grad()) wanted.push_back(views.back());
+  }
+  if (wanted.empty()) return grads;
+  const variable_list got = torch::autograd::grad({f(views)}, wanted, {g}, /*retain_graph=*/true, /*create_graph=*/true);
+  size_t k = 0;
+  for (size_t i = 0; i < tensors.size(); i++)
+    if (tensors[i].defined() && tensors[i].requires_grad()) grads[i] = got[k++];
+  return grads;
+}
+
+at::Tensor some(const Maybe &t) { return t ? *t : at::Tensor(); }
+Maybe some(const at::Tensor &t) { return t.defined() ? Maybe(t) : Maybe(); }
+bool needs(const at::Tensor &t) { return t.defined() && t.requires_grad(); }
+
+struct NormFn : torch::autograd::Function<NormFn> {
+  static at::Tensor forward(AutogradContext *ctx, const at::Tensor &x, const Maybe &w, const Maybe &b, int64_t groups, double eps, const std::string &act,
+                            const Maybe &lengths) {
+    auto [y, mean, rstd] = norm_fwd(x, groups, w, b, eps, act, lengths, true);
+    ctx->save_for_backward({x, some(w), some(b), some(lengths), mean, rstd});
+    ctx->saved_data["how"] = std::tuple<int64_t, double, int64_t>(groups, eps, act_of(act));
+    return y;
+  }
+  static variable_list backward(AutogradContext *ctx, variable_list g) {
+    const variable_list saved = ctx->get_saved_variables();
+    const at::Tensor &x = saved[0], &w = saved[1], &b = saved[2], &lengths = saved[3];
+    const auto how = ctx->saved_data["how"].to<std::tuple<int64_t, double, int64_t>>();
+    const auto [groups, eps, act] = how;
+    variable_list grads(7);
+    if (!g[0].defined()) return grads;
+    if (at::GradMode::is_enabled()) {   // a graph of the gradients is wanted
+      const int64_t G = groups, A = act;
+      const double e = eps;
+      const variable_list got = graph_grads([&](const variable_list &v) { return norm_from_torch(v[0], v[1], v[2], lengths, G, e, A); }, {x, w, b}, g[0]);
+      std::copy(got.begin(), got.end(), grads.begin());
+      return grads;
+    }
+    size_t at = 0;   // (tensors that were given are counted)
+    const bool need_x = ctx->needs_input_grad(at), need_w = w.defined() && ctx->needs_input_grad(++at), need_b = b.defined() && ctx->needs_input_grad(++at);
+    auto [gx, gw, gb] = norm_bwd(g[0], saved[4], saved[5], x, groups, some(w), some(b), (int)act, some(lengths), need_x, need_w, need_b);
+    grads[0] = gx, grads[1] = gw, grads[2] = gb;
+    return grads;
+  }
+};
+
+at::Tensor group_norm_act(const at::Tensor &x, int64_t groups, const Maybe &w, const Maybe &b, double eps, const std::string &act, const Maybe &lengths) {
+  if (at::GradMode::is_enabled() && (x.requires_grad() || (w && needs(*w)) || (b && needs(*b)))) {
+    norm_check(x, groups, w, b, lengths);   // (refusals come before anything is recorded)
+    return NormFn::apply(x, w, b, groups, eps, act, lengths);
+  }
+  return std::get<0>(norm_fwd(x, groups, w, b, eps, act, lengths, false));
 }
 
 // ---- linear layer ----
@@ -188,7 +276,7 @@ void linear_check(const at::Tensor &x, const at::Tensor &w) {
   if (w.size(0) > 0x7fffffff || w.size(1) > 0x7fffffff) throw py::value_error("GElib: too many channels");
 }
 
-std::tuple<at::Tensor, Maybe> linear_fwd(const at::Tensor &x, const at::Tensor &w, const Maybe &b, const Maybe &r, const std::string &act, bool keep) {
+std::tuple<at::Tensor, at::Tensor> linear_fwd(const at::Tensor &x, const at::Tensor &w, const Maybe &b, const Maybe &r, const std::string &act, bool keep) {
   linear_check(x, w);
   const int a = act_of(act);
   std::vector<int64_t> shape(x.sizes().begin(), x.sizes().end());
@@ -211,10 +299,10 @@ std::tuple<at::Tensor, Maybe> linear_fwd(const at::Tensor &x, const at::Tensor &
   const uint64_t bytes = gelib_hip_linear_act_workspace_bytes(0, type_of(x), X.rows, X.K, N);
   at::Tensor ws = workspace(bytes, x);
   done(gelib_hip_linear_act_fwd(ptr(y), ptr(slope), ptr(X.x), ptr(W), ptr(B), ptr(R), type_of(x), X.rows, X.K, N, X.stride, a, ptr(ws), bytes, on.stream));
-  return {y, slope.defined() ? Maybe(slope) : Maybe()};
+  return {y, slope};
 }
 
-std::tuple<Maybe, Maybe, Maybe> linear_bwd(const at::Tensor &gy_, const Maybe &slope, const at::Tensor &x, const at::Tensor &w, bool need_x, bool need_w,
+std::tuple<at::Tensor, at::Tensor, at::Tensor> linear_bwd(const at::Tensor &gy_, const Maybe &slope, const at::Tensor &x, const at::Tensor &w, bool need_x, bool need_w,
                                            bool need_b) {
   linear_check(x, w);
   OnDevice on(x);
@@ -231,8 +319,52 @@ std::tuple<Maybe, Maybe, Maybe> linear_bwd(const at::Tensor &gy_, const Maybe &s
   at::Tensor ws = workspace(bytes, x);
   done(gelib_hip_linear_act_bwd(ptr(gx), ptr(gw), ptr(gb), ptr(gy), slope ? ptr(*slope) : nullptr, ptr(X.x), ptr(W), type_of(x), X.rows, X.K, N, X.stride,
                                 ptr(ws), bytes, on.stream));
-  auto some = [](const at::Tensor &t) { return t.defined() ? Maybe(t) : Maybe(); };
-  return {some(gx), some(gw), some(gb)};
+  return {gx, gw, gb};
+}
+
+at::Tensor linear_from_torch(const at::Tensor &x, const at::Tensor &w, const at::Tensor &b, int64_t act) {
+  at::Tensor z = at::matmul(x.to(at::kFloat), w.to(at::kFloat));
+  if (b.defined()) z = z + b.to(at::kFloat);
+  return activated(z, act).to(x.scalar_type());
+}
+
+// Keeps act'(x w + bias) for the backward pass: the product is not formed again, and nothing else of its size is kept.
+struct LinearFn : torch::autograd::Function<LinearFn> {
+  static at::Tensor forward(AutogradContext *ctx, const at::Tensor &x, const at::Tensor &w, const Maybe &b, const Maybe &r, const std::string &act) {
+    auto [y, slope] = linear_fwd(x, w, b, r, act, true);
+    ctx->save_for_backward({x, w, some(b), slope});
+    ctx->saved_data["how"] = std::tuple<int64_t, bool>(act_of(act), r.has_value());
+    return y;
+  }
+  static variable_list backward(AutogradContext *ctx, variable_list g) {
+    const variable_list saved = ctx->get_saved_variables();
+    const at::Tensor &x = saved[0], &w = saved[1], &b = saved[2];
+    const auto how = ctx->saved_data["how"].to<std::tuple<int64_t, bool>>();
+    const int64_t act = std::get<0>(how);
+    variable_list grads(5);
+    if (!g[0].defined()) return grads;
+    size_t at = 1;
+    const bool need_x = ctx->needs_input_grad(0), need_w = ctx->needs_input_grad(1), need_b = b.defined() && ctx->needs_input_grad(++at),
+               need_r = std::get<1>(how) && ctx->needs_input_grad(++at);
+    if (need_r) grads[3] = g[0];
+    if (!need_x && !need_w && !need_b) return grads;
+    if (at::GradMode::is_enabled()) {   // a graph of the gradients is wanted
+      const variable_list got = graph_grads([&](const variable_list &v) { return linear_from_torch(v[0], v[1], v[2], act); }, {x, w, b}, g[0]);
+      std::copy(got.begin(), got.end(), grads.begin());
+      return grads;
+    }
+    auto [gx, gw, gb] = linear_bwd(g[0], some(saved[3]), x, w, need_x, need_w, need_b);
+    grads[0] = gx, grads[1] = gw, grads[2] = gb;
+    return grads;
+  }
+};
+
+at::Tensor linear_act(const at::Tensor &x, const at::Tensor &w, const Maybe &b, const Maybe &r, const std::string &act) {
+  if (at::GradMode::is_enabled() && (x.requires_grad() || w.requires_grad() || (b && needs(*b)) || (r && needs(*r)))) {
+    linear_check(x, w);   // (refusals come before anything is recorded)
+    return LinearFn::apply(x, w, b, r, act);
+  }
+  return std::get<0>(linear_fwd(x, w, b, r, act, false));
 }
 
 // ---- AdamW ----
@@ -306,10 +438,8 @@ void adamw_set_moments(const at::Tensor &m, const at::Tensor &v, const at::Tenso
 }  // namespace
 
 void bind_real_ops(py::module_ &m) {
-  m.def("group_norm_act_fwd", &norm_fwd);
-  m.def("group_norm_act_bwd", &norm_bwd);
-  m.def("linear_act_fwd", &linear_fwd);
-  m.def("linear_act_bwd", &linear_bwd);
+  m.def("group_norm_act", &group_norm_act);
+  m.def("linear_act", &linear_act);
   py::class_<AdamWGroup>(m, "AdamWGroup", "Parameters of one AdamW step, with the places of their moments")
       .def(py::init<std::vector<at::Tensor>, std::vector<int64_t>>())
       .def("step", &AdamWGroup::step)
