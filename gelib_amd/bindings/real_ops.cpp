@@ -39,7 +39,11 @@ void on_gpu(const at::Tensor &x) {
   if (!x.is_cuda()) throw py::value_error("GElib: tensors must be on GPU: these operators have no host form in this build");
 }
 
-at::Tensor plain(const at::Tensor &t) { return t.resolve_neg().contiguous(); }
+// t packed, and from a multiple of 16 bytes on
+at::Tensor plain(const at::Tensor &t) {
+  const at::Tensor p = t.resolve_neg().contiguous();
+  return p.numel() && (uintptr_t)p.data_ptr() % 16 ? p.clone() : p;
+}
 
 void *ptr(const at::Tensor &t) { return t.defined() && t.numel() ? t.data_ptr() : nullptr; }
 
@@ -140,9 +144,7 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor> norm_bwd(const at::Tensor &gy_, c
   norm_check(x, groups, w, b, lengths);
   OnDevice on(x);
   NormShape s = norm_shape(x);
-  at::Tensor gy = plain(gy_);
-  if ((uintptr_t)gy.data_ptr() % 16) gy = gy.clone();
-  at::Tensor W = w ? plain(*w) : at::Tensor(), B = b ? plain(*b) : at::Tensor(), L = lengths ? lengths->contiguous() : at::Tensor();
+  at::Tensor gy = plain(gy_), W = w ? plain(*w) : at::Tensor(), B = b ? plain(*b) : at::Tensor(), L = lengths ? lengths->contiguous() : at::Tensor();
   like(gy, x, "the gradient");
   if (gy.sizes() != x.sizes()) throw py::value_error("GElib: the gradient has another shape than x");
   const auto packed = x.options().memory_format(at::MemoryFormat::Contiguous);
@@ -241,7 +243,7 @@ at::Tensor group_norm_act(const at::Tensor &x, int64_t groups, const Maybe &w, c
 
 // ---- linear layer ----
 
-struct Rows {   // x as rows: itself where they are evenly spaced and contiguous, else a copy
+struct Rows {   // x as rows: itself where they are evenly spaced, contiguous and aligned as packed ones are, else a copy
   at::Tensor x;
   int64_t rows, stride;
   int K;
@@ -260,8 +262,10 @@ Rows rows_of(const at::Tensor &t) {
     }
     r.rows *= t.size(k);
   }
+  const int64_t width = r.K * t.element_size() % 16 == 0 ? 16 : 1;
+  if (even) even = (step < 0 || step * t.element_size() % width == 0) && (uintptr_t)r.x.data_ptr() % width == 0;
   if (!even || r.x.numel() == 0) {
-    r.x = r.x.contiguous();
+    r.x = r.x.is_contiguous() ? r.x.clone() : r.x.contiguous();
     step = r.K;
   }
   r.stride = step < 0 ? r.K : step;

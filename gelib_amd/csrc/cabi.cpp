@@ -15,6 +15,7 @@
 
 #include "cg_common.h"
 #include "cg_linear.h"
+#include "real_ops.h"
 #include "mix_vec.h"
 #include "cg_staged.h"
 #include "cg_unrolled.h"
@@ -1939,6 +1940,7 @@ int gelib_hip_set_option(const char *name, int value) {
     g_vec_mix = value;
     return GELIB_HIP_OK;
   }
+  if (!std::strncmp(name, "linear_act_", 11)) return linear_act_set_option(name, value);
   if (!std::strcmp(name, "linear_wgrad")) {
     g_linear_wgrad = value;
     return GELIB_HIP_OK;

@@ -44,9 +44,14 @@ int norm_shape(int dtype, int act, int64_t N, int64_t S, int C, int G, int64_t x
   return GELIB_HIP_OK;
 }
 
+// what rows of `cols` elements are aligned to: 16 bytes where they are a multiple of it long
+unsigned row_align(unsigned e, int64_t cols) { return cols * e % 16 == 0 ? 16 : e; }
+
 int linear_shape(int dtype, int act, int64_t rows, int K, int N, int64_t xs) {
   if (!types_ok(dtype, act) || rows < 0 || K < 0 || N < 0 || xs < 0) return GELIB_HIP_ERR_ARG;
   if (!product_ok(rows, K) || !product_ok(rows, N) || !product_ok(rows, xs)) return GELIB_HIP_ERR_ARG;
+  const unsigned e = (unsigned)dtype_bytes(dtype);
+  if (rows > 1 && xs * e % row_align(e, K) != 0) return GELIB_HIP_ERR_ARG;
   return GELIB_HIP_OK;
 }
 
@@ -124,7 +129,7 @@ int gelib_hip_linear_act_fwd(void *y, void *slope, const void *x, const void *w,
   Memory mem;
   mem.need(y, out * e, e);
   if (act != GELIB_HIP_ACT_NONE) mem.may(slope, out * e, e);   // (float32 or float16: as wide as the layer's type)
-  if (out && n_in) mem.need(x, ((rows - 1) * x_row_stride + n_in) * e, e), mem.need(w, (int64_t)n_in * n_out * e, e);
+  if (out && n_in) mem.need(x, ((rows - 1) * x_row_stride + n_in) * e, row_align(e, n_in)), mem.need(w, (int64_t)n_in * n_out * e, row_align(e, n_out));
   mem.may(bias, (int64_t)n_out * e, e);
   mem.may(residual, out * e, e);
   if (int rc = mem.rc()) return rc;
@@ -143,13 +148,13 @@ int gelib_hip_linear_act_bwd(void *gx, void *gw, void *gb, const void *gy, const
   const unsigned e = (unsigned)dtype_bytes(dtype);
   const int64_t out = rows * n_out;
   Memory mem;
-  mem.need(gy, out * e, e);
+  mem.need(gy, out * e, row_align(e, n_out));
   mem.may(slope, out * e, e);
   mem.may(gx, rows * n_in * e, e);
   mem.may(gw, (int64_t)n_in * n_out * e, e);
   mem.may(gb, (int64_t)n_out * e, e);
-  if (gx && rows && n_in) mem.need(w, (int64_t)n_in * n_out * e, e);
-  if (gw && out && n_in) mem.need(x, ((rows - 1) * x_row_stride + n_in) * e, e);
+  if (gx && rows && n_in) mem.need(w, (int64_t)n_in * n_out * e, row_align(e, n_out));
+  if (gw && out && n_in) mem.need(x, ((rows - 1) * x_row_stride + n_in) * e, row_align(e, n_in));
   if (int rc = mem.rc()) return rc;
   const int what = (gx ? 1 : 0) | (gw ? 2 : 0) | (gb ? 4 : 0) | (slope ? 8 : 0);
   if (int rc = check_workspace(workspace, workspace_bytes, linear_workspace(what, dtype, rows, n_in, n_out))) return rc;

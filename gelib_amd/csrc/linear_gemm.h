@@ -3,9 +3,9 @@
 //
 // An operand lies in memory either with k innermost (x in x w, gz and w in gz w^T) or with its own index innermost (w in x w, both
 // in x^T gz); the tile that a block stages is 128 bytes of k by R rows, or its transpose, either way R * 128 bytes of LDS, copied as
-// it lies in memory, 16 bytes a lane, straight into LDS where rows are 16-byte aligned (FAST) and through registers, element by
-// element at the ends, where they are not.  What is outside the matrix is staged as zero, so no tile needs a special case behind
-// this.  Transposing happens on the way from LDS into registers: 16-bit types with the LDS unit's transposing reads (a group of 16
+// it lies in memory, 16 bytes a lane, straight into LDS: rows start at multiples of 16 bytes and end in zeros up to the next one
+// (operands that do not are copied first, linear_act.hip).  What is outside the matrix is staged as zero, so no tile needs a special
+// case behind this.  Transposing happens on the way from LDS into registers: 16-bit types with the LDS unit's transposing reads (a group of 16
 // lanes reads 4 rows of 16 values and each lane gets a column of 4), float32 by giving a lane the 4 neighbouring columns that one
 // 16-byte read delivers: fragment j of a lane belongs to column 4 r + j, and the epilogue goes by that.
 // The order of 16-byte pieces in a row of LDS is permuted (exclusive or with the row) so that the lanes of a read spread over the banks.
@@ -24,7 +24,7 @@ struct GemmArgs {
   void *c;                  // (M, N) packed
   const void *bias, *res;   // epilogue: c = act(sum + bias) + res, slope = act'(sum + bias); each may be null
   void *slope;
-  float *part;              // [splits][M][N] sums of the pieces of k instead of c, or null
+  float *part;              // [splits][M][N up to a multiple of 4] sums of the pieces of k instead of c, or null
   long long M, K, kper;     // kper: k of a piece, a multiple of the step
   int N, act, splits, vec4;  // vec4: rows of c, res and slope take vectors of 4
   unsigned mtiles, ntiles;
@@ -37,7 +37,7 @@ constexpr int kGemmTiles = 4;
 constexpr int kGemmBM[kGemmTiles] = {256, 128, 64, 16}, kGemmBN[kGemmTiles] = {256, 128, 128, 256};
 
 template <typename T>
-int launch_gemm(GemmForm form, int tile, bool fast, const GemmArgs &a, hipStream_t s);
+int launch_gemm(GemmForm form, int tile, const GemmArgs &a, hipStream_t s);
 
 #ifdef __HIPCC__
 
@@ -72,7 +72,7 @@ __device__ __forceinline__ void load_to_lds(const char *from, char *to) {
 static __device__ const float4 gemm_zeros[1] = {};   // what lanes outside a matrix stage
 
 // One operand's tile.  R: its extent (BM or BN), KIN: k innermost in memory, G: neighbouring rows that fragments share in float32
-template <typename T, int R, bool KIN, bool FAST, int THREADS, int G>
+template <typename T, int R, bool KIN, int THREADS, int G>
 struct Stage {
   static constexpr int VEC = 16 / sizeof(T), BK = 128 / sizeof(T);
   static constexpr int CPR = KIN ? 8 : R * (int)sizeof(T) / 16;          // 16-byte pieces of a row in LDS
@@ -81,7 +81,6 @@ struct Stage {
   long long mn[NL];
   int k[NL];
   long long step;
-  float4 reg[FAST ? 1 : NL];
 
   static __device__ __forceinline__ int swizzle(int row) {
     if (KIN) return (row / G) & 7;
@@ -99,33 +98,13 @@ struct Stage {
     step = KIN ? BK : BK * ld;
   }
   // the tile whose first k has `left` more of it behind (k0 .. k0 + left)
-  __device__ __forceinline__ void issue(char *lds, long long left, long long MN) {
+  __device__ __forceinline__ void issue(char *lds, long long left) {
 #pragma unroll
     for (int u = 0; u < NL; u++) {
       if (R * 8 % THREADS != 0 && u * THREADS + threadIdx.x >= R * 8) continue;   // (whole waves)
       const bool in = mn[u] >= 0 && k[u] < left;
-      if (FAST) {
-        load_to_lds(in ? (const char *)p[u] : (const char *)gemm_zeros, lds + (u * THREADS + (threadIdx.x & ~63)) * 16);
-      } else {
-        const long long have = !in ? 0 : KIN ? left - k[u] : MN - mn[u];
-        T t[VEC];
-        if (have >= VEC) {
-          __builtin_memcpy(t, p[u], 16);
-        } else {
-#pragma unroll
-          for (int i = 0; i < VEC; i++) t[i] = i < have ? p[u][i] : (T)0.f;
-        }
-        __builtin_memcpy(&reg[u], t, 16);
-      }
+      load_to_lds(in ? (const char *)p[u] : (const char *)gemm_zeros, lds + (u * THREADS + (threadIdx.x & ~63)) * 16);
       p[u] += step;
-    }
-  }
-  __device__ __forceinline__ void commit(char *lds) {
-    if (FAST) return;
-#pragma unroll
-    for (int u = 0; u < NL; u++) {
-      if (R * 8 % THREADS != 0 && u * THREADS + threadIdx.x >= R * 8) continue;
-      *(float4 *)(lds + (u * THREADS + threadIdx.x) * 16) = reg[u];
     }
   }
   // 16-bit: the fragment of 16 rows from row0 on, k = ks * 32 + (lane / 16) * 8 + 0..7
@@ -205,12 +184,12 @@ __device__ __forceinline__ void epilogue4(const GemmArgs &a, long long m, int n,
   }
 }
 
-template <typename T, bool AK, bool BKIN, int BM, int BN, int WM, int WN, bool FAST, int ACT>
+template <typename T, bool AK, bool BKIN, int BM, int BN, int WM, int WN, int ACT>
 __global__ void __launch_bounds__(64 * (BM / WM) * (BN / WN)) gemm_kernel(const GemmArgs a) {
   constexpr int THREADS = 64 * (BM / WM) * (BN / WN), BK = 128 / sizeof(T), FM = WM / 16, FN = WN / 16;
   constexpr int GM = sizeof(T) == 4 ? (FM < 4 ? FM : 4) : 1, GN = sizeof(T) == 4 ? (FN < 4 ? FN : 4) : 1;
-  typedef Stage<T, BM, AK, FAST, THREADS, GM> SA;
-  typedef Stage<T, BN, BKIN, FAST, THREADS, GN> SB;
+  typedef Stage<T, BM, AK, THREADS, GM> SA;
+  typedef Stage<T, BN, BKIN, THREADS, GN> SB;
   __shared__ __align__(16) char lds[2][(BM + BN) * 128];
   // Blocks go round the eight XCDs in turn: each XCD gets a run of neighbouring tiles, so that its L2 holds what they share;
   // in a run, eight row tiles by all columns before the next eight.
@@ -235,20 +214,18 @@ __global__ void __launch_bounds__(64 * (BM / WM) * (BN / WN)) gemm_kernel(const 
   sb.init(a.b, a.ldb, n0, a.N, k0);
   long long left = k1 - k0;
   auto issue = [&](int buf) __attribute__((always_inline)) {
-    sa.issue(lds[buf], left, a.M);
-    sb.issue(lds[buf] + BM * 128, left, a.N);
+    sa.issue(lds[buf], left);
+    sb.issue(lds[buf] + BM * 128, left);
     left -= BK;
   };
-  auto commit = [&](int buf) __attribute__((always_inline)) {
-    sa.commit(lds[buf]);
-    sb.commit(lds[buf] + BM * 128);
-    if (FAST) asm volatile("s_waitcnt vmcnt(0)" : : : "memory");   // what this wave has copied into LDS is there
+  auto arrive = [&]() __attribute__((always_inline)) {
+    asm volatile("s_waitcnt vmcnt(0)" : : : "memory");   // what this wave has copied into LDS is there
     __syncthreads();
   };
   const int steps = left > 0 ? (int)((left + BK - 1) / BK) : 0;
   if (steps) {
     issue(0);
-    commit(0);
+    arrive();
   }
   for (int t = 0, buf = 0; t < steps; t++, buf ^= 1) {
     const bool more = t + 1 < steps;
@@ -283,22 +260,16 @@ __global__ void __launch_bounds__(64 * (BM / WM) * (BN / WN)) gemm_kernel(const 
             for (int j = 0; j < FN; j++) acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x4f32(fb[j][k], fa[i][k], acc[i][j], 0, 0, 0);
       }
     }
-    if (more) commit(buf ^ 1);
+    if (more) arrive();
   }
 
   const int lane = threadIdx.x % 64, c = lane % 16, q = lane / 16;
-  float *part = a.part ? a.part + (long long)blockIdx.y * a.M * a.N : nullptr;
+  const long long part_row = (a.N + 3) & ~3;
+  float *part = a.part ? a.part + (long long)blockIdx.y * a.M * part_row : nullptr;
   auto out = [&](long long m, long long n, const float *v) __attribute__((always_inline)) {
     if (m >= a.M || n >= a.N) return;
     if (part) {
-      float *to = part + m * a.N + n;
-      if (a.vec4) {
-        *(f32x4 *)to = f32x4{v[0], v[1], v[2], v[3]};
-      } else {
-#pragma unroll
-        for (int i = 0; i < 4; i++)
-          if (n + i < a.N) to[i] = v[i];
-      }
+      *(f32x4 *)(part + m * part_row + n) = f32x4{v[0], v[1], v[2], v[3]};
     } else {
       epilogue4<T, ACT>(a, m, (int)n, v);
     }
@@ -333,13 +304,12 @@ __global__ void __launch_bounds__(64 * (BM / WM) * (BN / WN)) gemm_kernel(const 
 }
 
 template <typename T, bool AK, bool BKIN, int ACT>
-void launch_tile(int tile, bool fast, const GemmArgs &a, hipStream_t s) {
+void launch_tile(int tile, const GemmArgs &a, hipStream_t s) {
   const dim3 grid(a.mtiles * a.ntiles, a.splits);
 #define GELIB_GEMM(BM, BN, WM, WN)                                                                                                                 \
   do {                                                                                                                                             \
     const dim3 block(64 * (BM / WM) * (BN / WN));                                                                                                  \
-    if (fast) hipLaunchKernelGGL((gemm_kernel<T, AK, BKIN, BM, BN, WM, WN, true, ACT>), grid, block, 0, s, a);                                     \
-    else hipLaunchKernelGGL((gemm_kernel<T, AK, BKIN, BM, BN, WM, WN, false, ACT>), grid, block, 0, s, a);                                         \
+    hipLaunchKernelGGL((gemm_kernel<T, AK, BKIN, BM, BN, WM, WN, ACT>), grid, block, 0, s, a);                                                     \
   } while (0)
   switch (tile) {
     case 0: GELIB_GEMM(256, 256, 128, 64); break;
@@ -351,15 +321,15 @@ void launch_tile(int tile, bool fast, const GemmArgs &a, hipStream_t s) {
 }
 
 template <typename T>
-int launch_gemm(GemmForm form, int tile, bool fast, const GemmArgs &a, hipStream_t s) {
+int launch_gemm(GemmForm form, int tile, const GemmArgs &a, hipStream_t s) {
   if (form == kFormXW) {
-    if (a.act == kActSilu) launch_tile<T, true, false, kActSilu>(tile, fast, a, s);
-    else if (a.act == kActGelu) launch_tile<T, true, false, kActGelu>(tile, fast, a, s);
-    else launch_tile<T, true, false, kActNone>(tile, fast, a, s);
+    if (a.act == kActSilu) launch_tile<T, true, false, kActSilu>(tile, a, s);
+    else if (a.act == kActGelu) launch_tile<T, true, false, kActGelu>(tile, a, s);
+    else launch_tile<T, true, false, kActNone>(tile, a, s);
   } else if (form == kFormGW) {
-    launch_tile<T, true, true, kActNone>(tile, fast, a, s);
+    launch_tile<T, true, true, kActNone>(tile, a, s);
   } else {
-    launch_tile<T, false, false, kActNone>(tile, fast, a, s);
+    launch_tile<T, false, false, kActNone>(tile, a, s);
   }
   const hipError_t e = hipGetLastError();
   return e == hipSuccess ? 0 : record_hip_error(e, "linear layer launch");

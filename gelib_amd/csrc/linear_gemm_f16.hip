@@ -2,5 +2,5 @@
 #include "linear_gemm.h"
 
 namespace gelib_hip {
-template int launch_gemm<half_t>(GemmForm, int, bool, const GemmArgs &, hipStream_t);
+template int launch_gemm<half_t>(GemmForm, int, const GemmArgs &, hipStream_t);
 }

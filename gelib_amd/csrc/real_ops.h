@@ -42,6 +42,7 @@ struct LinearArgs {
 size_t linear_workspace(int backward, int dtype, long long rows, int K, int N);   // backward: bits 1 gx, 2 gw, 4 gb, 8 slope; 0 forward
 int launch_linear_fwd(int dtype, const LinearArgs &a, hipStream_t s);
 int launch_linear_bwd(int dtype, const LinearArgs &a, hipStream_t s);
+int linear_act_set_option(const char *name, int value);
 
 // ---- AdamW (adamw.hip) ----
 constexpr int kAdamBlock = 256;   // elements that share a scale of 8-bit moments; parameters start at multiples of it

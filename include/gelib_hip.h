@@ -291,7 +291,8 @@ uint64_t gelib_hip_group_norm_act_workspace_bytes(int backward, int dtype, int64
                                                   int groups);
 
 /* Linear layer: z = x w + bias, y = act(z) + residual; x (rows, n_in) at a row stride, w (n_in, n_out) as the matrices of
- * SO3weights, bias (n_out) and residual (rows, n_out) may be NULL; y packed.  slope (NULL: not wanted; not written where act is
+ * SO3weights, bias (n_out) and residual (rows, n_out) may be NULL; y packed.  An operand whose rows are a multiple of 16 bytes
+ * long (x, w, gy) starts at one and has a row stride that is one (GELIB_HIP_ERR_ARG otherwise); others are copied to such rows.  slope (NULL: not wanted; not written where act is
  * GELIB_HIP_ACT_NONE): act'(z) for the backward pass, (rows, n_out) float32 for float32 layers and float16 for the others. */
 int gelib_hip_linear_act_fwd(void *y, void *slope, const void *x, const void *w, const void *bias, const void *residual, int dtype,
                              int64_t rows, int n_in, int n_out, int64_t x_row_stride, int act, void *workspace,
@@ -393,7 +394,8 @@ int gelib_hip_set_stream_workspace(void *stream, void *ptr, uint64_t bytes);
  * default), "bwd_lds_target" (LDS bytes per block the unrolled backward kernels aim at when they choose their cells per
  * block), "bwd_min_runs" (runs of 64 lane slots such a block should have at least, 0 = no such rule), "unrolled_bwd_l6" / "unrolled_fwd_l6" (1/0: the backward / forward kernels for operands up to l = 6),
  * "fwd_stream" / "diag6_stream" / "onepair_mfma_stream" (streaming stores of a product) and "bwd_once" / "diag6_once" / "onepair_mfma_once" (streaming
- * loads of its gradient; -1 by the shape, the default, 0 never, 1 always), "vec_mix" (the one launch that mixes all parts of a vector: -1 by the
+ * loads of its gradient; -1 by the shape, the default, 0 never, 1 always), "linear_act_tile" (-1: by the sizes; 0: 256 x 256, 1: 128 x 128, 2: 64 x 128, 3: 16 x 256 of a linear layer's products a block) and
+ * "linear_act_splits" (0: by the sizes; pieces that their sums are cut into), "vec_mix" (the one launch that mixes all parts of a vector: -1 by the
  * shape, the default, 0 only for parts that the matrix-core kernels do not take, 1 always), "onepair_mfma_pad" (1/0: the matrix-core
  * single-pair kernels at other channel counts up to 16 x 16 than those they are built for, and in rows that are not 16-byte aligned),
  * "staged_fwd_tile" (1, 2, 4), "staged_fwd_threads", "staged_fwd_coeffs_lds" (1/0), "staged_fwd_lds_target",
