@@ -3,8 +3,9 @@
 // with step_size = lr / (1 - b1^t), inv_sqrt_bc2 = (1 - b2^t)^-1/2; complex parameters are twice as many reals.
 //
 // Every parameter owns a run of the moment arrays that starts at a multiple of 256 elements; a block of 256 elements is what
-// one scale is kept for in 8 bits.  A wave owns such a block (4 elements a lane) and needs no other wave: the maximum is a
-// wavefront reduction.
+// one scale is kept for in 8 bits.  Half a wave owns such a block, 8 elements a lane in loads of up to 16 bytes, and needs nobody
+// else: the maximum is a reduction over 32 lanes.  The parameter that a wave works on is found by all lanes at once (one entry
+// of the table each).
 //
 // The 8-bit form works on the bits of float32 numbers.  u = (bits without the sign + r) >> 20 are the exponent and three bits of
 // the mantissa: eight steps an octave, and integers in the order of the values.  top = the largest u of a block (16 bits are
@@ -32,12 +33,13 @@ struct AdamTable {
     void *p;
     const void *g;
     long long n;
-    unsigned first, blocks_before;  // first block of moments, blocks of the launch before this parameter
+    unsigned first, waves_before;  // first block of moments, waves of the launch before this parameter
+    int aligned;                   // p and g start at multiples of 16 bytes
     float step_size, inv_sqrt_bc2;
     unsigned key;
   } t[kAdamTensors];
   int count;
-  unsigned blocks;
+  unsigned waves;
 };
 
 __device__ __forceinline__ unsigned mixed(unsigned index, unsigned key) {
@@ -51,9 +53,9 @@ __device__ __forceinline__ unsigned mixed_more(unsigned h) {
   return (h ^ (h >> 15)) & 0xffffu;
 }
 
-__device__ __forceinline__ int wave_max(int v) {
+__device__ __forceinline__ int half_wave_max(int v) {
 #pragma unroll
-  for (int d = 32; d >= 1; d >>= 1) v = max(v, __shfl_xor(v, d));
+  for (int d = 16; d >= 1; d >>= 1) v = max(v, __shfl_xor(v, d));
   return v;
 }
 
@@ -77,98 +79,152 @@ __device__ __forceinline__ int coded(float x, int u, int top, int steps) {
   return c >= 1 ? ((__float_as_uint(x) & 0x7fffffffu) ? c : 0) : ABOVE && (__float_as_uint(x) & 0x7fffffffu) ? 1 : 0;
 }
 
+constexpr int kAdamLane = 8;   // elements of a lane: 32 lanes a block
+
+template <typename T>
+__device__ __forceinline__ void load8(const T *p, bool whole, long long n, float *v) {
+  if (whole) {
+    T t[kAdamLane];
+    __builtin_memcpy(t, __builtin_assume_aligned(p, 16), sizeof(t));
+#pragma unroll
+    for (int i = 0; i < kAdamLane; i++) v[i] = to_f(t[i]);
+  } else {
+#pragma unroll
+    for (int i = 0; i < kAdamLane; i++) v[i] = i < n ? to_f(p[i]) : 0.f;
+  }
+}
+
 template <typename T, int BITS>
 __global__ void __launch_bounds__(256) adamw_kernel(const AdamTable tab, const AdamArgs a) {
-  const unsigned wave = blockIdx.x * 4 + threadIdx.x / 64, lane = threadIdx.x % 64;
-  if (wave >= tab.blocks) return;
-  int k = 0;
-  while (k + 1 < tab.count && wave >= tab.t[k + 1].blocks_before) k++;
-  const unsigned at = wave - tab.t[k].blocks_before;           // block of the parameter
-  const long long e0 = (long long)at * kAdamBlock + lane * 4;  // element of the parameter
-  const long long s0 = ((long long)tab.t[k].first + at) * kAdamBlock + lane * 4;
-  T *p = (T *)tab.t[k].p;
-  const T *g = (const T *)tab.t[k].g;
-  const long long n = tab.t[k].n;
-  const float step_size = tab.t[k].step_size, inv_sqrt_bc2 = tab.t[k].inv_sqrt_bc2;
-  const unsigned key = tab.t[k].key;
-  float m[4], v[4];
+  const unsigned lane = threadIdx.x % 64, wave = __builtin_amdgcn_readfirstlane(blockIdx.x * 4 + threadIdx.x / 64);
+  if (wave >= tab.waves) return;
+  const auto *t = (const AdamTable *)__builtin_amdgcn_kernarg_segment_ptr();
+  const int k = __popcll(__ballot((int)lane < tab.count && t->t[lane].waves_before <= wave)) - 1;
+  const auto &e = t->t[k];
+  const long long at = ((long long)(wave - e.waves_before) * 64 + lane) * kAdamLane;   // element of the parameter
+  const long long s0 = (long long)e.first * kAdamBlock + at;
+  const long long left = e.n - at;             // may be below zero: a lane whose elements pad the last block, or lie behind it
+  const bool own = at < (e.n + kAdamBlock - 1) / kAdamBlock * kAdamBlock;   // the moments are this parameter's
+  const bool whole = left >= kAdamLane && e.aligned;
+  T *p = (T *)e.p + at;
+  const T *g = (const T *)e.g + at;
+  float m[kAdamLane], v[kAdamLane], gr[kAdamLane], was[kAdamLane];
+  load8(g, whole, left, gr);
+  load8((const T *)p, whole, left, was);
+  int mt = 0, vt = 0;
   if (BITS == 32) {
-    for (int i = 0; i < 4; i++) m[i] = ((const float *)a.m)[s0 + i], v[i] = ((const float *)a.v)[s0 + i];
+    load8((const float *)a.m + s0, own, 0, m);
+    load8((const float *)a.v + s0, own, 0, v);
   } else {
-    const int mt = a.m_top[s0 / kAdamBlock], vt = a.v_top[s0 / kAdamBlock];
-    for (int i = 0; i < 4; i++) {
-      const int cm = ((const unsigned char *)a.m)[s0 + i], cv = ((const unsigned char *)a.v)[s0 + i];
-      m[i] = decoded(cm & 127, mt, 126, kNan);
-      if (cm & 128) m[i] = -m[i];
-      v[i] = decoded(cv, vt, 254, kInf);
+    uint2 cm = {}, cv = {};
+    if (own) {
+      cm = *(const uint2 *)((const char *)a.m + s0), cv = *(const uint2 *)((const char *)a.v + s0);
+      mt = a.m_top[s0 / kAdamBlock], vt = a.v_top[s0 / kAdamBlock];
+    }
+#pragma unroll
+    for (int i = 0; i < kAdamLane; i++) {
+      const int c = (i < 4 ? cm.x : cm.y) >> (i % 4 * 8) & 255, d = (i < 4 ? cv.x : cv.y) >> (i % 4 * 8) & 255;
+      m[i] = decoded(c & 127, mt, 126, kNan);
+      if (c & 128) m[i] = -m[i];
+      v[i] = decoded(d, vt, 254, kInf);
     }
   }
-  unsigned h[4];
-  for (int i = 0; i < 4; i++) {
-    const bool in = e0 + i < n;
-    const float gi = in ? to_f(g[e0 + i]) : 0.f;
-    m[i] = m[i] * a.b1 + gi * a.c1;
-    v[i] = v[i] * a.b2 + (gi * gi) * a.c2;
-    if (BITS == 8 || sizeof(T) == 2) h[i] = mixed((unsigned)(s0 + i), key + (unsigned)((s0 + i) >> 32) * 3144134277u);
-    if (in) {
-      const float denom = sqrtf(v[i]) * inv_sqrt_bc2 + a.eps;
-      const float was = to_f(p[e0 + i]);
-      const float np = (was - was * a.decay) - (m[i] * step_size) / denom;
-      if (sizeof(T) == 2) {
-        const unsigned b = __float_as_uint(np);
-        ((unsigned short *)p)[e0 + i] = (b & 0x7fffffffu) > kInf ? 0x7fc0 : (b & 0x7fffffffu) == kInf ? b >> 16 : (b + mixed_more(h[i])) >> 16;
-      } else {
-        p[e0 + i] = from_f<T>(np);
-      }
+  unsigned h[kAdamLane];
+  const unsigned key = e.key + (unsigned)(s0 >> 32) * 3144134277u;   // (a lane's eight elements share the upper half of their index)
+  float now[kAdamLane];
+#pragma unroll
+  for (int i = 0; i < kAdamLane; i++) {
+    m[i] = m[i] * a.b1 + gr[i] * a.c1;
+    v[i] = v[i] * a.b2 + (gr[i] * gr[i]) * a.c2;
+    if (BITS == 8 || sizeof(T) == 2) h[i] = mixed((unsigned)(s0 + i), key);
+    const float denom = sqrtf(v[i]) * e.inv_sqrt_bc2 + a.eps;
+    now[i] = (was[i] - was[i] * a.decay) - (m[i] * e.step_size) / denom;
+  }
+  T out[kAdamLane];
+#pragma unroll
+  for (int i = 0; i < kAdamLane; i++) {
+    if (sizeof(T) == 2) {
+      const unsigned b = __float_as_uint(now[i]), u = b & 0x7fffffffu;
+      const unsigned short r = u > kInf ? 0x7fc0 : u == kInf ? b >> 16 : (b + mixed_more(h[i])) >> 16;
+      __builtin_memcpy(&out[i], &r, 2);
+    } else {
+      __builtin_memcpy(&out[i], &now[i], sizeof(T));
     }
   }
-  if (BITS == 32) {
-    for (int i = 0; i < 4; i++) ((float *)a.m)[s0 + i] = m[i], ((float *)a.v)[s0 + i] = v[i];
+  if (whole) {
+    __builtin_memcpy(__builtin_assume_aligned(p, 16), out, sizeof(out));
   } else {
-    int um[4], uv[4], mt = 0, vt = 0;
-    for (int i = 0; i < 4; i++) {
+#pragma unroll
+    for (int i = 0; i < kAdamLane; i++)
+      if (i < left) p[i] = out[i];
+  }
+  if (BITS == 32) {
+    if (own) {
+      __builtin_memcpy(__builtin_assume_aligned((float *)a.m + s0, 16), m, sizeof(m));
+      __builtin_memcpy(__builtin_assume_aligned((float *)a.v + s0, 16), v, sizeof(v));
+    }
+  } else {
+    int um[kAdamLane], uv[kAdamLane];
+    mt = vt = 0;
+#pragma unroll
+    for (int i = 0; i < kAdamLane; i++) {
       um[i] = upper(m[i], h[i] & 0xfffffu), uv[i] = upper(v[i], h[i] >> 12);
       if (uv[i] < 0 && um[i] >= 0) m[i] = 0.f, um[i] = 0;   // v is infinite: its steps are zero whatever m is, and m as large as that
                                                             // would push the block's others below the smallest code
       mt = max(mt, um[i]), vt = max(vt, uv[i]);
     }
-    mt = wave_max(mt), vt = wave_max(vt);
-    for (int i = 0; i < 4; i++) {
-      const int c = coded<false>(m[i], um[i], mt, 126);
-      ((unsigned char *)a.m)[s0 + i] = c | (c && __float_as_uint(m[i]) >> 31 ? 128 : 0);
-      ((unsigned char *)a.v)[s0 + i] = coded<true>(v[i], uv[i], vt, 254);
+    mt = half_wave_max(mt), vt = half_wave_max(vt);
+    uint2 cm = {}, cv = {};
+#pragma unroll
+    for (int i = 0; i < kAdamLane; i++) {
+      const unsigned c = coded<false>(m[i], um[i], mt, 126), d = coded<true>(v[i], uv[i], vt, 254);
+      (i < 4 ? cm.x : cm.y) |= (c | (c && __float_as_uint(m[i]) >> 31 ? 128u : 0u)) << (i % 4 * 8);
+      (i < 4 ? cv.x : cv.y) |= d << (i % 4 * 8);
     }
-    if (lane == 0) a.m_top[s0 / kAdamBlock] = mt, a.v_top[s0 / kAdamBlock] = vt;
+    if (own) {
+      *(uint2 *)((char *)a.m + s0) = cm, *(uint2 *)((char *)a.v + s0) = cv;
+      if (lane % 32 == 0) a.m_top[s0 / kAdamBlock] = mt, a.v_top[s0 / kAdamBlock] = vt;
+    }
   }
 }
 
 // what 8-bit moments stand for, in bfloat16 (four significant bits: exact); n is a multiple of 256
 __global__ void __launch_bounds__(256) adamw_moments_kernel(unsigned short *mv, unsigned short *vv, const unsigned char *m, const unsigned char *v,
                                                             const short *mt, const short *vt, long long n) {
-  const long long i = (long long)blockIdx.x * 256 + threadIdx.x;
-  if (i >= n) return;
-  const float a = decoded(m[i] & 127, mt[i / kAdamBlock], 126, kNan), b = decoded(v[i], vt[i / kAdamBlock], 254, kInf);
-  mv[i] = __float_as_uint(m[i] & 128 ? -a : a) >> 16;
-  vv[i] = __float_as_uint(b) >> 16;
+  const long long s0 = ((long long)blockIdx.x * 256 + threadIdx.x) * kAdamLane;
+  if (s0 >= n) return;
+  const uint2 cm = *(const uint2 *)(m + s0), cv = *(const uint2 *)(v + s0);
+  const int tm = mt[s0 / kAdamBlock], tv = vt[s0 / kAdamBlock];
+  unsigned short a[kAdamLane], b[kAdamLane];
+#pragma unroll
+  for (int i = 0; i < kAdamLane; i++) {
+    const int c = (i < 4 ? cm.x : cm.y) >> (i % 4 * 8) & 255, d = (i < 4 ? cv.x : cv.y) >> (i % 4 * 8) & 255;
+    a[i] = __float_as_uint(decoded(c & 127, tm, 126, kNan)) >> 16 | (c & 128) << 8;
+    b[i] = __float_as_uint(decoded(d, tv, 254, kInf)) >> 16;
+  }
+  __builtin_memcpy(__builtin_assume_aligned(mv + s0, 16), a, 16);
+  __builtin_memcpy(__builtin_assume_aligned(vv + s0, 16), b, 16);
 }
 
 // 8-bit moments nearest to given values
 __global__ void __launch_bounds__(256) adamw_set_moments_kernel(unsigned char *m, unsigned char *v, short *m_top, short *v_top, const float *mv,
                                                                 const float *vv, long long n) {
-  const long long wave = (long long)blockIdx.x * 4 + threadIdx.x / 64, s0 = wave * kAdamBlock + threadIdx.x % 64 * 4;
-  if (s0 >= n) return;
-  int um[4], uv[4], mt = 0, vt = 0;
-  for (int i = 0; i < 4; i++) {
+  const long long s0 = ((long long)blockIdx.x * 256 + threadIdx.x) * kAdamLane;
+  if (s0 >= n) return;   // (half waves: n is a multiple of 256)
+  int um[kAdamLane], uv[kAdamLane], mt = 0, vt = 0;
+#pragma unroll
+  for (int i = 0; i < kAdamLane; i++) {
     um[i] = upper(mv[s0 + i], 1u << 19), uv[i] = upper(vv[s0 + i], 1u << 19);
     mt = max(mt, um[i]), vt = max(vt, uv[i]);
   }
-  mt = wave_max(mt), vt = wave_max(vt);
-  for (int i = 0; i < 4; i++) {
+  mt = half_wave_max(mt), vt = half_wave_max(vt);
+#pragma unroll
+  for (int i = 0; i < kAdamLane; i++) {
     const int c = coded<false>(mv[s0 + i], um[i], mt, 126);
     m[s0 + i] = c | (c && __float_as_uint(mv[s0 + i]) >> 31 ? 128 : 0);
     v[s0 + i] = coded<true>(vv[s0 + i], uv[i], vt, 254);
   }
-  if (threadIdx.x % 64 == 0) m_top[wave] = mt, v_top[wave] = vt;
+  if (threadIdx.x % 32 == 0) m_top[s0 / kAdamBlock] = mt, v_top[s0 / kAdamBlock] = vt;
 }
 
 int launched() {
@@ -183,7 +239,7 @@ int launch_adamw(int n, const AdamTensor *tensors, const AdamArgs &a, hipStream_
   std::memset(&tab, 0, sizeof(tab));
   auto flush = [&]() {
     if (tab.count == 0) return 0;
-    const dim3 grid((tab.blocks + 3) / 4);
+    const dim3 grid((tab.waves + 3) / 4);
     if (a.dtype == GELIB_HIP_F32) {
       if (a.bits == 32) hipLaunchKernelGGL((adamw_kernel<float, 32>), grid, dim3(256), 0, s, tab, a);
       else hipLaunchKernelGGL((adamw_kernel<float, 8>), grid, dim3(256), 0, s, tab, a);
@@ -191,7 +247,7 @@ int launch_adamw(int n, const AdamTensor *tensors, const AdamArgs &a, hipStream_
       if (a.bits == 32) hipLaunchKernelGGL((adamw_kernel<bhalf_t, 32>), grid, dim3(256), 0, s, tab, a);
       else hipLaunchKernelGGL((adamw_kernel<bhalf_t, 8>), grid, dim3(256), 0, s, tab, a);
     }
-    tab.count = 0, tab.blocks = 0;
+    tab.count = 0, tab.waves = 0;
     return launched();
   };
   // A launch has at most 2^26 waves (2^32 threads are HIP's limit), a larger parameter several.
@@ -200,14 +256,15 @@ int launch_adamw(int n, const AdamTensor *tensors, const AdamArgs &a, hipStream_
   for (int k = 0; k < n; k++)
     for (long long done = 0; done < tensors[k].n;) {
       const AdamTensor &from = tensors[k];
-      const long long left = from.n - done, now = std::min(left, most * kAdamBlock), blocks = (now + kAdamBlock - 1) / kAdamBlock;
-      if (tab.count == kAdamTensors || tab.blocks + blocks > most)
+      const long long left = from.n - done, now = std::min(left, most * 64 * kAdamLane), waves = (now + 64 * kAdamLane - 1) / (64 * kAdamLane);
+      if (tab.count == kAdamTensors || tab.waves + waves > most)
         if (int rc = flush()) return rc;
       auto &t = tab.t[tab.count];
       t.p = (char *)from.p + done * elem, t.g = (const char *)from.g + done * elem, t.n = now;
-      t.first = (unsigned)((from.first + done) / kAdamBlock), t.blocks_before = tab.blocks;
+      t.first = (unsigned)((from.first + done) / kAdamBlock), t.waves_before = tab.waves;
       t.step_size = from.step_size, t.inv_sqrt_bc2 = from.inv_sqrt_bc2, t.key = from.key;
-      tab.blocks += (unsigned)blocks;
+      t.aligned = ((uintptr_t)t.p | (uintptr_t)t.g) % 16 == 0;
+      tab.waves += (unsigned)waves;
       tab.count++;
       done += now;
     }
@@ -217,7 +274,7 @@ int launch_adamw(int n, const AdamTensor *tensors, const AdamArgs &a, hipStream_
 int launch_adamw_moments(void *mv, void *vv, const void *m, const void *v, const short *mt, const short *vt, long long n, hipStream_t s) {
   const long long most = 1LL << 31;   // elements of a launch
   for (long long i = 0; i < n; i += most)
-    hipLaunchKernelGGL(adamw_moments_kernel, dim3((unsigned)((std::min(n - i, most) + 255) / 256)), dim3(256), 0, s, (unsigned short *)mv + i,
+    hipLaunchKernelGGL(adamw_moments_kernel, dim3((unsigned)((std::min(n - i, most) / kAdamLane + 255) / 256)), dim3(256), 0, s, (unsigned short *)mv + i,
                        (unsigned short *)vv + i, (const unsigned char *)m + i, (const unsigned char *)v + i, mt + i / kAdamBlock,
                        vt + i / kAdamBlock, std::min(n - i, most));
   return launched();
@@ -226,7 +283,7 @@ int launch_adamw_moments(void *mv, void *vv, const void *m, const void *v, const
 int launch_adamw_set_moments(void *m, void *v, short *mt, short *vt, const float *mv, const float *vv, long long n, hipStream_t s) {
   const long long most = 1LL << 31;
   for (long long i = 0; i < n; i += most)
-    hipLaunchKernelGGL(adamw_set_moments_kernel, dim3((unsigned)((std::min(n - i, most) / kAdamBlock + 3) / 4)), dim3(256), 0, s,
+    hipLaunchKernelGGL(adamw_set_moments_kernel, dim3((unsigned)((std::min(n - i, most) / kAdamLane + 255) / 256)), dim3(256), 0, s,
                        (unsigned char *)m + i, (unsigned char *)v + i, mt + i / kAdamBlock, vt + i / kAdamBlock, mv + i, vv + i, std::min(n - i, most));
   return launched();
 }

@@ -184,8 +184,8 @@ int gelib_hip_adamw_step(int ntensors, void *const *p, const void *const *g, con
     if (n[k]) end = std::max(end, first[k] + (n[k] + kAdamBlock - 1) / kAdamBlock * kAdamBlock);
   }
   const unsigned s = state_bits / 8;
-  mem.need(m, end * s, 4);
-  mem.need(v, end * s, 4);
+  mem.need(m, end * s, 16);
+  mem.need(v, end * s, 16);
   if (state_bits == 8) mem.need(m_top, end / kAdamBlock * 2, 2), mem.need(v_top, end / kAdamBlock * 2, 2);
   if (int rc = mem.rc()) return rc;
   if (end == 0) return GELIB_HIP_OK;
@@ -221,8 +221,8 @@ static int check_moments(const void *mv, const void *vv, const void *m, const vo
   if (n < 0 || n % kAdamBlock) return GELIB_HIP_ERR_ARG;
   if (n > (1LL << 40)) return GELIB_HIP_ERR_ARG;
   Memory mem;
-  mem.need(mv, n * e, e), mem.need(vv, n * e, e);
-  mem.need(m, n, 4), mem.need(v, n, 4);
+  mem.need(mv, n * e, 16), mem.need(vv, n * e, 16);
+  mem.need(m, n, 16), mem.need(v, n, 16);
   mem.need(mt, n / kAdamBlock * 2, 2), mem.need(vt, n / kAdamBlock * 2, 2);
   return mem.rc();
 }

@@ -310,7 +310,7 @@ uint64_t gelib_hip_linear_act_workspace_bytes(int backward, int dtype, int64_t r
  *     m = beta1 m + (1 - beta1) g,  v = beta2 v + (1 - beta2) g^2,
  *     p = p (1 - lr weight_decay) - lr / (1 - beta1^t) m / (sqrt(v / (1 - beta2^t)) + eps),  t = step[k], from 1 on.
  * The moments of parameter k are elements first[k].. of the arrays m and v, first[k] a multiple of 256; runs do not overlap
- * and their unused ends are zero.  state_bits 32: float32 arrays, m_top and v_top NULL.  state_bits 8: a byte an element, and
+ * and their unused ends are zero.  All arrays of moments start at multiples of 16 bytes.  state_bits 32: float32 arrays, m_top and v_top NULL.  state_bits 8: a byte an element, and
  * m_top, v_top a 16-bit integer for every 256 elements: code c of v stands for the float whose bits are (c + top - 254) << 20
  * (0: zero, 255: not finite), code c of m for (c % 128 + top - 126) << 20 with sign c / 128 (0: zero, 127: not finite).  These
  * codes, and bfloat16 parameters, are rounded at random with bits that are a function of seed, step[k] and element alone. */
