@@ -91,8 +91,8 @@ __global__ void __launch_bounds__(256) join_kernel(const GemmArgs a, unsigned pe
   f32x4 s = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll 8
   for (int k = 0; k < a.splits; k++) s += *(const f32x4 *)(p + k * all);
-  const float v[4] = {s[0], s[1], s[2], s[3]};
-  epilogue4<T, ACT>(a, m, n, v);
+  const float v[1][4] = {{s[0], s[1], s[2], s[3]}};
+  epilogue<T, ACT, 1>(a, m, n, 0, v);
 }
 
 // bytes written for a result: the workspace is sized without knowing whether act' is kept, so it counts in every forward product
@@ -102,10 +102,9 @@ template <typename T>
 int product(GemmForm form, int dtype, GemmArgs a, float *part, hipStream_t s) {
   const Plan p = plan_of(dtype, a.M, a.N, a.K, out_bytes(form, dtype));
   const bool a_kin = form != kFormXG;
-  const bool vec4 = a.N % 4 == 0 && ((uintptr_t)a.c | (uintptr_t)a.res | (uintptr_t)a.slope) % (4 * sizeof(T)) == 0;
+  a.vec4 = a.N % 4 == 0 && ((uintptr_t)a.c | (uintptr_t)a.res | (uintptr_t)a.slope) % (4 * sizeof(T)) == 0;
   a.splits = p.splits, a.kper = p.kper;
   a.part = p.splits > 1 ? part : nullptr;
-  a.vec4 = vec4;
   a.ntiles = (unsigned)((a.N + kGemmBN[p.tile] - 1) / kGemmBN[p.tile]);
   // a launch takes 2^22 tiles at most (2^31 threads); further rows go to further launches
   const long long BM = kGemmBM[p.tile], most = std::max(1LL, (1LL << 22) / a.ntiles) * BM;

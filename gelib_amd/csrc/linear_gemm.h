@@ -9,7 +9,7 @@
 // lanes reads 4 rows of 16 values and each lane gets a column of 4), float32 by giving a lane the 4 neighbouring columns that one
 // 16-byte read delivers: fragment j of a lane belongs to column 4 r + j, and the epilogue goes by that.
 // The order of 16-byte pieces in a row of LDS is permuted (exclusive or with the row) so that the lanes of a read spread over the banks.
-// Two buffers: the next tile is on its way while this one is multiplied; one barrier a step.
+// Two buffers, one barrier a step, fragments read half a step ahead (below).
 //
 // The products are formed with B's fragment as the first operand, so that a lane's four results lie side by side in a row of C.
 #pragma once
@@ -22,7 +22,7 @@ struct GemmArgs {
   const void *a, *b;
   long long lda, ldb;       // elements between the rows in memory
   void *c;                  // (M, N) packed
-  const void *bias, *res;   // epilogue: c = act(sum + bias) + res, slope = act'(sum + bias); each may be null
+  const void *bias, *res;   // epilogue: c = act(bias + sum) + res, slope = act'(bias + sum); each may be null
   void *slope;
   float *part;              // [splits][M][N up to a multiple of 4] sums of the pieces of k instead of c, or null
   long long M, K, kper;     // kper: k of a piece, a multiple of the step
@@ -76,36 +76,37 @@ template <typename T, int R, bool KIN, int THREADS, int G>
 struct Stage {
   static constexpr int VEC = 16 / sizeof(T), BK = 128 / sizeof(T);
   static constexpr int CPR = KIN ? 8 : R * (int)sizeof(T) / 16;          // 16-byte pieces of a row in LDS
-  static constexpr int NL = (R * 8 + THREADS - 1) / THREADS;
-  const T *p[NL];
-  long long mn[NL];
-  int k[NL];
-  long long step;
-
+  static constexpr int PIECES = R * 8, NL = (PIECES + THREADS - 1) / THREADS, DOWN = THREADS / CPR;   // DOWN: rows between a thread's pieces
+  // a thread's pieces lie in one column of the permuted tile
+  static_assert(NL == 1 || (KIN ? DOWN / G % 8 == 0 && DOWN % G == 0 : DOWN % 4 == 0), "");
+  const char *p;       // its first piece of the tile to come
+  long long down, step;
+  int k, mn;           // k of that piece in the tile; rows (KIN) or columns of the matrix from it on
   static __device__ __forceinline__ int swizzle(int row) {
     if (KIN) return (row / G) & 7;
-    return sizeof(T) == 2 ? ((row & 3) << 1) & (CPR - 1) : 0;
+    // 16 lanes read 32 bytes of four neighbouring k, and the next 16 of the four k that are 8 further on: eight places of 256 bytes
+    // (without the second term every transposing read took twice its time: 25 % more LDS cycles in x w, 100 % in x^T gz)
+    return sizeof(T) == 2 ? ((row & 3) << 1 | (CPR >= 16 && DOWN % 16 == 0 ? (row & 8) : 0)) & (CPR - 1) : 0;
   }
   __device__ __forceinline__ void init(const void *base, long long ld, long long mn0, long long MN, long long k0) {
-#pragma unroll
-    for (int u = 0; u < NL; u++) {
-      const int L = u * THREADS + threadIdx.x, row = L / CPR, c = (L % CPR) ^ swizzle(row);
-      mn[u] = mn0 + (KIN ? row : c * VEC);
-      k[u] = KIN ? c * VEC : row;
-      if (mn[u] >= MN) mn[u] = -1;
-      p[u] = (const T *)base + (KIN ? mn[u] * ld + k0 + k[u] : (k0 + k[u]) * ld + mn[u]);
-    }
-    step = KIN ? BK : BK * ld;
+    const int row = threadIdx.x / CPR, c = (threadIdx.x % CPR) ^ swizzle(row);
+    const long long at = mn0 + (KIN ? row : c * VEC);
+    k = KIN ? c * VEC : row;
+    mn = (int)max(0LL, min(MN - at, 1LL << 30));
+    p = (const char *)((const T *)base + (KIN ? at * ld + k0 + k : (k0 + k) * ld + at));
+    down = DOWN * ld * (long long)sizeof(T);
+    step = (KIN ? BK : BK * ld) * (long long)sizeof(T);
   }
-  // the tile whose first k has `left` more of it behind (k0 .. k0 + left)
+  // the next tile, of which `left` k are there
   __device__ __forceinline__ void issue(char *lds, long long left) {
+    const int have = (int)min(left, (long long)BK);
 #pragma unroll
     for (int u = 0; u < NL; u++) {
-      if (R * 8 % THREADS != 0 && u * THREADS + threadIdx.x >= R * 8) continue;   // (whole waves)
-      const bool in = mn[u] >= 0 && k[u] < left;
-      load_to_lds(in ? (const char *)p[u] : (const char *)gemm_zeros, lds + (u * THREADS + (threadIdx.x & ~63)) * 16);
-      p[u] += step;
+      if (PIECES % THREADS != 0 && u * THREADS + threadIdx.x >= PIECES) continue;   // (whole waves)
+      const bool in = KIN ? u * DOWN < mn && k < have : mn > 0 && k + u * DOWN < have;
+      load_to_lds(in ? p + u * down : (const char *)gemm_zeros, lds + (u * THREADS + (threadIdx.x & ~63)) * 16);
     }
+    p += step;
   }
   // 16-bit: the fragment of 16 rows from row0 on, k = ks * 32 + (lane / 16) * 8 + 0..7
   static __device__ __forceinline__ s16x8 frag16(const char *lds, int row0, int ks) {
@@ -144,44 +145,58 @@ struct Stage {
   }
 };
 
-// four neighbouring results of a row
-template <typename T, int ACT>
-__device__ __forceinline__ void epilogue4(const GemmArgs &a, long long m, int n, const float *v) {
+// `count` vectors of four neighbouring results, `apart` columns from one to the next.  All of y is written before all of the
+// slopes: a line of either is then whole in the L2 when it leaves (written in turn, 16384 x 8192 results and slopes were 1.01 GB of
+// writes instead of 0.54).
+template <typename T, int ACT, int COUNT>
+__device__ __forceinline__ void epilogue(const GemmArgs &a, long long m, long long n0, int apart, const float (*v)[4]) {
   typedef typename SlopeOf<T>::type D;
-  const long long at = m * a.N + n;
+  const long long row = m * a.N;
   if (a.vec4) {
-    T t[4];
-    D d[4];
-    float b[4] = {0.f, 0.f, 0.f, 0.f}, r[4] = {0.f, 0.f, 0.f, 0.f};
-    if (a.bias) {
-      __builtin_memcpy(t, (const T *)a.bias + n, sizeof(t));
-#pragma unroll
-      for (int i = 0; i < 4; i++) b[i] = to_f(t[i]);
-    }
+    if (n0 >= a.N) return;
+    T t[COUNT][4];
+    D d[COUNT][4];
     if (a.res) {
-      __builtin_memcpy(t, __builtin_assume_aligned((const T *)a.res + at, sizeof(t)), sizeof(t));
 #pragma unroll
-      for (int i = 0; i < 4; i++) r[i] = to_f(t[i]);
+      for (int k = 0; k < COUNT; k++) {   // (a vector behind the row reads the first one again)
+        const long long n = n0 + k * apart < a.N ? n0 + k * apart : n0;
+        __builtin_memcpy(t[k], __builtin_assume_aligned((const T *)a.res + row + n, 4 * sizeof(T)), 4 * sizeof(T));
+      }
+    } else {
+#pragma unroll
+      for (int k = 0; k < COUNT; k++)
+#pragma unroll
+        for (int i = 0; i < 4; i++) t[k][i] = (T)0.f;
     }
 #pragma unroll
-    for (int i = 0; i < 4; i++) {
-      float y, s;
-      act_both<ACT>(v[i] + b[i], y, s, a.act == kActRelu);
-      t[i] = from_f<T>(y + r[i]);
-      d[i] = from_f<D>(s);
-    }
-    __builtin_memcpy(__builtin_assume_aligned((T *)a.c + at, sizeof(t)), t, sizeof(t));
-    if (a.slope) __builtin_memcpy(__builtin_assume_aligned((D *)a.slope + at, sizeof(d)), d, sizeof(d));
+    for (int k = 0; k < COUNT; k++)
+#pragma unroll
+      for (int i = 0; i < 4; i++) {
+        float y, s;
+        act_both<ACT>(v[k][i], y, s, a.act == kActRelu);
+        t[k][i] = from_f<T>(y + to_f(t[k][i]));
+        d[k][i] = from_f<D>(s);
+      }
+#pragma unroll
+    for (int k = 0; k < COUNT; k++)
+      if (n0 + k * apart < a.N) __builtin_memcpy(__builtin_assume_aligned((T *)a.c + row + n0 + k * apart, 4 * sizeof(T)), t[k], 4 * sizeof(T));
+    if (a.slope)
+#pragma unroll
+      for (int k = 0; k < COUNT; k++)
+        if (n0 + k * apart < a.N) __builtin_memcpy(__builtin_assume_aligned((D *)a.slope + row + n0 + k * apart, 4 * sizeof(D)), d[k], 4 * sizeof(D));
     return;
   }
 #pragma unroll
-  for (int i = 0; i < 4; i++) {
-    if (n + i >= a.N) break;
-    float y, s;
-    act_both<ACT>(v[i] + (a.bias ? to_f(((const T *)a.bias)[n + i]) : 0.f), y, s, a.act == kActRelu);
-    ((T *)a.c)[at + i] = from_f<T>(y + (a.res ? to_f(((const T *)a.res)[at + i]) : 0.f));
-    if (a.slope) ((D *)a.slope)[at + i] = from_f<D>(s);
-  }
+  for (int k = 0; k < COUNT; k++)
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+      const long long n = n0 + k * apart + i;
+      if (n >= a.N) break;
+      float y, s;
+      act_both<ACT>(v[k][i], y, s, a.act == kActRelu);
+      ((T *)a.c)[row + n] = from_f<T>(y + (a.res ? to_f(((const T *)a.res)[row + n]) : 0.f));
+      if (a.slope) ((D *)a.slope)[row + n] = from_f<D>(s);
+    }
 }
 
 template <typename T, bool AK, bool BKIN, int BM, int BN, int WM, int WN, int ACT>
@@ -202,11 +217,22 @@ __global__ void __launch_bounds__(64 * (BM / WM) * (BN / WN)) gemm_kernel(const 
   const long long k0 = blockIdx.y * a.kper, k1 = min(k0 + a.kper, a.K);
   const int wave = threadIdx.x / 64, wm = wave % (BM / WM) * WM, wn = wave / (BM / WM) * WN;
 
+  // sums begin with the bias (of the first piece of k)
   f32x4 acc[FM][FN];
+  const int lane = threadIdx.x % 64, c = lane % 16, q = lane / 16;
 #pragma unroll
-  for (int i = 0; i < FM; i++)
+  for (int j = 0; j < FN; j++) {
+    f32x4 b = {0.f, 0.f, 0.f, 0.f};
+    if (a.bias && blockIdx.y == 0) {
 #pragma unroll
-    for (int j = 0; j < FN; j++) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
+      for (int e = 0; e < 4; e++) {
+        const long long n = n0 + wn + j / GN * GN * 16 + (q * 4 + e) * GN + j % GN;
+        b[e] = to_f(((const T *)a.bias)[n < a.N ? n : a.N - 1]);
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < FM; i++) acc[i][j] = b;
+  }
 
   SA sa;
   SB sb;
@@ -218,87 +244,109 @@ __global__ void __launch_bounds__(64 * (BM / WM) * (BN / WN)) gemm_kernel(const 
     sb.issue(lds[buf] + BM * 128, left);
     left -= BK;
   };
-  auto arrive = [&]() __attribute__((always_inline)) {
-    asm volatile("s_waitcnt vmcnt(0)" : : : "memory");   // what this wave has copied into LDS is there
-    __syncthreads();
+  // the fragments of half a step, and their products
+  struct Half {
+    s16x8 a16[sizeof(T) == 2 ? FM : 1], b16[sizeof(T) == 2 ? FN : 1];
+    float a32[sizeof(T) == 4 ? FM : 1][4], b32[sizeof(T) == 4 ? FN : 1][4];
   };
-  const int steps = left > 0 ? (int)((left + BK - 1) / BK) : 0;
-  if (steps) {
-    issue(0);
-    arrive();
-  }
-  for (int t = 0, buf = 0; t < steps; t++, buf ^= 1) {
-    const bool more = t + 1 < steps;
-    if (more) issue(buf ^ 1);
+  auto read = [&](Half &h, int buf, int ks) __attribute__((always_inline)) {
     const char *la = lds[buf], *lb = lds[buf] + BM * 128;
     if constexpr (sizeof(T) == 2) {
 #pragma unroll
-      for (int ks = 0; ks < 2; ks++) {
-        s16x8 fa[FM], fb[FN];
+      for (int j = 0; j < FN; j++) h.b16[j] = SB::frag16(lb, wn + j * 16, ks);
 #pragma unroll
-        for (int i = 0; i < FM; i++) fa[i] = SA::frag16(la, wm + i * 16, ks);
+      for (int i = 0; i < FM; i++) h.a16[i] = SA::frag16(la, wm + i * 16, ks);
+    } else {
 #pragma unroll
-        for (int j = 0; j < FN; j++) fb[j] = SB::frag16(lb, wn + j * 16, ks);
+      for (int j = 0; j < FN; j += GN) SB::frag32(lb, wn + j * 16, ks, h.b32 + j);
+#pragma unroll
+      for (int i = 0; i < FM; i += GM) SA::frag32(la, wm + i * 16, ks, h.a32 + i);
+    }
+    if (sizeof(T) == 2) __builtin_amdgcn_sched_barrier(0);   // (asked for before the products that they are read beside)
+  };
+  auto multiply = [&](const Half &h) __attribute__((always_inline)) {
+    if constexpr (sizeof(T) == 2) {
+#pragma unroll
+      for (int i = 0; i < FM; i++)
+#pragma unroll
+        for (int j = 0; j < FN; j++) acc[i][j] = mfma(h.b16[j], h.a16[i], acc[i][j], T());
+    } else {
+#pragma unroll
+      for (int k = 0; k < 4; k++)
 #pragma unroll
         for (int i = 0; i < FM; i++)
 #pragma unroll
-          for (int j = 0; j < FN; j++) acc[i][j] = mfma(fb[j], fa[i], acc[i][j], T());
-      }
-    } else {
-#pragma unroll
-      for (int ks = 0; ks < 2; ks++) {
-        float fa[FM][4], fb[FN][4];
-#pragma unroll
-        for (int i = 0; i < FM; i += GM) SA::frag32(la, wm + i * 16, ks, fa + i);
-#pragma unroll
-        for (int j = 0; j < FN; j += GN) SB::frag32(lb, wn + j * 16, ks, fb + j);
-#pragma unroll
-        for (int k = 0; k < 4; k++)
-#pragma unroll
-          for (int i = 0; i < FM; i++)
-#pragma unroll
-            for (int j = 0; j < FN; j++) acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x4f32(fb[j][k], fa[i][k], acc[i][j], 0, 0, 0);
-      }
+          for (int j = 0; j < FN; j++) acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x4f32(h.b32[j][k], h.a32[i][k], acc[i][j], 0, 0, 0);
     }
-    if (more) arrive();
+    if (sizeof(T) == 2) __builtin_amdgcn_sched_barrier(0);
+  };
+  auto arrive = [&]() __attribute__((always_inline)) {
+    asm volatile("s_waitcnt vmcnt(0)" : : : "memory");   // what this wave has copied into LDS is there, and read from there
+    __syncthreads();
+  };
+  // Half a step is multiplied while the fragments of the next half are on their way from LDS.  The barrier of a step lies between
+  // its halves: everybody holds all of this tile then, so its buffer is free for the tile after next, and the next tile, asked for a
+  // whole step ago, is there.
+  const int steps = left > 0 ? (int)((left + BK - 1) / BK) : 0;
+  // (float32: a half is 1024 cycles of products to one LDS latency; the compiler's own order of reads and products is better there by
+  // 2 to 40 %.)
+  if constexpr (sizeof(T) == 4) {
+    Half h;
+    if (steps) {
+      issue(0);
+      arrive();
+    }
+    for (int t = 0; t < steps; t++) {
+      if (t + 1 < steps) issue((t + 1) & 1);
+      read(h, t & 1, 0);
+      multiply(h);
+      read(h, t & 1, 1);
+      multiply(h);
+      if (t + 1 < steps) arrive();
+    }
+  } else if (steps) {
+    Half h0, h1;
+    issue(0);
+    arrive();
+    if (steps > 1) issue(1);
+    read(h0, 0, 0);
+    for (int t = 0; t < steps; t++) {
+      read(h1, t & 1, 1);
+      multiply(h0);
+      if (t + 1 < steps) {
+        arrive();
+        if (t + 2 < steps) issue(t & 1);
+        read(h0, (t + 1) & 1, 0);
+      }
+      multiply(h1);
+    }
   }
 
-  const int lane = threadIdx.x % 64, c = lane % 16, q = lane / 16;
   const long long part_row = (a.N + 3) & ~3;
   float *part = a.part ? a.part + (long long)blockIdx.y * a.M * part_row : nullptr;
-  auto out = [&](long long m, long long n, const float *v) __attribute__((always_inline)) {
-    if (m >= a.M || n >= a.N) return;
-    if (part) {
-      *(f32x4 *)(part + m * part_row + n) = f32x4{v[0], v[1], v[2], v[3]};
-    } else {
-      epilogue4<T, ACT>(a, m, (int)n, v);
-    }
-  };
 #pragma unroll
   for (int i = 0; i < FM; i++) {
     const long long m = m0 + wm + (i / GM * GM) * 16 + c * GM + i % GM;
-    if (sizeof(T) == 2 || GN == 1) {
+    if (m >= a.M) continue;
 #pragma unroll
-      for (int j = 0; j < FN; j++) {
-        const float v[4] = {acc[i][j][0], acc[i][j][1], acc[i][j][2], acc[i][j][3]};
-        out(m, n0 + wn + j * 16 + q * 4, v);
+    for (int j = 0; j < FN; j += 4 < FN ? 4 : FN) {
+      // the vectors that a lane holds of four fragments (or of all): 4 q + 0..3 of each (16 bits), or columns G e + 0..G - 1, e = 4 q + 0..3,
+      // of the columns that they share
+      constexpr int COUNT = FN < 4 ? FN : 4;
+      float v[COUNT][4];
+      const int apart = GN == 1 ? 16 : 4;
+      const long long n = n0 + wn + j * 16 + (GN == 1 ? q * 4 : q * 4 * GN);
+#pragma unroll
+      for (int k = 0; k < COUNT; k++)
+#pragma unroll
+        for (int e = 0; e < 4; e++) v[k][e] = GN == 1 ? acc[i][j + k][e] : acc[i][j + (4 * k + e) % GN][(4 * k + e) / GN];
+      if (part) {
+#pragma unroll
+        for (int k = 0; k < COUNT; k++)
+          if (n + k * apart < a.N) *(f32x4 *)(part + m * part_row + n + k * apart) = f32x4{v[k][0], v[k][1], v[k][2], v[k][3]};
+      } else {
+        epilogue<T, ACT, COUNT>(a, m, n, apart, v);
       }
-    } else if constexpr (GN == 4) {
-#pragma unroll
-      for (int j = 0; j < FN; j += GN)
-#pragma unroll
-        for (int e = 0; e < 4; e++) {
-          const float v[4] = {acc[i][j][e], acc[i][(j + 1) % FN][e], acc[i][(j + 2) % FN][e], acc[i][(j + 3) % FN][e]};
-          out(m, n0 + wn + j * 16 + q * 16 + e * 4, v);
-        }
-    } else {   // two columns a lane: elements 2 e, 2 e + 1
-#pragma unroll
-      for (int j = 0; j < FN; j += GN)
-#pragma unroll
-        for (int e = 0; e < 4; e += 2) {
-          const float v[4] = {acc[i][j][e], acc[i][(j + 1) % FN][e], acc[i][j][e + 1], acc[i][(j + 1) % FN][e + 1]};
-          out(m, n0 + wn + j * 16 + q * 8 + e * 2, v);
-        }
     }
   }
 }
