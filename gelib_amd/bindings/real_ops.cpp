@@ -41,6 +41,7 @@ void on_gpu(const at::Tensor &x) {
 
 // t packed, and from a multiple of 16 bytes on
 at::Tensor plain(const at::Tensor &t) {
+  if (!t.is_neg() && t.is_contiguous() && (t.numel() == 0 || (uintptr_t)t.data_ptr() % 16 == 0)) return t;   // (no dispatch)
   const at::Tensor p = t.resolve_neg().contiguous();
   return p.numel() && (uintptr_t)p.data_ptr() % 16 ? p.clone() : p;
 }
@@ -77,7 +78,7 @@ struct NormShape {
 };
 NormShape norm_shape(const at::Tensor &t) {
   NormShape r;
-  r.x = t.resolve_neg();
+  r.x = t.is_neg() ? t.resolve_neg() : t;
   const int64_t d = t.dim();
   r.N = t.size(0), r.C = (int)t.size(d - 1), r.S = 1;
   for (int64_t k = 1; k < d - 1; k++) r.S *= t.size(k);
@@ -118,7 +119,7 @@ void norm_check(const at::Tensor &x, int64_t groups, const Maybe &w, const Maybe
   }
 }
 
-std::tuple<at::Tensor, at::Tensor, at::Tensor> norm_fwd(const at::Tensor &x, int64_t groups, const Maybe &w, const Maybe &b, double eps,
+std::tuple<at::Tensor, at::Tensor> norm_fwd(const at::Tensor &x, int64_t groups, const Maybe &w, const Maybe &b, double eps,
                                                         const std::string &act, const Maybe &lengths, bool keep) {
   norm_check(x, groups, w, b, lengths);
   const int a = act_of(act);
@@ -126,19 +127,16 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor> norm_fwd(const at::Tensor &x, int
   OnDevice on(x);
   NormShape s = norm_shape(x);
   at::Tensor W = w ? plain(*w) : at::Tensor(), B = b ? plain(*b) : at::Tensor(), L = lengths ? lengths->contiguous() : at::Tensor();
-  at::Tensor y = at::empty(x.sizes(), x.options().memory_format(at::MemoryFormat::Contiguous)), mean, rstd;
-  if (keep) {
-    const at::Tensor both = at::empty({2, s.N, groups}, x.options().dtype(at::kFloat));
-    mean = both[0], rstd = both[1];
-  }
+  at::Tensor y = at::empty(x.sizes(), x.options().memory_format(at::MemoryFormat::Contiguous)), stats;
+  if (keep) stats = at::empty({2, s.N, groups}, x.options().dtype(at::kFloat));   // mean, rstd
   const uint64_t bytes = gelib_hip_group_norm_act_workspace_bytes(0, type_of(x), s.N, s.S, s.C, (int)groups);
   at::Tensor ws = workspace(bytes, x);
-  done(gelib_hip_group_norm_act_fwd(ptr(y), (float *)ptr(mean), (float *)ptr(rstd), ptr(s.x), ptr(W), ptr(B), (int32_t *)ptr(L), type_of(x), s.N, s.S,
+  done(gelib_hip_group_norm_act_fwd(ptr(y), (float *)ptr(stats), ptr(stats) ? (float *)ptr(stats) + s.N * groups : nullptr, ptr(s.x), ptr(W), ptr(B), (int32_t *)ptr(L), type_of(x), s.N, s.S,
                                     s.C, (int)groups, s.xs, s.xp, (float)eps, a, ptr(ws), bytes, on.stream));
-  return {y, mean, rstd};
+  return {y, stats};
 }
 
-std::tuple<at::Tensor, at::Tensor, at::Tensor> norm_bwd(const at::Tensor &gy_, const at::Tensor &mean, const at::Tensor &rstd, const at::Tensor &x, int64_t groups,
+std::tuple<at::Tensor, at::Tensor, at::Tensor> norm_bwd(const at::Tensor &gy_, const at::Tensor &stats, const at::Tensor &x, int64_t groups,
                                          const Maybe &w, const Maybe &b, int act, const Maybe &lengths, bool need_x, bool need_w,
                                          bool need_b) {
   norm_check(x, groups, w, b, lengths);
@@ -152,7 +150,7 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor> norm_bwd(const at::Tensor &gy_, c
              gb = need_b ? at::empty({s.C}, packed) : at::Tensor();
   const uint64_t bytes = gelib_hip_group_norm_act_workspace_bytes(1, type_of(x), s.N, s.S, s.C, (int)groups);
   at::Tensor ws = workspace(bytes, x);
-  done(gelib_hip_group_norm_act_bwd(ptr(gx), ptr(gw), ptr(gb), ptr(gy), (float *)ptr(mean), (float *)ptr(rstd), ptr(s.x), ptr(W), ptr(B), (int32_t *)ptr(L),
+  done(gelib_hip_group_norm_act_bwd(ptr(gx), ptr(gw), ptr(gb), ptr(gy), (float *)ptr(stats), ptr(stats) ? (float *)ptr(stats) + s.N * groups : nullptr, ptr(s.x), ptr(W), ptr(B), (int32_t *)ptr(L),
                                     type_of(x), s.N, s.S, s.C, (int)groups, s.xs, s.xp, act, ptr(ws), bytes, on.stream));
   return {gx, gw, gb};
 }
@@ -206,28 +204,27 @@ bool needs(const at::Tensor &t) { return t.defined() && t.requires_grad(); }
 struct NormFn : torch::autograd::Function<NormFn> {
   static at::Tensor forward(AutogradContext *ctx, const at::Tensor &x, const Maybe &w, const Maybe &b, int64_t groups, double eps, const std::string &act,
                             const Maybe &lengths) {
-    auto [y, mean, rstd] = norm_fwd(x, groups, w, b, eps, act, lengths, true);
-    ctx->save_for_backward({x, some(w), some(b), some(lengths), mean, rstd});
-    ctx->saved_data["how"] = std::tuple<int64_t, double, int64_t>(groups, eps, act_of(act));
+    auto [y, stats] = norm_fwd(x, groups, w, b, eps, act, lengths, true);
+    ctx->save_for_backward({x, some(w), some(b), some(lengths), stats});
+    ctx->saved_data["how"] = groups * 4 + act_of(act);
+    ctx->saved_data["eps"] = eps;
     return y;
   }
   static variable_list backward(AutogradContext *ctx, variable_list g) {
     const variable_list saved = ctx->get_saved_variables();
     const at::Tensor &x = saved[0], &w = saved[1], &b = saved[2], &lengths = saved[3];
-    const auto how = ctx->saved_data["how"].to<std::tuple<int64_t, double, int64_t>>();
-    const auto [groups, eps, act] = how;
+    const int64_t how = ctx->saved_data["how"].toInt(), groups = how / 4, act = how % 4;
     variable_list grads(7);
     if (!g[0].defined()) return grads;
     if (at::GradMode::is_enabled()) {   // a graph of the gradients is wanted
-      const int64_t G = groups, A = act;
-      const double e = eps;
-      const variable_list got = graph_grads([&](const variable_list &v) { return norm_from_torch(v[0], v[1], v[2], lengths, G, e, A); }, {x, w, b}, g[0]);
+      const double eps = ctx->saved_data["eps"].toDouble();
+      const variable_list got = graph_grads([&](const variable_list &v) { return norm_from_torch(v[0], v[1], v[2], lengths, groups, eps, act); }, {x, w, b}, g[0]);
       std::copy(got.begin(), got.end(), grads.begin());
       return grads;
     }
     size_t at = 0;   // (tensors that were given are counted)
     const bool need_x = ctx->needs_input_grad(at), need_w = w.defined() && ctx->needs_input_grad(++at), need_b = b.defined() && ctx->needs_input_grad(++at);
-    auto [gx, gw, gb] = norm_bwd(g[0], saved[4], saved[5], x, groups, some(w), some(b), (int)act, some(lengths), need_x, need_w, need_b);
+    auto [gx, gw, gb] = norm_bwd(g[0], saved[4], x, groups, some(w), some(b), (int)act, some(lengths), need_x, need_w, need_b);
     grads[0] = gx, grads[1] = gw, grads[2] = gb;
     return grads;
   }
@@ -250,7 +247,7 @@ struct Rows {   // x as rows: itself where they are evenly spaced, contiguous an
 };
 Rows rows_of(const at::Tensor &t) {
   Rows r;
-  r.x = t.resolve_neg();
+  r.x = t.is_neg() ? t.resolve_neg() : t;
   const int64_t d = t.dim();
   r.K = (int)t.size(d - 1), r.rows = 1;
   bool even = t.stride(d - 1) == 1 || r.K == 1;
@@ -337,19 +334,18 @@ struct LinearFn : torch::autograd::Function<LinearFn> {
   static at::Tensor forward(AutogradContext *ctx, const at::Tensor &x, const at::Tensor &w, const Maybe &b, const Maybe &r, const std::string &act) {
     auto [y, slope] = linear_fwd(x, w, b, r, act, true);
     ctx->save_for_backward({x, w, some(b), slope});
-    ctx->saved_data["how"] = std::tuple<int64_t, bool>(act_of(act), r.has_value());
+    ctx->saved_data["how"] = (int64_t)(act_of(act) * 2 + r.has_value());
     return y;
   }
   static variable_list backward(AutogradContext *ctx, variable_list g) {
     const variable_list saved = ctx->get_saved_variables();
     const at::Tensor &x = saved[0], &w = saved[1], &b = saved[2];
-    const auto how = ctx->saved_data["how"].to<std::tuple<int64_t, bool>>();
-    const int64_t act = std::get<0>(how);
+    const int64_t how = ctx->saved_data["how"].toInt(), act = how / 2;
     variable_list grads(5);
     if (!g[0].defined()) return grads;
     size_t at = 1;
     const bool need_x = ctx->needs_input_grad(0), need_w = ctx->needs_input_grad(1), need_b = b.defined() && ctx->needs_input_grad(++at),
-               need_r = std::get<1>(how) && ctx->needs_input_grad(++at);
+               need_r = how % 2 && ctx->needs_input_grad(++at);
     if (need_r) grads[3] = g[0];
     if (!need_x && !need_w && !need_b) return grads;
     if (at::GradMode::is_enabled()) {   // a graph of the gradients is wanted

@@ -15,8 +15,8 @@ int g_linear_tile = -1, g_linear_splits = 0;   // options: -1 and 0 leave the ch
 }
 
 int linear_act_set_option(const char *name, int value) {
-  if (!std::strcmp(name, "linear_act_tile")) g_linear_tile = value;
-  else if (!std::strcmp(name, "linear_act_splits")) g_linear_splits = value;
+  if (!std::strcmp(name, "linear_act_tile") && value >= -1 && value < kGemmTiles) g_linear_tile = value;
+  else if (!std::strcmp(name, "linear_act_splits") && value >= 0 && value <= 64) g_linear_splits = value;
   else return GELIB_HIP_ERR_ARG;
   return GELIB_HIP_OK;
 }
@@ -40,8 +40,8 @@ struct TileCost {
   double alone, full;
   int fit;
 };
-constexpr TileCost kCost16[kGemmTiles] = {{1.55, 2.0, 1}, {0.83, 0.57, 2}, {0.63, 0.32, 3}, {0.68, 0.34, 2}};
-constexpr TileCost kCost32[kGemmTiles] = {{7.5, 8.2, 1}, {2.2, 2.08, 2}, {1.27, 1.12, 3}, {0.94, 0.7, 2}};
+constexpr TileCost kCost16[kGemmTiles] = {{1.55, 2.0, 1}, {0.83, 0.57, 2}, {0.6, 0.34, 2}, {0.68, 0.34, 2}};
+constexpr TileCost kCost32[kGemmTiles] = {{7.5, 8.2, 1}, {2.2, 2.08, 2}, {1.2, 1.09, 2}, {0.94, 0.7, 2}};
 
 Plan plan_of(int dtype, long long M, long long N, long long K, int out) {
   const int bk = dtype == GELIB_HIP_F32 ? 32 : 64;
@@ -50,18 +50,18 @@ Plan plan_of(int dtype, long long M, long long N, long long K, int out) {
   Plan best = {};
   double least = 0;
   for (int t = 0; t < kGemmTiles; t++) {
-    if (g_linear_tile >= 0 && g_linear_tile < kGemmTiles && t != g_linear_tile) continue;
+    if (g_linear_tile >= 0 && t != g_linear_tile) continue;
     const TileCost &c = dtype == GELIB_HIP_F32 ? kCost32[t] : kCost16[t];
     const double tiles = std::ceil((double)M / kGemmBM[t]) * std::ceil((double)N / kGemmBN[t]);
-    for (long long want = 1; want <= 64 && want <= steps; want *= 2) {
-      if (g_linear_splits > 0 && want != g_linear_splits && want * 2 <= std::min(64LL, steps)) continue;
+    for (long long want = g_linear_splits > 0 ? std::min<long long>(g_linear_splits, steps) : 1; want <= 64 && want <= steps; want *= 2) {
       const long long per = (steps + want - 1) / want, pieces = (steps + per - 1) / per;
       const double blocks = std::ceil(tiles * pieces / 256), rounds = std::floor(blocks / c.fit), rest = blocks - rounds * c.fit;
       double us = per * (rounds * std::max(c.alone, c.fit * c.full) + (rest > 0 ? std::max(c.alone, rest * c.full) : 0)) + 1.5 * (rounds + (rest > 0));
-      const double write = results * (pieces > 1 ? 4.0 * pieces : out) / 4.5e6;
+      const double write = pieces > 1 ? results * 4.0 * pieces / 2.5e6 : results * out / 4.5e6;
       us = c.fit > 1 ? std::max(us, write) + 0.3 * write : us + write;
-      if (pieces > 1) us += 4 + results * (4.0 * pieces + out) / 4.5e6;
+      if (pieces > 1) us += 4 + results * (4.0 * pieces + out) / 2.5e6;
       if (best.splits == 0 || us < least) least = us, best = {t, (int)pieces, per * bk};
+      if (g_linear_splits > 0) break;
     }
   }
   return best;

@@ -9,7 +9,7 @@
 // lanes reads 4 rows of 16 values and each lane gets a column of 4), float32 by giving a lane the 4 neighbouring columns that one
 // 16-byte read delivers: fragment j of a lane belongs to column 4 r + j, and the epilogue goes by that.
 // The order of 16-byte pieces in a row of LDS is permuted (exclusive or with the row) so that the lanes of a read spread over the banks.
-// Two buffers, one barrier a step, fragments read half a step ahead (below).
+// Two or three buffers, one barrier a step, fragments read half a step ahead (below).
 //
 // The products are formed with B's fragment as the first operand, so that a lane's four results lie side by side in a row of C.
 #pragma once
@@ -199,13 +199,13 @@ __device__ __forceinline__ void epilogue(const GemmArgs &a, long long m, long lo
     }
 }
 
-template <typename T, bool AK, bool BKIN, int BM, int BN, int WM, int WN, int ACT>
+template <typename T, bool AK, bool BKIN, int BM, int BN, int WM, int WN, int BUFS, int ACT>
 __global__ void __launch_bounds__(64 * (BM / WM) * (BN / WN)) gemm_kernel(const GemmArgs a) {
   constexpr int THREADS = 64 * (BM / WM) * (BN / WN), BK = 128 / sizeof(T), FM = WM / 16, FN = WN / 16;
   constexpr int GM = sizeof(T) == 4 ? (FM < 4 ? FM : 4) : 1, GN = sizeof(T) == 4 ? (FN < 4 ? FN : 4) : 1;
   typedef Stage<T, BM, AK, THREADS, GM> SA;
   typedef Stage<T, BN, BKIN, THREADS, GN> SB;
-  __shared__ __align__(16) char lds[2][(BM + BN) * 128];
+  __shared__ __align__(16) char lds[BUFS][(BM + BN) * 128];
   // Blocks go round the eight XCDs in turn: each XCD gets a run of neighbouring tiles, so that its L2 holds what they share;
   // in a run, eight row tiles by all columns before the next eight.
   unsigned tile = blockIdx.x;
@@ -280,45 +280,49 @@ __global__ void __launch_bounds__(64 * (BM / WM) * (BN / WN)) gemm_kernel(const 
     }
     if (sizeof(T) == 2) __builtin_amdgcn_sched_barrier(0);
   };
-  auto arrive = [&]() __attribute__((always_inline)) {
-    asm volatile("s_waitcnt vmcnt(0)" : : : "memory");   // what this wave has copied into LDS is there, and read from there
+  // What this wave has copied into LDS is there, but for the copies of `behind` tiles asked for last; what it reads from there it has.
+  static_assert(BUFS == 2 || (SA::PIECES % THREADS == 0 && SB::PIECES % THREADS == 0), "every wave makes as many copies of a tile");
+  auto arrive = [&](bool behind) __attribute__((always_inline)) {
+    if (BUFS > 2 && behind) asm volatile("s_waitcnt vmcnt(%0)" : : "n"((BUFS - 2) * (SA::NL + SB::NL)) : "memory");
+    else asm volatile("s_waitcnt vmcnt(0)" : : : "memory");
     __syncthreads();
   };
   // Half a step is multiplied while the fragments of the next half are on their way from LDS.  The barrier of a step lies between
-  // its halves: everybody holds all of this tile then, so its buffer is free for the tile after next, and the next tile, asked for a
-  // whole step ago, is there.
+  // its halves: everybody holds all of this tile then, so its buffer is free for the tile BUFS steps on, and the next tile, asked for
+  // BUFS - 1 steps ago, is there.  (Three buffers for the tiles of small products, whose time is how soon their data come.)
   const int steps = left > 0 ? (int)((left + BK - 1) / BK) : 0;
+  if (steps) {
+    issue(0);
+    if (BUFS > 2 && steps > 1) issue(1);
+    arrive(steps > 1);
+  }
   // (float32: a half is 1024 cycles of products to one LDS latency; the compiler's own order of reads and products is better there by
   // 2 to 40 %.)
   if constexpr (sizeof(T) == 4) {
     Half h;
-    if (steps) {
-      issue(0);
-      arrive();
-    }
-    for (int t = 0; t < steps; t++) {
-      if (t + 1 < steps) issue((t + 1) & 1);
-      read(h, t & 1, 0);
+    for (int t = 0, buf = 0; t < steps; t++, buf = buf + 1 == BUFS ? 0 : buf + 1) {
+      if (t + BUFS - 1 < steps) issue(buf == 0 ? BUFS - 1 : buf - 1);
+      read(h, buf, 0);
       multiply(h);
-      read(h, t & 1, 1);
+      read(h, buf, 1);
       multiply(h);
-      if (t + 1 < steps) arrive();
+      if (t + 1 < steps) arrive(t + 2 < steps);
     }
   } else if (steps) {
     Half h0, h1;
-    issue(0);
-    arrive();
-    if (steps > 1) issue(1);
+    if (steps > BUFS - 1) issue(BUFS - 1);
     read(h0, 0, 0);
-    for (int t = 0; t < steps; t++) {
-      read(h1, t & 1, 1);
+    for (int t = 0, buf = 0; t < steps; t++) {
+      const int next = buf + 1 == BUFS ? 0 : buf + 1;
+      read(h1, buf, 1);
       multiply(h0);
       if (t + 1 < steps) {
-        arrive();
-        if (t + 2 < steps) issue(t & 1);
-        read(h0, (t + 1) & 1, 0);
+        arrive(t + 2 < steps);
+        if (t + BUFS < steps) issue(buf);
+        read(h0, next, 0);
       }
       multiply(h1);
+      buf = next;
     }
   }
 
@@ -354,16 +358,16 @@ __global__ void __launch_bounds__(64 * (BM / WM) * (BN / WN)) gemm_kernel(const 
 template <typename T, bool AK, bool BKIN, int ACT>
 void launch_tile(int tile, const GemmArgs &a, hipStream_t s) {
   const dim3 grid(a.mtiles * a.ntiles, a.splits);
-#define GELIB_GEMM(BM, BN, WM, WN)                                                                                                                 \
+#define GELIB_GEMM(BM, BN, WM, WN, BUFS)                                                                                                                 \
   do {                                                                                                                                             \
     const dim3 block(64 * (BM / WM) * (BN / WN));                                                                                                  \
-    hipLaunchKernelGGL((gemm_kernel<T, AK, BKIN, BM, BN, WM, WN, ACT>), grid, block, 0, s, a);                                                     \
+    hipLaunchKernelGGL((gemm_kernel<T, AK, BKIN, BM, BN, WM, WN, BUFS, ACT>), grid, block, 0, s, a);                                                     \
   } while (0)
   switch (tile) {
-    case 0: GELIB_GEMM(256, 256, 128, 64); break;
-    case 1: GELIB_GEMM(128, 128, 64, 64); break;
-    case 2: GELIB_GEMM(64, 128, 64, 32); break;
-    default: GELIB_GEMM(16, 256, 16, 64); break;
+    case 0: GELIB_GEMM(256, 256, 128, 64, 2); break;
+    case 1: GELIB_GEMM(128, 128, 64, 64, 2); break;
+    case 2: GELIB_GEMM(64, 128, 64, 32, 3); break;
+    default: GELIB_GEMM(16, 256, 16, 64, 2); break;
   }
 #undef GELIB_GEMM
 }
