@@ -14,7 +14,8 @@ class AdamW(torch.optim.Optimizer):
     state_bits=32 keeps m and v in float32.  state_bits=8 keeps each in a byte, an exponent and three bits of the mantissa, with a scale
     for every 256 elements; these and bfloat16 parameters are rounded at random, so that steps far below a unit in the last place
     add up (to the nearest, v would not follow the gradients at all).  The random bits are a function of seed, step and element:
-    runs repeat.  t counts the steps of each parameter; one whose gradient is None takes none."""
+    runs repeat.  t counts the steps of each parameter; one whose gradient is None takes none.  (A step recorded into a graph is the step
+    of that t at every replay.)"""
 
     def __init__(self, params, lr=1e-3, betas=(0.9, 0.999), eps=1e-8, weight_decay=1e-2, state_bits=32, seed=0):
         if state_bits not in (8, 32):
@@ -27,7 +28,8 @@ class AdamW(torch.optim.Optimizer):
 
     def add_param_group(self, param_group):
         super().add_param_group(param_group)
-        params, device = self.param_groups[-1]["params"], self.param_groups[0]["params"][0].device
+        params = self.param_groups[-1]["params"]
+        device = next((p.device for g in self.param_groups for p in g["params"]), torch.device("cuda"))
         try:
             for p in params:
                 if p.dtype not in (torch.float32, torch.bfloat16, torch.complex64):

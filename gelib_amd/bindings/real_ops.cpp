@@ -373,10 +373,11 @@ at::Tensor linear_act(const at::Tensor &x, const at::Tensor &w, const Maybe &b, 
 // (one without a gradient takes none).
 struct AdamWGroup {
   std::vector<at::Tensor> params;
-  std::vector<int64_t> first, steps;
+  std::vector<int64_t> first, steps, sizes;   // sizes: bytes, which the places were made for
 
   AdamWGroup(std::vector<at::Tensor> p, std::vector<int64_t> f) : params(std::move(p)), first(std::move(f)), steps(params.size(), 0) {
     if (first.size() != params.size()) throw py::value_error("GElib: one place a parameter");
+    for (const at::Tensor &t : params) sizes.push_back(t.nbytes());
   }
 
   void step(const at::Tensor &m, const at::Tensor &v, const Maybe &mt, const Maybe &vt, int bits, double lr, double beta1, double beta2, double eps,
@@ -398,6 +399,7 @@ struct AdamWGroup {
       if (grad.is_sparse() || grad.scalar_type() != type) throw py::type_error("GElib: a gradient is dense and has its parameter's type");
       if (t.device() != m.device() || grad.device() != m.device()) throw py::value_error("GElib: parameters, gradients and moments are on one GPU");
       if (!t.is_contiguous() || t.is_conj() || t.is_neg()) throw py::value_error("GElib: parameters are contiguous in memory");
+      if ((int64_t)t.nbytes() != sizes[k]) throw py::value_error("GElib: a parameter has another size or type than the optimizer was made for");
       if (grad.sizes() != t.sizes()) throw py::value_error("GElib: a gradient is shaped like its parameter");
       const void *g = grad.data_ptr();
       if (!grad.is_contiguous() || grad.is_conj() || grad.is_neg()) {
@@ -443,7 +445,11 @@ void bind_real_ops(py::module_ &m) {
   py::class_<AdamWGroup>(m, "AdamWGroup", "Parameters of one AdamW step, with the places of their moments")
       .def(py::init<std::vector<at::Tensor>, std::vector<int64_t>>())
       .def("step", &AdamWGroup::step)
-      .def_readwrite("steps", &AdamWGroup::steps);
+      .def_property("steps", [](const AdamWGroup &g) { return g.steps; },
+                    [](AdamWGroup &g, std::vector<int64_t> s) {
+                      if (s.size() != g.params.size()) throw py::value_error("GElib: one number of steps a parameter");
+                      g.steps = std::move(s);
+                    });
   m.def("adamw_moments", &adamw_moments);
   m.def("adamw_set_moments", &adamw_set_moments);
 }

@@ -157,6 +157,23 @@ def test_groups_missing_gradients_and_state(gelib, bits):
     assert ((moved - 0.1).abs() < 1e-5).all()
 
 
+def test_a_group_that_comes_later(gelib):
+    a, b = make([(300,)], torch.float32, 4), make([(77,)], torch.float32, 5)
+    opt = gelib.AdamW(a, state_bits=8)
+    opt.step()
+    kept = [t.clone() for t in opt.moments(a[0])]
+    opt.add_param_group({"params": b, "lr": 0.5, "weight_decay": 0.0})
+    for x, y in zip(opt.moments(a[0]), kept):
+        assert torch.equal(x, y)
+    was = b[0].detach().clone()
+    opt.step()
+    assert ((b[0].detach() - was).abs() - 0.5).abs().max() < 1e-5 and [list(g.steps) for g in opt._groups] == [[2], [1]]
+    b[0].data = torch.zeros(5000, device="cuda")   # no room for its moments
+    b[0].grad = torch.zeros(5000, device="cuda")
+    with pytest.raises(ValueError):
+        opt.step()
+
+
 def test_scheduler_closure_zero_grad(gelib):
     p = torch.nn.Parameter(torch.ones(10, device="cuda"))
     opt = gelib.AdamW([p], lr=0.5, weight_decay=0.0)

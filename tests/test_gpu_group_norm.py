@@ -162,6 +162,24 @@ def test_values_behind_a_length_are_not_read(gelib):
     assert torch.equal(gelib.group_norm_act(x, 4, lengths=torch.full((5,), 1 << 30, device="cuda", dtype=torch.int32)), gelib.group_norm_act(x, 4))
 
 
+@pytest.mark.parametrize("shape", [(70000, 3, 10304), (3, 2250000, 320)], ids=str)
+def test_offsets_beyond_32_bits(gelib, shape):
+    """4.3 GB tensors: the last sample is what it is by itself (the same kernels on the same values), and so is its gradient."""
+    n, s, c = shape
+    x = torch.zeros(shape, device="cuda", dtype=torch.bfloat16)
+    x[-1].normal_()
+    g = torch.zeros_like(x)
+    g[-1].normal_()
+    leaf, alone = x.requires_grad_(), x[-1:].detach().clone().requires_grad_()
+    a, b = (gelib.group_norm_act(t, 32, act="silu") for t in (leaf, alone))
+    assert torch.isfinite(a[0].float()).all()
+    # (how a sample is cut may depend on how many there are: the order of sums, not more)
+    assert (a[-1].float() - b[0].float()).abs().max() < 0.04
+    ga, = torch.autograd.grad(a, leaf, g)
+    gb, = torch.autograd.grad(b, alone, g[-1:])
+    assert (ga[-1].float() - gb[0].float()).abs().max() < 0.04 and not ga[0].any()
+
+
 def test_large_mean(gelib):
     """Statistics are formed around the mean: a thousand standard deviations of it cost three digits, not six."""
     gen = torch.Generator(device="cuda").manual_seed(4)

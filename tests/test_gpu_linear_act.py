@@ -123,6 +123,30 @@ def test_memory_beside_the_operands_is_not_touched_or_read(gelib):
                 assert torch.isnan(t[:512]).all() and torch.isnan(t[-512:]).all()
 
 
+def test_offsets_beyond_32_bits(gelib):
+    """4.4 GB of x and 4.6 of the result: the last rows are what they are by themselves."""
+    m, k, n = 1050000, 2056, 2100
+    x = torch.zeros(m, k, device="cuda", dtype=torch.bfloat16)
+    x[-70:] = torch.randn(70, k, device="cuda")
+    w, b = (torch.randn(k, n, device="cuda") / 50).bfloat16(), torch.randn(n, device="cuda").bfloat16()
+    y = gelib.linear_act(x, w, b, residual=torch.zeros(1, 1, device="cuda", dtype=torch.bfloat16).expand(m, n), act="relu")
+    want = reference(x[-70:].double(), w.double(), b.double(), torch.zeros(70, n, device="cuda", dtype=torch.float64), "relu",
+                     torch.zeros(70, n, device="cuda", dtype=torch.float64), torch.bfloat16)["y"]
+    check(y[-70:], *want, "the last rows")
+    assert torch.equal(y[:5], b.clamp(min=0).expand(5, n)) and torch.equal(y[m // 2], b.clamp(min=0))
+    del y
+    x.requires_grad_()
+    w.requires_grad_()
+    g = torch.zeros(m, n, device="cuda", dtype=torch.bfloat16)
+    g[-70:] = torch.randn(70, n, device="cuda")
+    gx, gw = torch.autograd.grad(gelib.linear_act(x, w, b, act="none"), (x, w), g)
+    zero = torch.zeros(70, n, device="cuda", dtype=torch.float64)
+    want = reference(x[-70:].detach().double(), w.detach().double(), b.double(), zero, "none", g[-70:].double(), torch.bfloat16)
+    check(gx[-70:], *want["gx"], "gx")
+    check(gw, want["gw"][0], want["gw"][1] + 64 * u * want["gw"][0].abs(), "gw")   # (the other rows add zeros)
+    assert not gx[:-70].any()
+
+
 def test_infinities_stay_in_their_rows_and_columns(gelib):
     for dtype in (torch.float32, torch.bfloat16):
         for m, k, n in ((40, 96, 130), (300, 260, 200), (2, 520, 136)):
