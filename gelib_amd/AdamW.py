@@ -59,7 +59,6 @@ class AdamW(torch.optim.Optimizer):
                 a[:b.numel()] = b
         self._arrays, self._size = new, size
 
-    @torch.no_grad()
     def step(self, closure=None):
         loss = None
         if closure is not None:

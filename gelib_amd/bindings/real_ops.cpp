@@ -389,6 +389,7 @@ struct AdamWGroup {
     } lists[2];   // float32 and complex64, bfloat16
     std::vector<at::Tensor> copies;   // of gradients that are not contiguous
     std::vector<size_t> moved;
+    at::NoGradGuard no_grad;
     OnDevice on(m);
     for (size_t k = 0; k < params.size(); k++) {
       const at::Tensor &t = params[k], &grad = t.grad();
@@ -419,7 +420,10 @@ struct AdamWGroup {
         done(gelib_hip_adamw_step((int)l.p.size(), l.p.data(), l.g.data(), l.n.data(), l.first.data(), l.step.data(), ptr(m), ptr(v),
                                   mt ? (int16_t *)ptr(*mt) : nullptr, vt ? (int16_t *)ptr(*vt) : nullptr, b ? GELIB_HIP_BF16 : GELIB_HIP_F32, bits, lr,
                                   beta1, beta2, eps, decay, seed, on.stream));
-    for (size_t k : moved) steps[k]++;
+    for (size_t k : moved) {
+      steps[k]++;
+      params[k].unsafeGetTensorImpl()->bump_version();   // (changed in place, as far as autograd is concerned)
+    }
   }
 };
 

@@ -38,6 +38,8 @@ def reference(x, w, b, r, act, g, dtype):
 # are cut into pieces, odd sizes whose rows are not aligned, an empty sum
 SHAPES = [(1, 1, 1), (1, 512, 700), (3, 40, 8), (7, 33, 1), (16, 16, 16), (17, 4099, 65), (64, 64, 64), (65, 63, 129), (128, 256, 128), (129, 72, 257), (300, 1, 5),
           (255, 130, 384), (513, 96, 264), (1000, 8, 40), (5003, 24, 30), (2, 8, 5000), (260, 1024, 520), (5, 0, 6)]
+# up to four rows: any columns, k below and above what one batch of loads takes, and the first k that goes to the tiles
+SHAPES += [(1, 1024, 256), (1, 2049, 72), (2, 1000, 130), (3, 341, 64), (4, 512, 1040), (4, 100, 3), (1, 7, 4100)]
 
 
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16], ids=str)
