@@ -17,6 +17,11 @@
 // itself, a code step is 6 to 12, so rounding to the nearest would leave v where it is for ever.  bfloat16 parameters are
 // rounded at random too (a step is mostly below half a unit in their last place).
 // Every operation is rounded by itself (no contraction), so codes are a function of the inputs that a host can repeat.
+//
+// What bounds it: HBM.  40 M float32 parameters in 300 tensors, moments in 32 bits: 28 bytes an element in 240 us, 4.7 TB/s (a copy of
+// 1 GiB reaches 4.8).  128 M bfloat16 parameters, moments in 8 bits: 10 bytes an element in .32 ms, 4.0 TB/s, where the vector unit is
+// close behind (about 100 instructions an element, of which 3 multiplications of whole numbers at a quarter of the rate; with
+// every test for what is not finite made for every element, and a fourth multiplication, 128 and .35 ms).
 #pragma clang fp contract(off)
 #include <cstring>
 
@@ -42,14 +47,15 @@ struct AdamTable {
   unsigned waves;
 };
 
-__device__ __forceinline__ unsigned mixed(unsigned index, unsigned key) {
-  unsigned h = (index + key) * 2654435769u;
-  h = (h ^ (h >> 15)) * 3144134277u;
-  h = (h ^ (h >> 13)) * 1779033703u;
+constexpr unsigned kMixA = 2654435769u, kMixB = 3144134277u, kMixC = 1779033703u;   // 2^32 / golden ratio, 2^32 (sqrt 3 - 1) and the like: odd numbers
+// of h = (index + key) kMixA, which a lane forms once for its eight neighbouring elements
+__device__ __forceinline__ unsigned mixed(unsigned h) {
+  h = (h ^ (h >> 15)) * kMixB;
+  h = (h ^ (h >> 13)) * kMixC;
   return h ^ (h >> 16);
 }
 __device__ __forceinline__ unsigned mixed_more(unsigned h) {
-  h *= 2654435769u;
+  h *= kMixA;
   return (h ^ (h >> 15)) & 0xffffu;
 }
 
@@ -60,24 +66,38 @@ __device__ __forceinline__ int half_wave_max(int v) {
 }
 
 constexpr unsigned kInf = 0x7f800000u;
+constexpr unsigned kNan = 0x7fc00000u;
 constexpr int kTopOfFinite = 2039;   // u of the largest finite float; rounding up past it stays there
 
-constexpr unsigned kNan = 0x7fc00000u;
-
-__device__ __forceinline__ float decoded(int code, int top, int steps, unsigned not_finite) {
-  return __uint_as_float(code == 0 ? 0u : code > steps ? not_finite : (unsigned)max(code + top - steps, 0) << 20);
+// A block's top is at least steps + 1 (2^-111 for m, 2^-95 for v: what is below is as good as zero), so codes are only ever zero for
+// values that round to it.
+__device__ __forceinline__ unsigned decoded(int code, int top, int steps, unsigned not_finite) {
+  return code == 0 ? 0u : code > steps ? not_finite : (unsigned)(code + top - steps) << 20;
 }
-// u of a value (0 for zero, -1 where it is not finite)
+// the same where the lane has no code for what is not finite: base = (top - steps) << 20
+__device__ __forceinline__ unsigned decoded_finite(unsigned code, unsigned base) { return code ? (code << 20) + base : 0u; }
+
+// u of a value, -1 where it is not finite
 __device__ __forceinline__ int upper(float x, unsigned r) {
   const unsigned b = __float_as_uint(x) & 0x7fffffffu;
   return b >= kInf ? -1 : min((int)((b + r) >> 20), kTopOfFinite);
 }
-template <bool ABOVE>
-__device__ __forceinline__ int coded(float x, int u, int top, int steps) {
-  if (u < 0) return steps + 1;
-  const int c = u - top + steps;
-  return c >= 1 ? ((__float_as_uint(x) & 0x7fffffffu) ? c : 0) : ABOVE && (__float_as_uint(x) & 0x7fffffffu) ? 1 : 0;
+template <bool ABOVE, bool FINITE = false>
+__device__ __forceinline__ unsigned coded(int u, int top, int steps) {
+  return !FINITE && u < 0 ? steps + 1 : max(u - top + steps, ABOVE ? min(u, 1) : 0);
 }
+// the bytes of a lane's eight elements; x: m, whose signs they keep
+template <bool FINITE>
+__device__ __forceinline__ void coded8(const float *x, const int *um, const int *uv, int mt, int vt, uint2 &cm, uint2 &cv) {
+  cm = cv = make_uint2(0, 0);
+#pragma unroll
+  for (int i = 0; i < 8; i++) {
+    const unsigned c = coded<false, FINITE>(um[i], mt, 126);
+    (i < 4 ? cm.x : cm.y) |= (c | (__float_as_uint(x[i]) >> 24 & (c ? 128u : 0u))) << (i % 4 * 8);
+    (i < 4 ? cv.x : cv.y) |= coded<true, FINITE>(uv[i], vt, 254) << (i % 4 * 8);
+  }
+}
+__device__ __forceinline__ unsigned code_of(uint2 w, int i) { return (i < 4 ? w.x : w.y) >> (i % 4 * 8) & 255u; }
 
 constexpr int kAdamLane = 8;   // elements of a lane: 32 lanes a block
 
@@ -121,35 +141,55 @@ __global__ void __launch_bounds__(256) adamw_kernel(const AdamTable tab, const A
       cm = *(const uint2 *)((const char *)a.m + s0), cv = *(const uint2 *)((const char *)a.v + s0);
       mt = a.m_top[s0 / kAdamBlock], vt = a.v_top[s0 / kAdamBlock];
     }
+    // a byte of seven set bits (m), of eight (v): adding one to the seven carries into the eighth
+    const unsigned ones = 0x01010101u, low = 0x7f7f7f7fu;
+    const bool odd = ((((cm.x & low) + ones) | ((cm.y & low) + ones) | (((cv.x & low) + ones) & cv.x) | (((cv.y & low) + ones) & cv.y)) & ~low) != 0;
+    if (__builtin_expect(__any(odd), 0)) {
 #pragma unroll
-    for (int i = 0; i < kAdamLane; i++) {
-      const int c = (i < 4 ? cm.x : cm.y) >> (i % 4 * 8) & 255, d = (i < 4 ? cv.x : cv.y) >> (i % 4 * 8) & 255;
-      m[i] = decoded(c & 127, mt, 126, kNan);
-      if (c & 128) m[i] = -m[i];
-      v[i] = decoded(d, vt, 254, kInf);
+      for (int i = 0; i < kAdamLane; i++) {
+        const unsigned c = code_of(cm, i);
+        m[i] = __uint_as_float(decoded(c & 127, mt, 126, kNan) | (c & 128) << 24);
+        v[i] = __uint_as_float(decoded(code_of(cv, i), vt, 254, kInf));
+      }
+    } else {
+      const unsigned mbase = (unsigned)(mt - 126) << 20, vbase = (unsigned)(vt - 254) << 20;
+#pragma unroll
+      for (int i = 0; i < kAdamLane; i++) {
+        const unsigned c = code_of(cm, i);
+        m[i] = __uint_as_float(decoded_finite(c & 127, mbase) | (c & 128) << 24);
+        v[i] = __uint_as_float(decoded_finite(code_of(cv, i), vbase));
+      }
     }
   }
   unsigned h[kAdamLane];
-  const unsigned key = e.key + (unsigned)(s0 >> 32) * 3144134277u;   // (a lane's eight elements share the upper half of their index)
-  float now[kAdamLane];
+  // (a lane's eight elements share the upper half of their index)
+  const unsigned h0 = ((unsigned)s0 + e.key + (unsigned)(s0 >> 32) * kMixB) * kMixA;
+  float now[kAdamLane], odd = 0.f;
 #pragma unroll
   for (int i = 0; i < kAdamLane; i++) {
     m[i] = m[i] * a.b1 + gr[i] * a.c1;
     v[i] = v[i] * a.b2 + (gr[i] * gr[i]) * a.c2;
-    if (BITS == 8 || sizeof(T) == 2) h[i] = mixed((unsigned)(s0 + i), key);
+    if (BITS == 8 || sizeof(T) == 2) h[i] = mixed(h0 + i * kMixA);
     const float denom = sqrtf(v[i]) * e.inv_sqrt_bc2 + a.eps;
     now[i] = (was[i] - was[i] * a.decay) - (m[i] * e.step_size) / denom;
+    if (sizeof(T) == 2) odd = __builtin_fmaf(now[i], 0.f, odd);   // NaN once one of them is not finite
   }
   T out[kAdamLane];
+  if constexpr (sizeof(T) == 2) {
+    unsigned short r[kAdamLane];
+    if (__builtin_expect(__any(odd != 0.f), 0)) {
 #pragma unroll
-  for (int i = 0; i < kAdamLane; i++) {
-    if (sizeof(T) == 2) {
-      const unsigned b = __float_as_uint(now[i]), u = b & 0x7fffffffu;
-      const unsigned short r = u > kInf ? 0x7fc0 : u == kInf ? b >> 16 : (b + mixed_more(h[i])) >> 16;
-      __builtin_memcpy(&out[i], &r, 2);
+      for (int i = 0; i < kAdamLane; i++) {
+        const unsigned b = __float_as_uint(now[i]), u = b & 0x7fffffffu;
+        r[i] = u > kInf ? 0x7fc0 : u == kInf ? b >> 16 : (b + mixed_more(h[i])) >> 16;
+      }
     } else {
-      __builtin_memcpy(&out[i], &now[i], sizeof(T));
+#pragma unroll
+      for (int i = 0; i < kAdamLane; i++) r[i] = (__float_as_uint(now[i]) + mixed_more(h[i])) >> 16;
     }
+    __builtin_memcpy(out, r, sizeof(out));
+  } else {
+    __builtin_memcpy(out, now, sizeof(out));
   }
   if (whole) {
     __builtin_memcpy(__builtin_assume_aligned(p, 16), out, sizeof(out));
@@ -165,21 +205,27 @@ __global__ void __launch_bounds__(256) adamw_kernel(const AdamTable tab, const A
     }
   } else {
     int um[kAdamLane], uv[kAdamLane];
-    mt = vt = 0;
+    uint2 cm, cv;
+    mt = 127, vt = 255;
 #pragma unroll
     for (int i = 0; i < kAdamLane; i++) {
-      um[i] = upper(m[i], h[i] & 0xfffffu), uv[i] = upper(v[i], h[i] >> 12);
-      if (uv[i] < 0 && um[i] >= 0) m[i] = 0.f, um[i] = 0;   // v is infinite: its steps are zero whatever m is, and m as large as that
-                                                            // would push the block's others below the smallest code
+      um[i] = ((__float_as_uint(m[i]) & 0x7fffffffu) + (h[i] & 0xfffffu)) >> 20, uv[i] = (__float_as_uint(v[i]) + (h[i] >> 12)) >> 20;
       mt = max(mt, um[i]), vt = max(vt, uv[i]);
     }
     mt = half_wave_max(mt), vt = half_wave_max(vt);
-    uint2 cm = {}, cv = {};
+    if (__builtin_expect(__any(mt > kTopOfFinite || vt > kTopOfFinite), 0)) {   // something is not finite, or rounds up to it
+      mt = 127, vt = 255;
 #pragma unroll
-    for (int i = 0; i < kAdamLane; i++) {
-      const unsigned c = coded<false>(m[i], um[i], mt, 126), d = coded<true>(v[i], uv[i], vt, 254);
-      (i < 4 ? cm.x : cm.y) |= (c | (c && __float_as_uint(m[i]) >> 31 ? 128u : 0u)) << (i % 4 * 8);
-      (i < 4 ? cv.x : cv.y) |= d << (i % 4 * 8);
+      for (int i = 0; i < kAdamLane; i++) {
+        um[i] = upper(m[i], h[i] & 0xfffffu), uv[i] = upper(v[i], h[i] >> 12);
+        if (uv[i] < 0 && um[i] >= 0) um[i] = 0;   // v is infinite: its steps are zero whatever m is, and m as large as that would push
+                                                  // the block's others below the smallest code
+        mt = max(mt, um[i]), vt = max(vt, uv[i]);
+      }
+      mt = half_wave_max(mt), vt = half_wave_max(vt);
+      coded8<false>(m, um, uv, mt, vt, cm, cv);
+    } else {
+      coded8<true>(m, um, uv, mt, vt, cm, cv);
     }
     if (own) {
       *(uint2 *)((char *)a.m + s0) = cm, *(uint2 *)((char *)a.v + s0) = cv;
@@ -198,32 +244,32 @@ __global__ void __launch_bounds__(256) adamw_moments_kernel(unsigned short *mv, 
   unsigned short a[kAdamLane], b[kAdamLane];
 #pragma unroll
   for (int i = 0; i < kAdamLane; i++) {
-    const int c = (i < 4 ? cm.x : cm.y) >> (i % 4 * 8) & 255, d = (i < 4 ? cv.x : cv.y) >> (i % 4 * 8) & 255;
-    a[i] = __float_as_uint(decoded(c & 127, tm, 126, kNan)) >> 16 | (c & 128) << 8;
-    b[i] = __float_as_uint(decoded(d, tv, 254, kInf)) >> 16;
+    const unsigned c = code_of(cm, i);
+    a[i] = decoded(c & 127, tm, 126, kNan) >> 16 | (c & 128) << 8;
+    b[i] = decoded(code_of(cv, i), tv, 254, kInf) >> 16;
   }
   __builtin_memcpy(__builtin_assume_aligned(mv + s0, 16), a, 16);
   __builtin_memcpy(__builtin_assume_aligned(vv + s0, 16), b, 16);
 }
 
-// 8-bit moments nearest to given values
+// 8-bit moments nearest to given values (128 M elements .26 ms)
 __global__ void __launch_bounds__(256) adamw_set_moments_kernel(unsigned char *m, unsigned char *v, short *m_top, short *v_top, const float *mv,
                                                                 const float *vv, long long n) {
   const long long s0 = ((long long)blockIdx.x * 256 + threadIdx.x) * kAdamLane;
   if (s0 >= n) return;   // (half waves: n is a multiple of 256)
-  int um[kAdamLane], uv[kAdamLane], mt = 0, vt = 0;
+  int um[kAdamLane], uv[kAdamLane], mt = 127, vt = 255;
+  float x[kAdamLane], y[kAdamLane];
+  load8(mv + s0, true, 0, x);
+  load8(vv + s0, true, 0, y);
 #pragma unroll
   for (int i = 0; i < kAdamLane; i++) {
-    um[i] = upper(mv[s0 + i], 1u << 19), uv[i] = upper(vv[s0 + i], 1u << 19);
+    um[i] = upper(x[i], 1u << 19), uv[i] = upper(y[i], 1u << 19);
     mt = max(mt, um[i]), vt = max(vt, uv[i]);
   }
   mt = half_wave_max(mt), vt = half_wave_max(vt);
-#pragma unroll
-  for (int i = 0; i < kAdamLane; i++) {
-    const int c = coded<false>(mv[s0 + i], um[i], mt, 126);
-    m[s0 + i] = c | (c && __float_as_uint(mv[s0 + i]) >> 31 ? 128 : 0);
-    v[s0 + i] = coded<true>(vv[s0 + i], uv[i], vt, 254);
-  }
+  uint2 cm, cv;
+  coded8<false>(x, um, uv, mt, vt, cm, cv);
+  *(uint2 *)(m + s0) = cm, *(uint2 *)(v + s0) = cv;
   if (threadIdx.x % 32 == 0) m_top[s0 / kAdamBlock] = mt, v_top[s0 / kAdamBlock] = vt;
 }
 
