@@ -112,6 +112,17 @@ def lib():
         L.gelib_hip_vec_mix_workspace_bytes.argtypes = [ctypes.c_int] + [ctypes.c_void_p] * 3 + [ctypes.c_int]
         L.gelib_hip_vec_mix_channels.argtypes = ([ctypes.c_int] + [ctypes.c_void_p] * 6 + [ctypes.c_int, ctypes.c_void_p,
                                                  ctypes.c_uint64, ctypes.c_void_p])
+        v, i, l, u, d = ctypes.c_void_p, ctypes.c_int, ctypes.c_int64, ctypes.c_uint64, ctypes.c_double
+        L.gelib_hip_group_norm_act_fwd.argtypes = [v] * 7 + [i, l, l, i, i, l, l, ctypes.c_float, i, v, u, v]
+        L.gelib_hip_group_norm_act_bwd.argtypes = [v] * 10 + [i, l, l, i, i, l, l, i, v, u, v]
+        L.gelib_hip_group_norm_act_workspace_bytes.argtypes = [i, i, l, l, i, i]
+        L.gelib_hip_linear_act_fwd.argtypes = [v] * 6 + [i, l, i, i, l, i, v, u, v]
+        L.gelib_hip_linear_act_bwd.argtypes = [v] * 7 + [i, l, i, i, l, v, u, v]
+        L.gelib_hip_linear_act_workspace_bytes.argtypes = [i, i, l, i, i]
+        for name in ("gelib_hip_group_norm_act_workspace_bytes", "gelib_hip_linear_act_workspace_bytes"):
+            getattr(L, name).restype = u
+        L.gelib_hip_adamw_step.argtypes = [i] + [v] * 9 + [i, i] + [d] * 5 + [u, v]
+        L.gelib_hip_adamw_moments.argtypes = L.gelib_hip_adamw_set_moments.argtypes = [v] * 6 + [l, v]
         L.gelib_hip_set_option.argtypes = [ctypes.c_char_p, ctypes.c_int]
         L.gelib_hip_set_stream_workspace.argtypes = [ctypes.c_void_p, ctypes.c_void_p, ctypes.c_uint64]
         _lib = L

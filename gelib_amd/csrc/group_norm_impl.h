@@ -11,6 +11,12 @@
 // memory-side cache still holds up to its 256 MB.  What bounds either is HBM; sums go over channels first and groups after, so any
 // channels a group will do, and the channel sums are the gradients of w and b.
 // No atomics: sums have one order.
+//
+// Measured (us, bfloat16 unless said; a copy of 1 GiB reaches 4.8 TB/s): 64 x 1024 x 256, whole forward 27 (67 MB: 2.5 TB/s, one block a
+// compute unit, so that its loads, two reductions and stores follow one another), backward in chunks 18 + 20 and 9 for the two
+// joins; held whole backward it was 180 (410 registers spilled).  24 samples of up to 9216 x 320: statistics 22, y 34, sums 42, gx 52
+// (141 MB written by each of y and gx: 4.2 and 2.7 TB/s, the second beside 25 instructions an element and two exponentials'
+// worth of silu'), joins 18.  32768 x 1 x 64 float32: 14 forward, 18 + 4 backward: six barriers of a block one after the other.
 #pragma once
 
 #include <numeric>
