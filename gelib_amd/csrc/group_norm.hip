@@ -79,24 +79,34 @@ __global__ void __launch_bounds__(256) norm_wide_gx(const NormArgs a, long long 
   }
 }
 
-// a block per channel
+// a block per 64 channels: four rows at a time
 template <typename T, int ACT>
 __global__ void __launch_bounds__(256) norm_wide_gw(const NormArgs a) {
-  __shared__ float lds[4];
-  const int c = blockIdx.x, g = c / (a.C / a.G);
-  const float w = a.w ? to_f(((const T *)a.w)[c]) : 1.f, b = a.b ? to_f(((const T *)a.b)[c]) : 0.f;
+  __shared__ float lds[2][4][64];
+  const int c = blockIdx.x * 64 + threadIdx.x % 64, row = threadIdx.x / 64;
   float sw = 0.f, sb = 0.f;
-  for (long long i = threadIdx.x; i < a.N * a.S; i += 256) {
-    const long long n = i / a.S, s = i % a.S;
-    if (s >= length_of(a, n)) continue;
-    const float xh = (to_f(((const T *)a.x)[n * a.xs + s * a.xp + c]) - a.mean[n * a.G + g]) * a.rstd[n * a.G + g];
-    const float gz = to_f(((const T *)a.gy)[i * a.C + c]) * act_slope<ACT>(xh * w + b);
-    sw += gz * xh, sb += gz;
+  if (c < a.C) {
+    const int g = c / (a.C / a.G);
+    const float w = a.w ? to_f(((const T *)a.w)[c]) : 1.f, b = a.b ? to_f(((const T *)a.b)[c]) : 0.f;
+    for (long long n = 0; n < a.N; n++) {
+      const long long len = length_of(a, n);
+      const float mean = a.mean[n * a.G + g], rstd = a.rstd[n * a.G + g];
+      const T *x = (const T *)a.x + n * a.xs + c, *gy = (const T *)a.gy + n * a.S * a.C + c;
+      // (samples of one position go to the rows in turn, the positions of longer ones)
+      const long long first = a.S == 1 ? (n % 4 == row ? 0 : len) : row;
+#pragma unroll 4
+      for (long long s = first; s < len; s += 4) {
+        const float xh = (to_f(x[s * a.xp]) - mean) * rstd, gz = to_f(gy[s * a.C]) * act_slope<ACT>(xh * w + b);
+        sw += gz * xh, sb += gz;
+      }
+    }
   }
-  sw = block_sum(sw, lds), sb = block_sum(sb, lds);
-  if (threadIdx.x == 0) {
-    if (a.gw) ((T *)a.gw)[c] = from_f<T>(sw);
-    if (a.gb) ((T *)a.gb)[c] = from_f<T>(sb);
+  lds[0][row][threadIdx.x % 64] = sw, lds[1][row][threadIdx.x % 64] = sb;
+  __syncthreads();
+  if (row == 0 && c < a.C) {
+    const int t = threadIdx.x;
+    if (a.gw) ((T *)a.gw)[c] = from_f<T>((lds[0][0][t] + lds[0][1][t]) + (lds[0][2][t] + lds[0][3][t]));
+    if (a.gb) ((T *)a.gb)[c] = from_f<T>((lds[1][0][t] + lds[1][1][t]) + (lds[1][2][t] + lds[1][3][t]));
   }
 }
 
@@ -108,7 +118,7 @@ int run_wide(bool backward, const NormArgs &a, hipStream_t s) {
     if (!backward) hipLaunchKernelGGL((norm_wide_fwd<T, ACT>), grid, dim3(256), 0, s, a, t);
     else if (a.y) hipLaunchKernelGGL((norm_wide_gx<T, ACT>), grid, dim3(256), 0, s, a, t);
   }
-  if (backward && (a.gw || a.gb)) hipLaunchKernelGGL((norm_wide_gw<T, ACT>), dim3(a.C), dim3(256), 0, s, a);
+  if (backward && (a.gw || a.gb)) hipLaunchKernelGGL((norm_wide_gw<T, ACT>), dim3((a.C + 63) / 64), dim3(256), 0, s, a);
   const hipError_t e = hipGetLastError();
   return e == hipSuccess ? 0 : record_hip_error(e, "group norm launch");
 }

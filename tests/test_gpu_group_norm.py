@@ -180,6 +180,45 @@ def test_offsets_beyond_32_bits(gelib, shape):
     assert (ga[-1].float() - gb[0].float()).abs().max() < 0.04 and not ga[0].any()
 
 
+def test_memory_beside_the_operands_is_not_touched_or_read(gelib):
+    """Operands between NaNs and results between sentinels, through the C ABI, over every way that a call is cut."""
+    from gelib_amd import cabi
+    L = cabi.lib()
+    for dtype, code in ((torch.float32, 0), (torch.bfloat16, 1)):
+        for n, s, c, groups in ((3, 5, 12, 3), (2, 33, 30, 10), (700, 1, 64, 8), (1, 2500, 48, 6), (2, 300, 7, 1), (1, 4, 8200, 4)):
+            def framed(shape, fill=None, frame=float("nan"), t=dtype):
+                size = 1
+                for k in shape:
+                    size *= k
+                whole = torch.full((size + 1024,), frame, device="cuda", dtype=t)
+                inner = whole[512:512 + size].view(shape)
+                inner.normal_() if fill is None else inner.fill_(fill)
+                return whole, inner
+            (X, x), (W, w), (B, b), (G, g) = framed((n, s, c)), framed((c,)), framed((c,)), framed((n, s, c))
+            outs = [framed(k, 3.0, 5.0) for k in ((n, s, c), (n, s, c), (c,), (c,))]
+            (M, mean), (R, rstd) = (framed((n, groups), 3.0, 5.0, torch.float32) for _ in range(2))
+            y, gx, gw, gb = (t for _, t in outs)
+            stream = torch.cuda.current_stream().cuda_stream
+            P = [t.data_ptr() for t in (x, w, b, g)]
+
+            def work(back):
+                need = L.gelib_hip_group_norm_act_workspace_bytes(back, code, n, s, c, groups)
+                return torch.full((max(need, 16),), 255, device="cuda", dtype=torch.uint8), need
+            ws, need = work(0)
+            cabi.check(L.gelib_hip_group_norm_act_fwd(y.data_ptr(), mean.data_ptr(), rstd.data_ptr(), P[0], P[1], P[2], None, code, n, s, c, groups, s * c, c, 1e-3, 2,
+                                                      ws.data_ptr(), need, stream))
+            ws, need = work(1)
+            cabi.check(L.gelib_hip_group_norm_act_bwd(gx.data_ptr(), gw.data_ptr(), gb.data_ptr(), P[3], mean.data_ptr(), rstd.data_ptr(), P[0], P[1], P[2], None, code,
+                                                      n, s, c, groups, s * c, c, 2, ws.data_ptr(), need, stream))
+            with torch.no_grad():
+                want = reference(x.double(), groups, w.double(), b.double(), 1e-3, "silu", torch.full((n,), s, device="cuda"), g.double())
+            for got, k in ((y, "y"), (gx, "gx"), (gw, "gw"), (gb, "gb")):
+                v, tol = want[k]
+                check(got, v.reshape(got.shape), tol.reshape(got.shape), "%s of %s" % (k, (n, s, c, groups)))
+            for t in [t for t, _ in outs] + [M, R]:
+                assert (t[:512] == 5).all() and (t[-512:] == 5).all()
+
+
 def test_large_mean(gelib):
     """Statistics are formed around the mean: a thousand standard deviations of it cost three digits, not six."""
     gen = torch.Generator(device="cuda").manual_seed(4)

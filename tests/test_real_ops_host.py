@@ -50,6 +50,25 @@ def test_refusals_are_status_codes():
     assert norm(N=0, x=None, y=None) == 0 and linear(rows=0, x=None, y=None, w=None) == 0 and linear(n=0, x=None, y=None, w=None) == 0
 
 
+def test_rows_of_whole_16_bytes_are_aligned():
+    assert linear(k=8, xs=9) == 12 and linear(k=8, x=vp(0x1004)) == 12 and linear(n=4, w=vp(0x1008)) == 12
+    # others may lie anywhere: refused only because the memory is not the device's
+    assert linear(k=7, xs=9, x=vp(0x1004)) in (8, 10) and linear(k=8, rows=1, xs=9) in (8, 10)
+    assert cabi.lib().gelib_hip_adamw_moments(vp(0x1008), P, P, P, P, P, i64(256), None) == 12
+
+
+def test_workspaces_and_options():
+    L = cabi.lib()
+    assert L.gelib_hip_linear_act_workspace_bytes(0, 1, 4096, 64, 64) == 0                     # whole rows, one piece
+    assert L.gelib_hip_linear_act_workspace_bytes(0, 1, 4096, 63, 64) >= 4096 * 64 * 2         # x is copied to rows of 64
+    assert L.gelib_hip_linear_act_workspace_bytes(8 | 3, 1, 4096, 64, 64) >= 4096 * 64 * 2     # gz
+    assert L.gelib_hip_linear_act_workspace_bytes(16, 1, 4096, 64, 64) == 0 and L.gelib_hip_linear_act_workspace_bytes(0, 5, 4096, 64, 64) == 0
+    assert L.gelib_hip_group_norm_act_workspace_bytes(0, 0, 8, 3, 64, 8) == 0 and L.gelib_hip_group_norm_act_workspace_bytes(1, 0, 8, 100000, 64, 8) > 0
+    for name, bad in (("linear_act_tile", 4), ("linear_act_tile", -2), ("linear_act_splits", 65), ("linear_act_other", 0)):
+        with pytest.raises(cabi.GelibHipError):
+            cabi.set_option(name, bad)
+
+
 def test_host_memory_is_refused():
     buf = np.zeros(4096, np.float32)
     q = vp(buf.ctypes.data)
