@@ -39,7 +39,7 @@ struct Memory {
 };
 
 int norm_shape(int dtype, int act, int64_t N, int64_t S, int C, int G, int64_t xs, int64_t xp) {
-  if (!types_ok(dtype, act) || N < 0 || S < 0 || C < 1 || G < 1 || C % G || xs < 0 || xp < 0) return GELIB_HIP_ERR_ARG;
+  if (!types_ok(dtype, act) || N < 0 || S < 0 || C < 1 || C > (1 << 26) || G < 1 || C % G || xs < 0 || xp < 0) return GELIB_HIP_ERR_ARG;
   if (!product_ok(N, S) || !product_ok(N * S, C) || N > (1LL << 40) / G || !product_ok(N, xs) || !product_ok(S, xp)) return GELIB_HIP_ERR_ARG;
   return GELIB_HIP_OK;
 }

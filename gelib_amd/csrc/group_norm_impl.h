@@ -8,15 +8,17 @@
 // registers (16 loads a thread, 512 threads: 128 KB) it is read once, and the statistics are formed around the mean from registers;
 // the backward pass forms gz twice from what it holds.  Larger samples are cut into chunks of positions: every chunk's mean and sum of
 // squares around it (backward: its channel sums), joined by the parallel form of the variance, then a second pass over x, which the
-// memory-side cache still holds up to its 256 MB.  What bounds either is HBM; sums go over channels first and groups after, so any
-// channels a group will do, and the channel sums are the gradients of w and b.
+// memory-side cache still holds up to its 256 MB; groups wider than a chunk's block (256 loads a position) are summed in pieces of as
+// many channels each, joined like chunks.  What bounds either is HBM; sums go over channels first and groups after, so any channels a
+// group will do, and the channel sums are the gradients of w and b.
 // No atomics: sums have one order.
 //
 // Measured (us, bfloat16 unless said; a copy of 1 GiB reaches 4.8 TB/s): 64 x 1024 x 256, whole forward 27 (67 MB: 2.5 TB/s, one block a
 // compute unit, so that its loads, two reductions and stores follow one another), backward in chunks 18 + 20 and 9 for the two
 // joins; held whole backward it was 180 (410 registers spilled).  24 samples of up to 9216 x 320: statistics 22, y 34, sums 42, gx 52
 // (141 MB written by each of y and gx: 4.2 and 2.7 TB/s, the second beside 25 instructions an element and two exponentials'
-// worth of silu'), joins 18.  32768 x 1 x 64 float32: 14 forward, 18 + 4 backward: six barriers of a block one after the other.
+// worth of silu'), joins 18.  One group of 4096 channels, silu, with the host's part: 64 x 512 forward 168, both 521 (a block a group
+// alone: 11900 and 28600); 8192 x 1 forward 148, both 461 (202 and 594); 8192 x 1 x 8192 in chunks of one position 268 and 1970.  32768 x 1 x 64 float32: 14 forward, 18 + 4 backward: six barriers of a block one after the other.
 #pragma once
 
 #include <numeric>
@@ -31,14 +33,15 @@ struct NormPlan {
   int T;                      // threads
   long long rows, chunks;     // positions of a chunk, chunks of a sample (in chunks)
   long long blocks;           // along the samples (whole: they walk over the groups of NS samples)
+  int pieces;                 // in chunks: parts of a group that are summed by themselves (groups wider than a block), as many channels each
 };
 
 struct NormDev {
   NormArgs a;
   NormPlan p;
-  float *stats;   // in chunks, forward: [n][chunk][G] mean and sum of squares; backward: [n][chunk][2][C]
+  float *stats;   // in chunks, forward: [n][chunk][G pieces] mean and sum of squares; backward: [n][chunk][2][C]
   float *sums;    // backward: [blocks or n][2][C] channel sums of gz xh and of gz
-  float *means;   // in chunks, backward: [n][G][2] mean of q and of q xh
+  float *means;   // in chunks, backward: [n][G pieces][2] mean of q and of q xh
 };
 
 template <typename T>
@@ -176,6 +179,22 @@ __device__ __forceinline__ void group_sums(const NormDev &d, const Place &w, con
       for (int i = 0; i < cg; i++) s += p[i];
       f(g, s);
     }
+  } else if (groups < d.p.T / 64) {   // fewer groups than waves: all of them at every group (one wave took 3 us for 4096 channels)
+    __shared__ float part[kNormMostT / 64];
+    for (int g = 0; g < groups; g++) {
+      const float *p = in + g / gs * d.p.Cw + g % gs * cg;
+      float s = 0.f;
+      for (int i = threadIdx.x; i < cg; i += d.p.T) s += p[i];
+#pragma unroll
+      for (int m = 32; m >= 1; m >>= 1) s += __shfl_xor(s, m);
+      if (threadIdx.x % 64 == 0) part[threadIdx.x / 64] = s;
+      __syncthreads();
+      if (threadIdx.x == 0) {
+        for (int k = 1; k < d.p.T / 64; k++) s += part[k];
+        f(g, s);
+      }
+      __syncthreads();
+    }
   } else {
     const int waves = d.p.T / 64, lane = threadIdx.x % 64;
     for (int g = threadIdx.x / 64; g < groups && (int)threadIdx.x / 64 < waves; g += waves) {
@@ -210,6 +229,18 @@ __device__ __forceinline__ void load_channels(const void *from, const Place &w, 
 template <int V>
 __device__ __forceinline__ void groups_of(const NormDev &d, const Place &w, int *g) {
   const int cg = d.a.C / d.a.G, first = w.on ? w.tx * V : 0;
+  int at = first / cg, left = cg - (first - at * cg);
+#pragma unroll
+  for (int i = 0; i < V; i++) {
+    g[i] = at;
+    if (--left == 0) at++, left = cg;
+  }
+}
+
+// the group of each of a thread's channels, of the sample's: stripes may begin inside a group in the passes that only look groups up
+template <int V>
+__device__ __forceinline__ void groups_in_row(const NormDev &d, const Place &w, int *g) {
+  const int cg = d.a.C / d.a.G, first = w.on ? w.c0 + w.tx * V : 0;
   int at = first / cg, left = cg - (first - at * cg);
 #pragma unroll
   for (int i = 0; i < V; i++) {
@@ -477,22 +508,24 @@ static __global__ void __launch_bounds__(256) norm_stats_join(const NormDev d) {
   const long long at = (long long)blockIdx.x * 4 + threadIdx.x / 64, n = at / a.G;
   const int g = (int)(at - n * a.G), lane = threadIdx.x % 64;
   if (n >= a.N) return;
-  const long long len = length_of(a, n);
-  const float *p = d.stats + (n * d.p.chunks * a.G + g) * 2;
+  const long long len = length_of(a, n), stride = (long long)a.G * d.p.pieces * 2;
+  const int pieces = d.p.pieces, piece = a.C / a.G / pieces;   // channels of a piece
+  const float *p = d.stats + n * d.p.chunks * stride + g * pieces * 2;
+  const long long entries = (len + d.p.rows - 1) / d.p.rows * pieces;
   auto count = [&](long long k) { return (float)max(0LL, min(d.p.rows, len - k * d.p.rows)); };
   auto all = [](float s) {
 #pragma unroll
     for (int m = 32; m >= 1; m >>= 1) s += __shfl_xor(s, m);
     return s;
   };
-  // (means of chunks around the first one's: their sum is as exact as they are)
+  // (means around the first one: their sum is as exact as they are)
   const float first = len ? p[0] : 0.f;
   float s = 0.f, q = 0.f;
-  for (long long k = lane; k < d.p.chunks && k * d.p.rows < len; k += 64) s += count(k) * (p[k * a.G * 2] - first);
-  const float mean = first + (len ? all(s) / (float)len : 0.f);
-  for (long long k = lane; k < d.p.chunks && k * d.p.rows < len; k += 64) {
-    const float e = p[k * a.G * 2] - mean;
-    q += p[k * a.G * 2 + 1] + count(k) * (float)(a.C / a.G) * e * e;
+  for (long long e = lane; e < entries; e += 64) s += count(e / pieces) * (p[e / pieces * stride + e % pieces * 2] - first);
+  const float mean = first + (len ? all(s) / ((float)len * (float)pieces) : 0.f);
+  for (long long e = lane; e < entries; e += 64) {
+    const float *t = p + e / pieces * stride + e % pieces * 2, d = t[0] - mean;
+    q += t[1] + count(e / pieces) * (float)piece * d * d;
   }
   q = all(q);
   if (lane == 0) a.mean[at] = mean, a.rstd[at] = 1.f / sqrtf((len ? q / ((float)len * (float)(a.C / a.G)) : 0.f) + a.eps);
@@ -510,10 +543,10 @@ __global__ void __launch_bounds__(kNormChunkT) norm_apply_fwd(const NormDev d, l
   int g[V];
   load_channels<T, V>(a.w, w, 1.f, k);
   load_channels<T, V>(a.b, w, 0.f, B);
-  groups_of<V>(d, w, g);
+  groups_in_row<V>(d, w, g);
 #pragma unroll
   for (int i = 0; i < V; i++) {
-    const long long at = n * a.G + w.c0 / cg + g[i];
+    const long long at = n * a.G + g[i];
     mu[i] = a.mean[at], k[i] *= a.rstd[at];
   }
   const T *x = (const T *)a.x + n * a.xs + w.c0 + w.tx * V;
@@ -552,11 +585,11 @@ __global__ void __launch_bounds__(kNormChunkT) norm_chunk_sums(const NormDev d, 
   int g[V];
   load_channels<T, V>(a.w, w, 1.f, W);
   load_channels<T, V>(a.b, w, 0.f, B);
-  groups_of<V>(d, w, g);
+  groups_in_row<V>(d, w, g);
   if (w.on) {
 #pragma unroll
     for (int i = 0; i < V; i++) {
-      const long long at = n * a.G + w.c0 / cg + g[i];
+      const long long at = n * a.G + g[i];
       mu[i] = a.mean[at], k[i] = a.rstd[at];
     }
     const T *x = (const T *)a.x + n * a.xs + w.c0 + w.tx * V, *gy = (const T *)a.gy + n * a.S * a.C + w.c0 + w.tx * V;
@@ -632,11 +665,18 @@ __global__ void __launch_bounds__(kNormChunkT) norm_apply_bwd(const NormDev d, l
   int g[V];
   load_channels<T, V>(a.w, w, 1.f, W);
   load_channels<T, V>(a.b, w, 0.f, B);
-  groups_of<V>(d, w, g);
+  groups_in_row<V>(d, w, g);
 #pragma unroll
   for (int i = 0; i < V; i++) {
-    const long long at = n * a.G + w.c0 / cg + g[i];
-    mu[i] = a.mean[at], k[i] = a.rstd[at], m1[i] = d.means[2 * at], m2[i] = d.means[2 * at + 1];
+    const long long at = n * a.G + g[i];
+    mu[i] = a.mean[at], k[i] = a.rstd[at];
+    if (i && g[i] == g[i - 1]) {
+      m1[i] = m1[i - 1], m2[i] = m2[i - 1];
+    } else {
+      float s1 = 0.f, s2 = 0.f;
+      for (int q = 0; q < d.p.pieces; q++) s1 += d.means[2 * (at * d.p.pieces + q)], s2 += d.means[2 * (at * d.p.pieces + q) + 1];
+      m1[i] = s1 / (float)d.p.pieces, m2[i] = s2 / (float)d.p.pieces;
+    }
   }
   const T *x = (const T *)a.x + n * a.xs + w.c0 + w.tx * V, *gy = (const T *)a.gy + n * a.S * a.C + w.c0 + w.tx * V;
   T *gx = (T *)a.y + n * a.S * a.C + w.c0 + w.tx * V;
@@ -686,9 +726,9 @@ template <typename T, int V, int ACT>
 int run_norm(bool backward, const NormDev &d, hipStream_t s) {
   const NormArgs &a = d.a;
   const NormPlan &p = d.p;
-  const size_t lds = norm_lds_bytes(p, a.C / a.G);
   const dim3 block(p.T);
   if (p.R) {
+    const size_t lds = norm_lds_bytes(p, a.C / a.G);
     const dim3 grid((unsigned)p.blocks, p.stripes);
 #define GELIB_NORM(R)                                                                                              \
   do {                                                                                                             \
@@ -708,14 +748,18 @@ int run_norm(bool backward, const NormDev &d, hipStream_t s) {
       for (long long n = 0; n < a.N; n += most)
         hipLaunchKernelGGL(kernel, dim3(chunks, p.stripes, (unsigned)std::min(most, a.N - n)), block, bytes, s, d, n);
     };
+    NormDev j = d;   // the kernels that sum groups sum the pieces of them
+    j.a.G = a.G * p.pieces;
+    const size_t lds = norm_lds_bytes(p, a.C / j.a.G);
     if (!backward) {
-      each(norm_chunk_stats<T, V>, (unsigned)p.chunks, lds);
+      for (long long n = 0; n < a.N; n += most)
+        hipLaunchKernelGGL((norm_chunk_stats<T, V>), dim3((unsigned)p.chunks, p.stripes, (unsigned)std::min(most, a.N - n)), block, lds, s, j, n);
       hipLaunchKernelGGL(norm_stats_join, dim3((unsigned)((a.N * a.G + 3) / 4)), dim3(256), 0, s, d);
       each(norm_apply_fwd<T, V, ACT>, (unsigned)p.chunks, 0);
     } else {
       each(norm_chunk_sums<T, V, ACT>, (unsigned)p.chunks, lds);
-      NormDev j = d;   // (stripes of about 32 channels: their sums are short, blocks are wanted)
-      const int cg = a.C / a.G, Cq = V / std::gcd(V, cg) * cg;
+      // (stripes of about 32 channels: their sums are short, blocks are wanted)
+      const int cg = a.C / j.a.G, Cq = V / std::gcd(V, cg) * cg;
       j.p.Cw = std::min(p.Cw, std::max(1, 32 / Cq) * Cq), j.p.stripes = (a.C + j.p.Cw - 1) / j.p.Cw, j.p.TX = 1, j.p.TY = 1, j.p.T = kNormChunkT;
       for (long long n = 0; n < a.N; n += most)
         hipLaunchKernelGGL((norm_sums_join<T>), dim3(1, j.p.stripes, (unsigned)std::min(most, a.N - n)), dim3(kNormChunkT), norm_lds_bytes(j.p, cg), s, j, n);

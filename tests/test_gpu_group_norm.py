@@ -85,6 +85,10 @@ SHAPES = [(1, 1, 1, 1), (3, 1, 8, 2), (2, 5, 7, 7), (2, 19, 30, 10), (5, 33, 64,
           (3, 2050, 96, 32), (2, 700, 1024, 1), (2, 9, 2056, 257), (1, 30011, 5, 1), (260, 70, 33, 11), (1, 3, 8200, 4)]
 
 
+# groups wider than a block: in pieces, in as many pieces as channels (a prime number of them), one group of everything
+SHAPES += [(2, 40, 4104, 1), (2, 5, 4106, 2), (300, 1, 9000, 3), (1, 700, 6144, 2)]
+
+
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16], ids=str)
 @pytest.mark.parametrize("act", ["none", "relu", "silu", "gelu"])
 @pytest.mark.parametrize("shape", SHAPES, ids=lambda s: "x".join(map(str, s)))
