@@ -18,7 +18,9 @@
 // joins; held whole backward it was 180 (410 registers spilled).  24 samples of up to 9216 x 320: statistics 22, y 34, sums 42, gx 52
 // (141 MB written by each of y and gx: 4.2 and 2.7 TB/s, the second beside 25 instructions an element and two exponentials'
 // worth of silu'), joins 18.  One group of 4096 channels, silu, with the host's part: 64 x 512 forward 168, both 521 (a block a group
-// alone: 11900 and 28600); 8192 x 1 forward 148, both 461 (202 and 594); 8192 x 1 x 8192 in chunks of one position 268 and 1970.  32768 x 1 x 64 float32: 14 forward, 18 + 4 backward: six barriers of a block one after the other.
+// alone: 11900 and 28600); 8192 x 1 forward 148, both 461 (202 and 594).  8192 x 1 x 8192, chunks of one position: 271 and 990.
+// 64 x 512 x 4099, loads of one channel: 384 and 916.  32768 x 1 x 64 float32: 14 forward, 18 + 4 backward: six barriers of a block
+// one after the other.
 #pragma once
 
 #include <numeric>
@@ -502,33 +504,54 @@ __global__ void __launch_bounds__(kNormChunkT) norm_chunk_stats(const NormDev d,
   for (int k = threadIdx.x; k < w.cw / cg; k += d.p.T) to[2 * k] = l.first[k], to[2 * k + 1] = l.second[k];
 }
 
-// the chunks of a sample joined: a wave a group
-static __global__ void __launch_bounds__(256) norm_stats_join(const NormDev d) {
+// The chunks of a sample joined, and the pieces of a group: W waves a group.  One where they are few; 16 from 1024 entries on, which
+// only groups in many pieces have (64 x 512 x 4099, 131 k entries a group: forward 2280 us with one wave and a division an entry, 384 so).
+template <int W>
+static __global__ void __launch_bounds__(W == 1 ? 256 : 64 * W) norm_stats_join(const NormDev d) {
   const NormArgs &a = d.a;
-  const long long at = (long long)blockIdx.x * 4 + threadIdx.x / 64, n = at / a.G;
-  const int g = (int)(at - n * a.G), lane = threadIdx.x % 64;
-  if (n >= a.N) return;
+  constexpr int kGroups = W == 1 ? 4 : 1, kStep = 64 * W;
+  const long long at = (long long)blockIdx.x * kGroups + threadIdx.x / kStep, n = at / a.G;
+  const int g = (int)(at - n * a.G), t = threadIdx.x % kStep;
+  if (n >= a.N) return;   // (whole waves; whole blocks where W is more than one)
   const long long len = length_of(a, n), stride = (long long)a.G * d.p.pieces * 2;
   const int pieces = d.p.pieces, piece = a.C / a.G / pieces;   // channels of a piece
-  const float *p = d.stats + n * d.p.chunks * stride + g * pieces * 2;
-  const long long entries = (len + d.p.rows - 1) / d.p.rows * pieces;
-  auto count = [&](long long k) { return (float)max(0LL, min(d.p.rows, len - k * d.p.rows)); };
+  const float *p = d.stats + n * d.p.chunks * stride + (long long)g * pieces * 2;
+  const long long chunks = (len + d.p.rows - 1) / d.p.rows;
   auto all = [](float s) {
 #pragma unroll
     for (int m = 32; m >= 1; m >>= 1) s += __shfl_xor(s, m);
+    if (W > 1) {
+      __shared__ float part[W];
+      __syncthreads();
+      if (threadIdx.x % 64 == 0) part[threadIdx.x / 64] = s;
+      __syncthreads();
+      s = part[0];
+      for (int k = 1; k < W; k++) s += part[k];
+    }
     return s;
+  };
+  // f(count, mean and sum of squares) of every kStep-th entry from t on
+  const int down = kStep / pieces, across = kStep - down * pieces;
+  auto each = [&](auto f) {
+    int q = t % pieces;
+    for (long long k = t / pieces; k < chunks;) {
+      f((float)min(d.p.rows, len - k * d.p.rows), p + k * stride + 2 * q);
+      k += down, q += across;
+      if (q >= pieces) q -= pieces, k++;
+    }
   };
   // (means around the first one: their sum is as exact as they are)
   const float first = len ? p[0] : 0.f;
   float s = 0.f, q = 0.f;
-  for (long long e = lane; e < entries; e += 64) s += count(e / pieces) * (p[e / pieces * stride + e % pieces * 2] - first);
-  const float mean = first + (len ? all(s) / ((float)len * (float)pieces) : 0.f);
-  for (long long e = lane; e < entries; e += 64) {
-    const float *t = p + e / pieces * stride + e % pieces * 2, d = t[0] - mean;
-    q += t[1] + count(e / pieces) * (float)piece * d * d;
-  }
+  each([&](float count, const float *e) { s += count * (e[0] - first); });
+  s = all(s);
+  const float mean = first + (len ? s / ((float)len * (float)pieces) : 0.f);
+  each([&](float count, const float *e) {
+    const float off = e[0] - mean;
+    q += e[1] + count * (float)piece * off * off;
+  });
   q = all(q);
-  if (lane == 0) a.mean[at] = mean, a.rstd[at] = 1.f / sqrtf((len ? q / ((float)len * (float)(a.C / a.G)) : 0.f) + a.eps);
+  if (t == 0) a.mean[at] = mean, a.rstd[at] = 1.f / sqrtf((len ? q / ((float)len * (float)(a.C / a.G)) : 0.f) + a.eps);
 }
 
 // second pass: y of a chunk
@@ -537,7 +560,6 @@ __global__ void __launch_bounds__(kNormChunkT) norm_apply_fwd(const NormDev d, l
   const Place w = place_of(d);
   if (!w.on) return;
   const NormArgs &a = d.a;
-  const int cg = a.C / a.G;
   const long long n = nbase + blockIdx.z, s0 = blockIdx.x * d.p.rows, len = length_of(a, n), end = min(s0 + d.p.rows, a.S);
   float B[V], mu[V], k[V];
   int g[V];
@@ -628,7 +650,16 @@ __global__ void __launch_bounds__(kNormChunkT) norm_sums_join(const NormDev d, l
   __shared__ float part[kNormChunkT / 32][2][33];
   float *lens = l.second + d.p.Cw / cg;
   if (threadIdx.x == 0) lens[0] = (float)len;
-  for (int base = 0; base < w.cw; base += 32) {
+  if (chunks < runs) {   // few to sum: a thread a channel (8192 x 1 x 8192, one chunk: both directions 1970 us in runs, 990 so)
+    const float *p = d.stats + n * d.p.chunks * 2 * a.C + w.c0;
+    for (int c = threadIdx.x; c < w.cw; c += d.p.T) {
+      float s1 = 0.f, s2 = 0.f;
+      for (long long k = 0; k < chunks; k++) s2 += p[k * 2 * a.C + c], s1 += p[k * 2 * a.C + a.C + c];
+      l.chan[c] = s1, l.chan2[c] = s2;
+    }
+    __syncthreads();
+  }
+  for (int base = chunks < runs ? w.cw : 0; base < w.cw; base += 32) {
     const int c = base + threadIdx.x % 32;
     float s1 = 0.f, s2 = 0.f;
     if (c < w.cw) {
@@ -654,12 +685,22 @@ __global__ void __launch_bounds__(kNormChunkT) norm_sums_join(const NormDev d, l
   for (int k = threadIdx.x; k < gs; k += d.p.T) m[2 * k] = l.first[k], m[2 * k + 1] = l.second[k];
 }
 
+// the means of a group's pieces averaged into the first one's place: a wave a group
+static __global__ void __launch_bounds__(256) norm_means_join(const NormDev d) {
+  const long long at = (long long)blockIdx.x * 4 + threadIdx.x / 64;
+  if (at >= d.a.N * d.a.G) return;
+  float *m = d.means + at * d.p.pieces * 2, s = 0.f;
+  for (int k = threadIdx.x % 64; k < 2 * d.p.pieces; k += 64) s += m[k];   // (even lanes the first kind, odd ones the second)
+#pragma unroll
+  for (int j = 32; j >= 2; j >>= 1) s += __shfl_xor(s, j);
+  if (threadIdx.x % 64 < 2) m[threadIdx.x % 64] = s / (float)d.p.pieces;
+}
+
 template <typename T, int V, int ACT>
 __global__ void __launch_bounds__(kNormChunkT) norm_apply_bwd(const NormDev d, long long nbase) {
   const Place w = place_of(d);
   if (!w.on) return;
   const NormArgs &a = d.a;
-  const int cg = a.C / a.G;
   const long long n = nbase + blockIdx.z, s0 = blockIdx.x * d.p.rows, len = length_of(a, n), end = min(s0 + d.p.rows, a.S);
   float W[V], B[V], mu[V], k[V], m1[V], m2[V];
   int g[V];
@@ -670,13 +711,7 @@ __global__ void __launch_bounds__(kNormChunkT) norm_apply_bwd(const NormDev d, l
   for (int i = 0; i < V; i++) {
     const long long at = n * a.G + g[i];
     mu[i] = a.mean[at], k[i] = a.rstd[at];
-    if (i && g[i] == g[i - 1]) {
-      m1[i] = m1[i - 1], m2[i] = m2[i - 1];
-    } else {
-      float s1 = 0.f, s2 = 0.f;
-      for (int q = 0; q < d.p.pieces; q++) s1 += d.means[2 * (at * d.p.pieces + q)], s2 += d.means[2 * (at * d.p.pieces + q) + 1];
-      m1[i] = s1 / (float)d.p.pieces, m2[i] = s2 / (float)d.p.pieces;
-    }
+    m1[i] = d.means[2 * at * d.p.pieces], m2[i] = d.means[2 * at * d.p.pieces + 1];
   }
   const T *x = (const T *)a.x + n * a.xs + w.c0 + w.tx * V, *gy = (const T *)a.gy + n * a.S * a.C + w.c0 + w.tx * V;
   T *gx = (T *)a.y + n * a.S * a.C + w.c0 + w.tx * V;
@@ -754,7 +789,8 @@ int run_norm(bool backward, const NormDev &d, hipStream_t s) {
     if (!backward) {
       for (long long n = 0; n < a.N; n += most)
         hipLaunchKernelGGL((norm_chunk_stats<T, V>), dim3((unsigned)p.chunks, p.stripes, (unsigned)std::min(most, a.N - n)), block, lds, s, j, n);
-      hipLaunchKernelGGL(norm_stats_join, dim3((unsigned)((a.N * a.G + 3) / 4)), dim3(256), 0, s, d);
+      if (p.chunks * p.pieces >= 1024) hipLaunchKernelGGL(norm_stats_join<16>, dim3((unsigned)(a.N * a.G)), dim3(1024), 0, s, d);
+      else hipLaunchKernelGGL(norm_stats_join<1>, dim3((unsigned)((a.N * a.G + 3) / 4)), dim3(256), 0, s, d);
       each(norm_apply_fwd<T, V, ACT>, (unsigned)p.chunks, 0);
     } else {
       each(norm_chunk_sums<T, V, ACT>, (unsigned)p.chunks, lds);
@@ -763,6 +799,7 @@ int run_norm(bool backward, const NormDev &d, hipStream_t s) {
       j.p.Cw = std::min(p.Cw, std::max(1, 32 / Cq) * Cq), j.p.stripes = (a.C + j.p.Cw - 1) / j.p.Cw, j.p.TX = 1, j.p.TY = 1, j.p.T = kNormChunkT;
       for (long long n = 0; n < a.N; n += most)
         hipLaunchKernelGGL((norm_sums_join<T>), dim3(1, j.p.stripes, (unsigned)std::min(most, a.N - n)), dim3(kNormChunkT), norm_lds_bytes(j.p, cg), s, j, n);
+      if (a.y && p.pieces > 1) hipLaunchKernelGGL(norm_means_join, dim3((unsigned)((a.N * a.G + 3) / 4)), dim3(256), 0, s, d);
       if (a.y) each(norm_apply_bwd<T, V, ACT>, (unsigned)p.chunks, 0);
       if (a.gw || a.gb)
         hipLaunchKernelGGL((norm_join<T>), dim3((2 * a.C + 31) / 32), dim3(256), 0, s, (const float *)d.sums, (T *)a.gw, (T *)a.gb, a.N, a.C);

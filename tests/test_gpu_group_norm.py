@@ -86,7 +86,7 @@ SHAPES = [(1, 1, 1, 1), (3, 1, 8, 2), (2, 5, 7, 7), (2, 19, 30, 10), (5, 33, 64,
 
 
 # groups wider than a block: in pieces, in as many pieces as channels (a prime number of them), one group of everything
-SHAPES += [(2, 40, 4104, 1), (2, 5, 4106, 2), (300, 1, 9000, 3), (1, 700, 6144, 2)]
+SHAPES += [(2, 40, 4104, 1), (2, 5, 4106, 2), (300, 1, 9000, 3), (1, 700, 6144, 2), (2, 40, 2053, 1), (3, 400, 257, 1)]
 
 
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16], ids=str)
