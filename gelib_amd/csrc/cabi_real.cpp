@@ -128,7 +128,7 @@ int gelib_hip_linear_act_fwd(void *y, void *slope, const void *x, const void *w,
   const int64_t out = rows * n_out;
   Memory mem;
   mem.need(y, out * e, e);
-  if (act != GELIB_HIP_ACT_NONE) mem.may(slope, out * e, e);   // (float32 or float16: as wide as the layer's type)
+  if (act != GELIB_HIP_ACT_NONE) mem.may(slope, out * e, e);   // (as wide as the layer's type)
   if (out && n_in) mem.need(x, ((rows - 1) * x_row_stride + n_in) * e, row_align(e, n_in)), mem.need(w, (int64_t)n_in * n_out * e, row_align(e, n_out));
   mem.may(bias, (int64_t)n_out * e, e);
   mem.may(residual, out * e, e);

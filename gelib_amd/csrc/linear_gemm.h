@@ -52,8 +52,11 @@ typedef short s16x8 __attribute__((ext_vector_type(8)));
 typedef bhalf_t bf16x8 __attribute__((ext_vector_type(8)));
 typedef half_t f16x8 __attribute__((ext_vector_type(8)));
 
+// what act'(z) is kept in: float16 is 1/8 of a bfloat16 layer's rounding
 template <typename T>
 struct SlopeOf { typedef half_t type; };
+template <>
+struct SlopeOf<half_t> { typedef slope16_t type; };
 template <>
 struct SlopeOf<float> { typedef float type; };
 
