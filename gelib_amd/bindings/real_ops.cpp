@@ -2,7 +2,10 @@
 // are checked and results allocated here, one call of the C ABI does the rest on torch's current stream of the tensors' GPU.
 // (A step over hundreds of parameters, or a layer on a few rows, would spend longer in Python than on the GPU.)
 #include <torch/extension.h>
+#include <c10/core/impl/LocalDispatchKeySet.h>
+#include <c10/core/impl/TorchDispatchModeTLS.h>
 #include <c10/hip/HIPStream.h>
+#include <torch/csrc/jit/frontend/tracer.h>
 
 #include "real_ops.h"
 
@@ -45,6 +48,18 @@ at::Tensor plain(const at::Tensor &t) {
   const at::Tensor p = t.resolve_neg().contiguous();
   return p.numel() && (uintptr_t)p.data_ptr() % 16 ? p.clone() : p;
 }
+
+// Is a call left to torch's own operations?  Only they know of forward-mode derivatives, function transforms, tracing and dispatch modes
+// (shapes without data, counters of operations): a kernel would read the memory below, and its result would be a constant to them.
+bool left_to_torch(std::initializer_list<const at::Tensor *> ts) {
+  if (torch::jit::tracer::isTracing() || c10::impl::TorchDispatchModeTLS::any_modes_set() ||
+      c10::impl::tls_is_dispatch_key_included(c10::DispatchKey::FuncTorchDynamicLayerFrontMode))
+    return true;
+  for (const at::Tensor *t : ts)
+    if (t && t->defined() && (t->_fw_grad(/*level=*/0).defined() || t->unsafeGetTensorImpl()->is_python_dispatch())) return true;
+  return false;
+}
+const at::Tensor *address(const Maybe &t) { return t ? &*t : nullptr; }
 
 void *ptr(const at::Tensor &t) { return t.defined() && t.numel() ? t.data_ptr() : nullptr; }
 
@@ -101,6 +116,9 @@ NormShape norm_shape(const at::Tensor &t) {
   return r;
 }
 
+void eps_check(double eps) {
+  if (!(eps >= 0)) throw py::value_error("GElib: eps is not below zero");
+}
 void norm_check(const at::Tensor &x, int64_t groups, const Maybe &w, const Maybe &b, const Maybe &lengths) {
   on_gpu(x);
   type_of(x);
@@ -123,7 +141,7 @@ std::tuple<at::Tensor, at::Tensor> norm_fwd(const at::Tensor &x, int64_t groups,
                                                         const std::string &act, const Maybe &lengths, bool keep) {
   norm_check(x, groups, w, b, lengths);
   const int a = act_of(act);
-  if (!(eps >= 0)) throw py::value_error("GElib: eps is not below zero");
+  eps_check(eps);
   OnDevice on(x);
   NormShape s = norm_shape(x);
   at::Tensor W = w ? plain(*w) : at::Tensor(), B = b ? plain(*b) : at::Tensor(), L = lengths ? lengths->contiguous() : at::Tensor();
@@ -155,9 +173,10 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor> norm_bwd(const at::Tensor &gy_, c
   return {gx, gw, gb};
 }
 
-// The same from torch's own operations: for gradients of gradients.
+// The same from torch's own operations: for gradients of gradients, and where only torch's operations will do.
+// (silu as a product: the gradient of torch's silu has no forward-mode derivative)
 at::Tensor activated(const at::Tensor &z, int64_t act) {
-  return act == GELIB_HIP_ACT_RELU ? at::relu(z) : act == GELIB_HIP_ACT_SILU ? at::silu(z) : act == GELIB_HIP_ACT_GELU ? at::gelu(z) : z;
+  return act == GELIB_HIP_ACT_RELU ? at::relu(z) : act == GELIB_HIP_ACT_SILU ? z * at::sigmoid(z) : act == GELIB_HIP_ACT_GELU ? at::gelu(z) : z;
 }
 at::Tensor norm_from_torch(const at::Tensor &x, const at::Tensor &w, const at::Tensor &b, const at::Tensor &lengths, int64_t groups, double eps, int64_t act) {
   const int64_t n = x.size(0), c = x.size(-1);
@@ -180,9 +199,10 @@ at::Tensor norm_from_torch(const at::Tensor &x, const at::Tensor &w, const at::T
   return t.to(x.scalar_type());
 }
 
-// Gradients with a graph of their own of f(tensors) for those that need one.
+// Gradients of f(tensors) for those that need one, with a graph of their own where the caller wants one.
 template <typename F>
 variable_list graph_grads(F f, const variable_list &tensors, const at::Tensor &g) {
+  const bool graph = at::GradMode::is_enabled();
   at::AutoGradMode on(true);
   variable_list views, wanted, grads(tensors.size());
   for (const at::Tensor &t : tensors) {
@@ -190,7 +210,7 @@ variable_list graph_grads(F f, const variable_list &tensors, const at::Tensor &g
     if (t.defined() && t.requires_grad()) wanted.push_back(views.back());
   }
   if (wanted.empty()) return grads;
-  const variable_list got = torch::autograd::grad({f(views)}, wanted, {g}, /*retain_graph=*/true, /*create_graph=*/true);
+  const variable_list got = torch::autograd::grad({f(views)}, wanted, {g}, /*retain_graph=*/graph, /*create_graph=*/graph);
   size_t k = 0;
   for (size_t i = 0; i < tensors.size(); i++)
     if (tensors[i].defined() && tensors[i].requires_grad()) grads[i] = got[k++];
@@ -216,7 +236,7 @@ struct NormFn : torch::autograd::Function<NormFn> {
     const int64_t how = ctx->saved_data["how"].toInt(), groups = how / 4, act = how % 4;
     variable_list grads(7);
     if (!g[0].defined()) return grads;
-    if (at::GradMode::is_enabled()) {   // a graph of the gradients is wanted
+    if (at::GradMode::is_enabled() || left_to_torch({&g[0], &x, &w, &b})) {   // a graph of the gradients is wanted, or their tangents
       const double eps = ctx->saved_data["eps"].toDouble();
       const variable_list got = graph_grads([&](const variable_list &v) { return norm_from_torch(v[0], v[1], v[2], lengths, groups, eps, act); }, {x, w, b}, g[0]);
       std::copy(got.begin(), got.end(), grads.begin());
@@ -231,6 +251,11 @@ struct NormFn : torch::autograd::Function<NormFn> {
 };
 
 at::Tensor group_norm_act(const at::Tensor &x, int64_t groups, const Maybe &w, const Maybe &b, double eps, const std::string &act, const Maybe &lengths) {
+  if (left_to_torch({&x, address(w), address(b), address(lengths)})) {
+    norm_check(x, groups, w, b, lengths);
+    eps_check(eps);
+    return norm_from_torch(x, some(w), some(b), some(lengths), groups, eps, act_of(act));
+  }
   if (at::GradMode::is_enabled() && (x.requires_grad() || (w && needs(*w)) || (b && needs(*b)))) {
     norm_check(x, groups, w, b, lengths);   // (refusals come before anything is recorded)
     return NormFn::apply(x, w, b, groups, eps, act, lengths);
@@ -277,9 +302,9 @@ void linear_check(const at::Tensor &x, const at::Tensor &w) {
   if (w.size(0) > 0x7fffffff || w.size(1) > 0x7fffffff) throw py::value_error("GElib: too many channels");
 }
 
-std::tuple<at::Tensor, at::Tensor> linear_fwd(const at::Tensor &x, const at::Tensor &w, const Maybe &b, const Maybe &r, const std::string &act, bool keep) {
+// the shape of the result, which bias and residual fit
+std::vector<int64_t> linear_shape(const at::Tensor &x, const at::Tensor &w, const Maybe &b, const Maybe &r) {
   linear_check(x, w);
-  const int a = act_of(act);
   std::vector<int64_t> shape(x.sizes().begin(), x.sizes().end());
   shape.back() = w.size(1);
   if (b) {
@@ -290,6 +315,12 @@ std::tuple<at::Tensor, at::Tensor> linear_fwd(const at::Tensor &x, const at::Ten
     like(*r, x, "residual");
     if (r->sizes() != at::IntArrayRef(shape)) throw py::value_error("GElib: residual is shaped like the result");
   }
+  return shape;
+}
+
+std::tuple<at::Tensor, at::Tensor> linear_fwd(const at::Tensor &x, const at::Tensor &w, const Maybe &b, const Maybe &r, const std::string &act, bool keep) {
+  const std::vector<int64_t> shape = linear_shape(x, w, b, r);
+  const int a = act_of(act);
   OnDevice on(x);
   Rows X = rows_of(x);
   at::Tensor W = plain(w), B = b ? plain(*b) : at::Tensor(), R = r ? plain(*r) : at::Tensor();
@@ -323,10 +354,12 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor> linear_bwd(const at::Tensor &gy_,
   return {gx, gw, gb};
 }
 
-at::Tensor linear_from_torch(const at::Tensor &x, const at::Tensor &w, const at::Tensor &b, int64_t act) {
+at::Tensor linear_from_torch(const at::Tensor &x, const at::Tensor &w, const at::Tensor &b, const at::Tensor &r, int64_t act) {
   at::Tensor z = at::matmul(x.to(at::kFloat), w.to(at::kFloat));
   if (b.defined()) z = z + b.to(at::kFloat);
-  return activated(z, act).to(x.scalar_type());
+  z = activated(z, act);
+  if (r.defined()) z = z + r.to(at::kFloat);
+  return z.to(x.scalar_type());
 }
 
 // Keeps act'(x w + bias) for the backward pass: the product is not formed again, and nothing else of its size is kept.
@@ -348,8 +381,8 @@ struct LinearFn : torch::autograd::Function<LinearFn> {
                need_r = how % 2 && ctx->needs_input_grad(++at);
     if (need_r) grads[3] = g[0];
     if (!need_x && !need_w && !need_b) return grads;
-    if (at::GradMode::is_enabled()) {   // a graph of the gradients is wanted
-      const variable_list got = graph_grads([&](const variable_list &v) { return linear_from_torch(v[0], v[1], v[2], act); }, {x, w, b}, g[0]);
+    if (at::GradMode::is_enabled() || left_to_torch({&g[0], &x, &w, &b})) {   // a graph of the gradients is wanted, or their tangents
+      const variable_list got = graph_grads([&](const variable_list &v) { return linear_from_torch(v[0], v[1], v[2], {}, act); }, {x, w, b}, g[0]);
       std::copy(got.begin(), got.end(), grads.begin());
       return grads;
     }
@@ -360,6 +393,10 @@ struct LinearFn : torch::autograd::Function<LinearFn> {
 };
 
 at::Tensor linear_act(const at::Tensor &x, const at::Tensor &w, const Maybe &b, const Maybe &r, const std::string &act) {
+  if (left_to_torch({&x, &w, address(b), address(r)})) {
+    linear_shape(x, w, b, r);
+    return linear_from_torch(x, w, some(b), some(r), act_of(act));
+  }
   if (at::GradMode::is_enabled() && (x.requires_grad() || w.requires_grad() || (b && needs(*b)) || (r && needs(*r)))) {
     linear_check(x, w);   // (refusals come before anything is recorded)
     return LinearFn::apply(x, w, b, r, act);

@@ -11,5 +11,6 @@ def group_norm_act(x, groups, weight=None, bias=None, eps=1e-5, act="none", leng
     padded molecule, cells of a smaller grid) over its first lengths[n] positions, counted through all dimensions between the first
     and the last: the others are not read, and are zero in the result and in the gradient of x.  act: "none", "relu", "silu" or
     "gelu" (with the error function).  weight and bias: one value a channel, of x's type.  Statistics are formed in float32 around
-    the mean; results are rounded to x's type once.  Differentiable in x, weight and bias, twice by torch's own operations."""
+    the mean; results are rounded to x's type once.  Differentiable in x, weight and bias, twice by torch's own operations, which
+    forward-mode derivatives, function transforms, tracing and dispatch modes get from the start."""
     return backend().group_norm_act(x, groups, weight, bias, eps, act, lengths)

@@ -9,5 +9,5 @@ def linear_act(x, w, bias=None, residual=None, act="none"):
     act: "none", "relu", "silu" or "gelu" (with the error function); bias (n_out), residual (..., n_out).  The product is summed in
     float32 and the result rounded once.  Differentiable in all four tensors, twice by torch's own operations; the forward pass keeps
     act'(x w + bias) for it, and in 16-bit layers the gradient that enters the two products of the backward pass is rounded to the
-    layer's type."""
+    layer's type.  Forward-mode derivatives, function transforms, tracing and dispatch modes get torch's own operations."""
     return backend().linear_act(x, w, bias, residual, act)
