@@ -286,7 +286,7 @@ __global__ void __launch_bounds__(1024) few_rows_kernel(const LinearArgs l, int 
       for (int e = threadIdx.x; e < left * cols; e += 1024) few_lds[e] += few_lds[e + left * cols];
     }
     __syncthreads();
-    const long long n = n0 + threadIdx.x, at = m * l.N + n;
+    const long long n = n0 + threadIdx.x, at = (long long)m * l.N + n;
     if (m >= l.rows || (int)threadIdx.x >= cols || n >= l.N) continue;
     float z = 0.f, y, slope;
     for (int g = 0; g < left; g++) z += few_lds[g * cols + threadIdx.x];
@@ -301,7 +301,10 @@ __global__ void __launch_bounds__(1024) few_rows_kernel(const LinearArgs l, int 
 // Which forward products go there: up to four rows, while a thread's loads are one or two batches.  bfloat16, here / tiles: 1 x 1024 -> 4096
 // 4.4 / 7.4, 2 x 1024 -> 4096 6.0 / 7.6, 4 x 1024 -> 4096 9.3 / 7.6, 1 x 4096 -> 4096 13.4 / 8.2, 1 x 333 -> 517 4.0 / 9.0, 4 x 333 -> 517
 // 5.7 / 9.1 us; float32: 4 x 1024 -> 4096 7.8 / 8.0, 1 x 4096 -> 4096 15.0 / 16.3, 3 x 4096 -> 64 8.8 / 9.0, 1 x 32768 -> 256 71 / 23 us.
-bool few_rows_case(int dtype, long long rows, int K) { return rows <= 4 && K > 0 && rows * K <= 1024 * (long long)dtype_bytes(dtype) && g_linear_tile < 0; }
+// (1024 threads for 64 columns: beyond 2^28 columns a launch would have more threads than the 2^32 that HIP takes.)
+bool few_rows_case(int dtype, long long rows, int K, int N) {
+  return rows <= 4 && K > 0 && rows * K <= 1024 * (long long)dtype_bytes(dtype) && N <= 1 << 27 && g_linear_tile < 0;
+}
 
 template <typename T, int V, int M>
 void launch_few(const LinearArgs &l, hipStream_t s) {
@@ -332,7 +335,7 @@ int few_rows(const LinearArgs &l, hipStream_t s) {
 template <typename T>
 int fwd(int dtype, const LinearArgs &l, hipStream_t s) {
   if (!l.rows || !l.N) return 0;
-  if (few_rows_case(dtype, l.rows, l.K)) return few_rows<T>(l, s);
+  if (few_rows_case(dtype, l.rows, l.K, l.N)) return few_rows<T>(l, s);
   GemmArgs a = {};
   a.lda = l.xs, a.ldb = l.N;
   Copies<T> copies(l.ws);
@@ -409,7 +412,7 @@ int bwd(int dtype, const LinearArgs &l, hipStream_t s) {
 }  // namespace
 
 size_t linear_workspace(int what, int dtype, long long rows, int K, int N) {
-  if (what == 0 && few_rows_case(dtype, rows, K)) return 0;
+  if (what == 0 && few_rows_case(dtype, rows, K, N)) return 0;
   if (what == 0) return copy_bytes(dtype, rows, K) + copy_bytes(dtype, K, N) + part_bytes(dtype, rows, N, K, out_bytes(kFormXW, dtype));
   size_t n = 0, parts = 0;
   const int V = 16 / (int)dtype_bytes(dtype);

@@ -1,0 +1,42 @@
+"""The operators on real channels at sizes where 32-bit indexes and the limits of a launch end.  Rows and columns that are compared
+are few; everything else is there to be counted past."""
+import ctypes
+
+import pytest
+import torch
+
+import gelib_amd as gelib
+from gelib_amd import cabi
+
+i64 = ctypes.c_int64
+
+
+@pytest.fixture(autouse=True)
+def memory():
+    yield
+    if torch.cuda.is_available():
+        torch.cuda.empty_cache()
+
+
+def linear_workspace(what, dtype, rows, k, n):
+    return cabi.lib().gelib_hip_linear_act_workspace_bytes(what, dtype, i64(rows), k, n)
+
+
+def test_a_few_rows_of_many_columns_go_to_the_tiles():
+    """Without a workspace: one launch without tiles.  A row of one value is copied to 16 bytes for the tiles."""
+    assert linear_workspace(0, 1, 4, 1, 1 << 27) == 0
+    for n in (1 << 28, 800000000, 2000000000):
+        assert linear_workspace(0, 1, 4, 1, n) > 0
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("n", [1 << 27, (1 << 28) + 8, 800000000])
+def test_a_few_rows_of_many_columns(n):
+    """The last row's last result lies behind 2^31 elements at 800 million columns (y: 6.4 GB)."""
+    x = torch.tensor([[1.0], [-2.0], [3.0], [0.5]], device="cuda", dtype=torch.bfloat16)
+    w = torch.ones(1, n, device="cuda", dtype=torch.bfloat16)
+    w[0, -3:] = torch.tensor([4.0, 5.0, 6.0])
+    y = gelib.linear_act(x, w)
+    assert y.shape == (4, n)
+    for m in range(4):
+        assert (y[m, :-3] == x[m]).all() and torch.equal(y[m, -3:], x[m] * w[0, -3:])
