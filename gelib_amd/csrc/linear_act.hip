@@ -169,7 +169,7 @@ struct Copies {
     if (cols % V == 0 || rows == 0 || cols == 0) return p;
     auto &m = a.m[a.count++];
     m = {p, ws, stride, rows, a.threads, cols};
-    stride = (cols + V - 1) / V * V;
+    stride = (cols + V - 1LL) / V * V;
     a.threads += rows * (stride / V);
     ws += up((size_t)rows * stride * sizeof(T));
     return m.to;
@@ -180,7 +180,7 @@ struct Copies {
 };
 size_t copy_bytes(int dtype, long long rows, int cols) {
   const int V = 16 / (int)dtype_bytes(dtype);
-  return cols % V ? up((size_t)rows * ((cols + V - 1) / V * 16)) : 0;
+  return cols % V ? up((size_t)rows * ((cols + V - 1LL) / V * 16)) : 0;
 }
 
 // gz = gy slope (slope null: gy), rounded to T, into gz unless that is null (rows of ldz, zeros behind N), and its unrounded column sums over chunks of rows
@@ -301,7 +301,8 @@ __global__ void __launch_bounds__(1024) few_rows_kernel(const LinearArgs l, int 
 // Which forward products go there: up to four rows, while a thread's loads are one or two batches.  bfloat16, here / tiles: 1 x 1024 -> 4096
 // 4.4 / 7.4, 2 x 1024 -> 4096 6.0 / 7.6, 4 x 1024 -> 4096 9.3 / 7.6, 1 x 4096 -> 4096 13.4 / 8.2, 1 x 333 -> 517 4.0 / 9.0, 4 x 333 -> 517
 // 5.7 / 9.1 us; float32: 4 x 1024 -> 4096 7.8 / 8.0, 1 x 4096 -> 4096 15.0 / 16.3, 3 x 4096 -> 64 8.8 / 9.0, 1 x 32768 -> 256 71 / 23 us.
-// (1024 threads for 64 columns: beyond 2^28 columns a launch would have more threads than the 2^32 that HIP takes.)
+// (1024 threads for 64 columns: from 2^28 columns on a launch has 2^32 threads, of which HIP runs what is left after that many, and
+// reports nothing.)
 bool few_rows_case(int dtype, long long rows, int K, int N) {
   return rows <= 4 && K > 0 && rows * K <= 1024 * (long long)dtype_bytes(dtype) && N <= 1 << 27 && g_linear_tile < 0;
 }
@@ -416,7 +417,7 @@ size_t linear_workspace(int what, int dtype, long long rows, int K, int N) {
   if (what == 0) return copy_bytes(dtype, rows, K) + copy_bytes(dtype, K, N) + part_bytes(dtype, rows, N, K, out_bytes(kFormXW, dtype));
   size_t n = 0, parts = 0;
   const int V = 16 / (int)dtype_bytes(dtype);
-  if ((what & 3) && K && (what & 8 || N % V)) n += up((size_t)rows * ((N + V - 1) / V * 16));
+  if ((what & 3) && K && (what & 8 || N % V)) n += up((size_t)rows * ((N + V - 1LL) / V * 16));
   if (what & 4) n += up((size_t)chunks_of(rows, N) * N * 4);
   if (what & 1) n += copy_bytes(dtype, K, N), parts = std::max(parts, part_bytes(dtype, rows, K, N, out_bytes(kFormGW, dtype)));
   if (what & 2) n += copy_bytes(dtype, rows, K), parts = std::max(parts, part_bytes(dtype, K, N, rows, out_bytes(kFormXG, dtype)));

@@ -29,6 +29,15 @@ def test_a_few_rows_of_many_columns_go_to_the_tiles():
         assert linear_workspace(0, 1, 4, 1, n) > 0
 
 
+def test_workspaces_of_wide_odd_rows():
+    """Copies to rows of whole 16 bytes, of 2^31 bytes and more each: the size that is asked for is theirs and what pieces may add."""
+    for dtype, e, n in ((1, 2, (1 << 30) + 1), (0, 4, (1 << 29) + 1), (2, 2, (1 << 31) - 1025)):
+        copy = -(-n * e // 16) * 16
+        assert 0 <= linear_workspace(0, dtype, 5, 8, n) - 8 * copy <= 1024               # w
+        assert 0 <= linear_workspace(0, dtype, 5, n, 8) - 5 * copy <= 64 * 8 * 5 * 4 + 1024   # x, 64 pieces
+        assert 0 <= linear_workspace(8 | 2, dtype, 3, 8, n) - 3 * copy <= 1024           # gz
+
+
 @pytest.mark.gpu
 @pytest.mark.parametrize("n", [1 << 27, (1 << 28) + 8, 800000000])
 def test_a_few_rows_of_many_columns(n):
