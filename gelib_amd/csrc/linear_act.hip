@@ -184,13 +184,14 @@ size_t copy_bytes(int dtype, long long rows, int cols) {
 }
 
 // gz = gy slope (slope null: gy), rounded to T, into gz unless that is null (rows of ldz, zeros behind N), and its unrounded column sums over chunks of rows
-// into sums[chunk][N] unless that is null (col_chunk rows a chunk).  A block: 64 threads of V columns by 4 rows at a time.
+// into sums[chunk][N] unless that is null (col_chunk rows a chunk).  A block: 64 threads of V columns by 4 rows at a time; `colblocks` of
+// them side by side from the `first` on.
 template <typename T, int V>
-__global__ void __launch_bounds__(256) gz_kernel(const T *gy, const typename SlopeOf<T>::type *slope, T *gz, float *sums, long long rows, int N, int ldz, unsigned colblocks, int col_chunk) {
+__global__ void __launch_bounds__(256) gz_kernel(const T *gy, const typename SlopeOf<T>::type *slope, T *gz, float *sums, long long rows, int N, int ldz, unsigned colblocks, unsigned first, int col_chunk) {
   typedef typename SlopeOf<T>::type D;
   __shared__ float lds[4][64 * V];
   const long long chunk = blockIdx.x / colblocks;
-  const long long n = ((long long)(blockIdx.x % colblocks) * 64 + threadIdx.x % 64) * V;
+  const long long n = ((long long)(first + blockIdx.x % colblocks) * 64 + threadIdx.x % 64) * V;
   const int tr = threadIdx.x / 64;
   float sum[V] = {};
   if (V == 1 && gz && n >= N && n < ldz)
@@ -221,21 +222,25 @@ __global__ void __launch_bounds__(256) gz_kernel(const T *gy, const typename Slo
     for (int i = 0; i < V; i++) sums[chunk * N + n + i] = (lds[0][i * 64 + threadIdx.x] + lds[1][i * 64 + threadIdx.x]) + (lds[2][i * 64 + threadIdx.x] + lds[3][i * 64 + threadIdx.x]);
 }
 
-// out[n] = sum over the chunks: 32 columns by 8 runs of chunks a block
+// out[n] = sum over the chunks: 32 columns at a time by 8 runs of chunks a block
 template <typename T>
 __global__ void __launch_bounds__(256) column_join_kernel(const float *sums, T *out, long long chunks, int N) {
   __shared__ float lds[8][32];
-  const int n = blockIdx.x * 32 + threadIdx.x % 32, run = threadIdx.x / 32;
-  float s = 0.f;
-  if (n < N) {
+  const int run = threadIdx.x / 32;
+  for (long long n0 = blockIdx.x * 32LL; n0 < N; n0 += gridDim.x * 32LL) {
+    const long long n = n0 + threadIdx.x % 32;
+    float s = 0.f;
+    if (n < N) {
 #pragma unroll 8
-    for (long long k = run; k < chunks; k += 8) s += sums[k * N + n];
-  }
-  lds[run][threadIdx.x % 32] = s;
-  __syncthreads();
-  if (run == 0 && n < N) {
-    for (int k = 1; k < 8; k++) s += lds[k][threadIdx.x];
-    out[n] = from_f<T>(s);
+      for (long long k = run; k < chunks; k += 8) s += sums[k * N + n];
+    }
+    lds[run][threadIdx.x % 32] = s;
+    __syncthreads();
+    if (run == 0 && n < N) {
+      for (int k = 1; k < 8; k++) s += lds[k][threadIdx.x];
+      out[n] = from_f<T>(s);
+    }
+    __syncthreads();
   }
 }
 
@@ -381,21 +386,23 @@ int bwd(int dtype, const LinearArgs &l, hipStream_t s) {
     const int col_chunk = rows_of_chunk(l.rows, l.N);
     const bool wide = l.N % V == 0 && ((uintptr_t)l.gy | (uintptr_t)l.slope) % 16 == 0;
     const int columns = wide ? 64 * V : 64;
-    const unsigned colblocks = (unsigned)((ldz + columns - 1) / columns);
-    const long long most = std::max(1LL, (1LL << 23) / colblocks);   // chunks of a launch
-    for (long long c = 0; c < chunks; c += most) {
-      const long long m = c * col_chunk, now = std::min(most, chunks - c), rows = std::min(now * col_chunk, l.rows - m);
-      const dim3 grid((unsigned)(now * colblocks));
-      const T *gy = (const T *)l.gy + m * l.N;
-      const D *d = l.slope ? (const D *)l.slope + m * l.N : nullptr;
-      T *to = keep ? (T *)gz + m * ldz : nullptr;
-      float *su = sums ? sums + c * l.N : nullptr;
-      if (wide) hipLaunchKernelGGL((gz_kernel<T, V>), grid, dim3(256), 0, s, gy, d, to, su, rows, l.N, (int)ldz, colblocks, col_chunk);
-      else hipLaunchKernelGGL((gz_kernel<T, 1>), grid, dim3(256), 0, s, gy, d, to, su, rows, l.N, (int)ldz, colblocks, col_chunk);
-    }
+    const unsigned all = (unsigned)((ldz + columns - 1) / columns), side = std::min(all, 1u << 23);   // blocks side by side, in one launch
+    const long long most = (1LL << 23) / side;   // chunks of a launch
+    for (unsigned first = 0; first < all; first += side)
+      for (long long c = 0; c < chunks; c += most) {
+        const unsigned colblocks = std::min(side, all - first);
+        const long long m = c * col_chunk, now = std::min(most, chunks - c), rows = std::min(now * col_chunk, l.rows - m);
+        const dim3 grid((unsigned)(now * colblocks));
+        const T *gy = (const T *)l.gy + m * l.N;
+        const D *d = l.slope ? (const D *)l.slope + m * l.N : nullptr;
+        T *to = keep ? (T *)gz + m * ldz : nullptr;
+        float *su = sums ? sums + c * l.N : nullptr;
+        if (wide) hipLaunchKernelGGL((gz_kernel<T, V>), grid, dim3(256), 0, s, gy, d, to, su, rows, l.N, (int)ldz, colblocks, first, col_chunk);
+        else hipLaunchKernelGGL((gz_kernel<T, 1>), grid, dim3(256), 0, s, gy, d, to, su, rows, l.N, (int)ldz, colblocks, first, col_chunk);
+      }
   }
   if (l.gb && l.N)
-    hipLaunchKernelGGL((column_join_kernel<T>), dim3((l.N + 31) / 32), dim3(256), 0, s, (const float *)sums, (T *)l.gb, chunks, l.N);
+    hipLaunchKernelGGL((column_join_kernel<T>), dim3((unsigned)std::min((l.N + 31LL) / 32, 1LL << 22)), dim3(256), 0, s, (const float *)sums, (T *)l.gb, chunks, l.N);
   GemmArgs a = {};
   if (gx) {
     a.a = gz, a.lda = ldz, a.b = w, a.ldb = ldw, a.c = l.gx;

@@ -18,6 +18,13 @@ def memory():
         torch.cuda.empty_cache()
 
 
+def scribbled(sizes):
+    """Memory of these sizes that the next allocations get holds sixes: what is not written does not pass for a result."""
+    torch.cuda.empty_cache()
+    ts = [torch.full((n,), 0x66, device="cuda", dtype=torch.uint8) for n in sizes]
+    del ts
+
+
 def linear_workspace(what, dtype, rows, k, n):
     return cabi.lib().gelib_hip_linear_act_workspace_bytes(what, dtype, i64(rows), k, n)
 
@@ -49,3 +56,22 @@ def test_a_few_rows_of_many_columns(n):
     assert y.shape == (4, n)
     for m in range(4):
         assert (y[m, :-3] == x[m]).all() and torch.equal(y[m, -3:], x[m] * w[0, -3:])
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("n", [(1 << 29) + 8, (1 << 30) + 1])
+def test_column_sums_of_many_columns(n):
+    """One row, so every sum is one value; behind 2^30 columns of an odd number also the copy of the gradient to aligned rows."""
+    x = torch.full((1, 1), 2.0, device="cuda", dtype=torch.bfloat16, requires_grad=True)
+    w = torch.zeros(1, n, device="cuda", dtype=torch.bfloat16)
+    w[0, -4:] = torch.tensor([1.0, 2.0, 3.0, 4.0])
+    w.requires_grad_()
+    b = torch.zeros(n, device="cuda", dtype=torch.bfloat16, requires_grad=True)
+    g = torch.ones(1, n, device="cuda", dtype=torch.bfloat16)
+    g[0, ::1000003] = 5.0
+    g[0, -1] = 7.0
+    y = gelib.linear_act(x, w, b)
+    scribbled(3 * [2 * n] + [4 * n])
+    gx, gw, gb = torch.autograd.grad(y, (x, w, b), g)
+    assert torch.equal(gb, g[0]) and torch.equal(gw, 2 * g)
+    assert gx.item() == (g[0, -4:] * w[0, -4:]).sum().item()
