@@ -299,7 +299,7 @@ void linear_check(const at::Tensor &x, const at::Tensor &w) {
   type_of(x);
   like(w, x, "w");
   if (x.dim() < 1 || w.dim() != 2 || w.size(0) != x.size(-1)) throw py::value_error("GElib: x (..., n_in) and w (n_in, n_out) are needed");
-  if (w.size(0) > 0x7fffffff || w.size(1) > 0x7fffffff) throw py::value_error("GElib: too many channels");
+  if (std::max(w.size(0), w.size(1)) > 0x7fffff00) throw py::value_error("GElib: too many channels");
 }
 
 // the shape of the result, which bias and residual fit

@@ -48,7 +48,7 @@ int norm_shape(int dtype, int act, int64_t N, int64_t S, int C, int G, int64_t x
 unsigned row_align(unsigned e, int64_t cols) { return cols * e % 16 == 0 ? 16 : e; }
 
 int linear_shape(int dtype, int act, int64_t rows, int K, int N, int64_t xs) {
-  if (!types_ok(dtype, act) || rows < 0 || K < 0 || N < 0 || xs < 0) return GELIB_HIP_ERR_ARG;
+  if (!types_ok(dtype, act) || rows < 0 || K < 0 || N < 0 || xs < 0 || std::max(K, N) > kLinearMostChannels) return GELIB_HIP_ERR_ARG;
   if (!product_ok(rows, K) || !product_ok(rows, N) || !product_ok(rows, xs)) return GELIB_HIP_ERR_ARG;
   const unsigned e = (unsigned)dtype_bytes(dtype);
   if (rows > 1 && xs * e % row_align(e, K) != 0) return GELIB_HIP_ERR_ARG;

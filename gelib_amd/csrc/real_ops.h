@@ -39,6 +39,7 @@ struct LinearArgs {
   int K, N, act;
   void *ws;
 };
+constexpr int kLinearMostChannels = 0x7fffff00;   // of either side: rounded up to whole tiles and vectors they stay below 2^31, and a row of tiles below 2^32 threads
 size_t linear_workspace(int backward, int dtype, long long rows, int K, int N);   // backward: bits 1 gx, 2 gw, 4 gb, 8 slope; 0 forward
 int launch_linear_fwd(int dtype, const LinearArgs &a, hipStream_t s);
 int launch_linear_bwd(int dtype, const LinearArgs &a, hipStream_t s);

@@ -291,7 +291,8 @@ uint64_t gelib_hip_group_norm_act_workspace_bytes(int backward, int dtype, int64
                                                   int groups);
 
 /* Linear layer: z = x w + bias, y = act(z) + residual; x (rows, n_in) at a row stride, w (n_in, n_out) as the matrices of
- * SO3weights, bias (n_out) and residual (rows, n_out) may be NULL; y packed.  An operand whose rows are a multiple of 16 bytes
+ * SO3weights, bias (n_out) and residual (rows, n_out) may be NULL; y packed.  n_in and n_out are at most 2^31 - 256
+ * (GELIB_HIP_ERR_ARG beyond).  An operand whose rows are a multiple of 16 bytes
  * long (x, w, gy) starts at one and has a row stride that is one (GELIB_HIP_ERR_ARG otherwise); others are copied to such rows.
  * slope (NULL: not wanted; not written where act is GELIB_HIP_ACT_NONE): act'(z) for the backward pass, (rows, n_out) values as wide
  * as the layer's type: float32 for float32 layers, float16 for bfloat16 ones, a 16-bit code for float16 ones that only the

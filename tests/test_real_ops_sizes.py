@@ -45,6 +45,18 @@ def test_workspaces_of_wide_odd_rows():
         assert 0 <= linear_workspace(8 | 2, dtype, 3, 8, n) - 3 * copy <= 1024           # gz
 
 
+def test_widths_that_do_not_round_up_within_31_bits():
+    """Widths are rounded up to vectors and tiles: within 255 of 2^31 they are refused, by either side, before anything else is looked at."""
+    L, vp = cabi.lib(), ctypes.c_void_p
+    most = (1 << 31) - 256
+    for k, n in ((most, 1), (1, most), (most + 1, 1), (1, most + 1), ((1 << 31) - 1, 8), (8, (1 << 31) - 1)):
+        args = (1, i64(2), k, n, i64(k))
+        fwd = L.gelib_hip_linear_act_fwd(None, None, None, None, None, None, *args, 0, None, 0, None)
+        bwd = L.gelib_hip_linear_act_bwd(None, None, None, None, None, None, None, *args, None, 0, None)
+        assert (fwd, bwd) == ((1, 1) if max(k, n) <= most else (12, 12))
+        assert (linear_workspace(2, 1, 2, k, n) == 0) == (max(k, n) > most)
+
+
 @pytest.mark.gpu
 @pytest.mark.parametrize("n", [1 << 27, (1 << 28) + 8, 800000000])
 def test_a_few_rows_of_many_columns(n):
