@@ -54,7 +54,9 @@ Plan plan_of(int dtype, long long M, long long N, long long K, int out) {
     if (g_linear_tile >= 0 && t != g_linear_tile) continue;
     const TileCost &c = dtype == GELIB_HIP_F32 ? kCost32[t] : kCost16[t];
     const double tiles = std::ceil((double)M / kGemmBM[t]) * std::ceil((double)N / kGemmBN[t]);
-    for (long long want = g_linear_splits > 0 ? std::min<long long>(g_linear_splits, steps) : 1; want <= 64 && want <= steps; want *= 2) {
+    // pieces only where all tiles go into one launch (the rows of a piece begin at its first), and the threads of the join
+    const int forced = tiles > (1 << 22) || results > 0x1p32 ? 1 : g_linear_splits;
+    for (long long want = forced > 0 ? std::min<long long>(forced, steps) : 1; want <= 64 && want <= steps; want *= 2) {
       const long long per = (steps + want - 1) / want, pieces = (steps + per - 1) / per;
       const double blocks = std::ceil(tiles * pieces / 256), rounds = std::floor(blocks / c.fit), rest = blocks - rounds * c.fit;
       double us = per * (rounds * std::max(c.alone, c.fit * c.full) + (rest > 0 ? std::max(c.alone, rest * c.full) : 0)) + 1.5 * (rounds + (rest > 0));
@@ -62,7 +64,7 @@ Plan plan_of(int dtype, long long M, long long N, long long K, int out) {
       us = c.fit > 1 ? std::max(us, write) + 0.3 * write : us + write;
       if (pieces > 1) us += 4 + results * (4.0 * pieces + out) / 2.5e6;
       if (best.splits == 0 || us < least) least = us, best = {t, (int)pieces, per * bk};
-      if (g_linear_splits > 0) break;
+      if (forced > 0) break;
     }
   }
   return best;

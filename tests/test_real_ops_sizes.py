@@ -57,6 +57,36 @@ def test_widths_that_do_not_round_up_within_31_bits():
         assert (linear_workspace(2, 1, 2, k, n) == 0) == (max(k, n) > most)
 
 
+@pytest.fixture
+def two_pieces():
+    cabi.set_option("linear_act_tile", 3)
+    cabi.set_option("linear_act_splits", 2)
+    yield
+    cabi.set_option("linear_act_tile", -1)
+    cabi.set_option("linear_act_splits", 0)
+
+
+MANY_ROWS = (1 << 26) + 100   # more than 2^22 tiles of 16 rows: two launches
+
+
+def test_products_of_several_launches_are_not_cut_into_pieces(two_pieces):
+    assert linear_workspace(0, 1, 1000, 72, 8) >= 2 * 1000 * 8 * 4
+    assert linear_workspace(0, 1, MANY_ROWS, 72, 8) == 0
+
+
+@pytest.mark.gpu
+def test_rows_of_several_launches(two_pieces):
+    x = torch.zeros(MANY_ROWS, 72, device="cuda", dtype=torch.bfloat16)
+    x[:200].normal_()
+    x[-200:].normal_()
+    w = torch.randn(72, 8, device="cuda").bfloat16()
+    y = gelib.linear_act(x, w)
+    for part in (slice(0, 200), slice(-200, None)):
+        want = x[part].double() @ w.double()
+        assert ((y[part].double() - want).abs() <= 2.0 ** -8 * want.abs() + 80 * 2.0 ** -24 * (x[part].double().abs() @ w.double().abs())).all()
+    assert not y[200:-200].any()
+
+
 @pytest.mark.gpu
 @pytest.mark.parametrize("n", [1 << 27, (1 << 28) + 8, 800000000])
 def test_a_few_rows_of_many_columns(n):
