@@ -44,6 +44,7 @@ struct NormDev {
   float *stats;   // in chunks, forward: [n][chunk][G pieces] mean and sum of squares; backward: [n][chunk][2][C]
   float *sums;    // backward: [blocks or n][2][C] channel sums of gz xh and of gz
   float *means;   // in chunks, backward: [n][G pieces][2] mean of q and of q xh
+  long long first[3];   // in chunks: chunk, stripe and sample of the launch's first block
 };
 
 template <typename T>
@@ -119,7 +120,7 @@ __device__ __forceinline__ Place place_of(const NormDev &d) {
   w.tx = t - rest * d.p.TX;
   w.ty = rest / d.p.NS;
   w.ns = rest - w.ty * d.p.NS;
-  w.c0 = blockIdx.y * d.p.Cw;
+  w.c0 = ((int)d.first[1] + blockIdx.y) * d.p.Cw;
   w.cw = min(d.p.Cw, d.a.C - w.c0);
   w.col = w.ns * d.p.Cw + w.tx * d.p.V;
   w.on = w.ty < d.p.TY && w.tx * d.p.V < w.cw;
@@ -482,14 +483,14 @@ __global__ void __launch_bounds__(kNormMostT) norm_whole_bwd(const NormDev d) {
 
 // ---- samples in chunks ----
 
-// mean and sum of squares of a chunk's groups: block (chunk, stripe) of sample blockIdx.z
+// mean and sum of squares of a chunk's groups: a block a chunk, stripe and sample
 template <typename T, int V>
-__global__ void __launch_bounds__(kNormChunkT) norm_chunk_stats(const NormDev d, long long nbase) {
+__global__ void __launch_bounds__(kNormChunkT) norm_chunk_stats(const NormDev d) {
   const Place w = place_of(d);
   const Lds l = lds_of(d);
   const NormArgs &a = d.a;
   const int cg = a.C / a.G;
-  const long long n = nbase + blockIdx.z, s0 = blockIdx.x * d.p.rows, len = max(0LL, min(d.p.rows, length_of(a, n) - s0));
+  const long long n = d.first[2] + blockIdx.z, chunk = d.first[0] + blockIdx.x, s0 = chunk * d.p.rows, len = max(0LL, min(d.p.rows, length_of(a, n) - s0));
   const T *x = (const T *)a.x + n * a.xs + s0 * a.xp + w.c0 + w.tx * V;
   Pack<T, V> xr[kNormMostR];
 #pragma unroll
@@ -500,17 +501,18 @@ __global__ void __launch_bounds__(kNormChunkT) norm_chunk_stats(const NormDev d,
   int g[V];
   groups_of<V>(d, w, g);
   block_stats<T, V, kNormMostR>(d, w, g, xr, len, l.scratch, l.chan, l.first, l.second);
-  float *to = d.stats + ((n * d.p.chunks + blockIdx.x) * a.G + w.c0 / cg) * 2;
+  float *to = d.stats + ((n * d.p.chunks + chunk) * a.G + w.c0 / cg) * 2;
   for (int k = threadIdx.x; k < w.cw / cg; k += d.p.T) to[2 * k] = l.first[k], to[2 * k + 1] = l.second[k];
 }
 
-// The chunks of a sample joined, and the pieces of a group: W waves a group.  One where they are few; 16 from 1024 entries on, which
-// only groups in many pieces have (64 x 512 x 4099, 131 k entries a group: forward 2280 us with one wave and a division an entry, 384 so).
+// The chunks of a sample joined, and the pieces of a group: W waves a group, of the groups from `base` on.  One where they are few; 16
+// from 1024 entries on, which groups in many pieces have (64 x 512 x 4099, 131 k entries a group: forward 2280 us with one wave and a
+// division an entry, 384 so) and very long samples.
 template <int W>
-static __global__ void __launch_bounds__(W == 1 ? 256 : 64 * W) norm_stats_join(const NormDev d) {
+static __global__ void __launch_bounds__(W == 1 ? 256 : 64 * W) norm_stats_join(const NormDev d, long long base) {
   const NormArgs &a = d.a;
   constexpr int kGroups = W == 1 ? 4 : 1, kStep = 64 * W;
-  const long long at = (long long)blockIdx.x * kGroups + threadIdx.x / kStep, n = at / a.G;
+  const long long at = base + (long long)blockIdx.x * kGroups + threadIdx.x / kStep, n = at / a.G;
   const int g = (int)(at - n * a.G), t = threadIdx.x % kStep;
   if (n >= a.N) return;   // (whole waves; whole blocks where W is more than one)
   const long long len = length_of(a, n), stride = (long long)a.G * d.p.pieces * 2;
@@ -556,11 +558,11 @@ static __global__ void __launch_bounds__(W == 1 ? 256 : 64 * W) norm_stats_join(
 
 // second pass: y of a chunk
 template <typename T, int V, int ACT>
-__global__ void __launch_bounds__(kNormChunkT) norm_apply_fwd(const NormDev d, long long nbase) {
+__global__ void __launch_bounds__(kNormChunkT) norm_apply_fwd(const NormDev d) {
   const Place w = place_of(d);
   if (!w.on) return;
   const NormArgs &a = d.a;
-  const long long n = nbase + blockIdx.z, s0 = blockIdx.x * d.p.rows, len = length_of(a, n), end = min(s0 + d.p.rows, a.S);
+  const long long n = d.first[2] + blockIdx.z, chunk = d.first[0] + blockIdx.x, s0 = chunk * d.p.rows, len = length_of(a, n), end = min(s0 + d.p.rows, a.S);
   float B[V], mu[V], k[V];
   int g[V];
   load_channels<T, V>(a.w, w, 1.f, k);
@@ -597,12 +599,12 @@ __global__ void __launch_bounds__(kNormChunkT) norm_apply_fwd(const NormDev d, l
 
 // channel sums of gz and gz xh of a chunk
 template <typename T, int V, int ACT>
-__global__ void __launch_bounds__(kNormChunkT) norm_chunk_sums(const NormDev d, long long nbase) {
+__global__ void __launch_bounds__(kNormChunkT) norm_chunk_sums(const NormDev d) {
   const Place w = place_of(d);
   const Lds l = lds_of(d);
   const NormArgs &a = d.a;
   const int cg = a.C / a.G;
-  const long long n = nbase + blockIdx.z, s0 = blockIdx.x * d.p.rows, end = min(s0 + d.p.rows, length_of(a, n));
+  const long long n = d.first[2] + blockIdx.z, chunk = d.first[0] + blockIdx.x, s0 = chunk * d.p.rows, end = min(s0 + d.p.rows, length_of(a, n));
   float W[V], B[V], mu[V], k[V], s1[V] = {}, s2[V] = {};
   int g[V];
   load_channels<T, V>(a.w, w, 1.f, W);
@@ -634,18 +636,18 @@ __global__ void __launch_bounds__(kNormChunkT) norm_chunk_sums(const NormDev d, 
   }
   column_sums<V>(d, w, s1, l.scratch, l.chan);
   column_sums<V>(d, w, s2, l.scratch, l.chan2);
-  float *to = d.stats + (n * d.p.chunks + blockIdx.x) * 2 * a.C + w.c0;
+  float *to = d.stats + (n * d.p.chunks + chunk) * 2 * a.C + w.c0;
   for (int c = threadIdx.x; c < w.cw; c += d.p.T) to[c] = l.chan2[c], to[a.C + c] = l.chan[c];
 }
 
-// the chunks of a sample joined: block (stripe) of sample blockIdx.z.  32 channels at a time by T / 32 runs of chunks.
+// the chunks of a sample joined: a block a stripe and sample.  32 channels at a time by T / 32 runs of chunks.
 template <typename T>
-__global__ void __launch_bounds__(kNormChunkT) norm_sums_join(const NormDev d, long long nbase) {
+__global__ void __launch_bounds__(kNormChunkT) norm_sums_join(const NormDev d) {
   const Place w = place_of(d);
   const Lds l = lds_of(d);
   const NormArgs &a = d.a;
   const int cg = a.C / a.G, gs = w.cw / cg, runs = d.p.T / 32, run = threadIdx.x / 32;
-  const long long n = nbase + blockIdx.z, len = length_of(a, n);
+  const long long n = d.first[2] + blockIdx.z, len = length_of(a, n);
   const long long chunks = (len + d.p.rows - 1) / d.p.rows;
   __shared__ float part[kNormChunkT / 32][2][33];
   float *lens = l.second + d.p.Cw / cg;
@@ -685,9 +687,9 @@ __global__ void __launch_bounds__(kNormChunkT) norm_sums_join(const NormDev d, l
   for (int k = threadIdx.x; k < gs; k += d.p.T) m[2 * k] = l.first[k], m[2 * k + 1] = l.second[k];
 }
 
-// the means of a group's pieces averaged into the first one's place: a wave a group
-static __global__ void __launch_bounds__(256) norm_means_join(const NormDev d) {
-  const long long at = (long long)blockIdx.x * 4 + threadIdx.x / 64;
+// the means of a group's pieces averaged into the first one's place: a wave a group, of the groups from `base` on
+static __global__ void __launch_bounds__(256) norm_means_join(const NormDev d, long long base) {
+  const long long at = base + (long long)blockIdx.x * 4 + threadIdx.x / 64;
   if (at >= d.a.N * d.a.G) return;
   float *m = d.means + at * d.p.pieces * 2, s = 0.f;
   for (int k = threadIdx.x % 64; k < 2 * d.p.pieces; k += 64) s += m[k];   // (even lanes the first kind, odd ones the second)
@@ -697,11 +699,11 @@ static __global__ void __launch_bounds__(256) norm_means_join(const NormDev d) {
 }
 
 template <typename T, int V, int ACT>
-__global__ void __launch_bounds__(kNormChunkT) norm_apply_bwd(const NormDev d, long long nbase) {
+__global__ void __launch_bounds__(kNormChunkT) norm_apply_bwd(const NormDev d) {
   const Place w = place_of(d);
   if (!w.on) return;
   const NormArgs &a = d.a;
-  const long long n = nbase + blockIdx.z, s0 = blockIdx.x * d.p.rows, len = length_of(a, n), end = min(s0 + d.p.rows, a.S);
+  const long long n = d.first[2] + blockIdx.z, chunk = d.first[0] + blockIdx.x, s0 = chunk * d.p.rows, len = length_of(a, n), end = min(s0 + d.p.rows, a.S);
   float W[V], B[V], mu[V], k[V], m1[V], m2[V];
   int g[V];
   load_channels<T, V>(a.w, w, 1.f, W);
@@ -778,29 +780,39 @@ int run_norm(bool backward, const NormDev &d, hipStream_t s) {
     if (backward && d.sums)
       hipLaunchKernelGGL((norm_join<T>), dim3((2 * a.C + 31) / 32), dim3(256), 0, s, (const float *)d.sums, (T *)a.gw, (T *)a.gb, p.blocks, a.C);
   } else {
-    const long long most = std::min(a.N, 32768LL);   // samples of a launch (its third dimension)
-    auto each = [&](auto kernel, unsigned chunks, size_t bytes) {
-      for (long long n = 0; n < a.N; n += most)
-        hipLaunchKernelGGL(kernel, dim3(chunks, p.stripes, (unsigned)std::min(most, a.N - n)), block, bytes, s, d, n);
+    // A launch takes 2^22 chunks, 32768 stripes and as many samples at most, a join 2^21 groups: from 2^32 threads on HIP runs what is
+    // left after that many, and reports nothing.
+    auto each = [&](auto kernel, NormDev v, long long chunks, size_t bytes) {
+      const long long count[3] = {chunks, v.p.stripes, a.N}, most[3] = {1LL << 22, 32768, 32768};
+      for (v.first[2] = 0; v.first[2] < a.N; v.first[2] += most[2])
+        for (v.first[1] = 0; v.first[1] < count[1]; v.first[1] += most[1])
+          for (v.first[0] = 0; v.first[0] < count[0]; v.first[0] += most[0]) {
+            unsigned n[3];
+            for (int k = 0; k < 3; k++) n[k] = (unsigned)std::min(most[k], count[k] - v.first[k]);
+            hipLaunchKernelGGL(kernel, dim3(n[0], n[1], n[2]), dim3(v.p.T), bytes, s, v);
+          }
+    };
+    auto join = [&](auto kernel, int groups, int threads) {   // groups of a block
+      const long long all = a.N * a.G, most = 1LL << 21;
+      for (long long g = 0; g < all; g += most)
+        hipLaunchKernelGGL(kernel, dim3((unsigned)((std::min(most, all - g) + groups - 1) / groups)), dim3(threads), 0, s, d, g);
     };
     NormDev j = d;   // the kernels that sum groups sum the pieces of them
     j.a.G = a.G * p.pieces;
     const size_t lds = norm_lds_bytes(p, a.C / j.a.G);
     if (!backward) {
-      for (long long n = 0; n < a.N; n += most)
-        hipLaunchKernelGGL((norm_chunk_stats<T, V>), dim3((unsigned)p.chunks, p.stripes, (unsigned)std::min(most, a.N - n)), block, lds, s, j, n);
-      if (p.chunks * p.pieces >= 1024) hipLaunchKernelGGL(norm_stats_join<16>, dim3((unsigned)(a.N * a.G)), dim3(1024), 0, s, d);
-      else hipLaunchKernelGGL(norm_stats_join<1>, dim3((unsigned)((a.N * a.G + 3) / 4)), dim3(256), 0, s, d);
-      each(norm_apply_fwd<T, V, ACT>, (unsigned)p.chunks, 0);
+      each(norm_chunk_stats<T, V>, j, p.chunks, lds);
+      if (p.chunks * p.pieces >= 1024) join(norm_stats_join<16>, 1, 1024);
+      else join(norm_stats_join<1>, 4, 256);
+      each(norm_apply_fwd<T, V, ACT>, d, p.chunks, 0);
     } else {
-      each(norm_chunk_sums<T, V, ACT>, (unsigned)p.chunks, lds);
+      each(norm_chunk_sums<T, V, ACT>, d, p.chunks, lds);
       // (stripes of about 32 channels: their sums are short, blocks are wanted)
       const int cg = a.C / j.a.G, Cq = V / std::gcd(V, cg) * cg;
       j.p.Cw = std::min(p.Cw, std::max(1, 32 / Cq) * Cq), j.p.stripes = (a.C + j.p.Cw - 1) / j.p.Cw, j.p.TX = 1, j.p.TY = 1, j.p.T = kNormChunkT;
-      for (long long n = 0; n < a.N; n += most)
-        hipLaunchKernelGGL((norm_sums_join<T>), dim3(1, j.p.stripes, (unsigned)std::min(most, a.N - n)), dim3(kNormChunkT), norm_lds_bytes(j.p, cg), s, j, n);
-      if (a.y && p.pieces > 1) hipLaunchKernelGGL(norm_means_join, dim3((unsigned)((a.N * a.G + 3) / 4)), dim3(256), 0, s, d);
-      if (a.y) each(norm_apply_bwd<T, V, ACT>, (unsigned)p.chunks, 0);
+      each(norm_sums_join<T>, j, 1, norm_lds_bytes(j.p, cg));
+      if (a.y && p.pieces > 1) join(norm_means_join, 4, 256);
+      if (a.y) each(norm_apply_bwd<T, V, ACT>, d, p.chunks, 0);
       if (a.gw || a.gb)
         hipLaunchKernelGGL((norm_join<T>), dim3((2 * a.C + 31) / 32), dim3(256), 0, s, (const float *)d.sums, (T *)a.gw, (T *)a.gb, a.N, a.C);
     }

@@ -117,3 +117,59 @@ def test_column_sums_of_many_columns(n):
     gx, gw, gb = torch.autograd.grad(y, (x, w, b), g)
     assert torch.equal(gb, g[0]) and torch.equal(gw, 2 * g)
     assert gx.item() == (g[0, -4:] * w[0, -4:]).sum().item()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("n,s,c,groups", [((1 << 22) + 8, 1, 1031, 1), ((1 << 20) + 16, 241, 65, 65)])
+def test_norms_of_many_groups(n, s, c, groups):
+    """More groups than one launch has blocks (1024 threads a group of many pieces) or waves for: the last samples are what they are by
+    themselves, but for the order of sums."""
+    x = torch.zeros(n, s, c, device="cuda", dtype=torch.bfloat16)
+    for part in (x[:3], x[-9:]):
+        part.normal_()
+    scribbled([cabi.lib().gelib_hip_group_norm_act_workspace_bytes(0, 1, i64(n), i64(s), c, groups), x.numel() * 2])
+    y = gelib.group_norm_act(x, groups)
+    for part in (slice(0, 3), slice(-9, None)):
+        alone = gelib.group_norm_act(x[part].contiguous(), groups)
+        assert ((y[part].float() - alone.float()).abs() <= 2.0 ** -7 * alone.float().abs() + 1e-4).all()
+    assert not y[3:-9].any()
+
+
+@pytest.mark.gpu
+def test_norms_of_many_stripes():
+    """16777217 channels in groups of 97 are 86481 stripes of two groups."""
+    from tests.test_gpu_group_norm import check, reference
+    c, groups = 16777217, 172961
+    gen = torch.Generator(device="cuda").manual_seed(1)
+    x, w, b, g = (torch.randn(*k, device="cuda", generator=gen) for k in ((1, 1, c), (c,), (c,), (1, 1, c)))
+    leaves = [t.requires_grad_() for t in (x, w, b)]
+    y = gelib.group_norm_act(x, groups, w, b, act="silu")
+    got = dict(zip(("gx", "gw", "gb"), torch.autograd.grad(y, leaves, g)), y=y.detach())
+    with torch.no_grad():
+        want = reference(x.double(), groups, w.double(), b.double(), 1e-5, "silu", torch.ones(1, device="cuda", dtype=torch.long), g.double())
+    for k, t in got.items():
+        check(t, want[k][0].reshape(t.shape), want[k][1].reshape(t.shape), k)
+
+
+@pytest.mark.gpu
+def test_norms_of_many_chunks():
+    """67 million positions of 129 channels in chunks of 16: more than a launch takes.  Zeros but for both ends, so that the formulas are
+    sums over these; a value is rounded to bfloat16 and the statistics to far less."""
+    s, c = (1 << 26) + 33, 129
+    ends = [slice(0, 40), slice(-40, None)]
+    x, g = (torch.zeros(1, s, c, device="cuda", dtype=torch.bfloat16) for _ in range(2))
+    for t in (x, g):
+        for e in ends:
+            t[0, e].normal_()
+    leaf = x.requires_grad_()
+    y = gelib.group_norm_act(leaf, 1, eps=1e-3)
+    gx, = torch.autograd.grad(y, leaf, g)
+    X, G = (torch.cat([t.detach()[0, e].double() for e in ends]) for t in (x, g))
+    mean = X.sum() / (s * c)
+    rstd = ((X.square().sum()) / (s * c) - mean.square() + 1e-3).rsqrt()
+    xh = (X - mean) * rstd
+    want_y, want_gx = xh, rstd * (G - G.sum() / (s * c) - xh * ((G * xh).sum() / (s * c)))
+    for got, want in ((y, want_y), (gx, want_gx)):
+        mine = torch.cat([got.detach()[0, e].double() for e in ends])
+        assert ((mine - want).abs() <= 2.0 ** -8 * want.abs() + 2.0 ** -12 * want.abs().max()).all()
+        assert got.detach()[0, 40:-40].abs().max() <= 1e-2
