@@ -184,7 +184,7 @@ at::Tensor norm_from_torch(const at::Tensor &x, const at::Tensor &w, const at::T
   if (lengths.defined()) {
     const at::Tensor held = lengths.clamp(0, t.size(1));
     live = at::arange(t.size(1), held.options()).lt(held.unsqueeze(1)).view({n, -1, 1, 1});
-    count = (held.clamp_min(1) * t.size(3)).view({n, 1, 1, 1});
+    count = (held.clamp_min(1).to(at::kLong) * t.size(3)).view({n, 1, 1, 1});   // (2^31 values and more are a large group, not a wrong one)
     t = t.masked_fill(live.logical_not(), 0);
   } else {
     count = at::full({}, (double)t.size(1) * t.size(3), t.options());

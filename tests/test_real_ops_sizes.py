@@ -173,3 +173,19 @@ def test_norms_of_many_chunks():
         mine = torch.cat([got.detach()[0, e].double() for e in ends])
         assert ((mine - want).abs() <= 2.0 ** -8 * want.abs() + 2.0 ** -12 * want.abs().max()).all()
         assert got.detach()[0, 40:-40].abs().max() <= 1e-2
+
+
+@pytest.mark.gpu
+def test_gradients_with_a_graph_of_groups_of_2_31_values():
+    """The gradients that have a graph (torch's operations) are those of the kernels."""
+    s, c = 131073, 16384
+    gen = torch.Generator(device="cuda").manual_seed(2)
+    x, g = (torch.randn(1, s, c, device="cuda", generator=gen, dtype=torch.bfloat16) for _ in range(2))
+    lengths = torch.full((1,), s, device="cuda", dtype=torch.int32)
+    leaf = (x + 3).requires_grad_()
+    y = gelib.group_norm_act(leaf, 1, lengths=lengths)
+    a, = torch.autograd.grad(y, leaf, g, retain_graph=True)
+    b, = torch.autograd.grad(y, leaf, g, create_graph=True)
+    b = b.detach()
+    for part in (slice(0, 500), slice(-500, None)):
+        assert ((a[0, part].float() - b[0, part].float()).abs() <= 2.0 ** -7 * a[0, part].float().abs() + 1e-4).all()
