@@ -98,16 +98,20 @@ struct slope16_t {
 
 enum Act { kActNone = 0, kActRelu = 1, kActSilu = 2, kActGelu = 3 };
 
-// Phi(z), the normal distribution, given e = exp(-z^2 / 2): 1/2 erfc(|z| / sqrt 2) as e times a polynomial in 1 / (1 + p |z| / sqrt 2)
-// (Abramowitz & Stegun, Handbook of Mathematical Functions, 7.1.26: erf to 1.5e-7), reflected for z > 0.  The exponential serves
-// the density in gelu' too: value and slope together are 16 instructions, where the library's erff is 40 and exp comes on top.
+// Phi(z), the normal distribution, given e = exp(-z^2 / 2): 1/2 erfc(|z| / sqrt 2) as e times a polynomial in t = 1 / (1 + p |z| / sqrt 2),
+// reflected for z > 0.  (The form is Abramowitz & Stegun's, Handbook of Mathematical Functions, 7.1.25 to 28; p and seven coefficients are
+// fitted here, for the least largest error of erfc over 0..6: 4e-10, so that what is left is the roundings of float32.)  The exponential
+// serves the density in gelu' too.  Root mean square errors of gelu and gelu' over normally distributed z, in units of 2^-24: 0.41 and 0.63;
+// with the handbook's five coefficients (1.5e-7) 0.93 and 1.10, in the same time (to 1 %); with the library's erff 0.42 and 0.46, at 4 % more
+// time for a float32 layer (32768 x 256 -> 512, both directions) and 11 % for a norm (64 x 1024 x 256).
 __device__ __forceinline__ float normal_cdf(float z, float e) {
-  const float t = __builtin_amdgcn_rcpf(1.f + 0.3275911f * 0.70710678118654752f * __builtin_fabsf(z));
-  const float tail = 0.5f * e * t * (0.254829592f + t * (-0.284496736f + t * (1.421413741f + t * (-1.453152027f + t * 1.061405429f))));
+  const float t = __builtin_amdgcn_rcpf(1.f + 0.47f * 0.70710678118654752f * __builtin_fabsf(z));
+  const float tail = e * (t * (0.13292666f + t * (0.12584779f + t * (0.16198763f + t * (-0.05227607f + t * (0.29318786f + t * (-0.20470048f + t * 0.04302663f)))))));
   return z > 0.f ? 1.f - tail : tail;
 }
 
-// act(z) and act'(z).  exp and the reciprocal are the hardware's (1 ulp): the sums in front of them are the coarser part.
+// act(z) and act'(z).  exp and the reciprocal are the hardware's (1 ulp).  Over normally distributed z silu is 0.47 units of 2^-24 off and
+// silu' 0.49, 0.39 and 0.48 in torch's float32 operations; with the library's expf and a division 0.45 and 0.48, at 2 and 11 % more time for the same two.
 // kActNone stands for relu too where a flag says so.
 template <int ACT>
 __device__ __forceinline__ void act_both(float z, float &value, float &slope, bool relu = false) {
@@ -122,18 +126,6 @@ __device__ __forceinline__ void act_both(float z, float &value, float &slope, bo
   } else {
     value = z, slope = 1.f;
   }
-}
-template <int ACT>
-__device__ __forceinline__ float act_value(float z) {
-  float v, s;
-  act_both<ACT>(z, v, s);
-  return v;
-}
-template <int ACT>
-__device__ __forceinline__ float act_slope(float z) {
-  float v, s;
-  act_both<ACT>(z, v, s);
-  return s;
 }
 #endif
 
