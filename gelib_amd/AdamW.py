@@ -41,6 +41,10 @@ class AdamW(torch.optim.Optimizer):
         except (TypeError, ValueError):
             self.param_groups.pop()
             raise
+        self._grow(self._place(params), device)
+
+    def _place(self, params):
+        """Gives the parameters of a further group their places behind the others; where the next ones would begin."""
         first, size = [], self._size
         for p in params:
             n = p.numel() * (2 if p.is_complex() else 1)
@@ -48,7 +52,7 @@ class AdamW(torch.optim.Optimizer):
             first.append(size)
             size += -(-n // BLOCK) * BLOCK
         self._groups.append(backend().AdamWGroup(params, first))
-        self._grow(size, device)
+        return size
 
     def _grow(self, size, device):
         of = [torch.float32] * 2 if self.state_bits == 32 else [torch.uint8] * 2 + [torch.int16] * 2
@@ -106,6 +110,20 @@ class AdamW(torch.optim.Optimizer):
             k = len(group.steps)
             group.steps = list(steps[at:at + k])
             at += k
+
+    def __getstate__(self):   # (of copies and pickles; the groups that hold the places in memory are made again)
+        return dict(super().__getstate__(), state_bits=self.state_bits, seed=self.seed, _arrays=self._arrays, steps=[list(g.steps) for g in self._groups])
+
+    def __setstate__(self, state):
+        state = dict(state)
+        steps = state.pop("steps", None)
+        super().__setstate__(state)
+        if steps is None:         # (what Optimizer.load_state_dict sets: hyperparameters)
+            return
+        self._groups, self._places, self._size = [], {}, 0
+        for group, k in zip(self.param_groups, steps):
+            self._size = self._place(group["params"])
+            self._groups[-1].steps = k
 
     def state_dict(self):
         d = super().state_dict()
