@@ -15,7 +15,7 @@ class AdamW(torch.optim.Optimizer):
     for every 256 elements; these and bfloat16 parameters are rounded at random, so that steps far below a unit in the last place
     add up (to the nearest, v would not follow the gradients at all).  The random bits are a function of seed, step and element:
     runs repeat.  t counts the steps of each parameter; one whose gradient is None takes none.  (A step recorded into a graph is the step
-    of that t at every replay.)"""
+    of that t at every replay, so one that rounds at random cannot be recorded: its bits would be the same ones every time.)"""
 
     def __init__(self, params, lr=1e-3, betas=(0.9, 0.999), eps=1e-8, weight_decay=1e-2, state_bits=32, seed=0):
         if state_bits not in (8, 32):

@@ -452,11 +452,16 @@ struct AdamWGroup {
       l.step.push_back(steps[k] + 1);
       moved.push_back(k);
     }
-    for (int b = 0; b < 2; b++)
-      if (Lists &l = lists[b]; !l.p.empty())
-        done(gelib_hip_adamw_step((int)l.p.size(), l.p.data(), l.g.data(), l.n.data(), l.first.data(), l.step.data(), ptr(m), ptr(v),
+    for (int b = 1; b >= 0; b--)   // (bfloat16 first: where it is refused nothing has been launched)
+      if (Lists &l = lists[b]; !l.p.empty()) {
+        const int status = gelib_hip_adamw_step((int)l.p.size(), l.p.data(), l.g.data(), l.n.data(), l.first.data(), l.step.data(), ptr(m), ptr(v),
                                   mt ? (int16_t *)ptr(*mt) : nullptr, vt ? (int16_t *)ptr(*vt) : nullptr, b ? GELIB_HIP_BF16 : GELIB_HIP_F32, bits, lr,
-                                  beta1, beta2, eps, decay, seed, on.stream));
+                                  beta1, beta2, eps, decay, seed, on.stream);
+        if (status == GELIB_HIP_ERR_UNSUPPORTED)
+          throw std::runtime_error("GElib: a step with moments in 8 bits or bfloat16 parameters cannot be recorded into a graph: every replay would round by the "
+                                   "same random bits");
+        done(status);
+      }
     for (size_t k : moved) {
       steps[k]++;
       params[k].unsafeGetTensorImpl()->bump_version();   // (changed in place, as far as autograd is concerned)

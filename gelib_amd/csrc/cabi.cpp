@@ -1483,7 +1483,7 @@ const char *gelib_hip_strerror(int status) {
       return "the packed matrix of n_in x n_out channels exceeds the 8 MiB array of the entry point that allocates "
              "nothing; use gelib_hip_part_mix_channels with a workspace";
     case GELIB_HIP_ERR_UNSUPPORTED:
-      return "shapes outside what the fused kernel takes; form the product and mix its channels in two calls";
+      return "shapes outside what the fused kernel takes; form the product and mix its channels in two calls (AdamW: rounding at random under stream capture)";
   }
   return "unknown status";
 }

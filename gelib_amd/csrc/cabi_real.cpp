@@ -189,6 +189,11 @@ int gelib_hip_adamw_step(int ntensors, void *const *p, const void *const *g, con
   if (state_bits == 8) mem.need(m_top, end / kAdamBlock * 2, 2), mem.need(v_top, end / kAdamBlock * 2, 2);
   if (int rc = mem.rc()) return rc;
   if (end == 0) return GELIB_HIP_OK;
+  if (state_bits == 8 || dtype == GELIB_HIP_BF16) {
+    hipStreamCaptureStatus recorded = hipStreamCaptureStatusNone;
+    if (hipStreamIsCapturing((hipStream_t)stream, &recorded) != hipSuccess) (void)hipGetLastError();
+    if (recorded != hipStreamCaptureStatusNone) return GELIB_HIP_ERR_UNSUPPORTED;   // every replay would round by the same random bits
+  }
   AdamArgs a;
   a.m = m, a.v = v, a.m_top = m_top, a.v_top = v_top, a.dtype = dtype, a.bits = state_bits;
   a.decay = (float)(lr * weight_decay);

@@ -56,7 +56,8 @@ enum gelib_hip_status {
   GELIB_HIP_ERR_ARG = 12,          /* negative offset, negative stride or other malformed argument                   */
   GELIB_HIP_ERR_WORKSPACE = 13,    /* workspace missing, not 16-byte aligned or smaller than the size query says     */
   GELIB_HIP_ERR_TOO_LARGE = 14,    /* sizes beyond the stated maximum of gelib_hip_part_mix_channels_static          */
-  GELIB_HIP_ERR_UNSUPPORTED = 15   /* gelib_hip_so3vec_cg_linear_fwd / _bwd: shapes outside what the call takes      */
+  GELIB_HIP_ERR_UNSUPPORTED = 15   /* gelib_hip_so3vec_cg_linear_fwd / _bwd: shapes outside what the call takes;
+                                      gelib_hip_adamw_step: rounding at random under stream capture                 */
 };
 
 #define GELIB_HIP_MAX_L 32          /* largest l of an operand part                     */
@@ -316,7 +317,8 @@ uint64_t gelib_hip_linear_act_workspace_bytes(int backward, int dtype, int64_t r
  * and their unused ends are zero.  All arrays of moments start at multiples of 16 bytes.  state_bits 32: float32 arrays, m_top and v_top NULL.  state_bits 8: a byte an element, and
  * m_top, v_top a 16-bit integer for every 256 elements: code c of v stands for the float whose bits are (c + top - 254) << 20
  * (0: zero, 255: not finite), code c of m for (c % 128 + top - 126) << 20 with sign c / 128 (0: zero, 127: not finite).  These
- * codes, and bfloat16 parameters, are rounded at random with bits that are a function of seed, step[k] and element alone. */
+ * codes, and bfloat16 parameters, are rounded at random with bits that are a function of seed, step[k] and element alone: on a
+ * stream that is being captured either returns GELIB_HIP_ERR_UNSUPPORTED, since every replay would be rounded by the same bits. */
 int gelib_hip_adamw_step(int ntensors, void *const *p, const void *const *g, const int64_t *n, const int64_t *first,
                          const int64_t *step, void *m, void *v, int16_t *m_top, int16_t *v_top, int dtype, int state_bits,
                          double lr, double beta1, double beta2, double eps, double weight_decay, uint64_t seed, void *stream);
