@@ -173,12 +173,18 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor> norm_bwd(const at::Tensor &gy_, c
   return {gx, gw, gb};
 }
 
+// torch's operations in the types that are written here: under autocast a product of float32 values would be one of 16-bit values.
+struct AsWritten {
+  c10::impl::ExcludeDispatchKeyGuard guard{c10::autocast_dispatch_keyset};
+};
+
 // The same from torch's own operations: for gradients of gradients, and where only torch's operations will do.
 // (silu as a product: the gradient of torch's silu has no forward-mode derivative)
 at::Tensor activated(const at::Tensor &z, int64_t act) {
   return act == GELIB_HIP_ACT_RELU ? at::relu(z) : act == GELIB_HIP_ACT_SILU ? z * at::sigmoid(z) : act == GELIB_HIP_ACT_GELU ? at::gelu(z) : z;
 }
 at::Tensor norm_from_torch(const at::Tensor &x, const at::Tensor &w, const at::Tensor &b, const at::Tensor &lengths, int64_t groups, double eps, int64_t act) {
+  AsWritten types;
   const int64_t n = x.size(0), c = x.size(-1);
   at::Tensor t = x.reshape({n, -1, groups, c / groups}).to(at::kFloat), live, count;
   if (lengths.defined()) {
@@ -203,6 +209,7 @@ at::Tensor norm_from_torch(const at::Tensor &x, const at::Tensor &w, const at::T
 template <typename F>
 variable_list graph_grads(F f, const variable_list &tensors, const at::Tensor &g) {
   const bool graph = at::GradMode::is_enabled();
+  AsWritten types;
   at::AutoGradMode on(true);
   variable_list views, wanted, grads(tensors.size());
   for (const at::Tensor &t : tensors) {
@@ -355,6 +362,7 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor> linear_bwd(const at::Tensor &gy_,
 }
 
 at::Tensor linear_from_torch(const at::Tensor &x, const at::Tensor &w, const at::Tensor &b, const at::Tensor &r, int64_t act) {
+  AsWritten types;
   at::Tensor z = at::matmul(x.to(at::kFloat), w.to(at::kFloat));
   if (b.defined()) z = z + b.to(at::kFloat);
   z = activated(z, act);

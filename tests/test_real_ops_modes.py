@@ -120,3 +120,19 @@ def test_function_transforms():
         many = torch.stack([ts[0], 2 * ts[0]])
         both = vmap(lambda x: f(x, *ts[1:]))(many)
         assert near(both[0], y) and near(both[1], f(2 * ts[0], *ts[1:]))
+
+
+@pytest.mark.gpu
+def test_autocast():
+    """Gradients with a graph, and calls that are left to torch's operations, keep the types of their tensors under autocast."""
+    for f, ts, k in cases():
+        leaves = [t.clone().requires_grad_() for t in ts[:k]]
+        y = f(*leaves, *ts[k:])
+        v = torch.randn_like(y)
+        want = torch.autograd.grad(y, leaves, v, retain_graph=True)
+        with torch.autocast("cuda", dtype=torch.bfloat16):
+            for a, b in zip(torch.autograd.grad(f(*leaves, *ts[k:]), leaves, v, create_graph=True), want):
+                assert a.dtype == torch.float32 and near(a, b)
+            with fwad.dual_level():
+                value, _ = fwad.unpack_dual(f(*[fwad.make_dual(t, t) for t in ts[:k]], *ts[k:]))
+                assert value.dtype == torch.float32 and near(value, y)
