@@ -26,3 +26,22 @@ def gelib():
 @pytest.mark.parametrize("shape", SHAPES, ids=lambda s: "x".join(map(str, s)))
 def test_values_and_gradients(gelib, shape, act, dtype):
     G.test_values_and_gradients(gelib, shape, act, dtype)
+
+
+@pytest.mark.parametrize("shape", [(5, 1, 24, 3), (3, 40, 48, 4), (2, 900, 64, 8), (2, 30, 4100, 1)], ids=lambda s: "x".join(map(str, s)))
+def test_each_gradient_by_itself(gelib, shape):
+    """Whichever of x, weight and bias need a gradient, and whichever of weight and bias there are."""
+    n, s, c, groups = shape
+    gen = torch.Generator(device="cuda").manual_seed(6)
+    x, w, b, g = (torch.randn(*k, device="cuda", generator=gen) for k in ((n, s, c), (c,), (c,), (n, s, c)))
+    for given in ("xwb", "xw", "xb", "x"):
+        full = {"x": x, "w": w if "w" in given else torch.ones_like(w), "b": b if "b" in given else torch.zeros_like(b)}
+        leaves = {k: t.clone().requires_grad_() for k, t in full.items()}
+        want = dict(zip("xwb", torch.autograd.grad(gelib.group_norm_act(leaves["x"], groups, leaves["w"], leaves["b"], act="silu"), list(leaves.values()), g)))
+        for needed in ("x", "w", "b", "xw", "wb", "xb"):
+            if not set(needed) <= set(given):
+                continue
+            ts = {k: full[k].clone().requires_grad_(k in needed) if k in given else None for k in "xwb"}
+            y = gelib.group_norm_act(ts["x"], groups, ts["w"], ts["b"], act="silu")
+            for k, got in zip(needed, torch.autograd.grad(y, [ts[k] for k in needed], g)):
+                assert torch.equal(got, want[k]), (given, needed, k)

@@ -136,3 +136,21 @@ def test_autocast():
             with fwad.dual_level():
                 value, _ = fwad.unpack_dual(f(*[fwad.make_dual(t, t) for t in ts[:k]], *ts[k:]))
                 assert value.dtype == torch.float32 and near(value, y)
+
+
+@pytest.mark.gpu
+def test_kernels_run_elsewhere():
+    """After all of it, and beside it for tensors without a tangent, calls go to the kernels (path 7)."""
+    from gelib_amd import cabi
+    L = cabi.lib()
+    for f, ts, k in cases():
+        torch.func.vmap(lambda x: f(x, *ts[1:]))(torch.stack([ts[0], ts[0]]))
+        for forward in (False, True):
+            cabi.check(L.gelib_hip_adamw_step(0, None, None, None, None, None, None, None, None, None, 0, 32, 0.0, 0.0, 0.0, 0.0, 0.0, 0, None))
+            assert L.gelib_hip_last_path() == 0
+            if forward:
+                with fwad.dual_level():
+                    f(*ts)
+            else:
+                f(*ts)
+            assert L.gelib_hip_last_path() == 7
