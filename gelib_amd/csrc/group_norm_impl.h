@@ -383,8 +383,11 @@ __device__ __forceinline__ void keep_sums(const NormDev &d, const Place &w, cons
 #pragma unroll
   for (int j = 0; j < J; j++) {
     const int c = threadIdx.x + j * d.p.T;
-    if (c < w.cw)
-      for (int k = 0; k < d.p.NS; k++) acc[j] += chan[k * d.p.Cw + c];
+    if (c < w.cw) {
+      float s = 0.f;   // (a chain of its own: one over all samples rounds as often as it has terms)
+      for (int k = 0; k < d.p.NS; k++) s += chan[k * d.p.Cw + c];
+      acc[j] += s;
+    }
   }
 }
 // sums of q = gz w and of q xh of the groups, divided by their count, from the column sums of gz and gz xh
@@ -739,17 +742,23 @@ __global__ void __launch_bounds__(kNormChunkT) norm_apply_bwd(const NormDev d) {
   }
 }
 
-// gw and gb: sums of `rows` rows of [2][C]; 32 columns by 8 runs of rows a block
+// gw and gb: sums of `rows` rows of [2][C]; 32 columns by 8 runs of rows a block, a run in four chains
 template <typename T>
 __global__ void __launch_bounds__(256) norm_join(const float *sums, T *gw, T *gb, long long rows, int C) {
   __shared__ float lds[8][32];
   const long long c = (long long)blockIdx.x * 32 + threadIdx.x % 32;
   const int run = threadIdx.x / 32;
-  float s = 0.f;
+  float chain[4] = {};
   if (c < 2LL * C) {
-#pragma unroll 8
-    for (long long k = run; k < rows; k += 8) s += sums[k * 2 * C + c];
+    long long k = run;
+#pragma unroll 2
+    for (; k + 24 < rows; k += 32) {
+#pragma unroll
+      for (int u = 0; u < 4; u++) chain[u] += sums[(k + 8 * u) * 2 * C + c];
+    }
+    for (; k < rows; k += 8) chain[0] += sums[k * 2 * C + c];
   }
+  float s = (chain[0] + chain[1]) + (chain[2] + chain[3]);
   lds[run][threadIdx.x % 32] = s;
   __syncthreads();
   if (run == 0 && c < 2LL * C) {

@@ -36,3 +36,16 @@ def test_as_exact_as_torchs_float32_operations(by, act):
         k = name == "slope"
         ours, plain = ((a.detach().double().view(-1) - outs[1][k].view(-1)).square().mean().sqrt() for a in (got, outs[0][k]))
         assert ours <= times * plain, (name, float(ours / plain))
+
+
+def test_sums_over_many_samples():
+    """The gradient of a norm's bias over 32768 samples is as far from float64 as torch's float32 sum of as many terms (1.3 times: both add in short
+    chains, of a term's rounding each)."""
+    import gelib_amd as gelib
+    gen = torch.Generator(device="cuda").manual_seed(2)
+    x, g = (torch.randn(32768, 1, 64, device="cuda", generator=gen) for _ in range(2))
+    b = torch.zeros(64, device="cuda", requires_grad=True)
+    got, = torch.autograd.grad(gelib.group_norm_act(x, 8, None, b), b, g)
+    want = g.double().sum((0, 1))
+    ours, plain = ((t.double() - want).square().mean().sqrt() for t in (got, g.sum((0, 1))))
+    assert ours <= 1.3 * plain + 2.0 ** -24 * want.abs().max(), (float(ours), float(plain))
