@@ -17,9 +17,9 @@
 // compute unit, so that its loads, two reductions and stores follow one another), backward in chunks 18 + 20 and 9 for the two
 // joins; held whole backward it was 180 (410 registers spilled).  24 samples of up to 9216 x 320: statistics 22, y 34, sums 42, gx 52
 // (141 MB written by each of y and gx: 4.2 and 2.7 TB/s, the second beside 25 instructions an element and two exponentials'
-// worth of silu'), joins 18.  One group of 4096 channels, silu, with the host's part: 64 x 512 forward 168, both 521 (a block a group
-// alone: 11900 and 28600); 8192 x 1 forward 148, both 461 (202 and 594).  8192 x 1 x 8192, chunks of one position: 271 and 990.
-// 64 x 512 x 4099, loads of one channel: 384 and 916.  32768 x 1 x 64 float32: 14 forward, 18 + 4 backward: six barriers of a block
+// worth of silu'), joins 18.  One group of 4096 channels, silu, with the host's part: 64 x 512 forward 168, both 528 (a block a group
+// alone: 11900 and 28600); 8192 x 1 forward 148, both 462 (202 and 594).  8192 x 1 x 8192, chunks of one position: 257 and 978.
+// 64 x 512 x 4099, loads of one channel: 383 and 910.  32768 x 1 x 64 float32: 14 forward, 18 + 4 backward: six barriers of a block
 // one after the other.
 #pragma once
 

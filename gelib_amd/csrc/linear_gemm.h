@@ -13,9 +13,9 @@
 //
 // The products are formed with B's fragment as the first operand, so that a lane's four results lie side by side in a row of C.
 //
-// What bounds it: the matrix cores, and below about 2000 rows the latency of the steps.  bfloat16 16384 x 2048 -> 8192: x w 545 to 640 us, gz w^T
-// 500 to 520, x^T gz 490 to 510, by the clock that the card's power allows (1.0 to 1.1 PFLOP/s; the library's products 440 to 580, 450 and
-// 590); a step of a 256 x 256 tile 1.7 us, of which the products are 1.0 at the full rate; with gelu and its slope 690 (0.54 GB written).
+// What bounds it: the matrix cores, and below about 2000 rows the latency of the steps.  bfloat16 16384 x 2048 -> 8192: x w 515 to 640 us, gz w^T
+// 465 to 520, x^T gz 480 to 510, by the clock that the card's power allows (0.9 to 1.2 PFLOP/s; the library's products 440 to 580, 450 and
+// 590); a step of a 256 x 256 tile 1.7 us, of which the products are 1.0 at the full rate; with gelu and its slope 620 to 690 (0.54 GB written).
 // float32, the same sizes: 4.1, 4.0 and 3.9 ms, 134 to 141 TFLOP/s (the library 148 to 152).
 #pragma once
 

@@ -77,8 +77,8 @@ __device__ __forceinline__ T from_f(float v) { return (T)v; }   // round to near
 // the layer's own, and gw, which is rounded twice besides (gz, and itself), came out 1.54 to 1.73 times as far off as with one
 // rounding; these steps are 1/16 of float16's over [0.5, 1), where most slopes are.  All of [-0.18, 1.14] has a code, which silu'
 // (-0.10 to 1.10) and gelu' (-0.13 to 1.13) stay within; what is not a number has its own.  16384 x 2048 -> 8192, forward and both
-// directions: silu 611 and 1781 us, gelu 641 and 1821, beside 597 and 1737, 628 and 1735 in bfloat16 (without an activation 579 and
-// 1630 beside 595 and 1597): the codes take about 15 us forward and 20 to 50 in gz.
+// directions, on one card: silu 588 and 1792 us, gelu 622 and 1824, without an activation 580 and 1630; in bfloat16, whose products draw
+// less power, 521 and 1700, 547 and 1728, 517 and 1539: the codes take about 5 to 10 us forward and nothing that shows in gz.
 struct slope16_t {
   static constexpr int kFloats = 0x2800, kNan = 50000;   // the float16 codes below 2^-5; positive codes end at 46572, negative ones begin at 50421
   unsigned short code;
