@@ -49,14 +49,14 @@ at::Tensor plain(const at::Tensor &t) {
   return p.numel() && (uintptr_t)p.data_ptr() % 16 ? p.clone() : p;
 }
 
-// Is a call left to torch's own operations?  Only they know of forward-mode derivatives, function transforms, tracing and dispatch modes
-// (shapes without data, counters of operations): a kernel would read the memory below, and its result would be a constant to them.
+// Is a call left to torch's own operations?  Only they know of forward-mode derivatives, function transforms, tracing, dispatch modes
+// (shapes without data, counters of operations) and batches of gradients: a kernel would read the memory below, and its result would be a constant to them.
 bool left_to_torch(std::initializer_list<const at::Tensor *> ts) {
   if (torch::jit::tracer::isTracing() || c10::impl::TorchDispatchModeTLS::any_modes_set() ||
       c10::impl::tls_is_dispatch_key_included(c10::DispatchKey::FuncTorchDynamicLayerFrontMode))
     return true;
   for (const at::Tensor *t : ts)
-    if (t && t->defined() && (t->_fw_grad(/*level=*/0).defined() || t->unsafeGetTensorImpl()->is_python_dispatch())) return true;
+    if (t && t->defined() && (t->_fw_grad(/*level=*/0).defined() || t->unsafeGetTensorImpl()->is_python_dispatch() || !t->has_storage())) return true;
   return false;
 }
 const at::Tensor *address(const Maybe &t) { return t ? &*t : nullptr; }

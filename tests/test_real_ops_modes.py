@@ -154,3 +154,16 @@ def test_kernels_run_elsewhere():
             else:
                 f(*ts)
             assert L.gelib_hip_last_path() == 7
+
+
+@pytest.mark.gpu
+def test_batches_of_gradients():
+    """Several gradients of one result in one call, as a vectorised Jacobian asks for them."""
+    for f, ts, k in cases():
+        leaves = [t.clone().requires_grad_() for t in ts[:k]]
+        y = f(*leaves, *ts[k:])
+        vs = torch.randn(3, *y.shape, device="cuda")
+        got = torch.autograd.grad(y, leaves, vs, is_grads_batched=True, retain_graph=True)
+        for i in range(3):
+            for a, b in zip(got, torch.autograd.grad(y, leaves, vs[i], retain_graph=True)):
+                assert near(a[i], b)
