@@ -19,6 +19,9 @@ from gelib_amd.gather_map import gather_map  # noqa: F401
 from gelib_amd.group_norm_act import group_norm_act  # noqa: F401
 from gelib_amd.linear_act import linear_act  # noqa: F401
 from gelib_amd.AdamW import AdamW  # noqa: F401
+from gelib_amd.embedding import embedding  # noqa: F401
+from gelib_amd.attention import attention  # noqa: F401
+from gelib_amd.linear_cross_entropy import linear_cross_entropy  # noqa: F401
 from gelib_amd.O3 import O3element, O3irrep, O3type, O3part, O3vec, O3vec_CGproductFn, O3vec_DiagCGproductFn  # noqa: F401
 
 

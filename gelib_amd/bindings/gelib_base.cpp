@@ -93,6 +93,7 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("version", []() { return std::string(_GELIB_VERSION); });
 
   bind_real_ops(m);
+  bind_point_ops(m);
 
   m.def("in_memory", [](const py::args &ts) {
     for (const py::handle t : ts) {

@@ -1,4 +1,4 @@
-// What gelib_base.cpp needs of real_ops.cpp.
+// What gelib_base.cpp needs of real_ops.cpp and point_ops.cpp.
 #pragma once
 
 #include <torch/extension.h>
@@ -6,3 +6,4 @@
 #include "gelib_hip.h"
 
 void bind_real_ops(pybind11::module_ &m);
+void bind_point_ops(pybind11::module_ &m);

@@ -14,10 +14,10 @@ PKG = os.path.join(ROOT, "gelib_amd")
 
 ext = ce.CppExtension(
     name="gelib_amd.gelib_base",
-    sources=[os.path.join(HERE, "gelib_base.cpp"), os.path.join(HERE, "real_ops.cpp")],
+    sources=[os.path.join(HERE, "gelib_base.cpp"), os.path.join(HERE, "real_ops.cpp"), os.path.join(HERE, "point_ops.cpp")],
     # the class mirror is header-only: the module must be rebuilt when any of these changes
     depends=[os.path.join(ROOT, "include", "gelib", "GElib.hpp"), os.path.join(ROOT, "include", "gelib", "cnine_min.hpp"),
-             os.path.join(ROOT, "include", "gelib_hip.h"), os.path.join(HERE, "real_ops.h")],
+             os.path.join(ROOT, "include", "gelib_hip.h"), os.path.join(HERE, "real_ops.h"), os.path.join(HERE, "tensors.h")],
     include_dirs=[os.path.join(ROOT, "include"), "/opt/rocm/include"],
     define_macros=[("__HIP_PLATFORM_AMD__", "1"), ("USE_ROCM", "1")],
     extra_compile_args=["-O2", "-g0", "-std=c++17", "-Wno-unused-function"],

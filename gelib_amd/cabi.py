@@ -29,6 +29,9 @@ SYMBOLS = [
     "gelib_hip_group_norm_act_fwd", "gelib_hip_group_norm_act_bwd", "gelib_hip_group_norm_act_workspace_bytes",
     "gelib_hip_linear_act_fwd", "gelib_hip_linear_act_bwd", "gelib_hip_linear_act_workspace_bytes",
     "gelib_hip_adamw_step", "gelib_hip_adamw_moments", "gelib_hip_adamw_set_moments",
+    "gelib_hip_embedding_fwd", "gelib_hip_embedding_bwd", "gelib_hip_embedding_workspace_bytes",
+    "gelib_hip_attention_fwd", "gelib_hip_attention_bwd", "gelib_hip_attention_workspace_bytes",
+    "gelib_hip_linear_cross_entropy_fwd", "gelib_hip_linear_cross_entropy_bwd", "gelib_hip_linear_cross_entropy_workspace_bytes",
     "gelib_hip_malloc", "gelib_hip_free", "gelib_hip_memcpy", "gelib_hip_memset", "gelib_hip_synchronize",
 ]
 

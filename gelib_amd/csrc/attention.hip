@@ -1,0 +1,391 @@
+// Attention over the points of documents: which kernels a call takes (attention_impl.h has them), the joins of pieces, the sums of the
+// gradients of points over heads and of slopes over rows.
+#include "attention_impl.h"
+
+namespace gelib_hip {
+
+namespace {
+
+constexpr int kSlopeRows = 128;   // rows whose slopes' gradients one block sums
+
+int bn_of(int dtype, int dims) { return dims * dtype_bytes(dtype) >= 512 ? 32 : 64; }
+
+// What one pass over `own` rows of a document (on the average) with `streamed` rows of the other side takes.
+struct Pass {
+  bool wide, blocked;
+  long long slots;
+  int splits;
+};
+Pass pass_of(const AttnCall &c, AttnPass pass) {
+  const bool own_q = pass != kAttnKeys;
+  const long long G = c.heads / c.kv_heads, per = own_q ? G : 1, other = own_q ? 1 : G;
+  const long long all = own_q ? c.nq : c.nk, streamed_all = (own_q ? c.nk : c.nq) * other;
+  const double docs = c.packed ? (double)std::max(1LL, c.docs) : 1.0;
+  const double own = all * per / docs, streamed = streamed_all / docs;
+  Pass p;
+  p.wide = own > 64;
+  // Heads of a group by tiles, where distances are formed: both sides of a tile pair share them.  Positions are filled up to 16, which costs
+  // less than it gives from two such tiles on.
+  const int own_rows = attention_rows(pass, (int)dtype_bytes(c.dtype), attention_dims(c.dim), true);
+  p.blocked = c.slopes && p.wide && (G == 2 || G == 4 || G == 8) && c.nq / docs >= 32 && (!own_q || own_rows % (16 * G) == 0);
+  const int rows = attention_rows(pass, (int)dtype_bytes(c.dtype), attention_dims(c.dim), p.wide);
+  const long long in_doc = own_q && p.blocked ? (all + 15) / 16 * 16 * per : all * per;
+  p.slots = c.packed ? all * per / rows + c.docs + 3 : c.docs * ((in_doc + rows - 1) / rows);
+  // pieces of the streamed side where blocks do not fill the compute units, four tiles each at least
+  const double blocks = std::max(1.0, own / rows) * (c.packed ? docs : (double)c.docs) * c.kv_heads, want = p.wide ? 512 : 2048;
+  const double most = streamed / bn_of(c.dtype, attention_dims(c.dim)) / 4;
+  p.splits = (int)std::max(1.0, std::min({want / blocks, most, 64.0}));
+  return p;
+}
+
+size_t up(size_t n) { return (n + 255) & ~(size_t)255; }
+
+// Operands whose heads do not lie at multiples of 16 bytes, copied to (row, head, values up to a multiple of 16 bytes): a thread 16
+// bytes of the copy.
+struct Operand {
+  const void *from;
+  long long s, p, h;   // strides of samples, positions, heads
+  long long docs, n;
+  int heads;
+};
+struct AttnCopies {
+  struct {
+    Operand o;
+    void *to;
+    long long first;   // thread
+  } m[5];
+  int count, dim, per;   // per: pieces of a head
+  long long threads;
+};
+template <typename T>
+__global__ void __launch_bounds__(256) attention_copy_kernel(const AttnCopies a) {
+  constexpr int V = 16 / sizeof(T);
+  for (long long t = (long long)blockIdx.x * 256 + threadIdx.x; t < a.threads; t += (long long)gridDim.x * 256) {
+    int k = 0;
+    while (k + 1 < a.count && t >= a.m[k + 1].first) k++;
+    const Operand &o = a.m[k].o;
+    const long long at = t - a.m[k].first, rh = at / a.per, row = rh / o.heads, doc = row / o.n;
+    const int c = (int)(at - rh * a.per) * V;
+    const T *p = (const T *)o.from + doc * o.s + (row - doc * o.n) * o.p + (rh - row * o.heads) * o.h + c;
+    T v[V];
+#pragma unroll
+    for (int i = 0; i < V; i++) v[i] = c + i < a.dim ? p[i] : (T)0.f;
+    __builtin_memcpy(__builtin_assume_aligned((T *)a.m[k].to + at * V, 16), v, 16);
+  }
+}
+
+int padded_dim(const AttnCall &c) {
+  const int v = 16 / (int)dtype_bytes(c.dtype);
+  return (c.dim + v - 1) / v * v;
+}
+bool aligned(const AttnCall &c, const void *p, const long long *s) {
+  const long long e = (long long)dtype_bytes(c.dtype);
+  return c.dim * e % 16 == 0 && ((long long)(uintptr_t)p | (c.packed ? 0 : s[0] * e) | s[1] * e | s[2] * e) % 16 == 0;
+}
+
+// Where everything lies in the workspace
+struct Space {
+  size_t q = 0, k = 0, v = 0, y = 0, gy = 0, part_q = 0, part_p = 0, part_d = 0, part_k = 0, part_v = 0, ml = 0, delta = 0, geo_q = 0, geo_p = 0, geo_k = 0, slopes = 0, bytes = 0;
+};
+long long rows_of(const AttnCall &c, bool q) { return c.packed ? (q ? c.nq : c.nk) : c.docs * (q ? c.nq : c.nk); }
+Space space_of(const AttnCall &c, bool backward, bool geometry) {
+  Space s;
+  const long long rq = rows_of(c, true) * c.heads, rk = rows_of(c, false) * c.kv_heads;
+  auto take = [&](size_t &at, size_t bytes) { at = s.bytes, s.bytes += up(bytes); };
+  const size_t head = (size_t)padded_dim(c) * dtype_bytes(c.dtype);
+  if (!aligned(c, c.q, c.qs)) take(s.q, rq * head);
+  if (!aligned(c, c.k, c.ks)) take(s.k, rk * head);
+  if (!aligned(c, c.v, c.vs)) take(s.v, rk * head);
+  if (backward && padded_dim(c) != c.dim) take(s.y, rq * head), take(s.gy, rq * head);
+  const Pass r = pass_of(c, backward ? kAttnRows : kAttnForward);
+  if (r.splits > 1) take(s.part_q, (size_t)r.splits * rq * c.dim * 4);
+  if (!backward) {
+    if (r.splits > 1) take(s.ml, (size_t)r.splits * rq * 8);
+    return s;
+  }
+  if (r.splits > 1 && c.dtype != GELIB_HIP_F32) {
+    take(s.part_p, (size_t)r.splits * rq * c.dim * 4), take(s.part_d, (size_t)r.splits * rq * 4);
+    if (geometry) take(s.geo_p, (size_t)r.splits * rq * 16);
+  }
+  const Pass k = pass_of(c, kAttnKeys);
+  if (k.splits > 1) take(s.part_k, (size_t)k.splits * rk * c.dim * 4), take(s.part_v, (size_t)k.splits * rk * c.dim * 4);
+  take(s.delta, (size_t)rq * 4);
+  if (geometry) {
+    take(s.geo_q, (size_t)r.splits * rq * 16);
+    take(s.geo_k, (size_t)k.splits * rk * 16);
+    take(s.slopes, (size_t)((rows_of(c, true) + kSlopeRows - 1) / kSlopeRows) * c.heads * 4);
+  }
+  return s;
+}
+
+int launched() {
+  const hipError_t e = hipGetLastError();
+  return e == hipSuccess ? 0 : record_hip_error(e, "attention launch");
+}
+
+constexpr long long kMostThreads = 1LL << 30;   // of a launch
+
+// y of one (row, head): pieces' results to their common maximum
+template <typename T>
+__global__ void __launch_bounds__(256) attention_join_kernel(const AttnArgs a, long long first, long long all, int per_row) {
+  const long long at = first + (long long)blockIdx.x * 256 + threadIdx.x;
+  if (at >= all) return;
+  const long long row = at / per_row;
+  const int d = (int)(at - row * per_row) * 4, n = min(4, a.dim - d);
+  const long long rows = a.rows_q * a.H;
+  float top = kLowest;
+  for (int s = 0; s < a.splits; s++) top = fmaxf(top, a.part_ml[s * rows + row].x);
+  float sum = 0.f, v[4] = {0.f, 0.f, 0.f, 0.f};
+  for (int s = 0; s < a.splits; s++) {
+    const float2 ml = a.part_ml[s * rows + row];
+    if (ml.y == 0.f) continue;
+    const float by = __builtin_amdgcn_exp2f(ml.x - top);
+    sum += ml.y * by;
+    const float *p = a.part_q + (s * rows + row) * a.dim + d;
+    for (int i = 0; i < n; i++) v[i] += p[i] * by;
+  }
+  const float by = sum == 0.f ? 0.f : 1.f / sum;
+  for (int i = 0; i < n; i++) ((T *)a.y)[row * a.dim + d + i] = from_f<T>(v[i] * by);
+  if (d == 0 && a.lse) a.lse[row] = sum == 0.f ? INFINITY : top + __builtin_amdgcn_logf(sum);
+}
+
+// 16-bit types: gq of one (row, head) from the sums of its pieces, less what D0 lacks times the sums with p (attention_impl.h), and the same
+// for the gradients of points and slopes, which are left in the first piece's place; D
+template <typename T>
+__global__ void __launch_bounds__(256) attention_mend_kernel(const AttnArgs a, long long first, long long all, int per_row) {
+  const long long at = first + (long long)blockIdx.x * 256 + threadIdx.x;
+  if (at >= all) return;
+  const long long row = at / per_row, rows = a.rows_q * a.H;
+  const int d = (int)(at - row * per_row) * 4, n = min(4, a.dim - d);
+  float lacks = 0.f;
+  for (int s = 0; s < a.splits; s++) lacks += a.part_d[s * rows + row];
+  float v[4] = {0.f, 0.f, 0.f, 0.f};
+  for (int s = 0; s < a.splits; s++) {
+    const long long p = (s * rows + row) * a.dim + d;
+    for (int i = 0; i < n; i++) v[i] += a.part_q[p + i] - lacks * a.part_p[p + i];
+  }
+  if (a.gq)
+    for (int i = 0; i < n; i++) ((T *)a.gq)[row * a.dim + d + i] = from_f<T>(v[i]);
+  if (d) return;
+  a.delta[row] += lacks;
+  if (!a.geo_q) return;
+  float4 g = {0.f, 0.f, 0.f, 0.f};
+  for (int s = 0; s < a.splits; s++) {
+    const float4 q = a.geo_q[s * rows + row], p = a.geo_p[s * rows + row];
+    g.x += q.x - lacks * p.x, g.y += q.y - lacks * p.y, g.z += q.z - lacks * p.z, g.w += q.w - lacks * p.w;
+  }
+  a.geo_q[row] = g;
+}
+
+// out[i] = sum of the pieces' values
+template <typename T>
+__global__ void __launch_bounds__(256) attention_sum_kernel(T *out, const float *part, long long first, long long n, int splits) {
+  const long long at = first + (long long)blockIdx.x * 256 + threadIdx.x;
+  if (at >= n) return;
+  float v = 0.f;
+  for (int s = 0; s < splits; s++) v += part[s * n + at];
+  out[at] = from_f<T>(v);
+}
+
+// gradients of points: sums over heads and pieces, of queries (geo_q), keys (geo_k) or, where they are the same points, both
+__global__ void __launch_bounds__(256) attention_points_kernel(float *out, const float4 *gq, int splits_q, int H, const float4 *gk, int splits_k, int KV,
+                                                               long long first, long long rows) {
+  const long long row = first + (long long)blockIdx.x * 256 + threadIdx.x;
+  if (row >= rows) return;
+  float x = 0.f, y = 0.f, z = 0.f;
+  if (gq)
+    for (int s = 0; s < splits_q; s++)
+      for (int h = 0; h < H; h++) {
+        const float4 g = gq[(s * rows + row) * H + h];
+        x += g.x, y += g.y, z += g.z;
+      }
+  if (gk)
+    for (int s = 0; s < splits_k; s++)
+      for (int h = 0; h < KV; h++) {
+        const float4 g = gk[(s * rows + row) * KV + h];
+        x += g.x, y += g.y, z += g.z;
+      }
+  out[row * 3] = x, out[row * 3 + 1] = y, out[row * 3 + 2] = z;
+}
+
+// gradients of slopes: of kSlopeRows rows, a block; then of all blocks
+__global__ void __launch_bounds__(256) attention_slopes_kernel(float *part, const float4 *geo, int splits, long long rows, int H) {
+  const long long r0 = (long long)blockIdx.x * kSlopeRows, r1 = min(rows, r0 + kSlopeRows);
+  for (int h = threadIdx.x; h < H; h += 256) {
+    float v = 0.f;
+    for (int s = 0; s < splits; s++)
+      for (long long r = r0; r < r1; r++) v += geo[(s * rows + r) * H + h].w;
+    part[(long long)blockIdx.x * H + h] = v;
+  }
+}
+__global__ void __launch_bounds__(256) attention_slopes_join_kernel(float *out, const float *part, long long blocks, int H) {
+  __shared__ float lds[256];
+  float v = 0.f;
+  for (long long b = threadIdx.x; b < blocks; b += 256) v += part[b * H + blockIdx.x];
+  lds[threadIdx.x] = v;
+  __syncthreads();
+  for (int k = 128; k; k /= 2) {
+    if ((int)threadIdx.x < k) lds[threadIdx.x] += lds[threadIdx.x + k];
+    __syncthreads();
+  }
+  if (threadIdx.x == 0) out[blockIdx.x] = lds[0];
+}
+
+template <typename F>
+int in_launches(long long threads, F f) {
+  for (long long first = 0; first < threads; first += kMostThreads) {
+    f(first, dim3((unsigned)((std::min(kMostThreads, threads - first) + 255) / 256)));
+    if (int rc = launched()) return rc;
+  }
+  return 0;
+}
+
+template <typename T>
+int sum_pieces(void *out, const float *part, long long n, int splits, hipStream_t s) {
+  return in_launches(n, [&](long long first, dim3 grid) { hipLaunchKernelGGL(attention_sum_kernel<T>, grid, dim3(256), 0, s, (T *)out, part, first, n, splits); });
+}
+
+// The call's operands, copied where they have to be (y and gy: of the backward pass).
+template <typename T>
+AttnArgs args_of(const AttnCall &c, const void *y, const void *gy, const Space &at, char *ws, hipStream_t s) {
+  AttnArgs a = {};
+  const int dim = padded_dim(c), H = c.heads, KV = c.kv_heads;
+  a.q = c.q, a.k = c.k, a.v = c.v, a.y = (void *)y, a.gy = gy;
+  a.qs = c.qs[0], a.qp = c.qs[1], a.qh = c.qs[2], a.ks = c.ks[0], a.kp = c.ks[1], a.kh = c.ks[2], a.vs = c.vs[0], a.vp = c.vs[1], a.vh = c.vs[2];
+  if (c.packed) a.qs = a.ks = a.vs = 0;
+  a.x = c.x, a.xk = c.xk, a.slopes = c.slopes, a.q_marks = c.q_marks, a.k_marks = c.k_marks;
+  a.docs = c.docs, a.nq = c.nq, a.nk = c.nk, a.rows_q = rows_of(c, true), a.rows_k = rows_of(c, false);
+  a.packed = c.packed, a.H = H, a.KV = KV, a.G = H / KV, a.dim = c.dim, a.ldy = c.dim;
+  if (a.G > 1) {   // n / G = n magic >> (31 + bits) for n < 2^31
+    int bits = 1;
+    while (1LL << bits < a.G) bits++;
+    a.g_magic = (unsigned)((1ULL << (31 + bits)) / a.G + 1), a.g_shift = bits - 1;
+  }
+  a.scale = c.scale, a.scale2 = (float)(c.scale * 1.4426950408889634);
+  AttnCopies copies = {};
+  copies.dim = c.dim, copies.per = dim * (int)sizeof(T) / 16;
+  const long long docs = c.packed ? 1 : c.docs;
+  auto copy = [&](const void *&p, long long &ss, long long &sp, long long &sh, size_t where, long long n, int heads) {
+    if (docs * n == 0) return;
+    auto &m = copies.m[copies.count++];
+    m.o = {p, ss, sp, sh, docs, n, heads}, m.to = ws + where, m.first = copies.threads;
+    copies.threads += docs * n * heads * copies.per;
+    p = m.to, ss = n * heads * dim, sp = (long long)heads * dim, sh = dim;
+    if (c.packed) ss = 0;
+  };
+  if (!aligned(c, c.q, c.qs)) copy(a.q, a.qs, a.qp, a.qh, at.q, c.nq, H);
+  if (!aligned(c, c.k, c.ks)) copy(a.k, a.ks, a.kp, a.kh, at.k, c.nk, KV);
+  if (!aligned(c, c.v, c.vs)) copy(a.v, a.vs, a.vp, a.vh, at.v, c.nk, KV);
+  if (gy && dim != c.dim) {
+    const void *yp = y;
+    for (auto *p : {&yp, &a.gy}) {
+      long long ss = c.nq * H * c.dim, sp = (long long)H * c.dim, sh = c.dim;
+      copy(*p, ss, sp, sh, p == &yp ? at.y : at.gy, c.nq, H);
+    }
+    a.y = (void *)yp, a.ldy = dim;
+  }
+  if (copies.threads) hipLaunchKernelGGL(attention_copy_kernel<T>, dim3((unsigned)std::min((copies.threads + 255) / 256, 1LL << 22)), dim3(256), 0, s, copies);
+  return a;
+}
+
+// whether rows of results take vectors of four values
+bool whole4(const AttnCall &c, std::initializer_list<const void *> results) {
+  uintptr_t all = 0;
+  for (const void *p : results) all |= (uintptr_t)p;
+  return c.dim % 4 == 0 && all % (4 * dtype_bytes(c.dtype)) == 0;
+}
+
+AttnArgs pass_args(AttnArgs a, const Pass &p) {
+  a.slots = p.slots, a.splits = p.splits, a.head_major = p.wide, a.blocked = p.blocked;
+  return a;
+}
+
+template <typename T>
+int forward(const AttnCall &c, void *y, float *lse, void *ws, hipStream_t s) {
+  const Space at = space_of(c, false, false);
+  const Pass p = pass_of(c, kAttnForward);
+  AttnArgs a = pass_args(args_of<T>(c, y, nullptr, at, (char *)ws, s), p);
+  a.lse = lse, a.vec_y = whole4(c, {y});
+  if (p.splits > 1) a.part_q = (float *)((char *)ws + at.part_q), a.part_ml = (float2 *)((char *)ws + at.ml);
+  if (int rc = launch_attention_kernels<kAttnForward, T>({attention_dims(c.dim), c.slopes ? kBiasPoints : kBiasNone, p.wide}, a, s)) return rc;
+  if (p.splits == 1) return 0;
+  const int per_row = (c.dim + 3) / 4;
+  const long long all = a.rows_q * a.H * per_row;
+  return in_launches(all, [&](long long first, dim3 grid) { hipLaunchKernelGGL(attention_join_kernel<T>, grid, dim3(256), 0, s, a, first, all, per_row); });
+}
+
+template <typename T>
+int backward(const AttnCall &c, const AttnGrads &g, void *ws, hipStream_t s) {
+  const bool geometry = c.slopes && (g.gx || g.gxk || g.gslopes);
+  const Space at = space_of(c, true, geometry);
+  auto in_ws = [&](size_t where) { return (char *)ws + where; };
+  AttnArgs a = args_of<T>(c, g.y, g.gy, at, (char *)ws, s);
+  a.lse = (float *)g.lse, a.delta = (float *)in_ws(at.delta), a.vec_y = whole4(c, {g.gq, g.gk, g.gv});
+  a.gq = g.gq, a.gk = g.gk, a.gv = g.gv;
+  if (geometry) a.geo_q = (float4 *)in_ws(at.geo_q), a.geo_k = (float4 *)in_ws(at.geo_k);
+  const int bias = geometry ? kBiasGradients : c.slopes ? kBiasPoints : kBiasNone, dims = attention_dims(c.dim);
+  Pass pr = pass_of(c, kAttnRows);
+  const Pass pk = pass_of(c, kAttnKeys);
+  AttnArgs r = pass_args(a, pr), k = pass_args(a, pk);
+  const bool mend = pr.splits > 1 && sizeof(T) == 2;
+  if (pr.splits > 1) r.part_q = (float *)in_ws(at.part_q);
+  if (mend) {
+    r.part_p = (float *)in_ws(at.part_p), r.part_d = (float *)in_ws(at.part_d);
+    if (geometry) r.geo_p = (float4 *)in_ws(at.geo_p);
+  }
+  if (int rc = launch_attention_kernels<kAttnRows, T>({dims, bias, pr.wide}, r, s)) return rc;
+  if (mend) {
+    const int per_row = (c.dim + 3) / 4;
+    const long long all = a.rows_q * a.H * per_row;
+    if (int rc = in_launches(all, [&](long long first, dim3 grid) { hipLaunchKernelGGL(attention_mend_kernel<T>, grid, dim3(256), 0, s, r, first, all, per_row); })) return rc;
+    pr.splits = 1;   // (of the gradients of points, from here on)
+  } else if (pr.splits > 1 && g.gq)
+    if (int rc = sum_pieces<T>(g.gq, r.part_q, a.rows_q * a.H * a.dim, pr.splits, s)) return rc;
+  if (g.gk || g.gv || geometry) {
+    if (pk.splits > 1) k.part_k = (float *)in_ws(at.part_k), k.part_v = (float *)in_ws(at.part_v);
+    if (int rc = launch_attention_kernels<kAttnKeys, T>({dims, bias, pk.wide}, k, s)) return rc;
+    if (pk.splits > 1) {
+      const long long n = a.rows_k * a.KV * a.dim;
+      if (g.gk)
+        if (int rc = sum_pieces<T>(g.gk, k.part_k, n, pk.splits, s)) return rc;
+      if (g.gv)
+        if (int rc = sum_pieces<T>(g.gv, k.part_v, n, pk.splits, s)) return rc;
+    }
+  }
+  if (!geometry) return 0;
+  auto points = [&](float *out, bool of_q, bool of_k, long long rows) {
+    return in_launches(rows, [&](long long first, dim3 grid) {
+      hipLaunchKernelGGL(attention_points_kernel, grid, dim3(256), 0, s, out, of_q ? a.geo_q : nullptr, pr.splits, a.H, of_k ? a.geo_k : nullptr, pk.splits, a.KV, first, rows);
+    });
+  };
+  if (g.gx)
+    if (int rc = points(g.gx, true, g.same_points, a.rows_q)) return rc;
+  if (g.gxk)
+    if (int rc = points(g.gxk, false, true, a.rows_k)) return rc;
+  if (g.gslopes) {
+    float *part = (float *)in_ws(at.slopes);
+    const long long blocks = (a.rows_q + kSlopeRows - 1) / kSlopeRows;
+    if (blocks) {
+      hipLaunchKernelGGL(attention_slopes_kernel, dim3((unsigned)blocks), dim3(256), 0, s, part, a.geo_q, pr.splits, a.rows_q, a.H);
+      if (int rc = launched()) return rc;
+    }
+    hipLaunchKernelGGL(attention_slopes_join_kernel, dim3(a.H), dim3(256), 0, s, g.gslopes, part, blocks, a.H);
+    return launched();
+  }
+  return 0;
+}
+
+}  // namespace
+
+size_t attention_workspace(const AttnCall &c, bool backward, bool geometry) { return space_of(c, backward, geometry).bytes; }
+
+int launch_attention(const AttnCall &c, void *y, float *lse, void *ws, hipStream_t s) {
+  if (rows_of(c, true) == 0) return 0;
+  return c.dtype == GELIB_HIP_F32 ? forward<float>(c, y, lse, ws, s) : c.dtype == GELIB_HIP_BF16 ? forward<bhalf_t>(c, y, lse, ws, s) : forward<half_t>(c, y, lse, ws, s);
+}
+
+int launch_attention_bwd(const AttnCall &c, const AttnGrads &g, void *ws, hipStream_t s) {
+  return c.dtype == GELIB_HIP_F32 ? backward<float>(c, g, ws, s) : c.dtype == GELIB_HIP_BF16 ? backward<bhalf_t>(c, g, ws, s) : backward<half_t>(c, g, ws, s);
+}
+
+}  // namespace gelib_hip

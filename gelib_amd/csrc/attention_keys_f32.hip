@@ -1,0 +1,6 @@
+// The gradients of attention by keys, float32 (attention_impl.h).
+#include "attention_impl.h"
+
+namespace gelib_hip {
+template int launch_attention_kernels<kAttnKeys, float>(const AttnPlan &, const AttnArgs &, hipStream_t);
+}

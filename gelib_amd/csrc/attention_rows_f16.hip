@@ -1,0 +1,6 @@
+// The gradients of attention by query rows, float16 (attention_impl.h).
+#include "attention_impl.h"
+
+namespace gelib_hip {
+template int launch_attention_kernels<kAttnRows, half_t>(const AttnPlan &, const AttnArgs &, hipStream_t);
+}

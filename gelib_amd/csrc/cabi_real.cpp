@@ -4,48 +4,20 @@
 #include <new>
 #include <vector>
 
+#include "cabi_check.h"
 #include "real_ops.h"
 
 using namespace gelib_hip;
 
 namespace {
 
-constexpr int64_t kMostElements = 1LL << 46;   // of one tensor: products of two extents below it do not overflow
-
 bool types_ok(int dtype, int act) { return dtype >= GELIB_HIP_F32 && dtype <= GELIB_HIP_F16 && act >= GELIB_HIP_ACT_NONE && act <= GELIB_HIP_ACT_GELU; }
-
-// both factors are not below zero
-bool product_ok(int64_t a, int64_t b) { return a == 0 || b <= kMostElements / a; }
-
-int check_workspace(const void *ws, uint64_t have, uint64_t need) {
-  if (need == 0) return GELIB_HIP_OK;
-  if (!ws || have < need || ((uintptr_t)ws & 15)) return GELIB_HIP_ERR_WORKSPACE;
-  return check_memory(ws, (int64_t)need);
-}
-
-// Collects the first refusal: missing pointers before memory that is not the device's.
-struct Memory {
-  int missing = GELIB_HIP_OK, foreign = GELIB_HIP_OK;
-  void need(const void *p, int64_t bytes, unsigned align) {
-    if (bytes == 0 || missing) return;
-    if (!p) missing = GELIB_HIP_ERR_NULL;
-    else if ((uintptr_t)p % align) missing = GELIB_HIP_ERR_ARG;
-    else if (!foreign) foreign = check_memory(p, bytes);
-  }
-  void may(const void *p, int64_t bytes, unsigned align) {
-    if (p) need(p, bytes, align);
-  }
-  int rc() const { return missing ? missing : foreign; }
-};
 
 int norm_shape(int dtype, int act, int64_t N, int64_t S, int C, int G, int64_t xs, int64_t xp) {
   if (!types_ok(dtype, act) || N < 0 || S < 0 || C < 1 || C > (1 << 26) || G < 1 || C % G || xs < 0 || xp < 0) return GELIB_HIP_ERR_ARG;
   if (!product_ok(N, S) || !product_ok(N * S, C) || N > (1LL << 40) / G || !product_ok(N, xs) || !product_ok(S, xp)) return GELIB_HIP_ERR_ARG;
   return GELIB_HIP_OK;
 }
-
-// what rows of `cols` elements are aligned to: 16 bytes where they are a multiple of it long
-unsigned row_align(unsigned e, int64_t cols) { return cols * e % 16 == 0 ? 16 : e; }
 
 int linear_shape(int dtype, int act, int64_t rows, int K, int N, int64_t xs) {
   if (!types_ok(dtype, act) || rows < 0 || K < 0 || N < 0 || xs < 0 || std::max(K, N) > kLinearMostChannels) return GELIB_HIP_ERR_ARG;

@@ -33,7 +33,20 @@ struct GemmArgs {
   long long M, K, kper;     // kper: k of a piece, a multiple of the step
   int N, act, splits, vec4;  // vec4: rows of c, res and slope take vectors of 4
   unsigned mtiles, ntiles;
+  long long ldc;            // elements between the rows of c
+  const float *norm;        // results without an activation times this; null: 1
+  int add;                  // part holds sums already: add to them
+  // a layer's classes and their loss (linear_loss.hip), instead of c = act(..) + res
+  const long long *targets; // class of every row
+  long long n_first, N_all; // the first of these classes, all of them (bias begins with these)
+  const float *lse, *weight;   // kLossGrad: log of the sum of exp, the loss's gradient
+  float2 *tops;             // kLossSums: [rows][ntiles] largest logit of a tile and sum of exp(logit - it)
+  float *picked;            // kLossSums: logit of the row's class, where it has one
+  float *columns;           // kLossGrad: [rows / WM][N] sums of gz over rows, or null
 };
+
+// epilogues beside enum Act's
+constexpr int kLossSums = 16, kLossGrad = 17;
 
 enum GemmForm { kFormXW = 0, kFormGW = 1, kFormXG = 2 };   // x w, gz w^T, x^T gz
 
@@ -41,8 +54,13 @@ enum GemmForm { kFormXW = 0, kFormGW = 1, kFormXG = 2 };   // x w, gz w^T, x^T g
 constexpr int kGemmTiles = 4;
 constexpr int kGemmBM[kGemmTiles] = {256, 128, 64, 16}, kGemmBN[kGemmTiles] = {256, 128, 128, 256};
 
+constexpr int kGemmWM[kGemmTiles] = {128, 64, 64, 16};   // rows of a wave
+
 template <typename T>
 int launch_gemm(GemmForm form, int tile, const GemmArgs &a, hipStream_t s);
+// x w with the epilogue kLossSums or kLossGrad (one launch: up to 2^22 tiles)
+template <typename T>
+int launch_loss_gemm(int epilogue, int tile, const GemmArgs &a, hipStream_t s);
 
 #ifdef __HIPCC__
 
@@ -159,7 +177,8 @@ struct Stage {
 template <typename T, int ACT, int COUNT>
 __device__ __forceinline__ void epilogue(const GemmArgs &a, long long m, long long n0, int apart, const float (*v)[4]) {
   typedef typename SlopeOf<T>::type D;
-  const long long row = m * a.N;
+  const long long row = m * a.N, row_c = m * a.ldc;
+  const float norm = ACT == kActNone && a.norm ? *a.norm : 1.f;
   if (a.vec4) {
     if (n0 >= a.N) return;
     T t[COUNT][4];
@@ -181,13 +200,13 @@ __device__ __forceinline__ void epilogue(const GemmArgs &a, long long m, long lo
 #pragma unroll
       for (int i = 0; i < 4; i++) {
         float y, s;
-        act_both<ACT>(v[k][i], y, s, a.act == kActRelu);
+        act_both<ACT>(ACT == kActNone ? v[k][i] * norm : v[k][i], y, s, a.act == kActRelu);
         t[k][i] = from_f<T>(y + to_f(t[k][i]));
         d[k][i] = from_f<D>(s);
       }
 #pragma unroll
     for (int k = 0; k < COUNT; k++)
-      if (n0 + k * apart < a.N) __builtin_memcpy(__builtin_assume_aligned((T *)a.c + row + n0 + k * apart, 4 * sizeof(T)), t[k], 4 * sizeof(T));
+      if (n0 + k * apart < a.N) __builtin_memcpy(__builtin_assume_aligned((T *)a.c + row_c + n0 + k * apart, 4 * sizeof(T)), t[k], 4 * sizeof(T));
     if (a.slope)
 #pragma unroll
       for (int k = 0; k < COUNT; k++)
@@ -201,8 +220,8 @@ __device__ __forceinline__ void epilogue(const GemmArgs &a, long long m, long lo
       const long long n = n0 + k * apart + i;
       if (n >= a.N) break;
       float y, s;
-      act_both<ACT>(v[k][i], y, s, a.act == kActRelu);
-      ((T *)a.c)[row + n] = from_f<T>(y + (a.res ? to_f(((const T *)a.res)[row + n]) : 0.f));
+      act_both<ACT>(ACT == kActNone ? v[k][i] * norm : v[k][i], y, s, a.act == kActRelu);
+      ((T *)a.c)[row_c + n] = from_f<T>(y + (a.res ? to_f(((const T *)a.res)[row + n]) : 0.f));
       if (a.slope) ((D *)a.slope)[row + n] = from_f<D>(s);
     }
 }
@@ -334,6 +353,89 @@ __global__ void __launch_bounds__(64 * (BM / WM) * (BN / WN)) gemm_kernel(const 
     }
   }
 
+  if constexpr (ACT >= kLossSums) {
+    // a lane holds FN vectors of four neighbouring logits of FM rows
+    constexpr int apart = GN == 1 ? 16 : 4;
+    const long long nl = n0 + wn + (GN == 1 ? q * 4 : q * 4 * GN);
+    auto logit = [&](int i, int k, int e) __attribute__((always_inline)) { return GN == 1 ? acc[i][k][e] : acc[i][(4 * k + e) % GN][(4 * k + e) / GN]; };
+    static_assert(FN <= 4, "");
+    if constexpr (ACT == kLossSums) {
+      __shared__ float2 tops[BN / WN][BM];
+#pragma unroll
+      for (int i = 0; i < FM; i++) {
+        const int r = wm + (i / GM * GM) * 16 + c * GM + i % GM;
+        const long long t = m0 + r < a.M ? a.targets[m0 + r] : -1;
+        float top = -INFINITY, sum = 0.f;
+#pragma unroll
+        for (int k = 0; k < FN; k++)
+#pragma unroll
+          for (int e = 0; e < 4; e++) {
+            const long long n = nl + k * apart + e;
+            if (n < a.N) top = fmaxf(top, logit(i, k, e));
+            if (n == t && n < a.N) a.picked[m0 + r] = logit(i, k, e);
+          }
+        top = fmaxf(top, __shfl_xor(top, 16));
+        top = fmaxf(top, __shfl_xor(top, 32));
+        const float from = top == -INFINITY ? 0.f : top;
+#pragma unroll
+        for (int k = 0; k < FN; k++)
+#pragma unroll
+          for (int e = 0; e < 4; e++)
+            if (nl + k * apart + e < a.N) sum += __builtin_amdgcn_exp2f((logit(i, k, e) - from) * 1.44269504088896341f);
+        sum += __shfl_xor(sum, 16);
+        sum += __shfl_xor(sum, 32);
+        if (q == 0) tops[wn / WN][r] = make_float2(top, sum);
+      }
+      __syncthreads();
+      for (int r = threadIdx.x; r < BM; r += THREADS) {
+        if (m0 + r >= a.M) continue;
+        float2 v = tops[0][r];
+#pragma unroll
+        for (int k = 1; k < BN / WN; k++) {
+          const float2 o = tops[k][r];
+          const float top = fmaxf(v.x, o.x), from = top == -INFINITY ? 0.f : top;
+          v = make_float2(top, v.y * __builtin_amdgcn_exp2f((v.x - from) * 1.44269504088896341f) + o.y * __builtin_amdgcn_exp2f((o.x - from) * 1.44269504088896341f));
+        }
+        a.tops[(m0 + r) * a.ntiles + n0 / BN] = v;
+      }
+    } else {
+      float column[FN][4] = {};
+      const float norm = a.norm ? *a.norm : 1.f;
+#pragma unroll
+      for (int i = 0; i < FM; i++) {
+        const long long m = m0 + wm + (i / GM * GM) * 16 + c * GM + i % GM;
+        if (m >= a.M) continue;
+        const long long t = a.targets[m];
+        const float lse = a.lse[m], g = t < a.N_all ? a.weight[m] * norm : __builtin_nanf("");
+#pragma unroll
+        for (int k = 0; k < FN; k++) {
+          T v[4];
+#pragma unroll
+          for (int e = 0; e < 4; e++) {
+            const long long n = nl + k * apart + e;
+            const float p = __builtin_amdgcn_exp2f((logit(i, k, e) - lse) * 1.44269504088896341f);
+            const float gz = n < a.N && t >= 0 ? (p - (n + a.n_first == t ? 1.f : 0.f)) * g : 0.f;
+            column[k][e] += gz;
+            v[e] = from_f<T>(gz);
+          }
+          if (nl + k * apart < a.ldc) __builtin_memcpy(__builtin_assume_aligned((T *)a.c + m * a.ldc + nl + k * apart, 4 * sizeof(T)), v, 4 * sizeof(T));
+        }
+      }
+      if (a.columns) {
+#pragma unroll
+        for (int k = 0; k < FN; k++)
+#pragma unroll
+          for (int e = 0; e < 4; e++) {
+            float v = column[k][e];
+#pragma unroll
+            for (int d = 1; d < 16; d *= 2) v += __shfl_xor(v, d);
+            const long long n = nl + k * apart + e;
+            if (c == 0 && n < a.N && m0 + wm < a.M) a.columns[(m0 + wm) / WM * a.N + n] = v;
+          }
+      }
+    }
+    return;
+  }
   const long long part_row = (a.N + 3) & ~3;
   float *part = a.part ? a.part + (long long)blockIdx.y * a.M * part_row : nullptr;
 #pragma unroll
@@ -355,7 +457,11 @@ __global__ void __launch_bounds__(64 * (BM / WM) * (BN / WN)) gemm_kernel(const 
       if (part) {
 #pragma unroll
         for (int k = 0; k < COUNT; k++)
-          if (n + k * apart < a.N) *(f32x4 *)(part + m * part_row + n + k * apart) = f32x4{v[k][0], v[k][1], v[k][2], v[k][3]};
+          if (n + k * apart < a.N) {
+            f32x4 *to = (f32x4 *)(part + m * part_row + n + k * apart);
+            const f32x4 now = {v[k][0], v[k][1], v[k][2], v[k][3]};
+            *to = a.add ? *to + now : now;
+          }
       } else {
         epilogue<T, ACT, COUNT>(a, m, n, apart, v);
       }

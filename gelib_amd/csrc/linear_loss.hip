@@ -1,0 +1,289 @@
+// Softmax cross entropy of a linear layer's classes: z = x w + b, loss_i = log sum_c exp z_ic - z_i,t.  The logits leave the matrix product
+// as a largest value and a sum of exp for each row of a tile, and the logit of the row's own class: (rows, classes / 256) pairs instead of
+// (rows, classes) logits.
+// The gradient of the logits, gz = g (exp(z - lse) - onehot), needs them again: the product is formed a second time, and what leaves it is
+// gz, for as many classes at a time as kMostGradients bytes hold; each such piece goes through the two products gx += gz w^T and gw = x^T gz
+// while the next level of memory still has it.  Eight operations a weight and row instead of six, for rows * classes values that are
+// neither kept nor read and written once more in between.
+// gz is rounded to the layer's type for the two products, as in the layer itself (linear_act.hip); gb sums unrounded values.
+// float16: gz is scaled by a power of two that brings the largest |g| to 2^13 (gz stays below 2^14), so that probabilities down to
+// 2^-27 are float16 values of full precision; results are scaled back before they are rounded.
+#include <algorithm>
+
+#include "linear_products.h"
+
+namespace gelib_hip {
+
+namespace {
+
+constexpr size_t kMostGradients = 256u << 20;   // bytes of gz formed at a time
+
+// A row's pairs -> the log of its sum, its loss.  `lanes` lanes a row (a power of two)
+__global__ void __launch_bounds__(256) loss_join_kernel(float *loss, float *lse, const float2 *tops, const float *picked, const long long *targets, long long rows,
+                                                        int ntiles, int N, int lanes) {
+  const long long row = ((long long)blockIdx.x * 256 + threadIdx.x) / lanes;
+  const int lane = threadIdx.x % lanes;
+  float top = -INFINITY, sum = 0.f;
+  if (row < rows)
+    for (int k = lane; k < ntiles; k += lanes) {
+      const float2 v = tops[row * ntiles + k];
+      const float to = fmaxf(top, v.x), from = to == -INFINITY ? 0.f : to;
+      sum = sum * __builtin_amdgcn_exp2f((top - from) * 1.44269504088896341f) + v.y * __builtin_amdgcn_exp2f((v.x - from) * 1.44269504088896341f);
+      top = to;
+    }
+  for (int d = 1; d < lanes; d *= 2) {
+    const float otop = __shfl_xor(top, d), osum = __shfl_xor(sum, d);
+    const float to = fmaxf(top, otop), from = to == -INFINITY ? 0.f : to;
+    sum = sum * __builtin_amdgcn_exp2f((top - from) * 1.44269504088896341f) + osum * __builtin_amdgcn_exp2f((otop - from) * 1.44269504088896341f);
+    top = to;
+  }
+  if (row >= rows || lane) return;
+  const float l = top + logf(sum);
+  const long long t = targets[row];
+  if (lse) lse[row] = l;
+  loss[row] = t < 0 ? 0.f : t < N ? l - picked[row] : __builtin_nanf("");
+}
+
+// norm[0]: the power of two that brings the largest |g| of a row with a class to 2^13, norm[1]: one over it
+__global__ void __launch_bounds__(1024) loss_norm_kernel(float *norm, const float *g, const long long *targets, long long rows) {
+  __shared__ float lds[16];
+  float top = 0.f;
+  for (long long i = threadIdx.x; i < rows; i += 1024)
+    if (targets[i] >= 0 && fabsf(g[i]) < INFINITY) top = fmaxf(top, fabsf(g[i]));
+#pragma unroll
+  for (int d = 1; d < 64; d *= 2) top = fmaxf(top, __shfl_xor(top, d));
+  if (threadIdx.x % 64 == 0) lds[threadIdx.x / 64] = top;
+  __syncthreads();
+  if (threadIdx.x) return;
+  for (int k = 0; k < 16; k++) top = fmaxf(top, lds[k]);
+  const int e = top > 0.f ? max(-100, min(100, 13 - ilogbf(top))) : 0;
+  norm[0] = ldexpf(1.f, e), norm[1] = ldexpf(1.f, -e);
+}
+
+// out[n] = norm * sum over the chunks of their column sums: 32 columns by 8 runs of chunks a block
+template <typename T>
+__global__ void __launch_bounds__(256) loss_columns_kernel(T *out, const float *sums, long long chunks, int N, const float *norm) {
+  __shared__ float lds[8][32];
+  const int run = threadIdx.x / 32;
+  for (long long n0 = blockIdx.x * 32LL; n0 < N; n0 += gridDim.x * 32LL) {
+    const long long n = n0 + threadIdx.x % 32;
+    float s = 0.f;
+    if (n < N) {
+#pragma unroll 8
+      for (long long k = run; k < chunks; k += 8) s += sums[k * N + n];
+    }
+    lds[run][threadIdx.x % 32] = s;
+    __syncthreads();
+    if (run == 0 && n < N) {
+      for (int k = 1; k < 8; k++) s += lds[k][threadIdx.x];
+      out[n] = from_f<T>(norm ? s * *norm : s);
+    }
+    __syncthreads();
+  }
+}
+
+// gx from the sums over all pieces (rows of K up to a multiple of 4)
+template <typename T>
+__global__ void __launch_bounds__(256) loss_finish_kernel(T *gx, const float *sums, long long n, int K, const float *norm) {
+  const long long stride = (K + 3) & ~3;
+  for (long long at = (long long)blockIdx.x * 256 + threadIdx.x; at < n; at += (long long)gridDim.x * 256) {
+    const long long row = at / K;
+    gx[at] = from_f<T>(sums[row * stride + (at - row * K)] * (norm ? *norm : 1.f));
+  }
+}
+template <typename T>
+__global__ void __launch_bounds__(256) loss_zero_kernel(T *to, long long n) {
+  for (long long at = (long long)blockIdx.x * 256 + threadIdx.x; at < n; at += (long long)gridDim.x * 256) to[at] = (T)0.f;
+}
+template <typename T>
+void zero(void *to, long long n, hipStream_t s) {
+  if (to && n) hipLaunchKernelGGL(loss_zero_kernel<T>, dim3((unsigned)std::min((n + 255) / 256, 1LL << 16)), dim3(256), 0, s, (T *)to, n);
+}
+
+long long tiles_of(long long n, int b) { return (n + b - 1) / b; }
+
+// x w and one of the loss's epilogues, in launches of at most 2^22 tiles
+template <typename T>
+int logits(int epilogue, int dtype, const GemmArgs &g, hipStream_t s) {
+  const Plan p = plan_of(dtype, g.M, g.N, g.K, epilogue == kLossGrad ? (int)dtype_bytes(dtype) : 0, true);
+  const long long BM = kGemmBM[p.tile];
+  GemmArgs a = g;
+  a.splits = 1, a.kper = p.kper, a.part = nullptr;
+  a.ntiles = (unsigned)tiles_of(a.N, kGemmBN[p.tile]);
+  const long long most = std::max(1LL, (1LL << 22) / a.ntiles) * BM;
+  for (long long m = 0; m < g.M; m += most) {
+    GemmArgs b = a;
+    b.M = std::min(most, g.M - m);
+    b.mtiles = (unsigned)tiles_of(b.M, (int)BM);
+    b.a = (const T *)a.a + m * a.lda;
+    if (a.c) b.c = (T *)a.c + m * a.ldc;
+    b.targets += m;
+    if (a.lse) b.lse += m, b.weight += m;
+    if (a.tops) b.tops += m * a.ntiles, b.picked += m;
+    if (a.columns) b.columns += m / kGemmWM[p.tile] * a.N;
+    if (int rc = launch_loss_gemm<T>(epilogue, p.tile, b, s)) return rc;
+  }
+  return 0;
+}
+// the tile that logits() takes
+int tile_of(int dtype, long long M, long long N, long long K, int epilogue) {
+  return plan_of(dtype, M, N, K, epilogue == kLossGrad ? (int)dtype_bytes(dtype) : 0, true).tile;
+}
+
+struct Forward {
+  size_t tops, picked, bytes;
+  int ntiles;
+};
+Forward forward_space(int dtype, long long rows, int K, int N) {
+  Forward f;
+  f.ntiles = (int)tiles_of(N, kGemmBN[tile_of(dtype, rows, N, K, kLossSums)]);
+  size_t at = copy_bytes(dtype, rows, K) + copy_bytes(dtype, K, N);
+  f.tops = at, at += up((size_t)rows * f.ntiles * 8);
+  f.picked = at, at += up((size_t)rows * 4);
+  f.bytes = at;
+  return f;
+}
+
+// Classes of a piece of gz, and where everything lies
+struct Backward {
+  long long piece, ldz;
+  int pieces;
+  size_t gz, norm, columns, part, bytes;
+};
+Backward backward_space(int what, int dtype, long long rows, int K, int N) {
+  Backward b;
+  const long long e = dtype_bytes(dtype), V = 16 / e;
+  const long long most = std::max(256LL, (long long)(kMostGradients / (size_t)(rows * e)) / 256 * 256);
+  b.pieces = (int)tiles_of(N, (int)std::min<long long>(most, 1 << 30));
+  b.piece = b.pieces == 1 ? N : (tiles_of(N, b.pieces) + 255) / 256 * 256;
+  b.pieces = (int)((N + b.piece - 1) / b.piece);
+  b.ldz = (b.piece + V - 1) / V * V;
+  const long long last = N - (b.pieces - 1) * b.piece;
+  size_t at = copy_bytes(dtype, rows, K, what & 2) + copy_bytes(dtype, K, N);
+  b.gz = at, at += up((size_t)rows * b.ldz * e);
+  b.norm = at, at += up(8);
+  b.columns = at;
+  if (what & 4)
+    for (long long n : {b.piece, last}) at = std::max(at, b.columns + up((size_t)tiles_of(rows, kGemmWM[tile_of(dtype, rows, n, K, kLossGrad)]) * n * 4));
+  b.part = at;
+  size_t part = 0;
+  if (what & 1) part = b.pieces > 1 ? up((size_t)rows * ((K + 3) & ~3LL) * 4) : part_bytes(dtype, rows, K, N, out_bytes(kFormGW, dtype));
+  size_t part_w = 0;
+  if (what & 2)
+    for (long long n : {b.piece, last}) part_w = std::max(part_w, part_bytes(dtype, K, n, rows, out_bytes(kFormXG, dtype)));
+  // (sums over pieces of classes live through all of them; pieces of a product only until they are joined)
+  b.bytes = at + (b.pieces > 1 ? part + part_w : std::max(part, part_w));
+  return b;
+}
+
+template <typename T>
+int fwd(int dtype, const LossArgs &l, hipStream_t s) {
+  const Forward at = forward_space(dtype, l.rows, l.K, l.N);
+  GemmArgs a = {};
+  a.lda = l.xs, a.ldb = l.N;
+  Copies<T> copies(l.ws);
+  a.a = copies.rows(l.x, a.lda, l.rows, l.K);
+  a.b = copies.rows(l.w, a.ldb, l.K, l.N);
+  copies.run(s);
+  a.bias = l.b, a.M = l.rows, a.N = l.N, a.K = l.K;
+  a.targets = l.targets, a.N_all = l.N;
+  a.tops = (float2 *)((char *)l.ws + at.tops), a.picked = (float *)((char *)l.ws + at.picked);
+  if (int rc = logits<T>(kLossSums, dtype, a, s)) return rc;
+  int lanes = 1;
+  while (lanes < 64 && lanes < at.ntiles) lanes *= 2;
+  const long long most = (1LL << 30) / lanes;   // rows of a launch
+  for (long long m = 0; m < l.rows; m += most) {
+    const long long now = std::min(most, l.rows - m);
+    hipLaunchKernelGGL(loss_join_kernel, dim3((unsigned)((now * lanes + 255) / 256)), dim3(256), 0, s, l.loss + m, l.lse_out ? l.lse_out + m : nullptr,
+                       a.tops + m * at.ntiles, a.picked + m, l.targets + m, now, at.ntiles, l.N, lanes);
+  }
+  return launched();
+}
+
+template <typename T>
+int bwd(int dtype, const LossArgs &l, hipStream_t s) {
+  const int what = (l.gx ? 1 : 0) | (l.gw ? 2 : 0) | (l.gb ? 4 : 0);
+  if (l.rows == 0) {
+    zero<T>(l.gw, (long long)l.K * l.N, s);
+    zero<T>(l.gb, l.N, s);
+    return launched();
+  }
+  const Backward at = backward_space(what, dtype, l.rows, l.K, l.N);
+  char *ws = (char *)l.ws;
+  long long ldx = l.xs, ldw = l.N;
+  Copies<T> copies(ws);
+  // (a row that is left out may hold anything; times a gradient of zero it would still be something in gw)
+  const T *x = (const T *)copies.rows(l.x, ldx, l.rows, l.K, l.gw ? l.targets : nullptr), *w = (const T *)copies.rows(l.w, ldw, l.K, l.N);
+  copies.run(s);
+  float *norm = nullptr;
+  if (dtype == GELIB_HIP_F16) {
+    norm = (float *)(ws + at.norm);
+    hipLaunchKernelGGL(loss_norm_kernel, dim3(1), dim3(1024), 0, s, norm, l.g, l.targets, l.rows);
+  }
+  const float *back = norm ? norm + 1 : nullptr;
+  T *gz = (T *)(ws + at.gz);
+  const bool gx = l.gx && l.K, gw = l.gw && l.K;
+  float *part = (float *)(ws + at.part), *part_w = part;
+  if (at.pieces > 1 && (what & 1)) part_w = (float *)((char *)part + up((size_t)l.rows * ((l.K + 3) & ~3LL) * 4));
+  for (int k = 0; k < at.pieces; k++) {
+    const long long n0 = k * at.piece;
+    const int n = (int)std::min(at.piece, l.N - n0);
+    GemmArgs a = {};
+    a.a = x, a.lda = ldx, a.b = w + n0, a.ldb = ldw, a.bias = l.b ? (const T *)l.b + n0 : nullptr;
+    a.c = gz, a.ldc = at.ldz, a.M = l.rows, a.N = n, a.K = l.K;
+    a.targets = l.targets, a.n_first = n0, a.N_all = l.N, a.lse = l.lse, a.weight = l.g, a.norm = norm;
+    if (l.gb) a.columns = (float *)(ws + at.columns);
+    if (int rc = logits<T>(kLossGrad, dtype, a, s)) return rc;
+    if (l.gb) {
+      const long long chunks = tiles_of(l.rows, kGemmWM[tile_of(dtype, l.rows, n, l.K, kLossGrad)]);
+      hipLaunchKernelGGL(loss_columns_kernel<T>, dim3((unsigned)std::min((n + 31LL) / 32, 1LL << 22)), dim3(256), 0, s, (T *)l.gb + n0, (const float *)a.columns, chunks, n, back);
+    }
+    if (gx) {
+      GemmArgs p = {};
+      p.a = gz, p.lda = at.ldz, p.b = w + n0, p.ldb = ldw, p.c = l.gx, p.M = l.rows, p.N = l.K, p.K = n, p.norm = back;
+      if (at.pieces == 1) {
+        if (int rc = product<T>(kFormGW, dtype, p, part, s)) return rc;
+      } else {
+        const Plan plan = plan_of(dtype, p.M, p.N, p.K, 4, true);
+        p.splits = 1, p.kper = plan.kper, p.add = k > 0;
+        p.ntiles = (unsigned)tiles_of(p.N, kGemmBN[plan.tile]);
+        const long long BM = kGemmBM[plan.tile], most = std::max(1LL, (1LL << 22) / p.ntiles) * BM;
+        for (long long m = 0; m < l.rows; m += most) {
+          GemmArgs b = p;
+          b.M = std::min(most, l.rows - m), b.mtiles = (unsigned)tiles_of(b.M, (int)BM);
+          b.a = gz + m * at.ldz, b.part = part + m * ((l.K + 3) & ~3LL);
+          if (int rc = launch_gemm<T>(kFormGW, plan.tile, b, s)) return rc;
+        }
+      }
+    }
+    if (gw) {
+      GemmArgs p = {};
+      p.a = x, p.lda = ldx, p.b = gz, p.ldb = at.ldz, p.c = (T *)l.gw + n0, p.ldc = l.N, p.M = l.K, p.N = n, p.K = l.rows, p.norm = back;
+      if (int rc = product<T>(kFormXG, dtype, p, part_w, s)) return rc;
+    }
+  }
+  if (gx && at.pieces > 1) {
+    const long long all = l.rows * l.K;
+    hipLaunchKernelGGL(loss_finish_kernel<T>, dim3((unsigned)std::min((all + 255) / 256, 1LL << 20)), dim3(256), 0, s, (T *)l.gx, (const float *)part, all, l.K, back);
+  }
+  return launched();
+}
+
+}  // namespace
+
+size_t loss_workspace(int what, int dtype, long long rows, int K, int N) {
+  if (rows == 0) return 0;
+  return what ? backward_space(what, dtype, rows, K, N).bytes : forward_space(dtype, rows, K, N).bytes;
+}
+
+int launch_loss(int dtype, const LossArgs &a, hipStream_t s) {
+  if (a.rows == 0) return 0;
+  return dtype == GELIB_HIP_F32 ? fwd<float>(dtype, a, s) : dtype == GELIB_HIP_BF16 ? fwd<bhalf_t>(dtype, a, s) : fwd<half_t>(dtype, a, s);
+}
+
+int launch_loss_bwd(int dtype, const LossArgs &a, hipStream_t s) {
+  if (!a.gx && !a.gw && !a.gb) return 0;
+  return dtype == GELIB_HIP_F32 ? bwd<float>(dtype, a, s) : dtype == GELIB_HIP_BF16 ? bwd<bhalf_t>(dtype, a, s) : bwd<half_t>(dtype, a, s);
+}
+
+}  // namespace gelib_hip

@@ -64,6 +64,57 @@ int launch_adamw(int n, const AdamTensor *t, const AdamArgs &a, hipStream_t s);
 int launch_adamw_moments(void *mv, void *vv, const void *m, const void *v, const short *mt, const short *vt, long long n, hipStream_t s);
 int launch_adamw_set_moments(void *m, void *v, short *mt, short *vt, const float *mv, const float *vv, long long n, hipStream_t s);
 
+// ---- a linear layer's classes and their loss (linear_loss.hip) ----
+struct LossArgs {
+  float *loss, *lse_out;          // forward; lse_out may be null
+  void *gx, *gw, *gb;             // backward; any may be null
+  const void *x, *w, *b;
+  const long long *targets;
+  const float *g, *lse;
+  long long rows, xs;
+  int K, N;
+  void *ws;
+};
+size_t loss_workspace(int what, int dtype, long long rows, int K, int N);   // what: bits 1 gx, 2 gw, 4 gb; 0 forward
+int launch_loss(int dtype, const LossArgs &a, hipStream_t s);
+int launch_loss_bwd(int dtype, const LossArgs &a, hipStream_t s);
+
+// ---- embedding (embedding.hip) ----
+struct EmbeddingArgs {
+  void *y, *gtable;
+  const void *table, *gy, *tokens;
+  long long n, rows;
+  int wide, channels;   // wide: tokens of 64 bits
+  float scale;
+  void *ws;
+};
+size_t embedding_workspace(long long n, int channels);
+int launch_embedding(int dtype, const EmbeddingArgs &a, hipStream_t s);
+int launch_embedding_bwd(int dtype, const EmbeddingArgs &a, hipStream_t s);
+
+// ---- attention (attention.hip) ----
+struct AttnCall {
+  const void *q, *k, *v;
+  const float *x, *xk, *slopes;    // null: no distances
+  const int *q_marks, *k_marks;    // padded: lengths or null; packed: starts, docs + 1 of them
+  long long docs, nq, nk;          // padded: samples and rows of one; packed: documents and all rows
+  long long qs[3], ks[3], vs[3];   // strides of samples, positions, heads, in elements
+  int dtype, packed, heads, kv_heads, dim;
+  float scale;
+};
+struct AttnGrads {
+  const void *y, *gy;
+  const float *lse;
+  void *gq, *gk, *gv;              // any may be null
+  float *gx, *gxk, *gslopes;
+  bool same_points;                // gx takes the sums over queries and keys
+};
+constexpr int kAttnMostDim = 128;
+inline int attention_dims(int dim) { return dim <= 32 ? 32 : dim <= 64 ? 64 : 128; }
+size_t attention_workspace(const AttnCall &c, bool backward, bool geometry);
+int launch_attention(const AttnCall &c, void *y, float *lse, void *ws, hipStream_t s);
+int launch_attention_bwd(const AttnCall &c, const AttnGrads &g, void *ws, hipStream_t s);
+
 #ifdef __HIPCC__
 typedef _Float16 half_t;
 typedef __bf16 bhalf_t;

@@ -329,6 +329,61 @@ int gelib_hip_adamw_moments(void *m_values, void *v_values, const void *m, const
 int gelib_hip_adamw_set_moments(void *m, void *v, int16_t *m_top, int16_t *v_top, const float *m_values, const float *v_values,
                                 int64_t n, void *stream);
 
+/* ---- operators of a network over points: what a point is, points that look at each other, a class for every point ---------------
+ * Types, results, workspaces and orders of summation as for the operators on real channels above. */
+
+/* y[i] = scale table[tokens[i]], (tokens, channels) packed; table (rows, channels) packed.  tokens: int32 or int64 (token_bytes 4 or 8);
+ * a row of zeros where one is below zero, a row of NaN where it is rows or more (the table is not read there). */
+int gelib_hip_embedding_fwd(void *y, const void *table, const void *tokens, int token_bytes, int dtype, int64_t ntokens, int64_t rows,
+                            int channels, float scale, void *stream);
+/* gtable[r] = scale sum of gy[i] over the i with tokens[i] == r, in their order; every row is written.  ntokens is below 2^31. */
+int gelib_hip_embedding_bwd(void *gtable, const void *gy, const void *tokens, int token_bytes, int dtype, int64_t ntokens, int64_t rows,
+                            int channels, float scale, void *workspace, uint64_t workspace_bytes, void *stream);
+uint64_t gelib_hip_embedding_workspace_bytes(int dtype, int64_t ntokens, int64_t rows, int channels);
+
+/* Attention over the points of documents.  Heads h of q stand on heads h / (heads / kv_heads) of k and v:
+ *     s_ij = scale q_i . k_j - slopes[h] |points_i - key_points_j|,  y_i = sum_j softmax_j(s_ij) v_j
+ * over the keys j of i's document; zero where there are none.  Strides in elements: sample, position, head; values contiguous.
+ * packed 0: `documents` samples of queries and keys rows; query_marks and key_marks (either may be NULL: all rows) say how many of them
+ * exist, the others are not read and get zeros.  packed 1: queries and keys rows in all (sample strides are not used), document d
+ * is rows marks[d] to marks[d + 1] of either side (documents + 1 ascending int32 each); rows in no document get zeros.  Marks are held to
+ * what there is.  Heads of q, k and v that do not lie at multiples of 16 bytes, or are no multiple of them long, are copied to ones that do.
+ * points, key_points (rows, 3) and slopes (heads) float32, or all three NULL: no distances.  dim is at most 128. */
+typedef struct {
+  const void *q, *k, *v;
+  const float *points, *key_points, *slopes;
+  const int32_t *query_marks, *key_marks;
+  int64_t documents, queries, keys;
+  int64_t q_strides[3], k_strides[3], v_strides[3];
+  int dtype, packed, heads, kv_heads, dim;
+  float scale;
+} gelib_attention_desc;
+/* y: (query rows, heads, dim) packed.  lse: float32 (query rows, heads) for the backward call, or NULL. */
+int gelib_hip_attention_fwd(const gelib_attention_desc *a, void *y, float *lse, void *workspace, uint64_t workspace_bytes, void *stream);
+/* Gradients from gy, packed as y (both at a multiple of 16 bytes where dim is one): gq (query rows, heads, dim), gk, gv (key rows, kv_heads, dim), gpoints and gkey_points (rows, 3), gslopes
+ * (heads), all packed; any may be NULL.  same_points: points and key_points are one array, and gpoints takes both sides' sums
+ * (gkey_points NULL).  Two points in one place have no direction and add nothing to the gradients of points. */
+int gelib_hip_attention_bwd(const gelib_attention_desc *a, const void *y, const float *lse, const void *gy, void *gq, void *gk, void *gv,
+                            float *gpoints, float *gkey_points, float *gslopes, int same_points, void *workspace,
+                            uint64_t workspace_bytes, void *stream);
+/* what: 0 the forward call, 1 the backward call without gradients of points and slopes, 2 with some of them */
+uint64_t gelib_hip_attention_workspace_bytes(const gelib_attention_desc *a, int what);
+
+/* Softmax cross entropy of a linear layer's classes, the logits formed tile by tile and not kept:  z = x w + bias (x (rows, n_in) at a
+ * row stride, w (n_in, n_out), bias (n_out) or NULL),  loss[i] = log sum_c exp z_ic - z_i,targets[i], float32; zero where targets[i] is
+ * below zero, NaN where it is n_out or more.  lse: float32 (rows) for the backward call, or NULL.  Alignment as for the linear layer. */
+int gelib_hip_linear_cross_entropy_fwd(float *loss, float *lse, const void *x, const void *w, const void *bias, const int64_t *targets,
+                                       int dtype, int64_t rows, int n_in, int n_out, int64_t x_row_stride, void *workspace,
+                                       uint64_t workspace_bytes, void *stream);
+/* With g (rows, float32) the gradient of the losses and gz = g (softmax(z) - onehot(targets)), zero where a target is below zero:
+ * gx = gz w^T, gw = x^T gz, gb = sum of gz over the rows; any may be NULL.  gz is formed again for some classes after the other and, in
+ * 16-bit types, rounded to the layer's type for the two products, not for gb. */
+int gelib_hip_linear_cross_entropy_bwd(void *gx, void *gw, void *gb, const float *g, const float *lse, const void *x, const void *w,
+                                       const void *bias, const int64_t *targets, int dtype, int64_t rows, int n_in, int n_out,
+                                       int64_t x_row_stride, void *workspace, uint64_t workspace_bytes, void *stream);
+/* backward: bits 1, 2 and 4 for gx, gw and gb; 0 for the forward call */
+uint64_t gelib_hip_linear_cross_entropy_workspace_bytes(int backward, int dtype, int64_t rows, int n_in, int n_out);
+
 /* ---- gather: sums of slices along the batch or a grid dimension ---------------------------------------------------------
  * A gather map is a list of (source, target) pairs with 0 <= source < n_in, 0 <= target < n_out (the arguments of
  * cnine::GatherMapB(sources, targets), python/bindings/gather_map_py.cpp:17-18).  create() checks the indices, sorts the
