@@ -1,5 +1,6 @@
 // Attention over the points of documents: which kernels a call takes (attention_impl.h has them), the joins of pieces, the sums of the
 // gradients of points over heads and of slopes over rows.
+#include <cstdlib>
 #include "attention_impl.h"
 
 namespace gelib_hip {
@@ -8,6 +9,7 @@ namespace {
 
 constexpr int kSlopeRows = 128;   // rows whose slopes' gradients one block sums
 
+int g_attention_tiles = getenv("GT") ? atoi(getenv("GT")) : 4;
 int bn_of(int dtype, int dims) { return dims * dtype_bytes(dtype) >= 512 ? 32 : 64; }
 
 // What one pass over `own` rows of a document (on the average) with `streamed` rows of the other side takes.
@@ -33,7 +35,7 @@ Pass pass_of(const AttnCall &c, AttnPass pass) {
   p.slots = c.packed ? all * per / rows + c.docs + 3 : c.docs * ((in_doc + rows - 1) / rows);
   // pieces of the streamed side where blocks do not fill the compute units, four tiles each at least
   const double blocks = std::max(1.0, own / rows) * (c.packed ? docs : (double)c.docs) * c.kv_heads, want = p.wide ? 512 : 2048;
-  const double most = streamed / bn_of(c.dtype, attention_dims(c.dim)) / 4;
+  const double most = streamed / bn_of(c.dtype, attention_dims(c.dim)) / g_attention_tiles;
   p.splits = (int)std::max(1.0, std::min({want / blocks, most, 64.0}));
   return p;
 }
@@ -125,28 +127,39 @@ int launched() {
 
 constexpr long long kMostThreads = 1LL << 30;   // of a launch
 
-// y of one (row, head): pieces' results to their common maximum
+// y of a (row, head), a wave each: pieces' results to their common maximum.  Lane k has piece k's share (there are at most 64), four
+// groups of 16 lanes take every fourth piece, four values a lane.
 template <typename T>
-__global__ void __launch_bounds__(256) attention_join_kernel(const AttnArgs a, long long first, long long all, int per_row) {
-  const long long at = first + (long long)blockIdx.x * 256 + threadIdx.x;
-  if (at >= all) return;
-  const long long row = at / per_row;
-  const int d = (int)(at - row * per_row) * 4, n = min(4, a.dim - d);
-  const long long rows = a.rows_q * a.H;
-  float top = kLowest;
-  for (int s = 0; s < a.splits; s++) top = fmaxf(top, a.part_ml[s * rows + row].x);
-  float sum = 0.f, v[4] = {0.f, 0.f, 0.f, 0.f};
-  for (int s = 0; s < a.splits; s++) {
-    const float2 ml = a.part_ml[s * rows + row];
-    if (ml.y == 0.f) continue;
-    const float by = __builtin_amdgcn_exp2f(ml.x - top);
-    sum += ml.y * by;
-    const float *p = a.part_q + (s * rows + row) * a.dim + d;
-    for (int i = 0; i < n; i++) v[i] += p[i] * by;
-  }
+__global__ void __launch_bounds__(256) attention_join_kernel(const AttnArgs a, long long first, long long rows) {
+  const long long row = first + ((long long)blockIdx.x * 256 + threadIdx.x) / 64;
+  if (row >= rows) return;
+  const int lane = threadIdx.x % 64, d0 = lane % 16 * 4;
+  const float2 ml = lane < a.splits ? a.part_ml[lane * rows + row] : make_float2(kLowest, 0.f);
+  float top = ml.x;
+#pragma unroll
+  for (int k = 1; k < 64; k *= 2) top = fmaxf(top, __shfl_xor(top, k));
+  const float share = ml.y == 0.f ? 0.f : __builtin_amdgcn_exp2f(ml.x - top);
+  float sum = ml.y * share;
+#pragma unroll
+  for (int k = 1; k < 64; k *= 2) sum += __shfl_xor(sum, k);
   const float by = sum == 0.f ? 0.f : 1.f / sum;
-  for (int i = 0; i < n; i++) ((T *)a.y)[row * a.dim + d + i] = from_f<T>(v[i] * by);
-  if (d == 0 && a.lse) a.lse[row] = sum == 0.f ? INFINITY : top + __builtin_amdgcn_logf(sum);
+  for (int d = d0; d < (a.dim + 63) / 64 * 64; d += 64) {
+    float v[4] = {0.f, 0.f, 0.f, 0.f};
+    for (int s = lane / 16; s < (a.splits + 3) / 4 * 4; s += 4) {
+      const float w = __shfl(share, s);
+      const float *p = a.part_q + (s * rows + row) * a.dim + d;
+#pragma unroll
+      for (int i = 0; i < 4; i++)
+        if (w != 0.f && d + i < a.dim) v[i] += p[i] * w;
+    }
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+      v[i] += __shfl_xor(v[i], 16);
+      v[i] += __shfl_xor(v[i], 32);
+      if (lane < 16 && d + i < a.dim) ((T *)a.y)[row * a.dim + d + i] = from_f<T>(v[i] * by);
+    }
+  }
+  if (lane == 0 && a.lse) a.lse[row] = sum == 0.f ? INFINITY : top + __builtin_amdgcn_logf(sum);
 }
 
 // 16-bit types: gq of one (row, head) from the sums of its pieces, less what D0 lacks times the sums with p (attention_impl.h), and the same
@@ -208,15 +221,23 @@ __global__ void __launch_bounds__(256) attention_points_kernel(float *out, const
   out[row * 3] = x, out[row * 3 + 1] = y, out[row * 3 + 2] = z;
 }
 
-// gradients of slopes: of kSlopeRows rows, a block; then of all blocks
-__global__ void __launch_bounds__(256) attention_slopes_kernel(float *part, const float4 *geo, int splits, long long rows, int H) {
+// gradients of slopes: of kSlopeRows rows and up to 64 heads, a block (side: threads side by side on heads, a power of two); then of all blocks
+__global__ void __launch_bounds__(256) attention_slopes_kernel(float *part, const float4 *geo, int splits, long long rows, int H, int side) {
+  __shared__ float lds[256];
   const long long r0 = (long long)blockIdx.x * kSlopeRows, r1 = min(rows, r0 + kSlopeRows);
-  for (int h = threadIdx.x; h < H; h += 256) {
-    float v = 0.f;
+  const int h = blockIdx.y * side + threadIdx.x % side, down = 256 / side;
+  float v = 0.f;
+  if (h < H)
     for (int s = 0; s < splits; s++)
-      for (long long r = r0; r < r1; r++) v += geo[(s * rows + r) * H + h].w;
-    part[(long long)blockIdx.x * H + h] = v;
+#pragma unroll 4
+      for (long long r = r0 + threadIdx.x / side; r < r1; r += down) v += geo[(s * rows + r) * H + h].w;
+  lds[threadIdx.x] = v;
+  __syncthreads();
+  for (int k = 128; k >= side; k /= 2) {
+    if ((int)threadIdx.x < k) lds[threadIdx.x] += lds[threadIdx.x + k];
+    __syncthreads();
   }
+  if ((int)threadIdx.x < side && h < H) part[(long long)blockIdx.x * H + h] = lds[threadIdx.x];
 }
 __global__ void __launch_bounds__(256) attention_slopes_join_kernel(float *out, const float *part, long long blocks, int H) {
   __shared__ float lds[256];
@@ -309,9 +330,8 @@ int forward(const AttnCall &c, void *y, float *lse, void *ws, hipStream_t s) {
   if (p.splits > 1) a.part_q = (float *)((char *)ws + at.part_q), a.part_ml = (float2 *)((char *)ws + at.ml);
   if (int rc = launch_attention_kernels<kAttnForward, T>({attention_dims(c.dim), c.slopes ? kBiasPoints : kBiasNone, p.wide}, a, s)) return rc;
   if (p.splits == 1) return 0;
-  const int per_row = (c.dim + 3) / 4;
-  const long long all = a.rows_q * a.H * per_row;
-  return in_launches(all, [&](long long first, dim3 grid) { hipLaunchKernelGGL(attention_join_kernel<T>, grid, dim3(256), 0, s, a, first, all, per_row); });
+  const long long rows = a.rows_q * a.H;
+  return in_launches(rows * 64, [&](long long first, dim3 grid) { hipLaunchKernelGGL(attention_join_kernel<T>, grid, dim3(256), 0, s, a, first / 64, rows); });
 }
 
 template <typename T>
@@ -366,7 +386,9 @@ int backward(const AttnCall &c, const AttnGrads &g, void *ws, hipStream_t s) {
     float *part = (float *)in_ws(at.slopes);
     const long long blocks = (a.rows_q + kSlopeRows - 1) / kSlopeRows;
     if (blocks) {
-      hipLaunchKernelGGL(attention_slopes_kernel, dim3((unsigned)blocks), dim3(256), 0, s, part, a.geo_q, pr.splits, a.rows_q, a.H);
+      int side = 1;
+      while (side < 64 && side < a.H) side *= 2;
+      hipLaunchKernelGGL(attention_slopes_kernel, dim3((unsigned)blocks, (unsigned)((a.H + side - 1) / side)), dim3(256), 0, s, part, a.geo_q, pr.splits, a.rows_q, a.H, side);
       if (int rc = launched()) return rc;
     }
     hipLaunchKernelGGL(attention_slopes_join_kernel, dim3(a.H), dim3(256), 0, s, g.gslopes, part, blocks, a.H);

@@ -459,7 +459,7 @@ struct KeyTiles {
 };
 
 template <typename T, int DP, int WAVES, int QS, int BIAS, bool SHARE>
-__global__ void __launch_bounds__(64 * WAVES) attention_fwd_kernel(const AttnArgs a) {
+__global__ void __launch_bounds__(64 * WAVES, 2) attention_fwd_kernel(const AttnArgs a) {
   typedef AttnTile<T, DP> Tile;
   typedef KeyTiles<T, DP, WAVES, BIAS> Keys;
   constexpr int BN = Keys::BN, SUB = BN / 16, BM = 16 * QS * WAVES;
@@ -594,7 +594,7 @@ __global__ void __launch_bounds__(64 * WAVES) attention_fwd_kernel(const AttnArg
 // heads of 64, bfloat16: errors of the gradients of points and slopes .004 without it.)  The pass by keys has the D that is right.
 
 template <typename T, int DP, int WAVES, int QS, int BIAS, bool SHARE>
-__global__ void __launch_bounds__(64 * WAVES) attention_rows_kernel(const AttnArgs a) {
+__global__ void __launch_bounds__(64 * WAVES, 2) attention_rows_kernel(const AttnArgs a) {
   typedef AttnTile<T, DP> Tile;
   typedef KeyTiles<T, DP, WAVES, BIAS> Keys;
   constexpr int BN = Keys::BN, SUB = BN / 16, BM = 16 * QS * WAVES;
@@ -640,10 +640,11 @@ __global__ void __launch_bounds__(64 * WAVES) attention_rows_kernel(const AttnAr
   const Keys keys(a, doc, w.kv);
   keys.each(lds, t0, t1, [&](int t, const typename Keys::Buffer &b) __attribute__((always_inline)) {
     const int left = doc.kn - t * BN, subs = min(SUB, (left + 15) / 16);
-#pragma unroll
+#pragma unroll 1
     for (int j0 = 0; j0 < SUB; j0 += 2) {
       if (j0 >= subs) break;
       f32x4 ds[2][SETS];
+      float part[SETS][4] = {};   // (of 32 keys: sums over thousands of them one after the other would lose two digits)
 #pragma unroll
       for (int u = 0; u < 2; u++) {
         const int j = j0 + u;
@@ -687,17 +688,22 @@ __global__ void __launch_bounds__(64 * WAVES) attention_rows_kernel(const AttnAr
             if constexpr (BIAS == kBiasGradients) {
               const int n = SHARE ? 0 : s;
               const float gi = g * far.inv[n][i], pi = p * far.inv[n][i];
-              geo[s][3] = __builtin_fmaf(g, far.far[n][i], geo[s][3]);
+              part[s][3] = __builtin_fmaf(g, far.far[n][i], part[s][3]);
 #pragma unroll
-              for (int e = 0; e < 3; e++) geo[s][e] = __builtin_fmaf(gi, far.d[n][i][e], geo[s][e]);
+              for (int e = 0; e < 3; e++) part[s][e] = __builtin_fmaf(gi, far.d[n][i][e], part[s][e]);
               if constexpr (MEND) {
-                geo[QS + s][3] = __builtin_fmaf(p, far.far[n][i], geo[QS + s][3]);
+                part[QS + s][3] = __builtin_fmaf(p, far.far[n][i], part[QS + s][3]);
 #pragma unroll
-                for (int e = 0; e < 3; e++) geo[QS + s][e] = __builtin_fmaf(pi, far.d[n][i][e], geo[QS + s][e]);
+                for (int e = 0; e < 3; e++) part[QS + s][e] = __builtin_fmaf(pi, far.d[n][i][e], part[QS + s][e]);
               }
             }
           }
       }
+      if constexpr (BIAS == kBiasGradients)
+#pragma unroll
+        for (int s = 0; s < SETS; s++)
+#pragma unroll
+          for (int e = 0; e < 4; e++) geo[s][e] += part[s][e];
       Tile::template transposed<SETS>(acc, b.k, j0 * 16, ds[0], ds[1]);
     }
   });
@@ -744,7 +750,7 @@ __global__ void __launch_bounds__(64 * WAVES) attention_rows_kernel(const AttnAr
 // ---- gradients by keys: gk, gv, the points of keys ----
 
 template <typename T, int DP, int WAVES, int QS, int BIAS, bool SHARE>
-__global__ void __launch_bounds__(64 * WAVES) attention_keys_kernel(const AttnArgs a) {
+__global__ void __launch_bounds__(64 * WAVES, 2) attention_keys_kernel(const AttnArgs a) {
   typedef AttnTile<T, DP> Tile;
   constexpr int THREADS = 64 * WAVES, BUFS = WAVES > 1 ? 2 : 1, BN = kAttnBN<T, DP>, SUB = BN / 16, BM = 16 * QS * WAVES, ROW = BIAS ? 6 : 2;
   struct Buffer {
@@ -806,7 +812,7 @@ __global__ void __launch_bounds__(64 * WAVES) attention_keys_kernel(const AttnAr
   };
   each_tile<WAVES>(lds, t0, t1, copy, [&](int t, const Buffer &b) __attribute__((always_inline)) {
     const int subs = min(SUB, (rows - t * BN + 15) / 16);
-#pragma unroll
+#pragma unroll 1
     for (int j0 = 0; j0 < SUB; j0 += 2) {
       if (j0 >= subs) break;
       f32x4 p[2][QS], ds[2][QS];
