@@ -230,34 +230,44 @@ __global__ void __launch_bounds__(256) embedding_sum_kernel(const List<T> l, O *
   };
   if (b < e) {
     const u32 left = token_before(l, b);
-    constexpr int U = 8;   // loads under way
+    constexpr int U = sizeof(T) * V == 16 && sizeof(T) == sizeof(O) ? 8 : 16;   // rows under way
+    const int lane = threadIdx.x % 64;
     bool any = false;
-    for (long long i0 = b; i0 < e; i0 += U) {
-      u32 key[U];
-      Some<T, V> v[U];
+    for (long long i0 = b; i0 < e; i0 += 64) {
+      // 64 entries at a time, one a lane: what there is, and where its row lies
+      const bool in = i0 + lane < e;
+      const u32 keys = in ? l.key[i0 + lane] : kNoToken;
+      const u32 rows = in && l.at ? l.at[i0 + lane] : (u32)(i0 + lane);
+      unsigned long long there = __ballot(keys != kNoToken);
+      while (there) {
+        u32 key[U];
+        Some<T, V> v[U];
 #pragma unroll
-      for (int u = 0; u < U; u++) {
-        const long long i = i0 + u;
-        key[u] = i < e ? __builtin_amdgcn_readfirstlane(l.key[i]) : kNoToken;
-        if (key[u] != kNoToken && here) {
-          const long long row = l.at ? __builtin_amdgcn_readfirstlane(l.at[i]) : i;
-          v[u] = *(const Some<T, V> *)(l.rows + row * C + c);
+        for (int u = 0; u < U; u++) {
+          key[u] = kNoToken;
+          if (there) {
+            const int k = __ffsll(there) - 1;
+            there &= there - 1;
+            key[u] = __builtin_amdgcn_readlane(keys, k);
+            const long long row = (long long)(u32)__builtin_amdgcn_readlane(rows, k);
+            if (here) v[u] = *(const Some<T, V> *)(l.rows + row * C + c);
+          }
         }
-      }
 #pragma unroll
-      for (int u = 0; u < U; u++) {
-        if (key[u] == kNoToken) continue;
-        if (key[u] != run) {
-          finish(false);
-          from_left = !any && key[u] == left;
-          any = true;
-          run = key[u];
+        for (int u = 0; u < U; u++) {
+          if (key[u] == kNoToken) continue;
+          if (key[u] != run) {
+            finish(false);
+            from_left = !any && key[u] == left;
+            any = true;
+            run = key[u];
 #pragma unroll
-          for (int k = 0; k < V; k++) acc[k] = 0.f;
+            for (int k = 0; k < V; k++) acc[k] = 0.f;
+          }
+          if (here)
+#pragma unroll
+            for (int k = 0; k < V; k++) acc[k] += to_f(v[u].v[k]);
         }
-        if (here)
-#pragma unroll
-          for (int k = 0; k < V; k++) acc[k] += to_f(v[u].v[k]);
       }
     }
     // the first entry of the next piece, or the one behind it, would continue the last run
@@ -319,13 +329,13 @@ int forward(const EmbeddingArgs &a, hipStream_t s) {
 }
 
 // entries of a piece
-int piece_of(long long n) { return n >= 1 << 18 ? 128 : n >= 1 << 14 ? 64 : 32; }
+int piece_of(long long n) { return n >= 1 << 18 ? 128 : 64; }
 
 struct Space {
   size_t key[2], at[2], counts, totals, count, keys[2], rows[2], bytes = 0;
 };
 Space space_of(long long n, int C) {
-  Space s;
+  Space s = {};
   auto take = [&](size_t &at, size_t bytes) { at = s.bytes, s.bytes += up(bytes); };
   const long long blocks = (n + kSortTokens - 1) / kSortTokens;
   for (int k = 0; k < 2; k++) take(s.key[k], (size_t)n * 4), take(s.at[k], (size_t)n * 4);

@@ -356,35 +356,47 @@ __global__ void __launch_bounds__(64 * (BM / WM) * (BN / WN)) gemm_kernel(const 
   if constexpr (ACT >= kLossSums) {
     // a lane holds FN vectors of four neighbouring logits of FM rows
     constexpr int apart = GN == 1 ? 16 : 4;
-    const long long nl = n0 + wn + (GN == 1 ? q * 4 : q * 4 * GN);
+    const int nl = wn + (GN == 1 ? q * 4 : q * 4 * GN), left = (int)min((long long)BN, a.N - n0);   // columns of the tile: the first one's, how many there are
     auto logit = [&](int i, int k, int e) __attribute__((always_inline)) { return GN == 1 ? acc[i][k][e] : acc[i][(4 * k + e) % GN][(4 * k + e) / GN]; };
+    // the class of a row as a column of the tile, -1: in another tile, or none
+    auto column_of = [&](long long t) __attribute__((always_inline)) {
+      const long long at = t - a.n_first - n0;
+      return t >= 0 && at >= 0 && at < left ? (int)at : -1;
+    };
     static_assert(FN <= 4, "");
     if constexpr (ACT == kLossSums) {
       __shared__ float2 tops[BN / WN][BM];
+      const bool whole = left == BN;
 #pragma unroll
       for (int i = 0; i < FM; i++) {
         const int r = wm + (i / GM * GM) * 16 + c * GM + i % GM;
-        const long long t = m0 + r < a.M ? a.targets[m0 + r] : -1;
-        float top = -INFINITY, sum = 0.f;
+        const int t = m0 + r < a.M ? column_of(a.targets[m0 + r]) : -1;
+        float top = -INFINITY, sum = 0.f, own = 0.f;
 #pragma unroll
         for (int k = 0; k < FN; k++)
 #pragma unroll
           for (int e = 0; e < 4; e++) {
-            const long long n = nl + k * apart + e;
-            if (n < a.N) top = fmaxf(top, logit(i, k, e));
-            if (n == t && n < a.N) a.picked[m0 + r] = logit(i, k, e);
+            const int n = nl + k * apart + e;
+            const float z = logit(i, k, e);
+            top = fmaxf(top, whole || n < left ? z : -INFINITY);
+            own = n == t ? z : own;
           }
+        // (only the lane that has column t writes)
+        if (t >= 0 && t >= nl && (GN == 1 ? (t - nl) % 16 < 4 && t - nl < 16 * FN : t - nl < 4 * GN)) a.picked[m0 + r] = own;
         top = fmaxf(top, __shfl_xor(top, 16));
         top = fmaxf(top, __shfl_xor(top, 32));
-        const float from = top == -INFINITY ? 0.f : top;
+        const float from = (top == -INFINITY ? 0.f : top) * 1.44269504088896341f;
 #pragma unroll
         for (int k = 0; k < FN; k++)
 #pragma unroll
-          for (int e = 0; e < 4; e++)
-            if (nl + k * apart + e < a.N) sum += __builtin_amdgcn_exp2f((logit(i, k, e) - from) * 1.44269504088896341f);
+          for (int e = 0; e < 4; e++) {
+            const float p = __builtin_amdgcn_exp2f(__builtin_fmaf(logit(i, k, e), 1.44269504088896341f, -from));
+            sum += whole || nl + k * apart + e < left ? p : 0.f;
+          }
         sum += __shfl_xor(sum, 16);
         sum += __shfl_xor(sum, 32);
         if (q == 0) tops[wn / WN][r] = make_float2(top, sum);
+        __builtin_amdgcn_sched_barrier(0);   // (row by row: all of them at once do not fit the registers)
       }
       __syncthreads();
       for (int r = threadIdx.x; r < BM; r += THREADS) {
@@ -401,25 +413,30 @@ __global__ void __launch_bounds__(64 * (BM / WM) * (BN / WN)) gemm_kernel(const 
     } else {
       float column[FN][4] = {};
       const float norm = a.norm ? *a.norm : 1.f;
+      const int stored = (int)min((long long)BN, a.ldc - n0);
 #pragma unroll
       for (int i = 0; i < FM; i++) {
         const long long m = m0 + wm + (i / GM * GM) * 16 + c * GM + i % GM;
-        if (m >= a.M) continue;
-        const long long t = a.targets[m];
-        const float lse = a.lse[m], g = t < a.N_all ? a.weight[m] * norm : __builtin_nanf("");
+        if (m < a.M) {
+          const long long class_ = a.targets[m];
+          const int t = column_of(class_);
+          const float from = a.lse[m] * 1.44269504088896341f, g = class_ < a.N_all ? a.weight[m] * norm : __builtin_nanf("");
+          T *to = (T *)a.c + m * a.ldc + n0 + nl;
 #pragma unroll
-        for (int k = 0; k < FN; k++) {
-          T v[4];
+          for (int k = 0; k < FN; k++) {
+            T v[4];
 #pragma unroll
-          for (int e = 0; e < 4; e++) {
-            const long long n = nl + k * apart + e;
-            const float p = __builtin_amdgcn_exp2f((logit(i, k, e) - lse) * 1.44269504088896341f);
-            const float gz = n < a.N && t >= 0 ? (p - (n + a.n_first == t ? 1.f : 0.f)) * g : 0.f;
-            column[k][e] += gz;
-            v[e] = from_f<T>(gz);
+            for (int e = 0; e < 4; e++) {
+              const int n = nl + k * apart + e;
+              const float p = __builtin_amdgcn_exp2f(__builtin_fmaf(logit(i, k, e), 1.44269504088896341f, -from)) - (n == t ? 1.f : 0.f);
+              const float gz = n < left && class_ >= 0 ? p * g : 0.f;
+              column[k][e] += gz;
+              v[e] = from_f<T>(gz);
+            }
+            if (nl + k * apart < stored) __builtin_memcpy(__builtin_assume_aligned(to + k * apart, 4 * sizeof(T)), v, 4 * sizeof(T));
           }
-          if (nl + k * apart < a.ldc) __builtin_memcpy(__builtin_assume_aligned((T *)a.c + m * a.ldc + nl + k * apart, 4 * sizeof(T)), v, 4 * sizeof(T));
         }
+        __builtin_amdgcn_sched_barrier(0);
       }
       if (a.columns) {
 #pragma unroll
@@ -429,8 +446,8 @@ __global__ void __launch_bounds__(64 * (BM / WM) * (BN / WN)) gemm_kernel(const 
             float v = column[k][e];
 #pragma unroll
             for (int d = 1; d < 16; d *= 2) v += __shfl_xor(v, d);
-            const long long n = nl + k * apart + e;
-            if (c == 0 && n < a.N && m0 + wm < a.M) a.columns[(m0 + wm) / WM * a.N + n] = v;
+            const int n = nl + k * apart + e;
+            if (c == 0 && n < left && m0 + wm < a.M) a.columns[(m0 + wm) / WM * a.N + n0 + n] = v;
           }
       }
     }

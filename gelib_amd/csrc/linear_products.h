@@ -141,9 +141,15 @@ __global__ void __launch_bounds__(256) copy_rows_kernel(const CopyArgs a) {
     const long long at = t - a.m[k].first, row = at / per_row;
     const int c = (int)(at - row * per_row) * V;
     const T *p = (const T *)a.m[k].from + row * a.m[k].stride + c;
-    T v[V];
+    T v[V] = {};
+    if (!a.m[k].classes || a.m[k].classes[row] >= 0) {
+      if (a.m[k].cols % V == 0) {   // (whole rows are aligned, and copied for what they leave out)
+        __builtin_memcpy(v, __builtin_assume_aligned(p, 16), 16);
+      } else {
 #pragma unroll
-    for (int i = 0; i < V; i++) v[i] = c + i < a.m[k].cols && (!a.m[k].classes || a.m[k].classes[row] >= 0) ? p[i] : (T)0.f;
+        for (int i = 0; i < V; i++) v[i] = c + i < a.m[k].cols ? p[i] : (T)0.f;
+      }
+    }
     __builtin_memcpy(__builtin_assume_aligned((T *)a.m[k].to + at * V, 16), v, 16);
   }
 }
