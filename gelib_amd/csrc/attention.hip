@@ -28,14 +28,14 @@ Pass pass_of(const AttnCall &c, AttnPass pass) {
   p.wide = own > 64;
   // Heads of a group by tiles, where distances are formed: both sides of a tile pair share them.  Positions are filled up to 16, which costs
   // less than it gives from two such tiles on.
-  const int own_rows = attention_rows(pass, (int)dtype_bytes(c.dtype), attention_dims(c.dim), true);
+  const int own_rows = attention_rows(pass, (int)dtype_bytes(c.dtype), attention_dims(c.dtype, c.dim), true);
   p.blocked = c.slopes && p.wide && (G == 2 || G == 4 || G == 8) && c.nq / docs >= 32 && (!own_q || own_rows % (16 * G) == 0);
-  const int rows = attention_rows(pass, (int)dtype_bytes(c.dtype), attention_dims(c.dim), p.wide);
+  const int rows = attention_rows(pass, (int)dtype_bytes(c.dtype), attention_dims(c.dtype, c.dim), p.wide);
   const long long in_doc = own_q && p.blocked ? (all + 15) / 16 * 16 * per : all * per;
   p.slots = c.packed ? all * per / rows + c.docs + 3 : c.docs * ((in_doc + rows - 1) / rows);
   // pieces of the streamed side where blocks do not fill the compute units, four tiles each at least
   const double blocks = std::max(1.0, own / rows) * (c.packed ? docs : (double)c.docs) * c.kv_heads, want = p.wide ? 512 : 2048;
-  const double most = streamed / bn_of(c.dtype, attention_dims(c.dim)) / g_attention_tiles;
+  const double most = streamed / bn_of(c.dtype, attention_dims(c.dtype, c.dim)) / g_attention_tiles;
   p.splits = (int)std::max(1.0, std::min({want / blocks, most, 64.0}));
   return p;
 }
@@ -328,7 +328,7 @@ int forward(const AttnCall &c, void *y, float *lse, void *ws, hipStream_t s) {
   AttnArgs a = pass_args(args_of<T>(c, y, nullptr, at, (char *)ws, s), p);
   a.lse = lse, a.vec_y = whole4(c, {y});
   if (p.splits > 1) a.part_q = (float *)((char *)ws + at.part_q), a.part_ml = (float2 *)((char *)ws + at.ml);
-  if (int rc = launch_attention_kernels<kAttnForward, T>({attention_dims(c.dim), c.slopes ? kBiasPoints : kBiasNone, p.wide}, a, s)) return rc;
+  if (int rc = launch_attention_kernels<kAttnForward, T>({attention_dims(c.dtype, c.dim), c.slopes ? kBiasPoints : kBiasNone, p.wide}, a, s)) return rc;
   if (p.splits == 1) return 0;
   const long long rows = a.rows_q * a.H;
   return in_launches(rows * 64, [&](long long first, dim3 grid) { hipLaunchKernelGGL(attention_join_kernel<T>, grid, dim3(256), 0, s, a, first / 64, rows); });
@@ -343,7 +343,7 @@ int backward(const AttnCall &c, const AttnGrads &g, void *ws, hipStream_t s) {
   a.lse = (float *)g.lse, a.delta = (float *)in_ws(at.delta), a.vec_y = whole4(c, {g.gq, g.gk, g.gv});
   a.gq = g.gq, a.gk = g.gk, a.gv = g.gv;
   if (geometry) a.geo_q = (float4 *)in_ws(at.geo_q), a.geo_k = (float4 *)in_ws(at.geo_k);
-  const int bias = geometry ? kBiasGradients : c.slopes ? kBiasPoints : kBiasNone, dims = attention_dims(c.dim);
+  const int bias = geometry ? kBiasGradients : c.slopes ? kBiasPoints : kBiasNone, dims = attention_dims(c.dtype, c.dim);
   Pass pr = pass_of(c, kAttnRows);
   const Pass pk = pass_of(c, kAttnKeys);
   AttnArgs r = pass_args(a, pr), k = pass_args(a, pk);

@@ -14,6 +14,8 @@
 // A document's query rows are its (position, head of the group) pairs: heads that share keys stand in one tile.
 #pragma once
 
+#include <type_traits>
+
 #include "real_ops.h"
 
 namespace gelib_hip {
@@ -40,16 +42,16 @@ struct AttnArgs {
 
 enum AttnBias { kBiasNone = 0, kBiasPoints = 1, kBiasGradients = 2 };
 
-// what a launch is made for; dims: 32, 64 or 128 values of a head in LDS
+// what a launch is made for; dims: 16 (float32 only: a step of the 16-bit products is 32), 32, 64 or 128 values of a head in LDS
 struct AttnPlan {
   int dims, bias;
   bool wide;   // four waves a block
 };
 enum AttnPass { kAttnForward, kAttnRows, kAttnKeys };
-// 16 QS own rows a wave: two tiles share every fragment of the streamed side, where registers hold their operands and results
-constexpr int attention_qs(AttnPass pass, int element, int dims) { return dims == 128 && (pass == kAttnRows || (pass == kAttnKeys && element == 4)) ? 1 : 2; }
-constexpr int attention_rows(AttnPass pass, int element, int dims, bool wide) { return 16 * attention_qs(pass, element, dims) * (wide ? 4 : 1); }
-
+// 16 QS own rows a wave: four waves a block take two tiles each, which share every fragment of the streamed side, where registers hold
+// their operands and results; a wave alone one, since the documents are short.
+constexpr int attention_qs(AttnPass pass, int element, int dims, bool wide) { return !wide || (dims == 128 && (pass != kAttnForward || element == 4)) ? 1 : 2; }
+constexpr int attention_rows(AttnPass pass, int element, int dims, bool wide) { return 16 * attention_qs(pass, element, dims, wide) * (wide ? 4 : 1); }
 template <AttnPass PASS, typename T>
 int launch_attention_kernels(const AttnPlan &p, const AttnArgs &a, hipStream_t s);
 
@@ -371,28 +373,25 @@ __device__ __forceinline__ void piece_of(int tiles, int split, int splits, int &
   from = min(tiles, split * per), to = min(tiles, from + per);
 }
 
-// Distances of a lane's own rows from four neighbouring points of the streamed side, which its wave's tiles have in common where SHARE.
-template <int QS, bool SHARE, bool GRADIENTS>
-struct Distances {
-  static constexpr int N = SHARE ? 1 : QS;
-  float far[N][4], inv[GRADIENTS ? N : 1][4], d[GRADIENTS ? N : 1][4][3];
-  __device__ __forceinline__ void form(const float (*x)[3], const f32x4 *p) {
+// Distance of an own row from one point of the streamed side, and what its gradients take of it.
+template <int BIAS>
+struct Distance {
+  float far, inv, d[3];
+  __device__ __forceinline__ void form(const float *x, const f32x4 *p, int i) {
+    if constexpr (BIAS != kBiasNone) {
 #pragma unroll
-    for (int s = 0; s < N; s++)
+      for (int k = 0; k < 3; k++) d[k] = x[k] - p[k][i];
+      const float sq = d[0] * d[0] + d[1] * d[1] + d[2] * d[2];
+      if constexpr (BIAS == kBiasGradients) inv = __builtin_amdgcn_rsqf(fmaxf(sq, 1e-37f)), far = sq * inv;   // (in one place: d and far are zero)
+      else far = __builtin_amdgcn_sqrtf(sq);
+    }
+  }
+  // sums of g d / |d| and g |d|
+  __device__ __forceinline__ void add(float *sums, float g) const {
+    const float w = g * inv;
 #pragma unroll
-      for (int i = 0; i < 4; i++) {
-        float e[3];
-#pragma unroll
-        for (int k = 0; k < 3; k++) e[k] = x[s][k] - p[k][i];
-        const float sq = e[0] * e[0] + e[1] * e[1] + e[2] * e[2];
-        if constexpr (GRADIENTS) {
-          inv[s][i] = __builtin_amdgcn_rsqf(fmaxf(sq, 1e-37f)), far[s][i] = sq * inv[s][i];
-#pragma unroll
-          for (int k = 0; k < 3; k++) d[s][i][k] = e[k];
-        } else {
-          far[s][i] = __builtin_amdgcn_sqrtf(sq);
-        }
-      }
+    for (int k = 0; k < 3; k++) sums[k] = __builtin_fmaf(w, d[k], sums[k]);
+    sums[3] = __builtin_fmaf(g, far, sums[3]);
   }
 };
 
@@ -507,12 +506,15 @@ __global__ void __launch_bounds__(64 * WAVES, 2) attention_fwd_kernel(const Attn
         f32x4 p[3];
 #pragma unroll
         for (int e = 0; e < 3; e++) p[e] = *(const f32x4 *)&b.x[e][j * 16 + q4];
-        Distances<QS, SHARE, false> far;
-        far.form(own.x, p);
 #pragma unroll
-        for (int s = 0; s < QS; s++)
+        for (int i = 0; i < 4; i++) {
+          Distance<kBiasPoints> far;
 #pragma unroll
-          for (int i = 0; i < 4; i++) sc[s][j][i] = __builtin_fmaf(z[s][i], a.scale2, __builtin_fmaf(far.far[SHARE ? 0 : s][i], own.slope[s], -m[s]));
+          for (int s = 0; s < QS; s++) {
+            if (!SHARE || s == 0) far.form(own.x[s], p, i);   // (the wave's tiles have the same positions)
+            sc[s][j][i] = __builtin_fmaf(z[s][i], a.scale2, __builtin_fmaf(far.far, own.slope[s], -m[s]));
+          }
+        }
       } else {
 #pragma unroll
         for (int s = 0; s < QS; s++)
@@ -644,7 +646,7 @@ __global__ void __launch_bounds__(64 * WAVES, 2) attention_rows_kernel(const Att
     for (int j0 = 0; j0 < SUB; j0 += 2) {
       if (j0 >= subs) break;
       f32x4 ds[2][SETS];
-      float part[SETS][4] = {};   // (of 32 keys: sums over thousands of them one after the other would lose two digits)
+      float part[QS][4] = {};   // (of 32 keys: sums over thousands of them one after the other would lose two digits)
 #pragma unroll
       for (int u = 0; u < 2; u++) {
         const int j = j0 + u;
@@ -657,51 +659,38 @@ __global__ void __launch_bounds__(64 * WAVES, 2) attention_rows_kernel(const Att
 #pragma unroll
           for (int s = 0; s < QS; s++) z[s] = Tile::product(fk, own.q[s][k], z[s]), dp[s] = Tile::product(fv, fg[s][k], dp[s]);
         }
-        Distances<QS, SHARE, BIAS == kBiasGradients> far;
-        if constexpr (BIAS != kBiasNone) {
-          f32x4 p[3];
+        f32x4 point[3];
+        if (BIAS)
 #pragma unroll
-          for (int e = 0; e < 3; e++) p[e] = *(const f32x4 *)&b.x[e][j * 16 + q4];
-          far.form(own.x, p);
-        }
-        f32x4 prob[QS];
-#pragma unroll
-        for (int s = 0; s < QS; s++)
+          for (int e = 0; e < 3; e++) point[e] = *(const f32x4 *)&b.x[BIAS ? e : 0][j * 16 + q4];
+        // (everything of one key before the next one's: registers)
+        auto elements = [&](auto masked) __attribute__((always_inline)) {
 #pragma unroll
           for (int i = 0; i < 4; i++) {
-            if constexpr (BIAS != kBiasNone) prob[s][i] = __builtin_fmaf(z[s][i], a.scale2, __builtin_fmaf(far.far[SHARE ? 0 : s][i], own.slope[s], nlse[s]));
-            else prob[s][i] = __builtin_fmaf(z[s][i], a.scale2, nlse[s]);
-          }
-        if (left < j * 16 + 16)
+            const bool in = !masked.value || j * 16 + q4 + i < left;
+            Distance<BIAS> far;
 #pragma unroll
-          for (int i = 0; i < 4; i++)
-            if (j * 16 + q4 + i >= left)
-#pragma unroll
-              for (int s = 0; s < QS; s++) prob[s][i] = -INFINITY;
-#pragma unroll
-        for (int s = 0; s < QS; s++)
-#pragma unroll
-          for (int i = 0; i < 4; i++) {
-            const float p = __builtin_amdgcn_exp2f(prob[s][i]), g = p * dp[s][i];
-            ds[u][s][i] = g;
-            if constexpr (MEND) ds[u][QS + s][i] = p, rest[s] += g;
-            if constexpr (BIAS == kBiasGradients) {
-              const int n = SHARE ? 0 : s;
-              const float gi = g * far.inv[n][i], pi = p * far.inv[n][i];
-              part[s][3] = __builtin_fmaf(g, far.far[n][i], part[s][3]);
-#pragma unroll
-              for (int e = 0; e < 3; e++) part[s][e] = __builtin_fmaf(gi, far.d[n][i][e], part[s][e]);
-              if constexpr (MEND) {
-                part[QS + s][3] = __builtin_fmaf(p, far.far[n][i], part[QS + s][3]);
-#pragma unroll
-                for (int e = 0; e < 3; e++) part[QS + s][e] = __builtin_fmaf(pi, far.d[n][i][e], part[QS + s][e]);
+            for (int s = 0; s < QS; s++) {
+              if (!SHARE || s == 0) far.form(own.x[s], point, i);
+              float v = BIAS ? __builtin_fmaf(far.far, own.slope[s], nlse[s]) : nlse[s];
+              v = __builtin_fmaf(z[s][i], a.scale2, v);
+              if (masked.value) v = in ? v : -INFINITY;
+              const float p = __builtin_amdgcn_exp2f(v), g = p * dp[s][i];
+              ds[u][s][i] = g;
+              if constexpr (MEND) ds[u][QS + s][i] = p, rest[s] += g;
+              if constexpr (BIAS == kBiasGradients) {
+                far.add(part[s], g);
+                if constexpr (MEND) far.add(geo[QS + s], p);
               }
             }
           }
+        };
+        if (left < j * 16 + 16) elements(std::true_type());
+        else elements(std::false_type());
       }
       if constexpr (BIAS == kBiasGradients)
 #pragma unroll
-        for (int s = 0; s < SETS; s++)
+        for (int s = 0; s < QS; s++)
 #pragma unroll
           for (int e = 0; e < 4; e++) geo[s][e] += part[s][e];
       Tile::template transposed<SETS>(acc, b.k, j0 * 16, ds[0], ds[1]);
@@ -815,48 +804,57 @@ __global__ void __launch_bounds__(64 * WAVES, 2) attention_keys_kernel(const Att
 #pragma unroll 1
     for (int j0 = 0; j0 < SUB; j0 += 2) {
       if (j0 >= subs) break;
-      f32x4 p[2][QS], ds[2][QS];
-      Distances<QS, false, BIAS == kBiasGradients> far;
+      f32x4 p[2][QS], ds[2][QS];   // scores and gy . v - D, then p and ds
 #pragma unroll
       for (int u = 0; u < 2; u++) {
         const int j = j0 + u;
-        f32x4 z[QS], dp[QS];
-        const f32x4 delta = *(const f32x4 *)&b.r[1][j * 16 + q4], lse = *(const f32x4 *)&b.r[0][j * 16 + q4];
+        const f32x4 delta = *(const f32x4 *)&b.r[1][j * 16 + q4];
 #pragma unroll
-        for (int s = 0; s < QS; s++) z[s] = f32x4{0.f, 0.f, 0.f, 0.f}, dp[s] = -delta;
+        for (int s = 0; s < QS; s++) p[u][s] = f32x4{0.f, 0.f, 0.f, 0.f}, ds[u][s] = -delta;
 #pragma unroll
         for (int k = 0; k < Tile::KS; k++) {
           const typename Tile::Frag fq = Tile::frag(b.q, j * 16, k), fg = Tile::frag(b.g, j * 16, k);
 #pragma unroll
-          for (int s = 0; s < QS; s++) z[s] = Tile::product(fq, fk[s][k], z[s]), dp[s] = Tile::product(fg, fv[s][k], dp[s]);
+          for (int s = 0; s < QS; s++) p[u][s] = Tile::product(fq, fk[s][k], p[u][s]), ds[u][s] = Tile::product(fg, fv[s][k], ds[u][s]);
         }
-        f32x4 slope;
-        if constexpr (BIAS != kBiasNone) {
-          slope = *(const f32x4 *)&b.r[2][j * 16 + q4];
-          if (!SHARE || u == 0) {   // (the second 16 rows are the same positions)
-            f32x4 r[3];
+      }
+      // what rows are: the second 16 have the positions of the first where SHARE
+      f32x4 nlse[2], slope[2], point[SHARE ? 1 : 2][3];
 #pragma unroll
-            for (int e = 0; e < 3; e++) r[e] = *(const f32x4 *)&b.r[3 + e][j * 16 + q4];
-            far.form(x, r);
+      for (int u = 0; u < 2; u++) {
+        nlse[u] = -*(const f32x4 *)&b.r[0][(j0 + u) * 16 + q4];
+        if constexpr (BIAS != kBiasNone) {
+          slope[u] = *(const f32x4 *)&b.r[2][(j0 + u) * 16 + q4];
+          if (!SHARE || u == 0)
+#pragma unroll
+            for (int e = 0; e < 3; e++) point[u][e] = *(const f32x4 *)&b.r[3 + e][(j0 + u) * 16 + q4];
+        }
+      }
+      float part[QS][4] = {};
+#pragma unroll
+      for (int s = 0; s < QS; s++)
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+          Distance<BIAS> far;
+#pragma unroll
+          for (int u = 0; u < 2; u++) {
+            if (!SHARE || u == 0) far.form(x[s], point[u], i);   // (from the key: the sign that its gradient takes)
+            float v = nlse[u][i];
+            if constexpr (BIAS != kBiasNone) v = __builtin_fmaf(far.far, slope[u][i] * -1.44269504088896341f, v);
+            const float prob = __builtin_amdgcn_exp2f(__builtin_fmaf(p[u][s][i], a.scale2, v)), g = prob * ds[u][s][i];
+            p[u][s][i] = prob, ds[u][s][i] = g;
+            if constexpr (BIAS == kBiasGradients) {
+              const float w = g * far.inv * slope[u][i];
+#pragma unroll
+              for (int e = 0; e < 3; e++) part[s][e] = __builtin_fmaf(w, far.d[e], part[s][e]);
+            }
           }
         }
-        const f32x4 slope2 = slope * -1.44269504088896341f;
+      if constexpr (BIAS == kBiasGradients)
 #pragma unroll
         for (int s = 0; s < QS; s++)
 #pragma unroll
-          for (int i = 0; i < 4; i++) {
-            float v;
-            if constexpr (BIAS != kBiasNone) v = __builtin_fmaf(z[s][i], a.scale2, __builtin_fmaf(far.far[s][i], slope2[i], -lse[i]));
-            else v = __builtin_fmaf(z[s][i], a.scale2, -lse[i]);
-            const float prob = __builtin_amdgcn_exp2f(v), g = prob * dp[s][i];
-            p[u][s][i] = prob, ds[u][s][i] = g;
-            if constexpr (BIAS == kBiasGradients) {
-              const float gi = g * far.inv[s][i] * slope[i];
-#pragma unroll
-              for (int e = 0; e < 3; e++) geo[s][e] = __builtin_fmaf(gi, far.d[s][i][e], geo[s][e]);
-            }
-          }
-      }
+          for (int e = 0; e < 3; e++) geo[s][e] -= part[s][e];
       Tile::template transposed<QS>(av, b.g, j0 * 16, p[0], p[1]);
       Tile::template transposed<QS>(ak, b.q, j0 * 16, ds[0], ds[1]);
     }
@@ -872,7 +870,7 @@ __global__ void __launch_bounds__(64 * WAVES, 2) attention_keys_kernel(const Att
     if (BIAS == kBiasGradients) {
 #pragma unroll
       for (int e = 0; e < 3; e++) {
-        const float all = -over_row_sum(geo[s][e]);   // (x - p above: from the key's point)
+        const float all = over_row_sum(geo[s][e]);
         geo[s][e] = exists[s] ? all : 0.f;
       }
       if (mine[s] && q4 == 0) a.geo_k[at] = make_float4(geo[s][0], geo[s][1], geo[s][2], 0.f);
@@ -900,7 +898,7 @@ constexpr long long kAttnMostBlocks = 1 << 22;
 
 template <AttnPass PASS, typename T, int DP, int WAVES, int BIAS, bool SHARE>
 void launch_attention_pass(AttnArgs a, hipStream_t s) {
-  constexpr int QS = attention_qs(PASS, sizeof(T), DP);
+  constexpr int QS = attention_qs(PASS, sizeof(T), DP, WAVES > 1);
   const long long blocks = a.slots * a.KV * a.splits;
   for (a.first = 0; a.first < blocks; a.first += kAttnMostBlocks) {
     const dim3 grid((unsigned)std::min(kAttnMostBlocks, blocks - a.first)), block(64 * WAVES);
@@ -913,7 +911,7 @@ void launch_attention_pass(AttnArgs a, hipStream_t s) {
 template <AttnPass PASS, typename T, int DP, int BIAS>
 void launch_attention_bias(const AttnPlan &p, const AttnArgs &a, hipStream_t s) {
   // (own rows share where a wave has two tiles of them, streamed ones always)
-  constexpr bool SHARES = BIAS != kBiasNone && (PASS == kAttnKeys || attention_qs(PASS, sizeof(T), DP) == 2);
+  constexpr bool SHARES = BIAS != kBiasNone && (PASS == kAttnKeys || attention_qs(PASS, sizeof(T), DP, true) == 2);
   if (!p.wide) launch_attention_pass<PASS, T, DP, 1, BIAS, false>(a, s);
   else if (!SHARES || !a.blocked) launch_attention_pass<PASS, T, DP, 4, BIAS, false>(a, s);
   else if constexpr (SHARES) launch_attention_pass<PASS, T, DP, 4, BIAS, true>(a, s);
@@ -928,9 +926,11 @@ void launch_attention_dims(const AttnPlan &p, const AttnArgs &a, hipStream_t s) 
 
 template <AttnPass PASS, typename T>
 int launch_attention_kernels(const AttnPlan &p, const AttnArgs &a, hipStream_t s) {
+  if constexpr (sizeof(T) == 4)
+    if (p.dims == 16) launch_attention_dims<PASS, T, 16>(p, a, s);
   if (p.dims == 32) launch_attention_dims<PASS, T, 32>(p, a, s);
   else if (p.dims == 64) launch_attention_dims<PASS, T, 64>(p, a, s);
-  else launch_attention_dims<PASS, T, 128>(p, a, s);
+  else if (p.dims == 128) launch_attention_dims<PASS, T, 128>(p, a, s);
   const hipError_t e = hipGetLastError();
   return e == hipSuccess ? 0 : record_hip_error(e, "attention launch");
 }

@@ -207,6 +207,7 @@ __global__ void __launch_bounds__(256) embedding_sum_kernel(const List<T> l, O *
   const bool names = w - p * chunks == 0 && threadIdx.x % 64 == 0;
   const long long b = p * piece, e = min(n, b + piece);
   const bool here = c < C;
+  const int cc = here ? c : 0;
   float acc[V] = {};
   u32 run = kNoToken, head = kNoToken, tail = kNoToken;
   bool from_left = false;
@@ -230,7 +231,7 @@ __global__ void __launch_bounds__(256) embedding_sum_kernel(const List<T> l, O *
   };
   if (b < e) {
     const u32 left = token_before(l, b);
-    constexpr int U = sizeof(T) * V == 16 && sizeof(T) == sizeof(O) ? 8 : 16;   // rows under way
+    constexpr int U = 16;   // rows under way
     const int lane = threadIdx.x % 64;
     bool any = false;
     for (long long i0 = b; i0 < e; i0 += 64) {
@@ -240,18 +241,16 @@ __global__ void __launch_bounds__(256) embedding_sum_kernel(const List<T> l, O *
       const u32 rows = in && l.at ? l.at[i0 + lane] : (u32)(i0 + lane);
       unsigned long long there = __ballot(keys != kNoToken);
       while (there) {
+        // (loads without a branch between them: behind the last entry it is read again)
         u32 key[U];
         Some<T, V> v[U];
+        int k = 0;
 #pragma unroll
         for (int u = 0; u < U; u++) {
-          key[u] = kNoToken;
-          if (there) {
-            const int k = __ffsll(there) - 1;
-            there &= there - 1;
-            key[u] = __builtin_amdgcn_readlane(keys, k);
-            const long long row = (long long)(u32)__builtin_amdgcn_readlane(rows, k);
-            if (here) v[u] = *(const Some<T, V> *)(l.rows + row * C + c);
-          }
+          k = there ? __ffsll(there) - 1 : k;
+          key[u] = there ? __builtin_amdgcn_readlane(keys, k) : kNoToken;
+          there &= there - 1;
+          v[u] = *(const Some<T, V> *)(l.rows + (long long)(u32)__builtin_amdgcn_readlane(rows, k) * C + cc);
         }
 #pragma unroll
         for (int u = 0; u < U; u++) {
@@ -262,11 +261,10 @@ __global__ void __launch_bounds__(256) embedding_sum_kernel(const List<T> l, O *
             any = true;
             run = key[u];
 #pragma unroll
-            for (int k = 0; k < V; k++) acc[k] = 0.f;
+            for (int i = 0; i < V; i++) acc[i] = 0.f;
           }
-          if (here)
 #pragma unroll
-            for (int k = 0; k < V; k++) acc[k] += to_f(v[u].v[k]);
+          for (int i = 0; i < V; i++) acc[i] += to_f(v[u].v[i]);
         }
       }
     }
@@ -329,7 +327,7 @@ int forward(const EmbeddingArgs &a, hipStream_t s) {
 }
 
 // entries of a piece
-int piece_of(long long n) { return n >= 1 << 18 ? 128 : 64; }
+int piece_of(long long n) { return n >= 1 << 18 ? 256 : 64; }
 
 struct Space {
   size_t key[2], at[2], counts, totals, count, keys[2], rows[2], bytes = 0;

@@ -110,7 +110,7 @@ struct AttnGrads {
   bool same_points;                // gx takes the sums over queries and keys
 };
 constexpr int kAttnMostDim = 128;
-inline int attention_dims(int dim) { return dim <= 32 ? 32 : dim <= 64 ? 64 : 128; }
+inline int attention_dims(int dtype, int dim) { return dim <= 16 && dtype == GELIB_HIP_F32 ? 16 : dim <= 32 ? 32 : dim <= 64 ? 64 : 128; }
 size_t attention_workspace(const AttnCall &c, bool backward, bool geometry);
 int launch_attention(const AttnCall &c, void *y, float *lse, void *ws, hipStream_t s);
 int launch_attention_bwd(const AttnCall &c, const AttnGrads &g, void *ws, hipStream_t s);
