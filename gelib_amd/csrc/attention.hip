@@ -1,6 +1,5 @@
 // Attention over the points of documents: which kernels a call takes (attention_impl.h has them), the joins of pieces, the sums of the
 // gradients of points over heads and of slopes over rows.
-#include <cstdlib>
 #include "attention_impl.h"
 
 namespace gelib_hip {
@@ -9,14 +8,13 @@ namespace {
 
 constexpr int kSlopeRows = 128;   // rows whose slopes' gradients one block sums
 
-int g_attention_tiles = getenv("GT") ? atoi(getenv("GT")) : 4;
 int bn_of(int dtype, int dims) { return dims * dtype_bytes(dtype) >= 512 ? 32 : 64; }
 
 // What one pass over `own` rows of a document (on the average) with `streamed` rows of the other side takes.
 struct Pass {
   bool wide, blocked;
   long long slots;
-  int splits;
+  int splits, heads;   // heads: of keys, one after the other in a block
 };
 Pass pass_of(const AttnCall &c, AttnPass pass) {
   const bool own_q = pass != kAttnKeys;
@@ -28,14 +26,19 @@ Pass pass_of(const AttnCall &c, AttnPass pass) {
   p.wide = own > 64;
   // Heads of a group by tiles, where distances are formed: both sides of a tile pair share them.  Positions are filled up to 16, which costs
   // less than it gives from two such tiles on.
-  const int own_rows = attention_rows(pass, (int)dtype_bytes(c.dtype), attention_dims(c.dtype, c.dim), true);
-  p.blocked = c.slopes && p.wide && (G == 2 || G == 4 || G == 8) && c.nq / docs >= 32 && (!own_q || own_rows % (16 * G) == 0);
-  const int rows = attention_rows(pass, (int)dtype_bytes(c.dtype), attention_dims(c.dtype, c.dim), p.wide);
+  const int e = (int)dtype_bytes(c.dtype), dims = attention_dims(c.dtype, c.dim);
+  const bool shares = !own_q || attention_qs(pass, e, dims, true, true) == 2;
+  p.blocked = shares && c.slopes && p.wide && (G == 2 || G == 4 || G == 8) && c.nq / docs >= 32 && (!own_q || attention_rows(pass, e, dims, true, true) % (16 * G) == 0);
+  const int rows = attention_rows(pass, e, dims, p.wide, p.blocked);
   const long long in_doc = own_q && p.blocked ? (all + 15) / 16 * 16 * per : all * per;
   p.slots = c.packed ? all * per / rows + c.docs + 3 : c.docs * ((in_doc + rows - 1) / rows);
-  // pieces of the streamed side where blocks do not fill the compute units, four tiles each at least
-  const double blocks = std::max(1.0, own / rows) * (c.packed ? docs : (double)c.docs) * c.kv_heads, want = p.wide ? 512 : 2048;
-  const double most = streamed / bn_of(c.dtype, attention_dims(c.dtype, c.dim)) / g_attention_tiles;
+  // Short documents: a wave takes several heads, which finds its document once, while there are four waves to every SIMD.
+  p.heads = 1;
+  while (!p.wide && p.heads * 2 <= c.kv_heads && p.slots * ((c.kv_heads + p.heads * 2 - 1) / (p.heads * 2)) >= 4096) p.heads *= 2;
+  // pieces of the streamed side where blocks do not fill the compute units, two tiles each at least (8 x 1 queries of 16 heads, 4099 keys of 4,
+  // kernel and join: pieces of 4 tiles 15.5 + 5.2, 2 tiles 11.6 + 7.3, 1 tile 10.7 + 10.6 us)
+  const double blocks = std::max(1.0, own / rows) * (c.packed ? docs : (double)c.docs) * c.kv_heads / p.heads, want = p.wide ? 512 : 2048;
+  const double most = streamed / bn_of(c.dtype, attention_dims(c.dtype, c.dim)) / 2;
   p.splits = (int)std::max(1.0, std::min({want / blocks, most, 64.0}));
   return p;
 }
@@ -143,20 +146,24 @@ __global__ void __launch_bounds__(256) attention_join_kernel(const AttnArgs a, l
 #pragma unroll
   for (int k = 1; k < 64; k *= 2) sum += __shfl_xor(sum, k);
   const float by = sum == 0.f ? 0.f : 1.f / sum;
+  const bool whole = a.dim % 4 == 0;
   for (int d = d0; d < (a.dim + 63) / 64 * 64; d += 64) {
-    float v[4] = {0.f, 0.f, 0.f, 0.f};
+    float4 v = {0.f, 0.f, 0.f, 0.f};
     for (int s = lane / 16; s < (a.splits + 3) / 4 * 4; s += 4) {
-      const float w = __shfl(share, s);
+      const float w = __shfl(share, s);   // (all lanes: the loop is one for the wave)
+      if (w == 0.f || d >= a.dim) continue;   // (a piece without a share has written nothing to speak of)
       const float *p = a.part_q + (s * rows + row) * a.dim + d;
-#pragma unroll
-      for (int i = 0; i < 4; i++)
-        if (w != 0.f && d + i < a.dim) v[i] += p[i] * w;
+      float4 t = {0.f, 0.f, 0.f, 0.f};
+      if (whole) t = *(const float4 *)__builtin_assume_aligned(p, 16);
+      else t.x = p[0], t.y = d + 1 < a.dim ? p[1] : 0.f, t.z = d + 2 < a.dim ? p[2] : 0.f, t.w = d + 3 < a.dim ? p[3] : 0.f;
+      v.x += t.x * w, v.y += t.y * w, v.z += t.z * w, v.w += t.w * w;
     }
 #pragma unroll
     for (int i = 0; i < 4; i++) {
-      v[i] += __shfl_xor(v[i], 16);
-      v[i] += __shfl_xor(v[i], 32);
-      if (lane < 16 && d + i < a.dim) ((T *)a.y)[row * a.dim + d + i] = from_f<T>(v[i] * by);
+      float e = i == 0 ? v.x : i == 1 ? v.y : i == 2 ? v.z : v.w;
+      e += __shfl_xor(e, 16);
+      e += __shfl_xor(e, 32);
+      if (lane < 16 && d + i < a.dim) ((T *)a.y)[row * a.dim + d + i] = from_f<T>(e * by);
     }
   }
   if (lane == 0 && a.lse) a.lse[row] = sum == 0.f ? INFINITY : top + __builtin_amdgcn_logf(sum);
@@ -317,7 +324,7 @@ bool whole4(const AttnCall &c, std::initializer_list<const void *> results) {
 }
 
 AttnArgs pass_args(AttnArgs a, const Pass &p) {
-  a.slots = p.slots, a.splits = p.splits, a.head_major = p.wide, a.blocked = p.blocked;
+  a.slots = p.slots, a.splits = p.splits, a.head_major = p.wide, a.blocked = p.blocked, a.heads = p.heads;
   return a;
 }
 

@@ -34,7 +34,7 @@ struct AttnArgs {
   long long docs, nq, nk;       // padded: rows of a sample; packed: all rows
   long long rows_q, rows_k;     // all of them
   long long slots, first;       // blocks of the whole call (one piece, one head), the first of this launch
-  int packed, H, KV, G, dim, ldy, splits, g_shift, blocked;   // blocked: row order (RowAt)
+  int packed, H, KV, G, dim, ldy, splits, g_shift, blocked, heads;   // blocked: row order (RowAt); heads of keys, one after the other in a block
   unsigned g_magic;   // division of row numbers by G (group_of)
   int head_major, vec_y;   // vec_y: results take vectors of four
   float scale, scale2;          // scale2: times log2(e)
@@ -49,9 +49,11 @@ struct AttnPlan {
 };
 enum AttnPass { kAttnForward, kAttnRows, kAttnKeys };
 // 16 QS own rows a wave: four waves a block take two tiles each, which share every fragment of the streamed side, where registers hold
-// their operands and results; a wave alone one, since the documents are short.
-constexpr int attention_qs(AttnPass pass, int element, int dims, bool wide) { return !wide || (dims == 128 && (pass != kAttnForward || element == 4)) ? 1 : 2; }
-constexpr int attention_rows(AttnPass pass, int element, int dims, bool wide) { return 16 * attention_qs(pass, element, dims, wide) * (wide ? 4 : 1); }
+// their operands and results (share: and their distances, see RowAt); a wave alone one, since the documents are short.
+constexpr int attention_qs(AttnPass pass, int element, int dims, bool wide, bool share) {
+  return !wide || (dims == 128 && (pass != kAttnForward || element == 4)) || (dims == 64 && pass == kAttnRows && element == 2 && !share) ? 1 : 2;
+}
+constexpr int attention_rows(AttnPass pass, int element, int dims, bool wide, bool share) { return 16 * attention_qs(pass, element, dims, wide, share) * (wide ? 4 : 1); }
 template <AttnPass PASS, typename T>
 int launch_attention_kernels(const AttnPlan &p, const AttnArgs &a, hipStream_t s);
 
@@ -354,16 +356,18 @@ struct AttnWork {
   long long slot;
   int kv, split;
 };
+// (w.kv: the block's first head of keys)
 __device__ __forceinline__ AttnWork work_of(const AttnArgs &a) {
   AttnWork w;
   const unsigned even = gridDim.x / 8 * 8;
   unsigned id = blockIdx.x;
   if (id < even) id = id % 8 * (even / 8) + id / 8;
-  const long long at = a.first + id, all = a.slots * a.KV;
+  const int groups = (a.KV + a.heads - 1) / a.heads;
+  const long long at = a.first + id, all = a.slots * groups;
   w.split = (int)(at / all);
   const long long r = at - w.split * all;
-  if (a.head_major) w.kv = (int)(r / a.slots), w.slot = r - w.kv * a.slots;
-  else w.slot = r / a.KV, w.kv = (int)(r - w.slot * a.KV);
+  if (a.head_major) w.kv = (int)(r / a.slots), w.slot = r - w.kv * a.slots;   // (one head a block)
+  else w.slot = r / groups, w.kv = (int)(r - w.slot * groups) * a.heads;
   return w;
 }
 
@@ -386,12 +390,11 @@ struct Distance {
       else far = __builtin_amdgcn_sqrtf(sq);
     }
   }
-  // sums of g d / |d| and g |d|
+  // sums of g d / |d|
   __device__ __forceinline__ void add(float *sums, float g) const {
     const float w = g * inv;
 #pragma unroll
     for (int k = 0; k < 3; k++) sums[k] = __builtin_fmaf(w, d[k], sums[k]);
-    sums[3] = __builtin_fmaf(g, far, sums[3]);
   }
 };
 
@@ -401,15 +404,18 @@ struct QueryRows {
   typedef AttnTile<T, DP> Tile;
   typename Tile::Frag q[QS][Tile::KS];
   float x[QS][3], slope[QS];   // slope: of log2 units, negative
-  long long out[QS];           // row of the results: position * heads + head
   bool there[QS], mine[QS];    // it exists; it is this document's to write
+  // row of the results: position * heads + head (formed where it is wanted: registers)
+  static __device__ __forceinline__ long long out(const AttnArgs &a, const AttnDoc &doc, int kv, int row0, int s) {
+    const RowAt r = row_at(a, row0 + 16 * s + threadIdx.x % 16);
+    return (doc.out_q + r.pos) * a.H + kv * a.G + r.head;
+  }
   __device__ __forceinline__ void load(const AttnArgs &a, const AttnDoc &doc, int kv, int row0, int live) {
 #pragma unroll
     for (int s = 0; s < QS; s++) {
       const RowAt r = row_at(a, row0 + 16 * s + threadIdx.x % 16);
       const int h = kv * a.G + r.head;
       mine[s] = r.pos < doc.own_all, there[s] = r.pos < live;
-      out[s] = (doc.out_q + r.pos) * a.H + h;
       const T *row = (const T *)a.q + doc.sample * a.qs + (doc.q0 + r.pos) * a.qp + h * a.qh;
 #pragma unroll
       for (int k = 0; k < Tile::KS; k++) q[s][k] = Tile::frag_of(row, k, a.dim, there[s]);
@@ -458,17 +464,14 @@ struct KeyTiles {
 };
 
 template <typename T, int DP, int WAVES, int QS, int BIAS, bool SHARE>
-__global__ void __launch_bounds__(64 * WAVES, 2) attention_fwd_kernel(const AttnArgs a) {
+__device__ __forceinline__ void attention_fwd_head(const AttnArgs &a, const AttnWork &w, const AttnDoc &doc, typename KeyTiles<T, DP, WAVES, BIAS>::Buffer *lds) {
   typedef AttnTile<T, DP> Tile;
   typedef KeyTiles<T, DP, WAVES, BIAS> Keys;
   constexpr int BN = Keys::BN, SUB = BN / 16, BM = 16 * QS * WAVES;
-  __shared__ typename Keys::Buffer lds[Keys::BUFS];
-  const AttnWork w = work_of(a);
-  const AttnDoc doc = find_doc<true>(a, w.slot, BM);
-  if ((long long)doc.tile * BM >= rows_in(a, doc.own_all)) return;
   const int q4 = threadIdx.x % 64 / 16 * 4, live = doc.kn > 0 ? doc.qn : 0;
+  const int row0 = doc.tile * BM + threadIdx.x / 64 * (16 * QS);
   QueryRows<T, DP, QS, BIAS> own;
-  own.load(a, doc, w.kv, doc.tile * BM + threadIdx.x / 64 * (16 * QS), live);
+  own.load(a, doc, w.kv, row0, live);
 
   // Scores are formed less the maximum so far, m (log2).  It moves only when one is more than 8 above it: values are then at most 2^8
   // times what they would be (and within float16), and rescaling is rare.
@@ -569,7 +572,7 @@ __global__ void __launch_bounds__(64 * WAVES, 2) attention_fwd_kernel(const Attn
   for (int s = 0; s < QS; s++) {
     const float all = over_row_sum(l[s]), sum = own.there[s] ? all : 0.f;
     if (!own.mine[s]) continue;
-    const long long at = own.out[s];
+    const long long at = own.out(a, doc, w.kv, row0, s);
     if (a.part_q) {
       const long long in_part = w.split * a.rows_q * a.H + at;
       if (q4 == 0) a.part_ml[in_part] = make_float2(sum == 0.f ? kLowest : m[s], sum);
@@ -588,6 +591,20 @@ __global__ void __launch_bounds__(64 * WAVES, 2) attention_fwd_kernel(const Attn
   }
 }
 
+template <typename T, int DP, int WAVES, int QS, int BIAS, bool SHARE>
+__global__ void __launch_bounds__(64 * WAVES, sizeof(T) == 2 && DP <= 64 ? 3 : 2) attention_fwd_kernel(const AttnArgs a) {
+  constexpr int BM = 16 * QS * WAVES;
+  __shared__ typename KeyTiles<T, DP, WAVES, BIAS>::Buffer lds[WAVES > 1 ? 2 : 1];
+  AttnWork w = work_of(a);
+  const AttnDoc doc = find_doc<true>(a, w.slot, BM);
+  if ((long long)doc.tile * BM >= rows_in(a, doc.own_all)) return;
+  if constexpr (WAVES > 1) {
+    attention_fwd_head<T, DP, WAVES, QS, BIAS, SHARE>(a, w, doc, lds);
+  } else {
+    for (const int end = min(w.kv + a.heads, a.KV); w.kv < end; w.kv++) attention_fwd_head<T, DP, WAVES, QS, BIAS, SHARE>(a, w, doc, lds);
+  }
+}
+
 // ---- gradients by query rows: gq, the points and slopes of queries, D ----
 //
 // D from a y that was rounded to 16 bits, and formed from p that were, is off by 2^-9 of itself, and so would be every ds and, worse, the
@@ -596,29 +613,27 @@ __global__ void __launch_bounds__(64 * WAVES, 2) attention_fwd_kernel(const Attn
 // heads of 64, bfloat16: errors of the gradients of points and slopes .004 without it.)  The pass by keys has the D that is right.
 
 template <typename T, int DP, int WAVES, int QS, int BIAS, bool SHARE>
-__global__ void __launch_bounds__(64 * WAVES, 2) attention_rows_kernel(const AttnArgs a) {
+__device__ __forceinline__ void attention_rows_head(const AttnArgs &a, const AttnWork &w, const AttnDoc &doc, typename KeyTiles<T, DP, WAVES, BIAS>::Buffer *lds) {
   typedef AttnTile<T, DP> Tile;
   typedef KeyTiles<T, DP, WAVES, BIAS> Keys;
   constexpr int BN = Keys::BN, SUB = BN / 16, BM = 16 * QS * WAVES;
   constexpr bool MEND = sizeof(T) == 2;
   constexpr int SETS = MEND ? 2 * QS : QS;   // ds, p
-  __shared__ typename Keys::Buffer lds[Keys::BUFS];
-  const AttnWork w = work_of(a);
-  const AttnDoc doc = find_doc<true>(a, w.slot, BM);
-  if ((long long)doc.tile * BM >= rows_in(a, doc.own_all)) return;
   const int q4 = threadIdx.x % 64 / 16 * 4, live = doc.kn > 0 ? doc.qn : 0;
+  const int row0 = doc.tile * BM + threadIdx.x / 64 * (16 * QS);
   QueryRows<T, DP, QS, BIAS> own;
-  own.load(a, doc, w.kv, doc.tile * BM + threadIdx.x / 64 * (16 * QS), live);
+  own.load(a, doc, w.kv, row0, live);
 
   typename Tile::Frag fg[QS][Tile::KS];
   float nlse[QS], delta[QS], rest[QS];   // -lse, D0, the sum of ds
 #pragma unroll
   for (int s = 0; s < QS; s++) {
     delta[s] = 0.f, rest[s] = 0.f;
+    const long long at = own.out(a, doc, w.kv, row0, s);
 #pragma unroll
     for (int k = 0; k < Tile::KS; k++) {
-      fg[s][k] = Tile::frag_of((const T *)a.gy + own.out[s] * a.ldy, k, a.dim, own.there[s]);
-      const typename Tile::Frag fy = Tile::frag_of((const T *)a.y + own.out[s] * a.ldy, k, a.dim, own.there[s]);
+      fg[s][k] = Tile::frag_of((const T *)a.gy + at * a.ldy, k, a.dim, own.there[s]);
+      const typename Tile::Frag fy = Tile::frag_of((const T *)a.y + at * a.ldy, k, a.dim, own.there[s]);
       T gv[Tile::EP], yv[Tile::EP];
       __builtin_memcpy(gv, &fg[s][k], 16);
       __builtin_memcpy(yv, &fy, 16);
@@ -626,7 +641,7 @@ __global__ void __launch_bounds__(64 * WAVES, 2) attention_rows_kernel(const Att
       for (int e = 0; e < Tile::EP; e++) delta[s] += to_f(gv[e]) * to_f(yv[e]);
     }
     delta[s] = over_row_sum(delta[s]);
-    nlse[s] = own.there[s] ? -a.lse[own.out[s]] : -INFINITY;
+    nlse[s] = own.there[s] ? -a.lse[at] : -INFINITY;
   }
   f32x4 acc[SETS][Tile::NF];
   float geo[SETS][4];
@@ -669,6 +684,7 @@ __global__ void __launch_bounds__(64 * WAVES, 2) attention_rows_kernel(const Att
           for (int i = 0; i < 4; i++) {
             const bool in = !masked.value || j * 16 + q4 + i < left;
             Distance<BIAS> far;
+            float both = 0.f;
 #pragma unroll
             for (int s = 0; s < QS; s++) {
               if (!SHARE || s == 0) far.form(own.x[s], point, i);
@@ -679,8 +695,11 @@ __global__ void __launch_bounds__(64 * WAVES, 2) attention_rows_kernel(const Att
               ds[u][s][i] = g;
               if constexpr (MEND) ds[u][QS + s][i] = p, rest[s] += g;
               if constexpr (BIAS == kBiasGradients) {
-                far.add(part[s], g);
-                if constexpr (MEND) far.add(geo[QS + s], p);
+                // (heads of one position: their gradients of the point are one sum, kept with the first)
+                both = SHARE && s > 0 ? __builtin_fmaf(g, own.slope[s], both) : g * own.slope[s];
+                if (!SHARE || s == QS - 1) far.add(part[SHARE ? 0 : s], both);
+                part[s][3] = __builtin_fmaf(g, far.far, part[s][3]);
+                if constexpr (MEND) far.add(geo[QS + s], p), geo[QS + s][3] = __builtin_fmaf(p, far.far, geo[QS + s][3]);
               }
             }
           }
@@ -701,11 +720,11 @@ __global__ void __launch_bounds__(64 * WAVES, 2) attention_rows_kernel(const Att
   for (int s = 0; s < QS; s++) {
     const bool pieces = MEND && a.part_d;   // (what is lacking is known when all pieces are there)
     const float lacks = MEND ? over_row_sum(rest[s]) : 0.f;
-    const long long at = own.out[s], in_part = w.split * a.rows_q * a.H + at;
+    const long long at = own.out(a, doc, w.kv, row0, s), in_part = w.split * a.rows_q * a.H + at;
     if (BIAS == kBiasGradients) {
 #pragma unroll
       for (int e = 0; e < 4; e++) {
-        geo[s][e] = over_row_sum(geo[s][e]) * (e < 3 ? own.slope[s] * 0.69314718055994531f : -1.f);
+        geo[s][e] = over_row_sum(geo[s][e]) * (e < 3 ? 0.69314718055994531f : -1.f);
         if (MEND) geo[QS * MEND + s][e] = over_row_sum(geo[QS * MEND + s][e]) * (e < 3 ? own.slope[s] * 0.69314718055994531f : -1.f);
         if (MEND && !pieces) geo[s][e] -= lacks * geo[QS * MEND + s][e];
       }
@@ -736,20 +755,35 @@ __global__ void __launch_bounds__(64 * WAVES, 2) attention_rows_kernel(const Att
   }
 }
 
+template <typename T, int DP, int WAVES, int QS, int BIAS, bool SHARE>
+__global__ void __launch_bounds__(64 * WAVES, 2) attention_rows_kernel(const AttnArgs a) {
+  constexpr int BM = 16 * QS * WAVES;
+  __shared__ typename KeyTiles<T, DP, WAVES, BIAS>::Buffer lds[WAVES > 1 ? 2 : 1];
+  AttnWork w = work_of(a);
+  const AttnDoc doc = find_doc<true>(a, w.slot, BM);
+  if ((long long)doc.tile * BM >= rows_in(a, doc.own_all)) return;
+  if constexpr (WAVES > 1) {
+    attention_rows_head<T, DP, WAVES, QS, BIAS, SHARE>(a, w, doc, lds);
+  } else {
+    for (const int end = min(w.kv + a.heads, a.KV); w.kv < end; w.kv++) attention_rows_head<T, DP, WAVES, QS, BIAS, SHARE>(a, w, doc, lds);
+  }
+}
+
 // ---- gradients by keys: gk, gv, the points of keys ----
 
+// Tiles of query rows, gradients and what belongs to the rows on their way through LDS
+template <typename T, int DP, int BIAS>
+struct RowBuffer {
+  static constexpr int BN = kAttnBN<T, DP>;
+  __align__(16) char q[BN * AttnTile<T, DP>::W], g[BN * AttnTile<T, DP>::W];
+  __align__(16) float r[BIAS ? 6 : 2][64];   // lse, D, slope, points of the rows
+};
+
 template <typename T, int DP, int WAVES, int QS, int BIAS, bool SHARE>
-__global__ void __launch_bounds__(64 * WAVES, 2) attention_keys_kernel(const AttnArgs a) {
+__device__ __forceinline__ void attention_keys_head(const AttnArgs &a, const AttnWork &w, const AttnDoc &doc, RowBuffer<T, DP, BIAS> *lds) {
   typedef AttnTile<T, DP> Tile;
-  constexpr int THREADS = 64 * WAVES, BUFS = WAVES > 1 ? 2 : 1, BN = kAttnBN<T, DP>, SUB = BN / 16, BM = 16 * QS * WAVES, ROW = BIAS ? 6 : 2;
-  struct Buffer {
-    __align__(16) char q[BN * Tile::W], g[BN * Tile::W];
-    __align__(16) float r[ROW][64];   // lse, D, slope, points of the rows
-  };
-  __shared__ Buffer lds[BUFS];
-  const AttnWork w = work_of(a);
-  const AttnDoc doc = find_doc<false>(a, w.slot, BM);
-  if ((long long)doc.tile * BM >= doc.own_all) return;
+  constexpr int THREADS = 64 * WAVES, BN = kAttnBN<T, DP>, SUB = BN / 16, BM = 16 * QS * WAVES, ROW = BIAS ? 6 : 2;
+  typedef RowBuffer<T, DP, BIAS> Buffer;
   const int lane = threadIdx.x % 64, c = lane % 16, q4 = lane / 16 * 4;
   const int key0 = doc.tile * BM + threadIdx.x / 64 * (16 * QS);
 
@@ -830,12 +864,13 @@ __global__ void __launch_bounds__(64 * WAVES, 2) attention_keys_kernel(const Att
             for (int e = 0; e < 3; e++) point[u][e] = *(const f32x4 *)&b.r[3 + e][(j0 + u) * 16 + q4];
         }
       }
-      float part[QS][4] = {};
+      float part[QS][3] = {};
 #pragma unroll
       for (int s = 0; s < QS; s++)
 #pragma unroll
         for (int i = 0; i < 4; i++) {
           Distance<BIAS> far;
+          float both = 0.f;   // gradients of rows of one position, times their slopes
 #pragma unroll
           for (int u = 0; u < 2; u++) {
             if (!SHARE || u == 0) far.form(x[s], point[u], i);   // (from the key: the sign that its gradient takes)
@@ -844,9 +879,8 @@ __global__ void __launch_bounds__(64 * WAVES, 2) attention_keys_kernel(const Att
             const float prob = __builtin_amdgcn_exp2f(__builtin_fmaf(p[u][s][i], a.scale2, v)), g = prob * ds[u][s][i];
             p[u][s][i] = prob, ds[u][s][i] = g;
             if constexpr (BIAS == kBiasGradients) {
-              const float w = g * far.inv * slope[u][i];
-#pragma unroll
-              for (int e = 0; e < 3; e++) part[s][e] = __builtin_fmaf(w, far.d[e], part[s][e]);
+              both = SHARE && u == 1 ? __builtin_fmaf(g, slope[u][i], both) : g * slope[u][i];
+              if (!SHARE || u == 1) far.add(part[s], both);
             }
           }
         }
@@ -893,13 +927,27 @@ __global__ void __launch_bounds__(64 * WAVES, 2) attention_keys_kernel(const Att
   }
 }
 
+template <typename T, int DP, int WAVES, int QS, int BIAS, bool SHARE>
+__global__ void __launch_bounds__(64 * WAVES, sizeof(T) == 4 && DP >= 64 ? 1 : 2) attention_keys_kernel(const AttnArgs a) {
+  constexpr int BM = 16 * QS * WAVES;
+  __shared__ RowBuffer<T, DP, BIAS> lds[WAVES > 1 ? 2 : 1];
+  AttnWork w = work_of(a);
+  const AttnDoc doc = find_doc<false>(a, w.slot, BM);
+  if ((long long)doc.tile * BM >= doc.own_all) return;
+  if constexpr (WAVES > 1) {
+    attention_keys_head<T, DP, WAVES, QS, BIAS, SHARE>(a, w, doc, lds);
+  } else {
+    for (const int end = min(w.kv + a.heads, a.KV); w.kv < end; w.kv++) attention_keys_head<T, DP, WAVES, QS, BIAS, SHARE>(a, w, doc, lds);
+  }
+}
+
 // Launches of at most 2^22 blocks (2^30 threads) each.
 constexpr long long kAttnMostBlocks = 1 << 22;
 
 template <AttnPass PASS, typename T, int DP, int WAVES, int BIAS, bool SHARE>
 void launch_attention_pass(AttnArgs a, hipStream_t s) {
-  constexpr int QS = attention_qs(PASS, sizeof(T), DP, WAVES > 1);
-  const long long blocks = a.slots * a.KV * a.splits;
+  constexpr int QS = attention_qs(PASS, sizeof(T), DP, WAVES > 1, SHARE);
+  const long long blocks = a.slots * ((a.KV + a.heads - 1) / a.heads) * a.splits;
   for (a.first = 0; a.first < blocks; a.first += kAttnMostBlocks) {
     const dim3 grid((unsigned)std::min(kAttnMostBlocks, blocks - a.first)), block(64 * WAVES);
     if constexpr (PASS == kAttnForward) hipLaunchKernelGGL((attention_fwd_kernel<T, DP, WAVES, QS, BIAS, SHARE>), grid, block, 0, s, a);
@@ -911,7 +959,7 @@ void launch_attention_pass(AttnArgs a, hipStream_t s) {
 template <AttnPass PASS, typename T, int DP, int BIAS>
 void launch_attention_bias(const AttnPlan &p, const AttnArgs &a, hipStream_t s) {
   // (own rows share where a wave has two tiles of them, streamed ones always)
-  constexpr bool SHARES = BIAS != kBiasNone && (PASS == kAttnKeys || attention_qs(PASS, sizeof(T), DP, true) == 2);
+  constexpr bool SHARES = BIAS != kBiasNone && (PASS == kAttnKeys || attention_qs(PASS, sizeof(T), DP, true, true) == 2);
   if (!p.wide) launch_attention_pass<PASS, T, DP, 1, BIAS, false>(a, s);
   else if (!SHARES || !a.blocked) launch_attention_pass<PASS, T, DP, 4, BIAS, false>(a, s);
   else if constexpr (SHARES) launch_attention_pass<PASS, T, DP, 4, BIAS, true>(a, s);

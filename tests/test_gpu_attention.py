@@ -187,9 +187,28 @@ def test_queries_of_other_keys(gelib, geometry, docs, packed, dtype):
 
 
 @pytest.mark.parametrize("dtype", TYPES, ids=str)
-@pytest.mark.parametrize("dim", [16, 64, 128])
-def test_long(gelib, dim, dtype):
-    compare(gelib, dtype, [(1500, 1500), (300, 300)], 4, 2, dim, True, every=False)
+@pytest.mark.parametrize("dim", [16, 32, 64, 128])
+@pytest.mark.parametrize("heads,kv", [(4, 2), (3, 3), (4, 1), (8, 1), (3, 1)])
+def test_long(gelib, heads, kv, dim, dtype):
+    """Groups of two, four and eight heads, whose tiles share distances, and others."""
+    compare(gelib, dtype, [(1100, 1100), (300, 300)], heads, kv, dim, True, every=False)
+
+
+@pytest.mark.parametrize("dtype", TYPES, ids=str)
+@pytest.mark.parametrize("heads,kv", [(3, 3), (4, 2)])
+@pytest.mark.parametrize("dim", [16, 32, 64, 128])
+def test_long_without_points(gelib, dim, heads, kv, dtype):
+    compare(gelib, dtype, [(600, 600), (300, 300)], heads, kv, dim, False, geometry=False, every=False)
+
+
+@pytest.mark.parametrize("dtype", TYPES, ids=str)
+@pytest.mark.parametrize("dim", [16, 32, 64, 128])
+def test_many_short_documents(gelib, dim, dtype):
+    """So many that a wave takes several heads, one after the other."""
+    gen = torch.Generator().manual_seed(3)
+    docs = [(k, k) for k in torch.randint(0, 40, (700,), generator=gen).tolist()]
+    for packed in (True, False):
+        compare(gelib, dtype, docs, 14, 7, dim, packed, every=False)
 
 
 @pytest.mark.parametrize("dtype", TYPES, ids=str)
