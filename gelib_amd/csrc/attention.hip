@@ -85,7 +85,7 @@ int padded_dim(const AttnCall &c) {
 }
 bool aligned(const AttnCall &c, const void *p, const long long *s) {
   const long long e = (long long)dtype_bytes(c.dtype);
-  return c.dim * e % 16 == 0 && ((long long)(uintptr_t)p | (c.packed ? 0 : s[0] * e) | s[1] * e | s[2] * e) % 16 == 0;
+  return s[1] <= 0x7fffffff && s[2] <= 0x7fffffff && c.dim * e % 16 == 0 && ((long long)(uintptr_t)p | (c.packed ? 0 : s[0] * e) | s[1] * e | s[2] * e) % 16 == 0;
 }
 
 // Where everything lies in the workspace
@@ -279,7 +279,8 @@ AttnArgs args_of(const AttnCall &c, const void *y, const void *gy, const Space &
   AttnArgs a = {};
   const int dim = padded_dim(c), H = c.heads, KV = c.kv_heads;
   a.q = c.q, a.k = c.k, a.v = c.v, a.y = (void *)y, a.gy = gy;
-  a.qs = c.qs[0], a.qp = c.qs[1], a.qh = c.qs[2], a.ks = c.ks[0], a.kp = c.ks[1], a.kh = c.ks[2], a.vs = c.vs[0], a.vp = c.vs[1], a.vh = c.vs[2];
+  a.qs = c.qs[0], a.ks = c.ks[0], a.vs = c.vs[0];
+  long long qp = c.qs[1], qh = c.qs[2], kp = c.ks[1], kh = c.ks[2], vp = c.vs[1], vh = c.vs[2];
   if (c.packed) a.qs = a.ks = a.vs = 0;
   a.x = c.x, a.xk = c.xk, a.slopes = c.slopes, a.q_marks = c.q_marks, a.k_marks = c.k_marks;
   a.docs = c.docs, a.nq = c.nq, a.nk = c.nk, a.rows_q = rows_of(c, true), a.rows_k = rows_of(c, false);
@@ -301,9 +302,9 @@ AttnArgs args_of(const AttnCall &c, const void *y, const void *gy, const Space &
     p = m.to, ss = n * heads * dim, sp = (long long)heads * dim, sh = dim;
     if (c.packed) ss = 0;
   };
-  if (!aligned(c, c.q, c.qs)) copy(a.q, a.qs, a.qp, a.qh, at.q, c.nq, H);
-  if (!aligned(c, c.k, c.ks)) copy(a.k, a.ks, a.kp, a.kh, at.k, c.nk, KV);
-  if (!aligned(c, c.v, c.vs)) copy(a.v, a.vs, a.vp, a.vh, at.v, c.nk, KV);
+  if (!aligned(c, c.q, c.qs)) copy(a.q, a.qs, qp, qh, at.q, c.nq, H);
+  if (!aligned(c, c.k, c.ks)) copy(a.k, a.ks, kp, kh, at.k, c.nk, KV);
+  if (!aligned(c, c.v, c.vs)) copy(a.v, a.vs, vp, vh, at.v, c.nk, KV);
   if (gy && dim != c.dim) {
     const void *yp = y;
     for (auto *p : {&yp, &a.gy}) {
@@ -312,6 +313,7 @@ AttnArgs args_of(const AttnCall &c, const void *y, const void *gy, const Space &
     }
     a.y = (void *)yp, a.ldy = dim;
   }
+  a.qp = (int)qp, a.qh = (int)qh, a.kp = (int)kp, a.kh = (int)kh, a.vp = (int)vp, a.vh = (int)vh;
   if (copies.threads) hipLaunchKernelGGL(attention_copy_kernel<T>, dim3((unsigned)std::min((copies.threads + 255) / 256, 1LL << 22)), dim3(256), 0, s, copies);
   return a;
 }

@@ -23,7 +23,8 @@ namespace gelib_hip {
 struct AttnArgs {
   const void *q, *k, *v, *gy;   // backward: gy and y at a stride of ldy from one (row, head) to the next
   void *y, *gq, *gk, *gv;       // packed: (rows, heads, dim)
-  long long qs, qp, qh, ks, kp, kh, vs, vp, vh;   // strides of samples, positions, heads in elements
+  long long qs, ks, vs;          // strides of samples in elements
+  int qp, qh, kp, kh, vp, vh;    // of positions and heads: operands with larger ones are copied (a multiplication instead of five)
   const float *x, *xk, *slopes;   // points of queries and keys (rows, 3), heads
   const int *q_marks, *k_marks;   // padded: lengths or null (all rows); packed: starts, docs + 1 of them
   float *lse, *delta;           // (query rows, heads): log2 of the sum of exp; D
@@ -416,7 +417,7 @@ struct QueryRows {
       const RowAt r = row_at(a, row0 + 16 * s + threadIdx.x % 16);
       const int h = kv * a.G + r.head;
       mine[s] = r.pos < doc.own_all, there[s] = r.pos < live;
-      const T *row = (const T *)a.q + doc.sample * a.qs + (doc.q0 + r.pos) * a.qp + h * a.qh;
+      const T *row = (const T *)a.q + doc.sample * a.qs + (doc.q0 + r.pos) * a.qp + (long long)h * a.qh;
 #pragma unroll
       for (int k = 0; k < Tile::KS; k++) q[s][k] = Tile::frag_of(row, k, a.dim, there[s]);
       if (BIAS) {
@@ -439,16 +440,15 @@ struct KeyTiles {
   };
   const T *k, *v;
   const float *x;
-  long long kp, vp;
-  int dim, rows;
+  int kp, vp, dim, rows;
   __device__ __forceinline__ KeyTiles(const AttnArgs &a, const AttnDoc &doc, int kv)
-      : k((const T *)a.k + doc.sample * a.ks + doc.k0 * a.kp + kv * a.kh), v((const T *)a.v + doc.sample * a.vs + doc.k0 * a.vp + kv * a.vh), x(BIAS ? a.xk + doc.out_k * 3 : nullptr),
+      : k((const T *)a.k + doc.sample * a.ks + doc.k0 * a.kp + (long long)kv * a.kh), v((const T *)a.v + doc.sample * a.vs + doc.k0 * a.vp + (long long)kv * a.vh), x(BIAS ? a.xk + doc.out_k * 3 : nullptr),
         kp(a.kp), vp(a.vp), dim(a.dim), rows(doc.kn) {}
   __device__ __forceinline__ void copy(int t, Buffer &b) const {
     const int left = rows - t * BN;
     const T *kt = k + (long long)t * BN * kp, *vt = v + (long long)t * BN * vp;
-    copy_tile<T, DP, BN, THREADS>(b.k, [&](int row) { return row < left ? kt + row * kp : nullptr; }, left, dim);
-    copy_tile<T, DP, BN, THREADS>(b.v, [&](int row) { return row < left ? vt + row * vp : nullptr; }, left, dim);
+    copy_tile<T, DP, BN, THREADS>(b.k, [&](int row) { return kt + (long long)row * kp; }, left, dim);
+    copy_tile<T, DP, BN, THREADS>(b.v, [&](int row) { return vt + (long long)row * vp; }, left, dim);
     if (BIAS) {
       const float *xt = x + (long long)t * BN * 3;
 #pragma unroll
@@ -796,8 +796,8 @@ __device__ __forceinline__ void attention_keys_head(const AttnArgs &a, const Att
     const int key = key0 + 16 * s + c;
     exists[s] = key < doc.kn, mine[s] = key < doc.own_all;
     out[s] = (doc.out_k + key) * a.KV + w.kv;
-    const T *rk = (const T *)a.k + doc.sample * a.ks + (doc.k0 + key) * a.kp + w.kv * a.kh;
-    const T *rv = (const T *)a.v + doc.sample * a.vs + (doc.k0 + key) * a.vp + w.kv * a.vh;
+    const T *rk = (const T *)a.k + doc.sample * a.ks + (doc.k0 + key) * a.kp + (long long)w.kv * a.kh;
+    const T *rv = (const T *)a.v + doc.sample * a.vs + (doc.k0 + key) * a.vp + (long long)w.kv * a.vh;
 #pragma unroll
     for (int k = 0; k < Tile::KS; k++) fk[s][k] = Tile::frag_of(rk, k, a.dim, exists[s]), fv[s][k] = Tile::frag_of(rv, k, a.dim, exists[s]);
     if (BIAS)
@@ -817,11 +817,11 @@ __device__ __forceinline__ void attention_keys_head(const AttnArgs &a, const Att
   const int rows = doc.tile * BM < doc.kn ? (int)rows_in(a, doc.qn) : 0;
   int t0, t1;
   piece_of((int)(((long long)rows + BN - 1) / BN), w.split, a.splits, t0, t1);
-  const T *q0 = (const T *)a.q + doc.sample * a.qs + doc.q0 * a.qp + w.kv * a.G * a.qh;
+  const T *q0 = (const T *)a.q + doc.sample * a.qs + doc.q0 * a.qp + (long long)w.kv * a.G * a.qh;
   const long long o0 = doc.out_q * a.H + w.kv * a.G;
   auto copy = [&](int t, Buffer &b) __attribute__((always_inline)) {
     const int left = rows - t * BN;
-    copy_tile<T, DP, BN, THREADS>(b.q, [&](int row) { const RowAt r = row_at(a, t * BN + row); return r.pos < doc.qn ? q0 + r.pos * a.qp + r.head * a.qh : nullptr; }, left, a.dim);
+    copy_tile<T, DP, BN, THREADS>(b.q, [&](int row) { const RowAt r = row_at(a, t * BN + row); return r.pos < doc.qn ? q0 + (long long)r.pos * a.qp + (long long)r.head * a.qh : nullptr; }, left, a.dim);
     copy_tile<T, DP, BN, THREADS>(b.g, [&](int row) { const RowAt r = row_at(a, t * BN + row); return r.pos < doc.qn ? (const T *)a.gy + (o0 + (long long)r.pos * a.H + r.head) * a.ldy : nullptr; }, left, a.dim);
 #pragma unroll
     for (int e = 0; e < ROW; e++)
