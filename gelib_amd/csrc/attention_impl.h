@@ -661,7 +661,7 @@ __device__ __forceinline__ void attention_rows_head(const AttnArgs &a, const Att
     for (int j0 = 0; j0 < SUB; j0 += 2) {
       if (j0 >= subs) break;
       f32x4 ds[2][SETS];
-      float part[QS][4] = {};   // (of 32 keys: sums over thousands of them one after the other would lose two digits)
+      float part[QS][4] = {}, part_rest[QS] = {};   // (of 32 keys: sums over thousands of them one after the other would lose two digits)
 #pragma unroll
       for (int u = 0; u < 2; u++) {
         const int j = j0 + u;
@@ -693,7 +693,7 @@ __device__ __forceinline__ void attention_rows_head(const AttnArgs &a, const Att
               if (masked.value) v = in ? v : -INFINITY;
               const float p = __builtin_amdgcn_exp2f(v), g = p * dp[s][i];
               ds[u][s][i] = g;
-              if constexpr (MEND) ds[u][QS + s][i] = p, rest[s] += g;
+              if constexpr (MEND) ds[u][QS + s][i] = p, part_rest[s] += g;
               if constexpr (BIAS == kBiasGradients) {
                 // (heads of one position: their gradients of the point are one sum, kept with the first)
                 both = SHARE && s > 0 ? __builtin_fmaf(g, own.slope[s], both) : g * own.slope[s];
@@ -712,6 +712,9 @@ __device__ __forceinline__ void attention_rows_head(const AttnArgs &a, const Att
         for (int s = 0; s < QS; s++)
 #pragma unroll
           for (int e = 0; e < 4; e++) geo[s][e] += part[s][e];
+      if constexpr (MEND)
+#pragma unroll
+        for (int s = 0; s < QS; s++) rest[s] += part_rest[s];
       Tile::template transposed<SETS>(acc, b.k, j0 * 16, ds[0], ds[1]);
     }
   });

@@ -226,7 +226,7 @@ int bwd(int dtype, const LinearArgs &l, hipStream_t s) {
       }
   }
   if (l.gb && l.N)
-    hipLaunchKernelGGL((column_join_kernel<T>), dim3((unsigned)std::min((l.N + 31LL) / 32, 1LL << 22)), dim3(256), 0, s, (const float *)sums, (T *)l.gb, chunks, l.N);
+    hipLaunchKernelGGL((column_join_kernel<T>), dim3((unsigned)std::min((l.N + 31LL) / 32, 1LL << 22)), dim3(256), 0, s, (const float *)sums, (T *)l.gb, chunks, l.N, (const float *)nullptr);
   GemmArgs a = {};
   if (gx) {
     a.a = gz, a.lda = ldz, a.b = w, a.ldb = ldw, a.c = l.gx;

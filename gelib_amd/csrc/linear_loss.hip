@@ -60,35 +60,24 @@ __global__ void __launch_bounds__(1024) loss_norm_kernel(float *norm, const floa
   norm[0] = ldexpf(1.f, e), norm[1] = ldexpf(1.f, -e);
 }
 
-// out[n] = norm * sum over the chunks of their column sums: 32 columns by 8 runs of chunks a block
-template <typename T>
-__global__ void __launch_bounds__(256) loss_columns_kernel(T *out, const float *sums, long long chunks, int N, const float *norm) {
-  __shared__ float lds[8][32];
-  const int run = threadIdx.x / 32;
-  for (long long n0 = blockIdx.x * 32LL; n0 < N; n0 += gridDim.x * 32LL) {
-    const long long n = n0 + threadIdx.x % 32;
-    float s = 0.f;
-    if (n < N) {
-#pragma unroll 8
-      for (long long k = run; k < chunks; k += 8) s += sums[k * N + n];
-    }
-    lds[run][threadIdx.x % 32] = s;
-    __syncthreads();
-    if (run == 0 && n < N) {
-      for (int k = 1; k < 8; k++) s += lds[k][threadIdx.x];
-      out[n] = from_f<T>(norm ? s * *norm : s);
-    }
-    __syncthreads();
-  }
-}
-
 // gx from the sums over all pieces (rows of K up to a multiple of 4)
 template <typename T>
 __global__ void __launch_bounds__(256) loss_finish_kernel(T *gx, const float *sums, long long n, int K, const float *norm) {
   const long long stride = (K + 3) & ~3;
+  const float by = norm ? *norm : 1.f;
+  if (K % 4 == 0 && (uintptr_t)gx % (4 * sizeof(T)) == 0) {   // (as they lie)
+    for (long long at = (long long)blockIdx.x * 256 + threadIdx.x; at < n / 4; at += (long long)gridDim.x * 256) {
+      const f32x4 v = ((const f32x4 *)sums)[at];
+      T t[4];
+#pragma unroll
+      for (int i = 0; i < 4; i++) t[i] = from_f<T>(v[i] * by);
+      __builtin_memcpy(__builtin_assume_aligned(gx + at * 4, 4 * sizeof(T)), t, sizeof(t));
+    }
+    return;
+  }
   for (long long at = (long long)blockIdx.x * 256 + threadIdx.x; at < n; at += (long long)gridDim.x * 256) {
     const long long row = at / K;
-    gx[at] = from_f<T>(sums[row * stride + (at - row * K)] * (norm ? *norm : 1.f));
+    gx[at] = from_f<T>(sums[row * stride + (at - row * K)] * by);
   }
 }
 template <typename T>
@@ -98,6 +87,160 @@ __global__ void __launch_bounds__(256) loss_zero_kernel(T *to, long long n) {
 template <typename T>
 void zero(void *to, long long n, hipStream_t s) {
   if (to && n) hipLaunchKernelGGL(loss_zero_kernel<T>, dim3((unsigned)std::min((n + 255) / 256, 1LL << 16)), dim3(256), 0, s, (T *)to, n);
+}
+
+// ---- few rows and classes ----
+// Where a product's tiles leave compute units idle and its sums are long, it is cut along k as any other: its pieces hold all logits then (they
+// are few), and the epilogue is the join's.  512 x 2048 -> 118 float32, both directions: FEWNEW us, in one piece FEWOLD.
+
+__device__ __forceinline__ void sum_exp(float &top, float &sum, float otop, float osum) {
+  const float to = fmaxf(top, otop), from = to == -INFINITY ? 0.f : to;
+  sum = sum * __builtin_amdgcn_exp2f((top - from) * 1.44269504088896341f) + osum * __builtin_amdgcn_exp2f((otop - from) * 1.44269504088896341f);
+  top = to;
+}
+
+// top and sum of 256 threads' pairs, in every thread
+__device__ __forceinline__ void block_sum_exp(float &top, float &sum, float2 *lds) {
+#pragma unroll
+  for (int d = 1; d < 64; d *= 2) {
+    const float otop = __shfl_xor(top, d), osum = __shfl_xor(sum, d);
+    sum_exp(top, sum, otop, osum);
+  }
+  if (threadIdx.x % 64 == 0) lds[threadIdx.x / 64] = make_float2(top, sum);
+  __syncthreads();
+  top = lds[0].x, sum = lds[0].y;
+  for (int k = 1; k < 4; k++) sum_exp(top, sum, lds[k].x, lds[k].y);
+}
+
+// a row's logit from the pieces of its sum
+__device__ __forceinline__ float logit_of(const float *part, long long all, int splits, long long at) {
+  float z = 0.f;
+  for (int k = 0; k < splits; k++) z += part[k * all + at];
+  return z;
+}
+
+// A block a row
+__global__ void __launch_bounds__(256) loss_pieces_kernel(float *loss, float *lse, const float *part, int splits, const long long *targets, long long rows, int N) {
+  __shared__ float2 lds[4];
+  const long long row = blockIdx.x, stride = (N + 3) & ~3, at = row * stride;
+  float top = -INFINITY, sum = 0.f;
+  for (int n = threadIdx.x; n < N; n += 256) sum_exp(top, sum, logit_of(part, rows * stride, splits, at + n), 1.f);
+  block_sum_exp(top, sum, lds);
+  if (threadIdx.x) return;
+  const float l = top + logf(sum);
+  const long long t = targets[row];
+  if (lse) lse[row] = l;
+  loss[row] = t < 0 ? 0.f : t < N ? l - logit_of(part, rows * stride, splits, at + t) : __builtin_nanf("");
+}
+
+// gz of one logit
+__device__ __forceinline__ float gradient_of(float z, float lse, long long t, int n, int N, float g) {
+  const float p = __builtin_amdgcn_exp2f((z - lse) * 1.44269504088896341f) - (n == t ? 1.f : 0.f);
+  return t < 0 ? 0.f : p * (t < N ? g : __builtin_nanf(""));
+}
+
+constexpr int kGzRows = 32;   // of a block
+
+// gz (rows of ldz, zeros behind N) and its column sums over kGzRows rows: a thread a column
+template <typename T>
+__global__ void __launch_bounds__(256) loss_gz_kernel(T *gz, float *columns, const float *part, int splits, const float *lse, const float *g, const long long *targets,
+                                                      const float *norm, long long rows, int N, int ldz) {
+  const int n = blockIdx.y * 256 + threadIdx.x;
+  if (n >= ldz) return;
+  const long long r0 = (long long)blockIdx.x * kGzRows, stride = (N + 3) & ~3;
+  const float scale = norm ? *norm : 1.f;
+  float sum = 0.f;
+  for (long long r = r0; r < min(rows, r0 + kGzRows); r++) {
+    const float v = n < N ? gradient_of(logit_of(part, rows * stride, splits, r * stride + n), lse[r], targets[r], n, N, g[r] * scale) : 0.f;
+    sum += v;
+    gz[r * ldz + n] = from_f<T>(v);
+  }
+  if (columns && n < N) columns[(long long)blockIdx.x * N + n] = sum;
+}
+
+// ---- a handful of rows and classes: one launch forward, two backward, no matrix cores ----
+// What counts there is launches: 19 x 64 -> 118 float32, both directions: SMALLNEW us a pass, through the tiles (nine launches) 80.
+constexpr long long kSmallWork = 1 << 21;   // rows * n_in * n_out
+constexpr int kSmallSide = 2048;            // n_in and n_out (LDS)
+bool small_case(long long rows, int K, int N) { return K > 0 && K <= kSmallSide && N <= kSmallSide && rows <= kSmallWork && rows * K <= kSmallWork && rows * K * N <= kSmallWork; }
+
+// z of a row's classes threadIdx.x, threadIdx.x + 256, ... into LDS; x in LDS
+template <typename T>
+__device__ __forceinline__ void small_logits(float *z, const float *x, const T *w, const T *b, int K, int N) {
+  for (int n = threadIdx.x; n < N; n += 256) {
+    float v = b ? to_f(b[n]) : 0.f;
+    const T *p = w + n;
+#pragma unroll 8
+    for (int k = 0; k < K; k++) v = __builtin_fmaf(x[k], to_f(p[(long long)k * N]), v);
+    z[n] = v;
+  }
+}
+
+template <typename T>
+__global__ void __launch_bounds__(256) loss_small_kernel(const LossArgs l) {
+  __shared__ float x[kSmallSide], z[kSmallSide];
+  __shared__ float2 lds[4];
+  const long long row = blockIdx.x;
+  for (int k = threadIdx.x; k < l.K; k += 256) x[k] = to_f(((const T *)l.x)[row * l.xs + k]);
+  __syncthreads();
+  small_logits<T>(z, x, (const T *)l.w, (const T *)l.b, l.K, l.N);
+  float top = -INFINITY, sum = 0.f;
+  for (int n = threadIdx.x; n < l.N; n += 256) sum_exp(top, sum, z[n], 1.f);
+  block_sum_exp(top, sum, lds);   // (and z is there)
+  if (threadIdx.x) return;
+  const float lse = top + logf(sum);
+  const long long t = l.targets[row];
+  if (l.lse_out) l.lse_out[row] = lse;
+  l.loss[row] = t < 0 ? 0.f : t < l.N ? lse - z[t] : __builtin_nanf("");
+}
+
+// gz of a row, as float32 values rounded to the layer's type as for the tiles' products (float16: with norm), and gx: a wave a value of it at a time
+template <typename T>
+__global__ void __launch_bounds__(256) loss_small_rows_kernel(const LossArgs l, float *gz, const float *norm) {
+  __shared__ float x[kSmallSide], z[kSmallSide];
+  const long long row = blockIdx.x, t = l.targets[row];
+  for (int k = threadIdx.x; k < l.K; k += 256) x[k] = to_f(((const T *)l.x)[row * l.xs + k]);
+  __syncthreads();
+  small_logits<T>(z, x, (const T *)l.w, (const T *)l.b, l.K, l.N);
+  const float g = l.g[row] * (norm ? norm[0] : 1.f), lse = l.lse[row];
+  for (int n = threadIdx.x; n < l.N; n += 256) {   // (its own)
+    const float v = gradient_of(z[n], lse, t, n, l.N, g);
+    gz[row * l.N + n] = v;
+    z[n] = to_f(from_f<T>(v));
+  }
+  __syncthreads();
+  if (!l.gx) return;
+  const float back = norm ? norm[1] : 1.f;
+  for (int k = threadIdx.x / 64; k < l.K; k += 4) {
+    const T *w = (const T *)l.w + (long long)k * l.N;
+    float v = 0.f;
+    if (t >= 0)   // (what is left out gives nothing, whatever w holds)
+      for (int n = threadIdx.x % 64; n < l.N; n += 64) v = __builtin_fmaf(z[n], to_f(w[n]), v);
+#pragma unroll
+    for (int d = 1; d < 64; d *= 2) v += __shfl_xor(v, d);
+    if (threadIdx.x % 64 == 0) ((T *)l.gx)[row * l.K + k] = from_f<T>(v * back);
+  }
+}
+
+// gw, a thread a value, and gb (row K)
+template <typename T>
+__global__ void __launch_bounds__(256) loss_small_columns_kernel(const LossArgs l, const float *gz, const float *norm) {
+  const long long at = (long long)blockIdx.x * 256 + threadIdx.x;
+  const int k = (int)(at / l.N), n = (int)(at - (long long)k * l.N);
+  if (k > l.K || (k < l.K ? !l.gw : !l.gb)) return;
+  const float back = norm ? norm[1] : 1.f;
+  float v = 0.f;
+  if (k < l.K) {
+#pragma unroll 4
+    for (long long r = 0; r < l.rows; r++) {
+      const float x = to_f(((const T *)l.x)[r * l.xs + k]), g = to_f(from_f<T>(gz[r * l.N + n]));
+      if (l.targets[r] >= 0) v = __builtin_fmaf(x, g, v);
+    }
+    ((T *)l.gw)[at] = from_f<T>(v * back);
+  } else {
+    for (long long r = 0; r < l.rows; r++) v += gz[r * l.N + n];
+    ((T *)l.gb)[n] = from_f<T>(v * back);
+  }
 }
 
 long long tiles_of(long long n, int b) { return (n + b - 1) / b; }
@@ -130,12 +273,33 @@ int tile_of(int dtype, long long M, long long N, long long K, int epilogue) {
   return plan_of(dtype, M, N, K, epilogue == kLossGrad ? (int)dtype_bytes(dtype) : 0, true).tile;
 }
 
+// pieces of k that the logits' product is cut into (1: it has the loss's epilogue), and their bytes
+// (in pieces only where the kernels behind them fit one launch)
+Plan logits_plan(int dtype, long long rows, int K, int N) { return plan_of(dtype, rows, N, K, 4, rows > 1 << 20 || N > 1 << 20); }
+int logit_pieces(int dtype, long long rows, int K, int N) { return logits_plan(dtype, rows, K, N).splits; }
+
+// the logits of all classes in pieces
+template <typename T>
+int logits_in_pieces(int dtype, GemmArgs a, float *part, hipStream_t s) {
+  const Plan p = logits_plan(dtype, a.M, (int)a.K, a.N);
+  a.splits = p.splits, a.kper = p.kper, a.part = part, a.act = kActNone;
+  a.mtiles = (unsigned)tiles_of(a.M, kGemmBM[p.tile]), a.ntiles = (unsigned)tiles_of(a.N, kGemmBN[p.tile]);
+  return launch_gemm<T>(kFormXW, p.tile, a, s);
+}
+
 struct Forward {
-  size_t tops, picked, bytes;
-  int ntiles;
+  size_t tops, picked, part, bytes;
+  int ntiles, splits;
 };
 Forward forward_space(int dtype, long long rows, int K, int N) {
-  Forward f;
+  Forward f = {};
+  if (small_case(rows, K, N)) return f;
+  f.splits = logit_pieces(dtype, rows, K, N);
+  if (f.splits > 1) {
+    f.part = copy_bytes(dtype, rows, K) + copy_bytes(dtype, K, N);
+    f.bytes = f.part + part_bytes(dtype, rows, N, K, 4);
+    return f;
+  }
   f.ntiles = (int)tiles_of(N, kGemmBN[tile_of(dtype, rows, N, K, kLossSums)]);
   size_t at = copy_bytes(dtype, rows, K) + copy_bytes(dtype, K, N);
   f.tops = at, at += up((size_t)rows * f.ntiles * 8);
@@ -147,23 +311,29 @@ Forward forward_space(int dtype, long long rows, int K, int N) {
 // Classes of a piece of gz, and where everything lies
 struct Backward {
   long long piece, ldz;
-  int pieces;
+  int pieces, splits;   // splits: of the logits' product
   size_t gz, norm, columns, part, bytes;
 };
 Backward backward_space(int what, int dtype, long long rows, int K, int N) {
-  Backward b;
+  Backward b = {};
+  if (small_case(rows, K, N)) {
+    b.norm = up((size_t)rows * N * 4), b.bytes = b.norm + up(8);
+    return b;
+  }
   const long long e = dtype_bytes(dtype), V = 16 / e;
   const long long most = std::max(256LL, (long long)(kMostGradients / (size_t)(rows * e)) / 256 * 256);
   b.pieces = (int)tiles_of(N, (int)std::min<long long>(most, 1 << 30));
   b.piece = b.pieces == 1 ? N : (tiles_of(N, b.pieces) + 255) / 256 * 256;
   b.pieces = (int)((N + b.piece - 1) / b.piece);
   b.ldz = (b.piece + V - 1) / V * V;
+  b.splits = b.pieces == 1 ? logit_pieces(dtype, rows, K, N) : 1;
   const long long last = N - (b.pieces - 1) * b.piece;
   size_t at = copy_bytes(dtype, rows, K, what & 2) + copy_bytes(dtype, K, N);
   b.gz = at, at += up((size_t)rows * b.ldz * e);
   b.norm = at, at += up(8);
   b.columns = at;
-  if (what & 4)
+  if (what & 4 && b.splits > 1) at += up((size_t)tiles_of(rows, kGzRows) * N * 4);
+  else if (what & 4)
     for (long long n : {b.piece, last}) at = std::max(at, b.columns + up((size_t)tiles_of(rows, kGemmWM[tile_of(dtype, rows, n, K, kLossGrad)]) * n * 4));
   b.part = at;
   size_t part = 0;
@@ -171,6 +341,7 @@ Backward backward_space(int what, int dtype, long long rows, int K, int N) {
   size_t part_w = 0;
   if (what & 2)
     for (long long n : {b.piece, last}) part_w = std::max(part_w, part_bytes(dtype, K, n, rows, out_bytes(kFormXG, dtype)));
+  if (b.splits > 1) part = std::max(part, part_bytes(dtype, rows, N, K, 4));
   // (sums over pieces of classes live through all of them; pieces of a product only until they are joined)
   b.bytes = at + (b.pieces > 1 ? part + part_w : std::max(part, part_w));
   return b;
@@ -178,6 +349,10 @@ Backward backward_space(int what, int dtype, long long rows, int K, int N) {
 
 template <typename T>
 int fwd(int dtype, const LossArgs &l, hipStream_t s) {
+  if (small_case(l.rows, l.K, l.N)) {
+    hipLaunchKernelGGL(loss_small_kernel<T>, dim3((unsigned)l.rows), dim3(256), 0, s, l);
+    return launched();
+  }
   const Forward at = forward_space(dtype, l.rows, l.K, l.N);
   GemmArgs a = {};
   a.lda = l.xs, a.ldb = l.N;
@@ -187,6 +362,12 @@ int fwd(int dtype, const LossArgs &l, hipStream_t s) {
   copies.run(s);
   a.bias = l.b, a.M = l.rows, a.N = l.N, a.K = l.K;
   a.targets = l.targets, a.N_all = l.N;
+  if (at.splits > 1) {
+    float *part = (float *)((char *)l.ws + at.part);
+    if (int rc = logits_in_pieces<T>(dtype, a, part, s)) return rc;
+    hipLaunchKernelGGL(loss_pieces_kernel, dim3((unsigned)l.rows), dim3(256), 0, s, l.loss, l.lse_out, (const float *)part, at.splits, l.targets, l.rows, l.N);
+    return launched();
+  }
   a.tops = (float2 *)((char *)l.ws + at.tops), a.picked = (float *)((char *)l.ws + at.picked);
   if (int rc = logits<T>(kLossSums, dtype, a, s)) return rc;
   int lanes = 1;
@@ -210,16 +391,23 @@ int bwd(int dtype, const LossArgs &l, hipStream_t s) {
   }
   const Backward at = backward_space(what, dtype, l.rows, l.K, l.N);
   char *ws = (char *)l.ws;
-  long long ldx = l.xs, ldw = l.N;
-  Copies<T> copies(ws);
-  // (a row that is left out may hold anything; times a gradient of zero it would still be something in gw)
-  const T *x = (const T *)copies.rows(l.x, ldx, l.rows, l.K, l.gw ? l.targets : nullptr), *w = (const T *)copies.rows(l.w, ldw, l.K, l.N);
-  copies.run(s);
   float *norm = nullptr;
   if (dtype == GELIB_HIP_F16) {
     norm = (float *)(ws + at.norm);
     hipLaunchKernelGGL(loss_norm_kernel, dim3(1), dim3(1024), 0, s, norm, l.g, l.targets, l.rows);
   }
+  if (small_case(l.rows, l.K, l.N)) {
+    float *gz = (float *)ws;
+    hipLaunchKernelGGL(loss_small_rows_kernel<T>, dim3((unsigned)l.rows), dim3(256), 0, s, l, gz, (const float *)norm);
+    if (l.gw || l.gb)
+      hipLaunchKernelGGL(loss_small_columns_kernel<T>, dim3((unsigned)(((l.K + 1LL) * l.N + 255) / 256)), dim3(256), 0, s, l, (const float *)gz, (const float *)norm);
+    return launched();
+  }
+  long long ldx = l.xs, ldw = l.N;
+  Copies<T> copies(ws);
+  // (a row that is left out may hold anything; times a gradient of zero it would still be something in gw)
+  const T *x = (const T *)copies.rows(l.x, ldx, l.rows, l.K, l.gw ? l.targets : nullptr), *w = (const T *)copies.rows(l.w, ldw, l.K, l.N);
+  copies.run(s);
   const float *back = norm ? norm + 1 : nullptr;
   T *gz = (T *)(ws + at.gz);
   const bool gx = l.gx && l.K, gw = l.gw && l.K;
@@ -233,10 +421,14 @@ int bwd(int dtype, const LossArgs &l, hipStream_t s) {
     a.c = gz, a.ldc = at.ldz, a.M = l.rows, a.N = n, a.K = l.K;
     a.targets = l.targets, a.n_first = n0, a.N_all = l.N, a.lse = l.lse, a.weight = l.g, a.norm = norm;
     if (l.gb) a.columns = (float *)(ws + at.columns);
-    if (int rc = logits<T>(kLossGrad, dtype, a, s)) return rc;
+    if (at.splits > 1) {
+      if (int rc = logits_in_pieces<T>(dtype, a, part, s)) return rc;
+      hipLaunchKernelGGL(loss_gz_kernel<T>, dim3((unsigned)tiles_of(l.rows, kGzRows), (unsigned)tiles_of(at.ldz, 256)), dim3(256), 0, s, gz, a.columns, (const float *)part, at.splits,
+                         l.lse, l.g, l.targets, (const float *)norm, l.rows, n, (int)at.ldz);
+    } else if (int rc = logits<T>(kLossGrad, dtype, a, s)) return rc;
     if (l.gb) {
-      const long long chunks = tiles_of(l.rows, kGemmWM[tile_of(dtype, l.rows, n, l.K, kLossGrad)]);
-      hipLaunchKernelGGL(loss_columns_kernel<T>, dim3((unsigned)std::min((n + 31LL) / 32, 1LL << 22)), dim3(256), 0, s, (T *)l.gb + n0, (const float *)a.columns, chunks, n, back);
+      const long long chunks = at.splits > 1 ? tiles_of(l.rows, kGzRows) : tiles_of(l.rows, kGemmWM[tile_of(dtype, l.rows, n, l.K, kLossGrad)]);
+      hipLaunchKernelGGL(column_join_kernel<T>, dim3((unsigned)std::min((n + 31LL) / 32, 1LL << 22)), dim3(256), 0, s, (const float *)a.columns, (T *)l.gb + n0, chunks, n, back);
     }
     if (gx) {
       GemmArgs p = {};

@@ -180,9 +180,9 @@ size_t copy_bytes(int dtype, long long rows, int cols, bool always = false) {
   return cols % V || always ? up((size_t)rows * ((cols + V - 1LL) / V * 16)) : 0;
 }
 
-// out[n] = sum over the chunks: 32 columns at a time by 8 runs of chunks a block
+// out[n] = norm (null: 1) times the sum over the chunks: 32 columns at a time by 8 runs of chunks a block
 template <typename T>
-__global__ void __launch_bounds__(256) column_join_kernel(const float *sums, T *out, long long chunks, int N) {
+__global__ void __launch_bounds__(256) column_join_kernel(const float *sums, T *out, long long chunks, int N, const float *norm) {
   __shared__ float lds[8][32];
   const int run = threadIdx.x / 32;
   for (long long n0 = blockIdx.x * 32LL; n0 < N; n0 += gridDim.x * 32LL) {
@@ -196,7 +196,7 @@ __global__ void __launch_bounds__(256) column_join_kernel(const float *sums, T *
     __syncthreads();
     if (run == 0 && n < N) {
       for (int k = 1; k < 8; k++) s += lds[k][threadIdx.x];
-      out[n] = from_f<T>(s);
+      out[n] = from_f<T>(norm ? s * *norm : s);
     }
     __syncthreads();
   }

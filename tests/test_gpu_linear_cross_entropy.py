@@ -58,6 +58,8 @@ def case(m, k, n, dtype, seed=0, spread=1.5):
 # one of everything, sizes around the tiles (16, 64, 128, 256) and their steps, classes of one tile and of many, odd rows that are not aligned
 SIZES = [(1, 1, 1), (1, 8, 2), (3, 40, 118), (19, 64, 118), (16, 16, 256), (17, 33, 257), (64, 64, 128), (65, 63, 129), (128, 256, 1000), (129, 72, 513), (300, 1, 5), (257, 130, 384),
          (1000, 8, 40), (5003, 24, 30), (2, 8, 5000), (260, 455, 2052), (7, 0, 6), (40, 24, 36867)]
+# long sums of few tiles, which are cut along n_in; the largest that need no matrix cores, and the next
+SIZES += [(300, 2048, 118), (70, 4100, 301), (512, 1000, 33), (16, 256, 512), (17, 256, 512), (1, 2048, 1024), (1, 2049, 8), (1024, 64, 32)]
 
 
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16], ids=str)
