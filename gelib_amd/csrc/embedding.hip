@@ -8,8 +8,9 @@
 // the ends of a piece share with their neighbours goes to a list of two entries a piece, whose entries are in order again: the same kernel
 // sums that list, and so on until one piece is left.  Adding to rows in memory as they come would be one launch, but atomic additions are
 // in no order, and take turns where tokens are few (a million atoms of a dozen elements).
-#include <cstring>
-
+// (A table of sums in the LDS of every block instead of the sort, for 118 rows: 285 us with read, add and write, 670 with LDS's own additions.)
+// What bounds it: memory.  1048576 x 128 float32 of 118 rows: forward 132 us (4.1 TB/s), sort 24, sums 152 (rows of 512 bytes in sorted order, 3.5 TB/s) + 3
+// joins of 8; 65536 x 2048 bfloat16 of 65536 rows: forward 84, zeros 34, sort 36, sums 110 (4.9 TB/s) + 20.
 #include "real_ops.h"
 
 namespace gelib_hip {

@@ -5,6 +5,8 @@
 // gz, for as many classes at a time as kMostGradients bytes hold; each such piece goes through the two products gx += gz w^T and gw = x^T gz
 // while the next level of memory still has it.  Eight operations a weight and row instead of six, for rows * classes values that are
 // neither kept nor read and written once more in between.
+// bfloat16 8192 x 2048 -> 65536, both directions: 7.9 ms (forward 2.0, 1.1 PFLOP/s; four pieces of gz .56, gx .45, gw .46 each), at the library's rate for
+// a large product (1335 TFLOP/s) 6.6.
 // gz is rounded to the layer's type for the two products, as in the layer itself (linear_act.hip); gb sums unrounded values.
 // float16: gz is scaled by a power of two that brings the largest |g| to 2^13 (gz stays below 2^14), so that probabilities down to
 // 2^-27 are float16 values of full precision; results are scaled back before they are rounded.
@@ -91,7 +93,7 @@ void zero(void *to, long long n, hipStream_t s) {
 
 // ---- few rows and classes ----
 // Where a product's tiles leave compute units idle and its sums are long, it is cut along k as any other: its pieces hold all logits then (they
-// are few), and the epilogue is the join's.  512 x 2048 -> 118 float32, both directions: FEWNEW us, in one piece FEWOLD.
+// are few), and the loss is taken of their sum (logits_plan).
 
 __device__ __forceinline__ void sum_exp(float &top, float &sum, float otop, float osum) {
   const float to = fmaxf(top, otop), from = to == -INFINITY ? 0.f : to;
@@ -112,25 +114,19 @@ __device__ __forceinline__ void block_sum_exp(float &top, float &sum, float2 *ld
   for (int k = 1; k < 4; k++) sum_exp(top, sum, lds[k].x, lds[k].y);
 }
 
-// a row's logit from the pieces of its sum
-__device__ __forceinline__ float logit_of(const float *part, long long all, int splits, long long at) {
-  float z = 0.f;
-  for (int k = 0; k < splits; k++) z += part[k * all + at];
-  return z;
-}
-
 // A block a row
-__global__ void __launch_bounds__(256) loss_pieces_kernel(float *loss, float *lse, const float *part, int splits, const long long *targets, long long rows, int N) {
+__global__ void __launch_bounds__(256) loss_rows_kernel(float *loss, float *lse, const float *logits, const long long *targets, int N) {
   __shared__ float2 lds[4];
-  const long long row = blockIdx.x, stride = (N + 3) & ~3, at = row * stride;
+  const long long row = blockIdx.x;
+  const float *z = logits + row * ((N + 3) & ~3);
   float top = -INFINITY, sum = 0.f;
-  for (int n = threadIdx.x; n < N; n += 256) sum_exp(top, sum, logit_of(part, rows * stride, splits, at + n), 1.f);
+  for (int n = threadIdx.x; n < N; n += 256) sum_exp(top, sum, z[n], 1.f);
   block_sum_exp(top, sum, lds);
   if (threadIdx.x) return;
   const float l = top + logf(sum);
   const long long t = targets[row];
   if (lse) lse[row] = l;
-  loss[row] = t < 0 ? 0.f : t < N ? l - logit_of(part, rows * stride, splits, at + t) : __builtin_nanf("");
+  loss[row] = t < 0 ? 0.f : t < N ? l - z[t] : __builtin_nanf("");
 }
 
 // gz of one logit
@@ -139,19 +135,22 @@ __device__ __forceinline__ float gradient_of(float z, float lse, long long t, in
   return t < 0 ? 0.f : p * (t < N ? g : __builtin_nanf(""));
 }
 
-constexpr int kGzRows = 32;   // of a block
+constexpr int kGzRows = 8;   // of a block
 
 // gz (rows of ldz, zeros behind N) and its column sums over kGzRows rows: a thread a column
 template <typename T>
-__global__ void __launch_bounds__(256) loss_gz_kernel(T *gz, float *columns, const float *part, int splits, const float *lse, const float *g, const long long *targets,
+__global__ void __launch_bounds__(256) loss_gz_kernel(T *gz, float *columns, const float *logits, const float *lse, const float *g, const long long *targets,
                                                       const float *norm, long long rows, int N, int ldz) {
   const int n = blockIdx.y * 256 + threadIdx.x;
   if (n >= ldz) return;
   const long long r0 = (long long)blockIdx.x * kGzRows, stride = (N + 3) & ~3;
   const float scale = norm ? *norm : 1.f;
   float sum = 0.f;
-  for (long long r = r0; r < min(rows, r0 + kGzRows); r++) {
-    const float v = n < N ? gradient_of(logit_of(part, rows * stride, splits, r * stride + n), lse[r], targets[r], n, N, g[r] * scale) : 0.f;
+#pragma unroll
+  for (int k = 0; k < kGzRows; k++) {
+    const long long r = r0 + k;
+    if (r >= rows) break;
+    const float v = n < N ? gradient_of(logits[r * stride + n], lse[r], targets[r], n, N, g[r] * scale) : 0.f;
     sum += v;
     gz[r * ldz + n] = from_f<T>(v);
   }
@@ -159,7 +158,8 @@ __global__ void __launch_bounds__(256) loss_gz_kernel(T *gz, float *columns, con
 }
 
 // ---- a handful of rows and classes: one launch forward, two backward, no matrix cores ----
-// What counts there is launches: 19 x 64 -> 118 float32, both directions: SMALLNEW us a pass, through the tiles (nine launches) 80.
+// What counts there is launches: 19 x 64 -> 118 float32, both directions: 60 us a pass, nearly all of them the host's; through the tiles (nine
+// launches) 80.  128 x 128 -> 128, here / through the tiles: 59 / 70.
 constexpr long long kSmallWork = 1 << 21;   // rows * n_in * n_out
 constexpr int kSmallSide = 2048;            // n_in and n_out (LDS)
 bool small_case(long long rows, int K, int N) { return K > 0 && K <= kSmallSide && N <= kSmallSide && rows <= kSmallWork && rows * K <= kSmallWork && rows * K * N <= kSmallWork; }
@@ -273,18 +273,29 @@ int tile_of(int dtype, long long M, long long N, long long K, int epilogue) {
   return plan_of(dtype, M, N, K, epilogue == kLossGrad ? (int)dtype_bytes(dtype) : 0, true).tile;
 }
 
-// pieces of k that the logits' product is cut into (1: it has the loss's epilogue), and their bytes
-// (in pieces only where the kernels behind them fit one launch)
-Plan logits_plan(int dtype, long long rows, int K, int N) { return plan_of(dtype, rows, N, K, 4, rows > 1 << 20 || N > 1 << 20); }
+// Pieces of k that the logits' product is cut into (1: it has the loss's epilogue): where the kernels behind them fit one launch and the sums are long
+// enough for the launches more.  Both directions, in pieces / whole, us: float32 512 x 256 -> 118 110 / 94, x 512 107 / 94, 4096 x 512 -> 64 87 / 182,
+// 512 x 2048 -> 118 90 / 171, 256 x 1024 -> 4096 129 / 220; bfloat16 64 x 2048 -> 1000 106 / 89, x 4096 102 / 109, x 8192 101 / 180.
+Plan logits_plan(int dtype, long long rows, int K, int N) {
+  return plan_of(dtype, rows, N, K, 4, rows > 1 << 20 || N > 1 << 20 || K < (dtype == GELIB_HIP_F32 ? 512 : 4096));
+}
 int logit_pieces(int dtype, long long rows, int K, int N) { return logits_plan(dtype, rows, K, N).splits; }
 
-// the logits of all classes in pieces
+size_t logits_bytes(int dtype, long long rows, int K, int N) { return up(part_bytes(dtype, rows, N, K, 4)) + up((size_t)rows * ((N + 3) & ~3LL) * 4); }
+
+// the logits of all classes from pieces of k, rows of N up to a multiple of 4
 template <typename T>
-int logits_in_pieces(int dtype, GemmArgs a, float *part, hipStream_t s) {
+int logits_in_pieces(int dtype, GemmArgs a, void *space, const float *&logits, hipStream_t s) {
   const Plan p = logits_plan(dtype, a.M, (int)a.K, a.N);
-  a.splits = p.splits, a.kper = p.kper, a.part = part, a.act = kActNone;
+  a.splits = p.splits, a.kper = p.kper, a.part = (float *)space, a.act = kActNone;
   a.mtiles = (unsigned)tiles_of(a.M, kGemmBM[p.tile]), a.ntiles = (unsigned)tiles_of(a.N, kGemmBN[p.tile]);
-  return launch_gemm<T>(kFormXW, p.tile, a, s);
+  if (int rc = launch_gemm<T>(kFormXW, p.tile, a, s)) return rc;
+  a.c = (char *)space + up(part_bytes(dtype, a.M, a.N, a.K, 4)), a.ldc = (a.N + 3) & ~3, a.vec4 = a.N % 4 == 0;
+  a.bias = a.norm = nullptr;   // (in the first piece; of the gradients)
+  const unsigned per_row = (a.N + 3) / 4;
+  hipLaunchKernelGGL((join_kernel<float, kActNone>), dim3((unsigned)((a.M * per_row + 255) / 256)), dim3(256), 0, s, a, per_row);
+  logits = (const float *)a.c;
+  return launched();
 }
 
 struct Forward {
@@ -297,7 +308,7 @@ Forward forward_space(int dtype, long long rows, int K, int N) {
   f.splits = logit_pieces(dtype, rows, K, N);
   if (f.splits > 1) {
     f.part = copy_bytes(dtype, rows, K) + copy_bytes(dtype, K, N);
-    f.bytes = f.part + part_bytes(dtype, rows, N, K, 4);
+    f.bytes = f.part + logits_bytes(dtype, rows, K, N);
     return f;
   }
   f.ntiles = (int)tiles_of(N, kGemmBN[tile_of(dtype, rows, N, K, kLossSums)]);
@@ -341,7 +352,7 @@ Backward backward_space(int what, int dtype, long long rows, int K, int N) {
   size_t part_w = 0;
   if (what & 2)
     for (long long n : {b.piece, last}) part_w = std::max(part_w, part_bytes(dtype, K, n, rows, out_bytes(kFormXG, dtype)));
-  if (b.splits > 1) part = std::max(part, part_bytes(dtype, rows, N, K, 4));
+  if (b.splits > 1) part = std::max(part, logits_bytes(dtype, rows, K, N));
   // (sums over pieces of classes live through all of them; pieces of a product only until they are joined)
   b.bytes = at + (b.pieces > 1 ? part + part_w : std::max(part, part_w));
   return b;
@@ -363,9 +374,9 @@ int fwd(int dtype, const LossArgs &l, hipStream_t s) {
   a.bias = l.b, a.M = l.rows, a.N = l.N, a.K = l.K;
   a.targets = l.targets, a.N_all = l.N;
   if (at.splits > 1) {
-    float *part = (float *)((char *)l.ws + at.part);
-    if (int rc = logits_in_pieces<T>(dtype, a, part, s)) return rc;
-    hipLaunchKernelGGL(loss_pieces_kernel, dim3((unsigned)l.rows), dim3(256), 0, s, l.loss, l.lse_out, (const float *)part, at.splits, l.targets, l.rows, l.N);
+    const float *logits;
+    if (int rc = logits_in_pieces<T>(dtype, a, (char *)l.ws + at.part, logits, s)) return rc;
+    hipLaunchKernelGGL(loss_rows_kernel, dim3((unsigned)l.rows), dim3(256), 0, s, l.loss, l.lse_out, logits, l.targets, l.N);
     return launched();
   }
   a.tops = (float2 *)((char *)l.ws + at.tops), a.picked = (float *)((char *)l.ws + at.picked);
@@ -422,9 +433,9 @@ int bwd(int dtype, const LossArgs &l, hipStream_t s) {
     a.targets = l.targets, a.n_first = n0, a.N_all = l.N, a.lse = l.lse, a.weight = l.g, a.norm = norm;
     if (l.gb) a.columns = (float *)(ws + at.columns);
     if (at.splits > 1) {
-      if (int rc = logits_in_pieces<T>(dtype, a, part, s)) return rc;
-      hipLaunchKernelGGL(loss_gz_kernel<T>, dim3((unsigned)tiles_of(l.rows, kGzRows), (unsigned)tiles_of(at.ldz, 256)), dim3(256), 0, s, gz, a.columns, (const float *)part, at.splits,
-                         l.lse, l.g, l.targets, (const float *)norm, l.rows, n, (int)at.ldz);
+      const float *logits;
+      if (int rc = logits_in_pieces<T>(dtype, a, part, logits, s)) return rc;
+      hipLaunchKernelGGL(loss_gz_kernel<T>, dim3((unsigned)tiles_of(l.rows, kGzRows), (unsigned)tiles_of(at.ldz, 256)), dim3(256), 0, s, gz, a.columns, logits, l.lse, l.g, l.targets, (const float *)norm, l.rows, n, (int)at.ldz);
     } else if (int rc = logits<T>(kLossGrad, dtype, a, s)) return rc;
     if (l.gb) {
       const long long chunks = at.splits > 1 ? tiles_of(l.rows, kGzRows) : tiles_of(l.rows, kGemmWM[tile_of(dtype, l.rows, n, l.K, kLossGrad)]);

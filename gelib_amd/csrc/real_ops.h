@@ -1,5 +1,6 @@
 // The operators on real channels around the equivariant layers -- group norm with an activation, the linear layer with its
-// epilogue, the AdamW step -- as the C entry points (cabi_real.cpp) see them, and what their kernels share.
+// epilogue, the AdamW step -- and those of a network over points -- embedding, attention, cross entropy of a linear layer's classes -- as the C entry
+// points (cabi_real.cpp, cabi_points.cpp) see them, and what their kernels share.
 #pragma once
 
 #include <algorithm>

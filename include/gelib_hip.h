@@ -482,7 +482,7 @@ int gelib_hip_set_stream_workspace(void *stream, void *ptr, uint64_t bytes);
  * gelib_hip_last_path() tells which kernel family the last call of this thread used
  * (0 = none, 1 = generic, 2 = unrolled small-l kernels, 3 = staged any-l kernels, 4 = lane-per-channel Diag
  * kernels for operand l up to 6, 5 = single-pair kernels for large l, 6 = the product fused with the weight matrices, or
- * the matrices' gradients alone, straight from the operands, 7 = the operators on real channels).
+ * the matrices' gradients alone, straight from the operands, 7 = the operators on real channels and over points).
  */
 int gelib_hip_set_option(const char *name, int value);
 int gelib_hip_last_path(void);
