@@ -253,6 +253,20 @@ __global__ void __launch_bounds__(256) embedding_sum_kernel(const List<T> l, O *
           there &= there - 1;
           v[u] = *(const Some<T, V> *)(l.rows + (long long)(u32)__builtin_amdgcn_readlane(rows, k) * C + cc);
         }
+        if (key[0] == run && key[U - 1] == run) {   // (keys ascend: all of one row, summed in pairs first: smaller errors)
+#pragma unroll
+          for (int i = 0; i < V; i++) {
+            float t[U];
+#pragma unroll
+            for (int u = 0; u < U; u++) t[u] = to_f(v[u].v[i]);
+#pragma unroll
+            for (int m = U / 2; m; m /= 2)
+#pragma unroll
+              for (int u = 0; u < m; u++) t[u] += t[u + m];
+            acc[i] += t[0];
+          }
+          continue;
+        }
 #pragma unroll
         for (int u = 0; u < U; u++) {
           if (key[u] == kNoToken) continue;
