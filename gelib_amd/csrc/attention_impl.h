@@ -13,10 +13,10 @@
 // transposed fragments are read by the LDS unit's transposing loads.  float32: each of the four is one step of k).
 // A document's query rows are its (position, head of the group) pairs: heads that share keys stand in one tile.
 //
-// What bounds it: the vector unit, 70 to 75 % busy with the distances, exponentials and sums between the products.  8192 points, 16 heads of 64 on 4, bfloat16, with points: forward 520 us (530 TFLOP/s),
-// by rows 940, by keys 920; 16 on 16, without points: forward 408 us (675), both directions 1645 (585); 2 x 8192, 8 heads of 128 on 2, without points: forward
-// 599 (918).  Short documents: the instructions around the products (addresses, rows, results): 2048 packed documents of 32 on average, 8 heads of 32: 66, 97
-// and 103 us.
+// What bounds it: the vector unit, 70 to 75 % busy with the distances, exponentials and sums between the products.  8192 points, 16 heads of 64
+// on 4, bfloat16, with points: forward 520 us (530 TFLOP/s), by rows 940, by keys 920; 16 on 16, without points: forward 408 us (675), both
+// directions 1645 (585); 2 x 8192, 8 heads of 128 on 2, without points: forward 599 (918).  Short documents: the instructions around the
+// products (addresses, rows, results): 2048 packed documents of up to 60 rows, 8 heads of 32, bfloat16: 66, 97 and 103 us.
 #pragma once
 
 #include <type_traits>

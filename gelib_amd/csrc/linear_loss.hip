@@ -46,18 +46,28 @@ __global__ void __launch_bounds__(256) loss_join_kernel(float *loss, float *lse,
   loss[row] = t < 0 ? 0.f : t < N ? l - picked[row] : __builtin_nanf("");
 }
 
-// norm[0]: the power of two that brings the largest |g| of a row with a class to 2^13, norm[1]: one over it
+// norm[0]: the power of two that brings the largest |g| of a row with a class to 2^13, norm[1]: one over it.  Many rows: largest values of blocks first
+// (behind norm[1]; targets null: of these)
+constexpr int kNormBlocks = 256, kNormRows = 8192;   // of a block
+constexpr size_t kNormBytes = (2 + kNormBlocks) * 4;
 __global__ void __launch_bounds__(1024) loss_norm_kernel(float *norm, const float *g, const long long *targets, long long rows) {
   __shared__ float lds[16];
   float top = 0.f;
-  for (long long i = threadIdx.x; i < rows; i += 1024)
-    if (targets[i] >= 0 && fabsf(g[i]) < INFINITY) top = fmaxf(top, fabsf(g[i]));
+#pragma unroll 4
+  for (long long i = blockIdx.x * 1024LL + threadIdx.x; i < rows; i += gridDim.x * 1024LL) {
+    const float v = fabsf(g[i]);
+    if ((!targets || targets[i] >= 0) && v < INFINITY) top = fmaxf(top, v);
+  }
 #pragma unroll
   for (int d = 1; d < 64; d *= 2) top = fmaxf(top, __shfl_xor(top, d));
   if (threadIdx.x % 64 == 0) lds[threadIdx.x / 64] = top;
   __syncthreads();
   if (threadIdx.x) return;
   for (int k = 0; k < 16; k++) top = fmaxf(top, lds[k]);
+  if (gridDim.x > 1) {
+    norm[2 + blockIdx.x] = top;
+    return;
+  }
   const int e = top > 0.f ? max(-100, min(100, 13 - ilogbf(top))) : 0;
   norm[0] = ldexpf(1.f, e), norm[1] = ldexpf(1.f, -e);
 }
@@ -162,7 +172,10 @@ __global__ void __launch_bounds__(256) loss_gz_kernel(T *gz, float *columns, con
 // launches) 80.  128 x 128 -> 128, here / through the tiles: 59 / 70.
 constexpr long long kSmallWork = 1 << 21;   // rows * n_in * n_out
 constexpr int kSmallSide = 2048;            // n_in and n_out (LDS)
-bool small_case(long long rows, int K, int N) { return K > 0 && K <= kSmallSide && N <= kSmallSide && rows <= kSmallWork && rows * K <= kSmallWork && rows * K * N <= kSmallWork; }
+// A value of gw is one thread's sum over the rows, here / through the tiles, float32, both directions: 256 x 64 -> 128 53 / 63, 512 x 64 -> 64 59 / 58,
+// 1024 x 64 -> 32 98 / 59, 8192 x 16 -> 16 619 / 59.
+constexpr int kSmallRows = 256;
+bool small_case(long long rows, int K, int N) { return K > 0 && rows <= kSmallRows && K <= kSmallSide && N <= kSmallSide && rows * K * N <= kSmallWork; }
 
 // z of a row's classes threadIdx.x, threadIdx.x + 256, ... into LDS; x in LDS
 template <typename T>
@@ -328,7 +341,7 @@ struct Backward {
 Backward backward_space(int what, int dtype, long long rows, int K, int N) {
   Backward b = {};
   if (small_case(rows, K, N)) {
-    b.norm = up((size_t)rows * N * 4), b.bytes = b.norm + up(8);
+    b.norm = up((size_t)rows * N * 4), b.bytes = b.norm + up(kNormBytes);
     return b;
   }
   const long long e = dtype_bytes(dtype), V = 16 / e;
@@ -341,7 +354,7 @@ Backward backward_space(int what, int dtype, long long rows, int K, int N) {
   const long long last = N - (b.pieces - 1) * b.piece;
   size_t at = copy_bytes(dtype, rows, K, what & 2) + copy_bytes(dtype, K, N);
   b.gz = at, at += up((size_t)rows * b.ldz * e);
-  b.norm = at, at += up(8);
+  b.norm = at, at += up(kNormBytes);
   b.columns = at;
   if (what & 4 && b.splits > 1) at += up((size_t)tiles_of(rows, kGzRows) * N * 4);
   else if (what & 4)
@@ -405,7 +418,9 @@ int bwd(int dtype, const LossArgs &l, hipStream_t s) {
   float *norm = nullptr;
   if (dtype == GELIB_HIP_F16) {
     norm = (float *)(ws + at.norm);
-    hipLaunchKernelGGL(loss_norm_kernel, dim3(1), dim3(1024), 0, s, norm, l.g, l.targets, l.rows);
+    const unsigned blocks = (unsigned)std::max(1LL, std::min((long long)kNormBlocks, l.rows / kNormRows));
+    hipLaunchKernelGGL(loss_norm_kernel, dim3(blocks), dim3(1024), 0, s, norm, l.g, l.targets, l.rows);
+    if (blocks > 1) hipLaunchKernelGGL(loss_norm_kernel, dim3(1), dim3(1024), 0, s, norm, (const float *)(norm + 2), (const long long *)nullptr, (long long)blocks);
   }
   if (small_case(l.rows, l.K, l.N)) {
     float *gz = (float *)ws;

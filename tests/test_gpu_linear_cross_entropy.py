@@ -98,6 +98,20 @@ def test_more_classes_than_one_piece(gelib, dtype):
 
 
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16], ids=str)
+def test_many_rows_of_few(gelib, dtype):
+    """Long sums over rows, blocks of them for the largest gradient among them (float16); the largest is the last."""
+    for size in ((256, 64, 128), (257, 64, 128), (20003, 5, 7), (300001, 8, 9)):
+        x, w, b, targets, g = case(*size, dtype)
+        targets[-1], g[-1] = 0, 900.
+        loss = gelib.linear_cross_entropy(x, w, targets, b)
+        got = dict(zip(("gx", "gw", "gb"), torch.autograd.grad(loss, (x, w, b), g)), loss=loss.detach())
+        with torch.no_grad():
+            want = reference(x.double(), w.double(), b.double(), targets, g.double(), dtype)
+        for name, (v, tol) in want.items():
+            check(got[name], v, tol, "%s of %s" % (name, size))
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16], ids=str)
 def test_logits_far_apart(gelib, dtype):
     """Logits of hundreds: nothing overflows, a class that has everything leaves the others gradients of zero."""
     x, w, b, targets, g = case(70, 32, 600, dtype, spread=60.)
