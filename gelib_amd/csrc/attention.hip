@@ -207,44 +207,54 @@ __global__ void __launch_bounds__(256) attention_sum_kernel(T *out, const float 
   out[at] = from_f<T>(v);
 }
 
-// gradients of points: sums over heads and pieces, of queries (geo_q), keys (geo_k) or, where they are the same points, both
+// gradients of points: sums over heads and pieces, of queries (geo_q), keys (geo_k) or, where they are the same points, both.  16 lanes a row,
+// neighbouring heads side by side: one query of 128 heads on 65536 keys in 64 pieces, both directions of the call: 609 us,
+// with a thread a row 1411; 16 heads on 4: 371 / 471.
 __global__ void __launch_bounds__(256) attention_points_kernel(float *out, const float4 *gq, int splits_q, int H, const float4 *gk, int splits_k, int KV,
                                                                long long first, long long rows) {
-  const long long row = first + (long long)blockIdx.x * 256 + threadIdx.x;
-  if (row >= rows) return;
+  const long long row = (first + (long long)blockIdx.x * 256 + threadIdx.x) / 16;
+  const int lane = threadIdx.x % 16;
   float x = 0.f, y = 0.f, z = 0.f;
-  if (gq)
-    for (int s = 0; s < splits_q; s++)
-      for (int h = 0; h < H; h++) {
-        const float4 g = gq[(s * rows + row) * H + h];
-        x += g.x, y += g.y, z += g.z;
-      }
-  if (gk)
-    for (int s = 0; s < splits_k; s++)
-      for (int h = 0; h < KV; h++) {
-        const float4 g = gk[(s * rows + row) * KV + h];
-        x += g.x, y += g.y, z += g.z;
-      }
-  out[row * 3] = x, out[row * 3 + 1] = y, out[row * 3 + 2] = z;
+  auto add = [&](const float4 *g, int splits, int heads) {
+#pragma unroll 4
+    for (int i = lane; i < splits * heads; i += 16) {
+      const int s = splits == 1 ? 0 : i / heads;
+      const float4 v = g[(s * rows + row) * heads + (i - s * heads)];
+      x += v.x, y += v.y, z += v.z;
+    }
+  };
+  if (row < rows) {
+    if (gq) add(gq, splits_q, H);
+    if (gk) add(gk, splits_k, KV);
+  }
+#pragma unroll
+  for (int d = 1; d < 16; d *= 2) x += __shfl_xor(x, d), y += __shfl_xor(y, d), z += __shfl_xor(z, d);
+  if (row < rows && lane < 3) out[row * 3 + lane] = lane == 0 ? x : lane == 1 ? y : z;
 }
 
 // gradients of slopes: of kSlopeRows rows and up to 64 heads, a block (side: threads side by side on heads, a power of two); then of all blocks
-__global__ void __launch_bounds__(256) attention_slopes_kernel(float *part, const float4 *geo, int splits, long long rows, int H, int side) {
+__global__ void __launch_bounds__(256) attention_slopes_kernel(float *part, const float4 *geo, int splits, long long rows, int H, int side, long long blocks) {
   __shared__ float lds[256];
-  const long long r0 = (long long)blockIdx.x * kSlopeRows, r1 = min(rows, r0 + kSlopeRows);
   const int h = blockIdx.y * side + threadIdx.x % side, down = 256 / side;
-  float v = 0.f;
-  if (h < H)
-    for (int s = 0; s < splits; s++)
+  for (long long b = blockIdx.x; b < blocks; b += gridDim.x) {
+    const long long r0 = b * kSlopeRows;
+    const int n = (int)min((long long)kSlopeRows, rows - r0);
+    float v = 0.f;
+    if (h < H)
 #pragma unroll 4
-      for (long long r = r0 + threadIdx.x / side; r < r1; r += down) v += geo[(s * rows + r) * H + h].w;
-  lds[threadIdx.x] = v;
-  __syncthreads();
-  for (int k = 128; k >= side; k /= 2) {
-    if ((int)threadIdx.x < k) lds[threadIdx.x] += lds[threadIdx.x + k];
+      for (int i = threadIdx.x / side; i < n * splits; i += down) {
+        const int s = splits == 1 ? 0 : i / n;
+        v += geo[(s * rows + r0 + (i - s * n)) * H + h].w;
+      }
+    lds[threadIdx.x] = v;
+    __syncthreads();
+    for (int k = 128; k >= side; k /= 2) {
+      if ((int)threadIdx.x < k) lds[threadIdx.x] += lds[threadIdx.x + k];
+      __syncthreads();
+    }
+    if ((int)threadIdx.x < side && h < H) part[b * H + h] = lds[threadIdx.x];
     __syncthreads();
   }
-  if ((int)threadIdx.x < side && h < H) part[(long long)blockIdx.x * H + h] = lds[threadIdx.x];
 }
 __global__ void __launch_bounds__(256) attention_slopes_join_kernel(float *out, const float *part, long long blocks, int H) {
   __shared__ float lds[256];
@@ -383,7 +393,7 @@ int backward(const AttnCall &c, const AttnGrads &g, void *ws, hipStream_t s) {
   }
   if (!geometry) return 0;
   auto points = [&](float *out, bool of_q, bool of_k, long long rows) {
-    return in_launches(rows, [&](long long first, dim3 grid) {
+    return in_launches(rows * 16, [&](long long first, dim3 grid) {
       hipLaunchKernelGGL(attention_points_kernel, grid, dim3(256), 0, s, out, of_q ? a.geo_q : nullptr, pr.splits, a.H, of_k ? a.geo_k : nullptr, pk.splits, a.KV, first, rows);
     });
   };
@@ -397,7 +407,8 @@ int backward(const AttnCall &c, const AttnGrads &g, void *ws, hipStream_t s) {
     if (blocks) {
       int side = 1;
       while (side < 64 && side < a.H) side *= 2;
-      hipLaunchKernelGGL(attention_slopes_kernel, dim3((unsigned)blocks, (unsigned)((a.H + side - 1) / side)), dim3(256), 0, s, part, a.geo_q, pr.splits, a.rows_q, a.H, side);
+      const long long beside = (a.H + side - 1) / side, most = std::max(1LL, (1LL << 22) / beside);   // (blocks of a launch)
+      hipLaunchKernelGGL(attention_slopes_kernel, dim3((unsigned)std::min(blocks, most), (unsigned)beside), dim3(256), 0, s, part, a.geo_q, pr.splits, a.rows_q, a.H, side, blocks);
       if (int rc = launched()) return rc;
     }
     hipLaunchKernelGGL(attention_slopes_join_kernel, dim3(a.H), dim3(256), 0, s, g.gslopes, part, blocks, a.H);
