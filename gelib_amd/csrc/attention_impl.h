@@ -416,6 +416,14 @@ struct QueryRows {
     const RowAt r = row_at(a, row0 + 16 * s + threadIdx.x % 16);
     return (doc.out_q + r.pos) * a.H + kv * a.G + r.head;
   }
+  __device__ __forceinline__ void negate() {
+    typedef unsigned u32x4 __attribute__((ext_vector_type(4)));
+    const unsigned sign = sizeof(T) == 2 ? 0x80008000u : 0x80000000u;
+#pragma unroll
+    for (int s = 0; s < QS; s++)
+#pragma unroll
+      for (int k = 0; k < Tile::KS; k++) q[s][k] = __builtin_bit_cast(typename Tile::Frag, __builtin_bit_cast(u32x4, q[s][k]) ^ sign);
+  }
   __device__ __forceinline__ void load(const AttnArgs &a, const AttnDoc &doc, int kv, int row0, int live) {
 #pragma unroll
     for (int s = 0; s < QS; s++) {
@@ -478,13 +486,20 @@ __device__ __forceinline__ void attention_fwd_head(const AttnArgs &a, const Attn
   QueryRows<T, DP, QS, BIAS> own;
   own.load(a, doc, w.kv, row0, live);
 
-  // Scores are formed less the maximum so far, m (log2).  It moves only when one is more than 8 above it: values are then at most 2^8
-  // times what they would be (and within float16), and rescaling is rare.
+  // Exponentials are formed less the maximum so far, m (log2), which is that of the first tile with a score above -infinity (begun: a row
+  // has had one).  It moves only when a score is more than 8 above it: values are then at most 2^8 times what they would be (and within
+  // float16), and rescaling is rare.  Scores themselves are kept whole until then: less a maximum far below them they would lose digits.
+  // Without distances what is kept are products that the scale, which is above zero then, has not met yet (q takes its sign): it and the
+  // maximum are one instruction in front of the exponential.  8192 x 8192, 16 heads of 64, bfloat16: 411 us, with scores scaled at once 423, less the
+  // maximum from the start 397; with points (8192, 16 heads on 4) an instruction more than that, 540 and 506.
+  const float unit = BIAS ? 1.f : fmaxf(fabsf(a.scale2), 0x1p-149f);   // (not zero: times -infinity)
+  if (!BIAS && a.scale2 < 0.f) own.negate();
   float m[QS], l[QS];
+  bool begun[QS];
   f32x4 acc[QS][Tile::NF];
 #pragma unroll
   for (int s = 0; s < QS; s++) {
-    m[s] = 0.f, l[s] = 0.f;
+    m[s] = 0.f, l[s] = 0.f, begun[s] = false;
 #pragma unroll
     for (int f = 0; f < Tile::NF; f++) acc[s][f] = f32x4{0.f, 0.f, 0.f, 0.f};
   }
@@ -520,14 +535,14 @@ __device__ __forceinline__ void attention_fwd_head(const AttnArgs &a, const Attn
 #pragma unroll
           for (int s = 0; s < QS; s++) {
             if (!SHARE || s == 0) far.form(own.x[s], p, i);   // (the wave's tiles have the same positions)
-            sc[s][j][i] = __builtin_fmaf(z[s][i], a.scale2, __builtin_fmaf(far.far, own.slope[s], -m[s]));
+            sc[s][j][i] = __builtin_fmaf(z[s][i], a.scale2, far.far * own.slope[s]);
           }
         }
       } else {
 #pragma unroll
         for (int s = 0; s < QS; s++)
 #pragma unroll
-          for (int i = 0; i < 4; i++) sc[s][j][i] = __builtin_fmaf(z[s][i], a.scale2, -m[s]);
+          for (int i = 0; i < 4; i++) sc[s][j][i] = z[s][i];
       }
       if (left < j * 16 + 16)
 #pragma unroll
@@ -537,25 +552,23 @@ __device__ __forceinline__ void attention_fwd_head(const AttnArgs &a, const Attn
             for (int s = 0; s < QS; s++) sc[s][j][i] = -INFINITY;
     }
     float top[QS];
-    bool grown = t == t0;
+    bool grown = false;
 #pragma unroll
     for (int s = 0; s < QS; s++) {
       float v = kLowest;
 #pragma unroll
       for (int j = 0; j < SUB; j++) v = fmaxf(v, fmaxf(fmaxf(sc[s][j][0], sc[s][j][1]), fmaxf(sc[s][j][2], sc[s][j][3])));
       top[s] = over_row_max(v);
-      grown |= top[s] > 8.f;
+      grown |= begun[s] ? top[s] * unit > m[s] + 8.f : top[s] > kLowest;
     }
     if (__any(grown)) {
 #pragma unroll
       for (int s = 0; s < QS; s++) {
-        // (the first tile's maximum may lie anywhere, if it has one)
-        const float up = t == t0 ? (top[s] > kLowest ? top[s] : 0.f) : fmaxf(top[s], 0.f), by = t == t0 ? 0.f : __builtin_amdgcn_exp2f(-up);
-        m[s] += up, l[s] *= by;
+        const bool first = !begun[s] && top[s] > kLowest;
+        const float to = first || (begun[s] && top[s] * unit > m[s]) ? top[s] * unit : m[s], by = first ? 0.f : __builtin_amdgcn_exp2f(m[s] - to);
+        m[s] = to, l[s] *= by, begun[s] |= first;
 #pragma unroll
         for (int f = 0; f < Tile::NF; f++) acc[s][f] *= by;
-#pragma unroll
-        for (int j = 0; j < SUB; j++) sc[s][j] -= up;
       }
     }
 #pragma unroll
@@ -565,7 +578,7 @@ __device__ __forceinline__ void attention_fwd_head(const AttnArgs &a, const Attn
 #pragma unroll
       for (int s = 0; s < QS; s++) {
 #pragma unroll
-        for (int i = 0; i < 4; i++) p0[s][i] = __builtin_amdgcn_exp2f(sc[s][j][i]), p1[s][i] = __builtin_amdgcn_exp2f(sc[s][j + 1][i]);
+        for (int i = 0; i < 4; i++) p0[s][i] = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[s][j][i], unit, -m[s])), p1[s][i] = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[s][j + 1][i], unit, -m[s]));
         const f32x4 both = p0[s] + p1[s];
         l[s] += (both[0] + both[1]) + (both[2] + both[3]);
       }
