@@ -15,7 +15,7 @@ def attention(q, k, v, points=None, slopes=None, key_points=None, lengths=None, 
 
     Heads h of q stand on heads h / (heads / kv_heads) of k and v.  dim is at most 128; a head's channels are contiguous, other strides
     as they come.  points and key_points (rows of q and of k, three coordinates each; key_points None: points) and slopes (heads) are float32.
-    scale None: dim ** -0.5.  One query a sample (n_q = 1) reads a sample out.
+    Points are finite numbers below 1e38; a distance above 1.8e19, whose square float32 does not hold, counts as that.  scale None: dim ** -0.5.  One query a sample (n_q = 1) reads a sample out.
 
     Scores, softmax and sums are float32; 16-bit types round its values to their own for the second product, and results once.  Differentiable
     in q, k, v, points, slopes and key_points (points in one place have no direction and add nothing to each other's gradient), twice by torch's

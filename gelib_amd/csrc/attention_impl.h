@@ -391,7 +391,8 @@ struct Distance {
     if constexpr (BIAS != kBiasNone) {
 #pragma unroll
       for (int k = 0; k < 3; k++) d[k] = x[k] - p[k][i];
-      const float sq = d[0] * d[0] + d[1] * d[1] + d[2] * d[2];
+      // (a square beyond float32 counts as its largest: infinity would meet slopes, shares and inverses of zero.  NaN stays NaN)
+      const float sq = __builtin_elementwise_minimum(d[0] * d[0] + d[1] * d[1] + d[2] * d[2], 0x1.fffffep127f);
       if constexpr (BIAS == kBiasGradients) inv = __builtin_amdgcn_rsqf(fmaxf(sq, 1e-37f)), far = sq * inv;   // (in one place: d and far are zero)
       else far = __builtin_amdgcn_sqrtf(sq);
     }

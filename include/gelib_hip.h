@@ -348,7 +348,8 @@ uint64_t gelib_hip_embedding_workspace_bytes(int dtype, int64_t ntokens, int64_t
  * exist, the others are not read and get zeros.  packed 1: queries and keys rows in all (sample strides are not used), document d
  * is rows marks[d] to marks[d + 1] of either side (documents + 1 ascending int32 each); rows in no document get zeros.  Marks are held to
  * what there is.  Heads of q, k and v that do not lie at multiples of 16 bytes, or are no multiple of them long, are copied to ones that do.
- * points, key_points (rows, 3) and slopes (heads) float32, or all three NULL: no distances.  dim is at most 128. */
+ * points, key_points (rows, 3; finite, below 1e38) and slopes (heads) float32, or all three NULL: no distances.  A distance above 1.8e19, whose square
+ * float32 does not hold, counts as that.  dim is at most 128. */
 typedef struct {
   const void *q, *k, *v;
   const float *points, *key_points, *slopes;

@@ -94,6 +94,34 @@ def test_finite_scores_without_a_share(gelib, dim, nq, nk, first, dtype):
 
 
 @pytest.mark.parametrize("dtype", TYPES, ids=str)
+@pytest.mark.parametrize("first", [3, 128, 1500])
+@pytest.mark.parametrize("nq,nk", OTHERS, ids=lambda v: str(v))
+@pytest.mark.parametrize("heads,kv", [(4, 2), (3, 3)])
+def test_distances_whose_square_overflows(gelib, heads, kv, nq, nk, first, dtype):
+    """Points 1e20 away and more are keys without a share, in gradients as in values; those of points in the neighbourhood are what they are without them."""
+    for where in (1e20, -3e37):
+        far_points(gelib, 32, nq, nk, first, dtype, where, heads, kv)
+
+
+@pytest.mark.parametrize("dtype", TYPES, ids=str)
+def test_a_head_without_slope_beside_far_points(gelib, dtype):
+    """A slope of zero: the distance does not count, whatever it is."""
+    gen = torch.Generator(device="cuda").manual_seed(1)
+    for nq, nk in ((5, 70), (130, 200)):
+        q, k, v, g = (torch.randn(n, 2, 32, device="cuda", generator=gen).to(dtype) for n in (nq, nk, nk, nq))
+        x, xk, slopes = torch.randn(nq, 3, device="cuda", generator=gen), torch.randn(nk, 3, device="cuda", generator=gen), torch.zeros(2, device="cuda")
+        xk[::3, 2] = 1e30
+        leaves = [t.requires_grad_() for t in (q, k, v, x, xk)]
+        y = gelib.attention(q[None], k[None], v[None], x[None], slopes, key_points=xk[None])[0]
+        got = dict(zip(("gq", "gk", "gv", "gx", "gxk"), torch.autograd.grad(y, leaves, g)), y=y.detach())
+        with torch.no_grad():
+            want = document(q.double(), k.double(), v.double(), None, None, None, g.double(), 32 ** -0.5, dtype)
+        assert (got.pop("gx") == 0).all() and (got.pop("gxk") == 0).all()
+        for name, t in got.items():
+            check(t, *want[name], name)
+
+
+@pytest.mark.parametrize("dtype", TYPES, ids=str)
 @pytest.mark.parametrize("apart", [3e3, 1e5])
 def test_maximum_grows_by_much(gelib, apart, dtype):
     """The first keys have weights until nearer ones come, a step at a time: no digit of the nearer ones' scores is lost."""
