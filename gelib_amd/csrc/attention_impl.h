@@ -839,6 +839,7 @@ __device__ __forceinline__ void attention_keys_head(const AttnArgs &a, const Att
   const int rows = doc.tile * BM < doc.kn ? (int)rows_in(a, doc.qn) : 0;
   int t0, t1;
   piece_of((int)(((long long)rows + BN - 1) / BN), w.split, a.splits, t0, t1);
+  const int whole = (a.blocked ? doc.qn & ~15 : doc.qn) * a.G;   // rows before the first that does not exist
   const T *q0 = (const T *)a.q + doc.sample * a.qs + doc.q0 * a.qp + (long long)w.kv * a.G * a.qh;
   const long long o0 = doc.out_q * a.H + w.kv * a.G;
   auto copy = [&](int t, Buffer &b) __attribute__((always_inline)) {
@@ -885,6 +886,15 @@ __device__ __forceinline__ void attention_keys_head(const AttnArgs &a, const Att
 #pragma unroll
             for (int e = 0; e < 3; e++) point[u][e] = *(const f32x4 *)&b.r[3 + e][(j0 + u) * 16 + q4];
         }
+      }
+      if (j0 * 16 + 32 > whole - t * BN) {   // (zeros of rows that do not exist, times a key or value of infinity)
+#pragma unroll
+        for (int u = 0; u < 2; u++)
+#pragma unroll
+          for (int i = 0; i < 4; i++)
+            if (nlse[u][i] == -INFINITY)
+#pragma unroll
+              for (int s = 0; s < QS; s++) p[u][s][i] = 0.f, ds[u][s][i] = 0.f;
       }
       float part[QS][3] = {};
 #pragma unroll
