@@ -235,8 +235,8 @@ variable_list attention_bwd(const Attention &given, const at::Tensor &y, const a
 at::Tensor attention_from_torch(const variable_list &t, const Attention &a) {
   AsWritten types;
   auto batched = [&](const at::Tensor &x) { return a.packed && x.defined() ? x.unsqueeze(0) : x; };
-  const at::Tensor q = batched(t[0]).to(at::kFloat), points = batched(t[3]), key_points = t[5].defined() ? batched(t[5]) : points;
-  at::Tensor k = batched(t[1]).to(at::kFloat), v = batched(t[2]).to(at::kFloat);
+  at::Tensor q = batched(t[0]).to(at::kFloat), k = batched(t[1]).to(at::kFloat), v = batched(t[2]).to(at::kFloat);
+  at::Tensor points = batched(t[3]), key_points = t[5].defined() ? batched(t[5]) : points;
   const int64_t n = q.size(0), nq = q.size(1), nk = k.size(1), heads = q.size(2), kv = k.size(2), dim = q.size(3), G = heads / kv;
   // which queries see which keys
   at::Tensor sees, there_q, there_k;   // (n, nq, nk), (n, nq), (n, nk); undefined: all
@@ -253,10 +253,12 @@ at::Tensor attention_from_torch(const variable_list &t, const Attention &a) {
     if (a.q_marks.defined()) there_q = at::arange(nq, a.q_marks.options()).unsqueeze(0).lt(a.q_marks.unsqueeze(1));
     if (a.k_marks.defined()) there_k = at::arange(nk, a.k_marks.options()).unsqueeze(0).lt(a.k_marks.unsqueeze(1)), sees = there_k.unsqueeze(1).expand({n, nq, nk});
   }
-  if (there_k.defined()) {   // (what is not there may be no number)
-    const at::Tensor gone = there_k.logical_not().view({there_k.size(0), nk, 1, 1});
-    k = k.masked_fill(gone, 0), v = v.masked_fill(gone, 0);
-  }
+  // (what is not there may be no number, which times zero would still be none.  A row of shared points may be there on one side only)
+  auto without = [&](at::Tensor &x, const at::Tensor &there) {
+    if (x.defined() && there.defined()) x = x.masked_fill((x.dim() == 4 ? there.unsqueeze(2).unsqueeze(3) : there.unsqueeze(2)).logical_not(), 0);
+  };
+  without(q, there_q), without(points, there_q);
+  without(k, there_k), without(v, there_k), without(key_points, there_k);
   const at::Tensor kt = k.permute({0, 2, 3, 1}), vt = v.permute({0, 2, 1, 3});
   const at::Tensor rows = q.reshape({n, nq, kv, G, dim}).permute({0, 2, 3, 1, 4}).reshape({n, kv, G * nq, dim});
   at::Tensor s = at::matmul(rows, kt).reshape({n, kv, G, nq, nk}) * a.scale;
@@ -371,10 +373,13 @@ variable_list loss_bwd(const at::Tensor &g_, const at::Tensor &lse, const at::Te
 
 at::Tensor loss_from_torch(const at::Tensor &x, const at::Tensor &w, const at::Tensor &b, const at::Tensor &targets) {
   AsWritten types;
-  at::Tensor z = at::matmul(x.to(at::kFloat), w.to(at::kFloat));
+  // (a row left out may hold anything, and so may what it meets in w: zero before the product and after)
+  const at::Tensor out = targets.lt(0), out_row = out.unsqueeze(-1);
+  at::Tensor z = at::matmul(x.to(at::kFloat).masked_fill(out_row, 0), w.to(at::kFloat));
   if (b.defined()) z = z + b.to(at::kFloat);
+  z = z.masked_fill(out_row, 0);
   const at::Tensor of = at::gather(z, -1, targets.clamp(0, w.size(1) - 1).unsqueeze(-1)).squeeze(-1);
-  return (at::logsumexp(z, -1) - of).masked_fill(targets.lt(0), 0).masked_fill(targets.ge(w.size(1)), std::numeric_limits<double>::quiet_NaN());
+  return (at::logsumexp(z, -1) - of).masked_fill(out, 0).masked_fill(targets.ge(w.size(1)), std::numeric_limits<double>::quiet_NaN());
 }
 
 struct LossFn : torch::autograd::Function<LossFn> {
