@@ -385,12 +385,13 @@ __global__ void __launch_bounds__(64 * (BM / WM) * (BN / WN)) gemm_kernel(const 
         if (t >= 0 && t >= nl && (GN == 1 ? (t - nl) % 16 < 4 && t - nl < 16 * FN : t - nl < 4 * GN)) a.picked[m0 + r] = own;
         top = fmaxf(top, __shfl_xor(top, 16));
         top = fmaxf(top, __shfl_xor(top, 32));
-        const float from = (top == -INFINITY ? 0.f : top) * 1.44269504088896341f;
+        const float from = top == -INFINITY ? 0.f : top;
 #pragma unroll
         for (int k = 0; k < FN; k++)
 #pragma unroll
           for (int e = 0; e < 4; e++) {
-            const float p = __builtin_amdgcn_exp2f(__builtin_fmaf(logit(i, k, e), 1.44269504088896341f, -from));
+            // (the difference first: a product with log2(e) that is rounded before it loses what the logits differ by)
+            const float p = __builtin_amdgcn_exp2f((logit(i, k, e) - from) * 1.44269504088896341f);
             sum += whole || nl + k * apart + e < left ? p : 0.f;
           }
         sum += __shfl_xor(sum, 16);
@@ -420,7 +421,7 @@ __global__ void __launch_bounds__(64 * (BM / WM) * (BN / WN)) gemm_kernel(const 
         if (m < a.M) {
           const long long class_ = a.targets[m];
           const int t = column_of(class_);
-          const float from = a.lse[m] * 1.44269504088896341f, g = class_ < a.N_all ? a.weight[m] * norm : __builtin_nanf("");
+          const float from = a.lse[m], g = class_ < a.N_all ? a.weight[m] * norm : __builtin_nanf("");
           T *to = (T *)a.c + m * a.ldc + n0 + nl;
 #pragma unroll
           for (int k = 0; k < FN; k++) {
@@ -428,7 +429,7 @@ __global__ void __launch_bounds__(64 * (BM / WM) * (BN / WN)) gemm_kernel(const 
 #pragma unroll
             for (int e = 0; e < 4; e++) {
               const int n = nl + k * apart + e;
-              const float p = __builtin_amdgcn_exp2f(__builtin_fmaf(logit(i, k, e), 1.44269504088896341f, -from)) - (n == t ? 1.f : 0.f);
+              const float p = __builtin_amdgcn_exp2f((logit(i, k, e) - from) * 1.44269504088896341f) - (n == t ? 1.f : 0.f);
               const float gz = n < left && class_ >= 0 ? p * g : 0.f;
               column[k][e] += gz;
               v[e] = from_f<T>(gz);
