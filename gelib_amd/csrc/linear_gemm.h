@@ -171,6 +171,9 @@ struct Stage {
   }
 };
 
+// What a row's exponentials are formed less: its largest logit, where infinity less infinity is not what that would come to
+__device__ __forceinline__ float finite_or_zero(float top) { return fabsf(top) == INFINITY ? 0.f : top; }
+
 // `count` vectors of four neighbouring results, `apart` columns from one to the next.  All of y is written before all of the
 // slopes: a line of either is then whole in the L2 when it leaves (written in turn, 16384 x 8192 results and slopes were 1.01 GB of
 // writes instead of 0.54).
@@ -385,7 +388,7 @@ __global__ void __launch_bounds__(64 * (BM / WM) * (BN / WN)) gemm_kernel(const 
         if (t >= 0 && t >= nl && (GN == 1 ? (t - nl) % 16 < 4 && t - nl < 16 * FN : t - nl < 4 * GN)) a.picked[m0 + r] = own;
         top = fmaxf(top, __shfl_xor(top, 16));
         top = fmaxf(top, __shfl_xor(top, 32));
-        const float from = top == -INFINITY ? 0.f : top;
+        const float from = finite_or_zero(top);
 #pragma unroll
         for (int k = 0; k < FN; k++)
 #pragma unroll
@@ -406,7 +409,7 @@ __global__ void __launch_bounds__(64 * (BM / WM) * (BN / WN)) gemm_kernel(const 
 #pragma unroll
         for (int k = 1; k < BN / WN; k++) {
           const float2 o = tops[k][r];
-          const float top = fmaxf(v.x, o.x), from = top == -INFINITY ? 0.f : top;
+          const float top = fmaxf(v.x, o.x), from = finite_or_zero(top);
           v = make_float2(top, v.y * __builtin_amdgcn_exp2f((v.x - from) * 1.44269504088896341f) + o.y * __builtin_amdgcn_exp2f((o.x - from) * 1.44269504088896341f));
         }
         a.tops[(m0 + r) * a.ntiles + n0 / BN] = v;

@@ -29,13 +29,13 @@ __global__ void __launch_bounds__(256) loss_join_kernel(float *loss, float *lse,
   if (row < rows)
     for (int k = lane; k < ntiles; k += lanes) {
       const float2 v = tops[row * ntiles + k];
-      const float to = fmaxf(top, v.x), from = to == -INFINITY ? 0.f : to;
+      const float to = fmaxf(top, v.x), from = finite_or_zero(to);
       sum = sum * __builtin_amdgcn_exp2f((top - from) * 1.44269504088896341f) + v.y * __builtin_amdgcn_exp2f((v.x - from) * 1.44269504088896341f);
       top = to;
     }
   for (int d = 1; d < lanes; d *= 2) {
     const float otop = __shfl_xor(top, d), osum = __shfl_xor(sum, d);
-    const float to = fmaxf(top, otop), from = to == -INFINITY ? 0.f : to;
+    const float to = fmaxf(top, otop), from = finite_or_zero(to);
     sum = sum * __builtin_amdgcn_exp2f((top - from) * 1.44269504088896341f) + osum * __builtin_amdgcn_exp2f((otop - from) * 1.44269504088896341f);
     top = to;
   }
@@ -106,7 +106,7 @@ void zero(void *to, long long n, hipStream_t s) {
 // are few), and the loss is taken of their sum (logits_plan).
 
 __device__ __forceinline__ void sum_exp(float &top, float &sum, float otop, float osum) {
-  const float to = fmaxf(top, otop), from = to == -INFINITY ? 0.f : to;
+  const float to = fmaxf(top, otop), from = finite_or_zero(to);
   sum = sum * __builtin_amdgcn_exp2f((top - from) * 1.44269504088896341f) + osum * __builtin_amdgcn_exp2f((otop - from) * 1.44269504088896341f);
   top = to;
 }

@@ -55,3 +55,26 @@ def test_logits_far_from_zero(gelib, size):
         tol = 2.0 ** -8 / 20 + (n + 16) * u
         assert ((loss.double() - math.log(n)).abs() <= tol).all(), B
         assert ((gb[1:].double() * n / m - 1).abs() <= tol + (m + 16) * u).all(), B
+
+
+@pytest.mark.parametrize("size", SIZES, ids=lambda s: "x".join(map(str, s)))
+def test_infinite_logits(gelib, size):
+    """log of a sum with an infinite term is infinite: so is the loss of the other classes, and the loss of that class is none (infinity less infinity).
+    -infinity is a class without a share; where all are, there is no loss to speak of (NaN), in that row only."""
+    m, k, n = size
+    gen = torch.Generator(device="cuda").manual_seed(m)
+    x, w = torch.randn(m, k, device="cuda", generator=gen), torch.randn(k, n, device="cuda", generator=gen) / k ** 0.5
+    targets = torch.arange(m, device="cuda") % n
+    for at in (0, n // 2, n - 1):
+        b = torch.randn(n, device="cuda", generator=gen)
+        b[at] = float("inf")
+        loss = gelib.linear_cross_entropy(x, w, targets, b)
+        assert torch.isnan(loss[targets == at]).all() and (loss[targets != at] == float("inf")).all()
+        b[at] = float("-inf")
+        loss = gelib.linear_cross_entropy(x, w, targets, b)
+        keep = torch.arange(n, device="cuda") != at
+        other = gelib.linear_cross_entropy(x, w[:, keep].contiguous(), (targets - (targets > at).long()).clamp(max=n - 2), b[keep])
+        seen = targets != at
+        assert (loss[~seen] == float("inf")).all() and torch.allclose(loss[seen], other[seen], rtol=1e-5, atol=1e-5)
+    loss = gelib.linear_cross_entropy(x, w, targets, torch.full((n,), float("-inf"), device="cuda"))
+    assert torch.isnan(loss).all()
