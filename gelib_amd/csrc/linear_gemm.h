@@ -36,6 +36,7 @@ struct GemmArgs {
   long long ldc;            // elements between the rows of c
   const float *norm;        // results without an activation times this; null: 1
   int add;                  // part holds sums already: add to them
+  const long long *left_out;   // rows of c whose entry is below zero are zeros, in results without an activation; null: none
   // a layer's classes and their loss (linear_loss.hip), instead of c = act(..) + res
   const long long *targets; // class of every row
   long long n_first, N_all; // the first of these classes, all of them (bias begins with these)
@@ -182,6 +183,7 @@ __device__ __forceinline__ void epilogue(const GemmArgs &a, long long m, long lo
   typedef typename SlopeOf<T>::type D;
   const long long row = m * a.N, row_c = m * a.ldc;
   const float norm = ACT == kActNone && a.norm ? *a.norm : 1.f;
+  const bool out = ACT == kActNone && a.left_out && a.left_out[m] < 0;   // (gradients of zero times a weight that is no number)
   if (a.vec4) {
     if (n0 >= a.N) return;
     T t[COUNT][4];
@@ -203,7 +205,7 @@ __device__ __forceinline__ void epilogue(const GemmArgs &a, long long m, long lo
 #pragma unroll
       for (int i = 0; i < 4; i++) {
         float y, s;
-        act_both<ACT>(ACT == kActNone ? v[k][i] * norm : v[k][i], y, s, a.act == kActRelu);
+        act_both<ACT>(ACT == kActNone ? (out ? 0.f : v[k][i] * norm) : v[k][i], y, s, a.act == kActRelu);
         t[k][i] = from_f<T>(y + to_f(t[k][i]));
         d[k][i] = from_f<D>(s);
       }
@@ -223,7 +225,7 @@ __device__ __forceinline__ void epilogue(const GemmArgs &a, long long m, long lo
       const long long n = n0 + k * apart + i;
       if (n >= a.N) break;
       float y, s;
-      act_both<ACT>(ACT == kActNone ? v[k][i] * norm : v[k][i], y, s, a.act == kActRelu);
+      act_both<ACT>(ACT == kActNone ? (out ? 0.f : v[k][i] * norm) : v[k][i], y, s, a.act == kActRelu);
       ((T *)a.c)[row_c + n] = from_f<T>(y + (a.res ? to_f(((const T *)a.res)[row + n]) : 0.f));
       if (a.slope) ((D *)a.slope)[row + n] = from_f<D>(s);
     }

@@ -72,24 +72,25 @@ __global__ void __launch_bounds__(1024) loss_norm_kernel(float *norm, const floa
   norm[0] = ldexpf(1.f, e), norm[1] = ldexpf(1.f, -e);
 }
 
-// gx from the sums over all pieces (rows of K up to a multiple of 4)
+// gx from the sums over all pieces (rows of K up to a multiple of 4), zeros in rows that are left out
 template <typename T>
-__global__ void __launch_bounds__(256) loss_finish_kernel(T *gx, const float *sums, long long n, int K, const float *norm) {
+__global__ void __launch_bounds__(256) loss_finish_kernel(T *gx, const float *sums, const long long *targets, long long n, int K, const float *norm) {
   const long long stride = (K + 3) & ~3;
   const float by = norm ? *norm : 1.f;
   if (K % 4 == 0 && (uintptr_t)gx % (4 * sizeof(T)) == 0) {   // (as they lie)
     for (long long at = (long long)blockIdx.x * 256 + threadIdx.x; at < n / 4; at += (long long)gridDim.x * 256) {
       const f32x4 v = ((const f32x4 *)sums)[at];
+      const bool out = targets[at / (K / 4)] < 0;
       T t[4];
 #pragma unroll
-      for (int i = 0; i < 4; i++) t[i] = from_f<T>(v[i] * by);
+      for (int i = 0; i < 4; i++) t[i] = from_f<T>(out ? 0.f : v[i] * by);
       __builtin_memcpy(__builtin_assume_aligned(gx + at * 4, 4 * sizeof(T)), t, sizeof(t));
     }
     return;
   }
   for (long long at = (long long)blockIdx.x * 256 + threadIdx.x; at < n; at += (long long)gridDim.x * 256) {
     const long long row = at / K;
-    gx[at] = from_f<T>(sums[row * stride + (at - row * K)] * by);
+    gx[at] = from_f<T>(targets[row] < 0 ? 0.f : sums[row * stride + (at - row * K)] * by);
   }
 }
 template <typename T>
@@ -458,7 +459,7 @@ int bwd(int dtype, const LossArgs &l, hipStream_t s) {
     }
     if (gx) {
       GemmArgs p = {};
-      p.a = gz, p.lda = at.ldz, p.b = w + n0, p.ldb = ldw, p.c = l.gx, p.M = l.rows, p.N = l.K, p.K = n, p.norm = back;
+      p.a = gz, p.lda = at.ldz, p.b = w + n0, p.ldb = ldw, p.c = l.gx, p.M = l.rows, p.N = l.K, p.K = n, p.norm = back, p.left_out = l.targets;
       if (at.pieces == 1) {
         if (int rc = product<T>(kFormGW, dtype, p, part, s)) return rc;
       } else {
@@ -482,7 +483,7 @@ int bwd(int dtype, const LossArgs &l, hipStream_t s) {
   }
   if (gx && at.pieces > 1) {
     const long long all = l.rows * l.K;
-    hipLaunchKernelGGL(loss_finish_kernel<T>, dim3((unsigned)std::min((all + 255) / 256, 1LL << 20)), dim3(256), 0, s, (T *)l.gx, (const float *)part, all, l.K, back);
+    hipLaunchKernelGGL(loss_finish_kernel<T>, dim3((unsigned)std::min((all + 255) / 256, 1LL << 20)), dim3(256), 0, s, (T *)l.gx, (const float *)part, l.targets, all, l.K, back);
   }
   return launched();
 }

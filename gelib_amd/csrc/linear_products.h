@@ -105,6 +105,7 @@ int product(GemmForm form, int dtype, GemmArgs a, float *part, hipStream_t s) {
     b.mtiles = (unsigned)((b.M + BM - 1) / BM);
     b.a = (const T *)a.a + m * (a_kin ? a.lda : 1);
     b.c = (T *)a.c + m * a.ldc;
+    if (a.left_out) b.left_out = a.left_out + m;
     if (a.res) b.res = (const T *)a.res + m * a.N;
     if (a.slope) b.slope = (T *)a.slope + m * a.N;   // (as wide as T)
     if (int rc = launch_gemm<T>(form, p.tile, b, s)) return rc;

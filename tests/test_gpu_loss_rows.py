@@ -21,6 +21,32 @@ def gelib():
     return gelib_amd
 
 
+def left_out(gelib, m, k, n, dtype):
+    gen = torch.Generator(device="cuda").manual_seed(m + k)
+    x, w = torch.randn(m, k, device="cuda", generator=gen).to(dtype), (torch.randn(k, n, device="cuda", generator=gen) / k ** 0.5).to(dtype)
+    w[k // 2, n // 2], w[0, n - 1] = float("inf"), float("nan")
+    targets = torch.randint(0, n, (m,), device="cuda", generator=gen)
+    out = torch.rand(m, device="cuda", generator=gen) < 0.5
+    out[0], out[-1] = True, True
+    targets[out] = -1
+    x.requires_grad_(), w.requires_grad_()
+    loss = gelib.linear_cross_entropy(x, w, targets)
+    gx, = torch.autograd.grad(loss, x, torch.ones_like(loss))
+    assert (loss[out] == 0).all() and (gx[out] == 0).all() and torch.isnan(gx[~out]).all()
+
+
+@pytest.mark.parametrize("dtype", TYPES, ids=str)
+@pytest.mark.parametrize("size", SIZES, ids=lambda s: "x".join(map(str, s)))
+def test_rows_left_out_beside_infinite_weights(gelib, size, dtype):
+    left_out(gelib, *size, dtype)
+
+
+@pytest.mark.parametrize("dtype", TYPES, ids=str)
+def test_rows_left_out_of_more_classes_than_one_piece(gelib, dtype):
+    for k in (40, 41):
+        left_out(gelib, 4099 if dtype == torch.float32 else 8200, k, 20003, dtype)
+
+
 FAR = [(9, 8, 25), (300, 64, 124), (300, 5000, 124), (1500, 16, 1026)]   # (classes whose log is nearly a multiple of 2^-8)
 
 
