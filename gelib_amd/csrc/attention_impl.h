@@ -80,6 +80,22 @@ __device__ __forceinline__ f32x4 attn_mfma(s16x8 a, s16x8 b, f32x4 c, half_t) {
 
 constexpr float kLowest = -3.0e38f;
 
+// float16's least normal value is 2^-14, and what the second products take as float16 values may lie anywhere below: weights, one over the number
+// of keys, and their scores' gradients, which are as small or large as the loss's.  Powers of two bring them into its range, and the float32
+// results are scaled back.
+//   Forward: weights less the maximum stand at 2^7, and at 2^15 before the maximum is moved (kHalfTop).
+//   Backward: weights, at most one, stand at 2^12 (kHalfUp: 2^4 to spare for scores so large that exp(s - lse) is off by that).
+//   ds: each own row has a power of two of its own, which is chosen when its first ds come so that the largest is 2^11 to 2^12, and again when
+//   one is beyond 2^15 (Lift).
+template <typename T>
+constexpr bool kIsHalf = std::is_same<T, half_t>::value;
+template <typename T>
+constexpr float kHalfTop = kIsHalf<T> ? 7.f : 0.f;
+template <typename T>
+constexpr float kHalfUp = kIsHalf<T> ? 12.f : 0.f;       // log2
+template <typename T>
+constexpr float kHalfDown = kIsHalf<T> ? 0x1p-12f : 1.f;
+
 // A document as a block sees it: where its rows begin in the strided operands and in packed results, how many exist, and how many there
 // are to write (rows that do not exist get zeros).
 struct AttnDoc {
@@ -287,6 +303,60 @@ __device__ __forceinline__ float over_row_sum(float v) {
   return v + __shfl_xor(v, 32);
 }
 
+// The kernels that have no register to spare for Lift: float16, 64 values, gradients of points, four waves
+template <typename T, int DP, int BIAS, int WAVES>
+constexpr bool kFrugal = kIsHalf<T> && DP == 64 && BIAS == kBiasGradients && WAVES > 1;
+
+// Powers of two of the gradients of scores (float16 only)
+template <typename T, int QS>
+struct Lift {
+  float by[QS];   // zero: not chosen yet
+  __device__ __forceinline__ Lift() {
+#pragma unroll
+    for (int s = 0; s < QS; s++) by[s] = 0.f;
+  }
+  // d[u][s], of 32 streamed rows: times their powers of two, which acc, the sums so far, follow
+  template <int SETS, int NF>
+  __device__ __forceinline__ void apply(f32x4 (*d)[SETS], f32x4 (*acc)[NF]) {
+    if constexpr (!kIsHalf<T>) return;
+#pragma unroll
+    for (int s = 0; s < QS; s++) {
+      float top = 0.f;
+#pragma unroll
+      for (int u = 0; u < 2; u++)
+#pragma unroll
+        for (int i = 0; i < 4; i++) top = fmaxf(top, fabsf(d[u][s][i]));
+      // (a lane's own values tell whether there is anything to do: the row's other lanes are asked then only)
+      if (__any(by[s] == 0.f ? top > 0.f : top * by[s] > 0x1p15f)) {
+        top = over_row_max(top);
+        const bool grown = by[s] == 0.f ? top > 0.f : top * by[s] > 0x1p15f;
+        // (frexp's exponent of a value from 1/2 to 1 is zero, that of 2^n is n + 1)
+        const int to = max(-120, min(120, 12 - __builtin_amdgcn_frexp_expf(top))), more = grown ? to - (__builtin_amdgcn_frexp_expf(by[s]) - 1) : 0;
+#pragma unroll
+        for (int f = 0; f < NF; f++)
+#pragma unroll
+          for (int i = 0; i < 4; i++) acc[s][f][i] = ldexpf(acc[s][f][i], more);   // (zeros if nothing was chosen yet)
+        by[s] = grown ? ldexpf(1.f, to) : by[s];
+      }
+#pragma unroll
+      for (int u = 0; u < 2; u++) d[u][s] *= by[s];
+    }
+  }
+  // the sums as they are, but for a factor
+  template <int NF>
+  __device__ __forceinline__ void down(f32x4 (*acc)[NF], float besides) const {
+    if constexpr (!kIsHalf<T>) return;
+#pragma unroll
+    for (int s = 0; s < QS; s++) {
+      const int less = by[s] == 0.f ? 0 : 1 - __builtin_amdgcn_frexp_expf(by[s]);
+#pragma unroll
+      for (int f = 0; f < NF; f++)
+#pragma unroll
+        for (int i = 0; i < 4; i++) acc[s][f][i] = ldexpf(acc[s][f][i], less) * besides;
+    }
+  }
+};
+
 typedef __attribute__((address_space(3))) char *AttnLds;
 
 // 16 (or 4) bytes of every lane to LDS, lane after lane from `to` (the same for the whole wave) on.  Written out because the compiler, which
@@ -313,12 +383,15 @@ __device__ __forceinline__ void arrive() {
 
 // A tile of the streamed side straight into LDS, as far as whole pairs of 16 rows exist: row_of(row) is a row's address, null where it does
 // not exist (from `left` on none does).
-template <typename T, int DP, int BN, int THREADS, typename F>
+// FRUGAL: rows and places are formed for each tile again, which frees registers.
+template <typename T, int DP, int BN, int THREADS, bool FRUGAL, typename F>
 __device__ __forceinline__ void copy_tile(char *lds, F row_of, int left, int dim) {
   typedef AttnTile<T, DP> Tile;
   constexpr int NL = BN * Tile::PPR / THREADS, DOWN = THREADS / Tile::PPR;
   static_assert(BN * Tile::PPR % THREADS == 0 && THREADS % Tile::PPR == 0, "");
-  const int row0 = threadIdx.x / Tile::PPR, slot = threadIdx.x % Tile::PPR, wave0 = threadIdx.x & ~63;
+  int id = threadIdx.x;
+  if constexpr (FRUGAL) asm volatile("" : "+v"(id));   // (as far as the compiler knows another number each time)
+  const int row0 = id / Tile::PPR, slot = id % Tile::PPR, wave0 = threadIdx.x & ~63;
 #pragma unroll 4
   for (int u = 0; u < NL; u++) {
     if (u * DOWN >= ((left + 31) & ~31)) break;
@@ -461,8 +534,8 @@ struct KeyTiles {
   __device__ __forceinline__ void copy(int t, Buffer &b) const {
     const int left = rows - t * BN;
     const T *kt = k + (long long)t * BN * kp, *vt = v + (long long)t * BN * vp;
-    copy_tile<T, DP, BN, THREADS>(b.k, [&](int row) { return kt + (long long)row * kp; }, left, dim);
-    copy_tile<T, DP, BN, THREADS>(b.v, [&](int row) { return vt + (long long)row * vp; }, left, dim);
+    copy_tile<T, DP, BN, THREADS, kFrugal<T, DP, BIAS, WAVES>>(b.k, [&](int row) { return kt + (long long)row * kp; }, left, dim);
+    copy_tile<T, DP, BN, THREADS, kFrugal<T, DP, BIAS, WAVES>>(b.v, [&](int row) { return vt + (long long)row * vp; }, left, dim);
     if (BIAS) {
       const float *xt = x + (long long)t * BN * 3;
 #pragma unroll
@@ -488,8 +561,9 @@ __device__ __forceinline__ void attention_fwd_head(const AttnArgs &a, const Attn
   own.load(a, doc, w.kv, row0, live);
 
   // Exponentials are formed less the maximum so far, m (log2), which is that of the first tile with a score above -infinity (begun: a row
-  // has had one).  It moves only when a score is more than 8 above it: values are then at most 2^8 times what they would be (and within
-  // float16), and rescaling is rare.  Scores themselves are kept whole until then: less a maximum far below them they would lose digits.
+  // has had one).  It moves only when a score is more than 8 above it: values are then at most 2^8 times what they would be, and
+  // rescaling is rare.  (float16: m is 7 below the maximum, see kHalfTop.)  Scores themselves are kept whole until then: less a maximum
+  // far below them they would lose digits.
   // Without distances what is kept are products that the scale, which is above zero then, has not met yet (q takes its sign): it and the
   // maximum are one instruction in front of the exponential.  8192 x 8192, 16 heads of 64, bfloat16: 411 us, with scores scaled at once 423, less the
   // maximum from the start 397; with points (8192, 16 heads on 4) an instruction more than that, 540 and 506.
@@ -560,13 +634,13 @@ __device__ __forceinline__ void attention_fwd_head(const AttnArgs &a, const Attn
 #pragma unroll
       for (int j = 0; j < SUB; j++) v = fmaxf(v, fmaxf(fmaxf(sc[s][j][0], sc[s][j][1]), fmaxf(sc[s][j][2], sc[s][j][3])));
       top[s] = over_row_max(v);
-      grown |= begun[s] ? top[s] * unit > m[s] + 8.f : top[s] > kLowest;
+      grown |= begun[s] ? top[s] * unit > m[s] + (kHalfTop<T> + 8.f) : top[s] > kLowest;
     }
     if (__any(grown)) {
 #pragma unroll
       for (int s = 0; s < QS; s++) {
         const bool first = !begun[s] && top[s] > kLowest;
-        const float to = first || (begun[s] && top[s] * unit > m[s]) ? top[s] * unit : m[s], by = first ? 0.f : __builtin_amdgcn_exp2f(m[s] - to);
+        const float to = first || (begun[s] && top[s] * unit > m[s] + kHalfTop<T>) ? top[s] * unit - kHalfTop<T> : m[s], by = first ? 0.f : __builtin_amdgcn_exp2f(m[s] - to);
         m[s] = to, l[s] *= by, begun[s] |= first;
 #pragma unroll
         for (int f = 0; f < Tile::NF; f++) acc[s][f] *= by;
@@ -660,8 +734,9 @@ __device__ __forceinline__ void attention_rows_head(const AttnArgs &a, const Att
       for (int e = 0; e < Tile::EP; e++) delta[s] += to_f(gv[e]) * to_f(yv[e]);
     }
     delta[s] = over_row_sum(delta[s]);
-    nlse[s] = own.there[s] ? -a.lse[at] : -INFINITY;
+    nlse[s] = own.there[s] ? kHalfUp<T> - a.lse[at] : -INFINITY;   // (weights times 2^kHalfUp from here on)
   }
+  Lift<T, QS> lift;
   f32x4 acc[SETS][Tile::NF];
   float geo[SETS][4];
 #pragma unroll
@@ -734,20 +809,25 @@ __device__ __forceinline__ void attention_rows_head(const AttnArgs &a, const Att
       if constexpr (MEND)
 #pragma unroll
         for (int s = 0; s < QS; s++) rest[s] += part_rest[s];
+      lift.apply(ds, acc);
       Tile::template transposed<SETS>(acc, b.k, j0 * 16, ds[0], ds[1]);
     }
   });
 
+  lift.down(acc, kHalfDown<T>);
 #pragma unroll
   for (int s = 0; s < QS; s++) {
+    if constexpr (kIsHalf<T>)
+#pragma unroll
+      for (int f = 0; f < Tile::NF; f++) acc[QS + s][f] *= kHalfDown<T>;
     const bool pieces = MEND && a.part_d;   // (what is lacking is known when all pieces are there)
-    const float lacks = MEND ? over_row_sum(rest[s]) : 0.f;
+    const float lacks = MEND ? over_row_sum(rest[s]) * kHalfDown<T> : 0.f;
     const long long at = own.out(a, doc, w.kv, row0, s), in_part = w.split * a.rows_q * a.H + at;
     if (BIAS == kBiasGradients) {
 #pragma unroll
       for (int e = 0; e < 4; e++) {
-        geo[s][e] = over_row_sum(geo[s][e]) * (e < 3 ? 0.69314718055994531f : -1.f);
-        if (MEND) geo[QS * MEND + s][e] = over_row_sum(geo[QS * MEND + s][e]) * (e < 3 ? own.slope[s] * 0.69314718055994531f : -1.f);
+        geo[s][e] = over_row_sum(geo[s][e]) * (kHalfDown<T> * (e < 3 ? 0.69314718055994531f : -1.f));
+        if (MEND) geo[QS * MEND + s][e] = over_row_sum(geo[QS * MEND + s][e]) * (kHalfDown<T> * (e < 3 ? own.slope[s] * 0.69314718055994531f : -1.f));
         if (MEND && !pieces) geo[s][e] -= lacks * geo[QS * MEND + s][e];
       }
       if (own.mine[s] && q4 == 0) {
@@ -811,13 +891,11 @@ __device__ __forceinline__ void attention_keys_head(const AttnArgs &a, const Att
 
   typename Tile::Frag fk[QS][Tile::KS], fv[QS][Tile::KS];
   float x[QS][3];
-  long long out[QS];
   bool mine[QS], exists[QS];
 #pragma unroll
   for (int s = 0; s < QS; s++) {
     const int key = key0 + 16 * s + c;
     exists[s] = key < doc.kn, mine[s] = key < doc.own_all;
-    out[s] = (doc.out_k + key) * a.KV + w.kv;
     const T *rk = (const T *)a.k + doc.sample * a.ks + (doc.k0 + key) * a.kp + (long long)w.kv * a.kh;
     const T *rv = (const T *)a.v + doc.sample * a.vs + (doc.k0 + key) * a.vp + (long long)w.kv * a.vh;
 #pragma unroll
@@ -826,6 +904,7 @@ __device__ __forceinline__ void attention_keys_head(const AttnArgs &a, const Att
 #pragma unroll
       for (int e = 0; e < 3; e++) x[s][e] = exists[s] ? a.xk[(doc.out_k + key) * 3 + e] : 0.f;
   }
+  Lift<T, QS> lift;
   f32x4 ak[QS][Tile::NF], av[QS][Tile::NF];
   float geo[QS][3];
 #pragma unroll
@@ -844,8 +923,8 @@ __device__ __forceinline__ void attention_keys_head(const AttnArgs &a, const Att
   const long long o0 = doc.out_q * a.H + w.kv * a.G;
   auto copy = [&](int t, Buffer &b) __attribute__((always_inline)) {
     const int left = rows - t * BN;
-    copy_tile<T, DP, BN, THREADS>(b.q, [&](int row) { const RowAt r = row_at(a, t * BN + row); return r.pos < doc.qn ? q0 + (long long)r.pos * a.qp + (long long)r.head * a.qh : nullptr; }, left, a.dim);
-    copy_tile<T, DP, BN, THREADS>(b.g, [&](int row) { const RowAt r = row_at(a, t * BN + row); return r.pos < doc.qn ? (const T *)a.gy + (o0 + (long long)r.pos * a.H + r.head) * a.ldy : nullptr; }, left, a.dim);
+    copy_tile<T, DP, BN, THREADS, kFrugal<T, DP, BIAS, WAVES>>(b.q, [&](int row) { const RowAt r = row_at(a, t * BN + row); return r.pos < doc.qn ? q0 + (long long)r.pos * a.qp + (long long)r.head * a.qh : nullptr; }, left, a.dim);
+    copy_tile<T, DP, BN, THREADS, kFrugal<T, DP, BIAS, WAVES>>(b.g, [&](int row) { const RowAt r = row_at(a, t * BN + row); return r.pos < doc.qn ? (const T *)a.gy + (o0 + (long long)r.pos * a.H + r.head) * a.ldy : nullptr; }, left, a.dim);
 #pragma unroll
     for (int e = 0; e < ROW; e++)
       if (WAVES == 1 || (int)threadIdx.x / 64 == e % 4)
@@ -879,7 +958,7 @@ __device__ __forceinline__ void attention_keys_head(const AttnArgs &a, const Att
       f32x4 nlse[2], slope[2], point[SHARE ? 1 : 2][3];
 #pragma unroll
       for (int u = 0; u < 2; u++) {
-        nlse[u] = -*(const f32x4 *)&b.r[0][(j0 + u) * 16 + q4];
+        nlse[u] = kHalfUp<T> - *(const f32x4 *)&b.r[0][(j0 + u) * 16 + q4];   // (weights times 2^kHalfUp from here on)
         if constexpr (BIAS != kBiasNone) {
           slope[u] = *(const f32x4 *)&b.r[2][(j0 + u) * 16 + q4];
           if (!SHARE || u == 0)
@@ -921,14 +1000,19 @@ __device__ __forceinline__ void attention_keys_head(const AttnArgs &a, const Att
         for (int s = 0; s < QS; s++)
 #pragma unroll
           for (int e = 0; e < 3; e++) geo[s][e] -= part[s][e];
+      lift.apply(ds, ak);
       Tile::template transposed<QS>(av, b.g, j0 * 16, p[0], p[1]);
       Tile::template transposed<QS>(ak, b.q, j0 * 16, ds[0], ds[1]);
     }
   });
 
+  lift.down(ak, kHalfDown<T>);
 #pragma unroll
   for (int s = 0; s < QS; s++) {
-    const long long at = w.split * a.rows_k * a.KV + out[s];
+    const long long out = (doc.out_k + key0 + 16 * s + c) * a.KV + w.kv, at = w.split * a.rows_k * a.KV + out;
+    if constexpr (kIsHalf<T>)
+#pragma unroll
+      for (int f = 0; f < Tile::NF; f++) av[s][f] *= kHalfDown<T>;
     if (!exists[s]) {   // (its score is no -infinity above: its values and gradients are zeros here)
 #pragma unroll
       for (int f = 0; f < Tile::NF; f++) ak[s][f] = f32x4{0.f, 0.f, 0.f, 0.f}, av[s][f] = ak[s][f];
@@ -937,7 +1021,7 @@ __device__ __forceinline__ void attention_keys_head(const AttnArgs &a, const Att
 #pragma unroll
       for (int e = 0; e < 3; e++) {
         const float all = over_row_sum(geo[s][e]);
-        geo[s][e] = exists[s] ? all : 0.f;
+        geo[s][e] = exists[s] ? all * kHalfDown<T> : 0.f;
       }
       if (mine[s] && q4 == 0) a.geo_k[at] = make_float4(geo[s][0], geo[s][1], geo[s][2], 0.f);
     }
@@ -948,11 +1032,11 @@ __device__ __forceinline__ void attention_keys_head(const AttnArgs &a, const Att
       Tile::results(av[s], [&](int d, f32x4 v) { store4<float>(tv, d, a.dim, a.dim % 4 == 0, v); });
     } else {
       if (a.gk) {
-        T *to = (T *)a.gk + out[s] * a.dim;
+        T *to = (T *)a.gk + out * a.dim;
         Tile::results(ak[s], [&](int d, f32x4 v) { store4<T>(to, d, a.dim, a.vec_y, v * a.scale); });
       }
       if (a.gv) {
-        T *to = (T *)a.gv + out[s] * a.dim;
+        T *to = (T *)a.gv + out * a.dim;
         Tile::results(av[s], [&](int d, f32x4 v) { store4<T>(to, d, a.dim, a.vec_y, v); });
       }
     }
