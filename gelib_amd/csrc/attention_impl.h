@@ -306,6 +306,11 @@ __device__ __forceinline__ float over_row_sum(float v) {
 // The kernels that have no register to spare for Lift: float16, 64 values, gradients of points, four waves
 template <typename T, int DP, int BIAS, int WAVES>
 constexpr bool kFrugal = kIsHalf<T> && DP == 64 && BIAS == kBiasGradients && WAVES > 1;
+// They do one thing after the other (what the compiler would begin early takes registers)
+template <bool FRUGAL>
+__device__ __forceinline__ void in_turn() {
+  if constexpr (FRUGAL) __builtin_amdgcn_sched_barrier(0);
+}
 
 // Powers of two of the gradients of scores (float16 only)
 template <typename T, int QS>
@@ -918,13 +923,15 @@ __device__ __forceinline__ void attention_keys_head(const AttnArgs &a, const Att
   const int rows = doc.tile * BM < doc.kn ? (int)rows_in(a, doc.qn) : 0;
   int t0, t1;
   piece_of((int)(((long long)rows + BN - 1) / BN), w.split, a.splits, t0, t1);
-  const int whole = (a.blocked ? doc.qn & ~15 : doc.qn) * a.G;   // rows before the first that does not exist
   const T *q0 = (const T *)a.q + doc.sample * a.qs + doc.q0 * a.qp + (long long)w.kv * a.G * a.qh;
   const long long o0 = doc.out_q * a.H + w.kv * a.G;
   auto copy = [&](int t, Buffer &b) __attribute__((always_inline)) {
-    const int left = rows - t * BN;
-    copy_tile<T, DP, BN, THREADS, kFrugal<T, DP, BIAS, WAVES>>(b.q, [&](int row) { const RowAt r = row_at(a, t * BN + row); return r.pos < doc.qn ? q0 + (long long)r.pos * a.qp + (long long)r.head * a.qh : nullptr; }, left, a.dim);
-    copy_tile<T, DP, BN, THREADS, kFrugal<T, DP, BIAS, WAVES>>(b.g, [&](int row) { const RowAt r = row_at(a, t * BN + row); return r.pos < doc.qn ? (const T *)a.gy + (o0 + (long long)r.pos * a.H + r.head) * a.ldy : nullptr; }, left, a.dim);
+    const int left = rows - t * BN, whole = (left + 31) & ~31;
+    // (a row that does not exist is the last that does, whose lse, infinity, leaves it without a share: zeros times a key or value of infinity would be
+    // no number.  Testing for that in the loop cost the kernel for 128 values without points 11 %.)
+    auto row_of = [&](int row) __attribute__((always_inline)) { const RowAt r = row_at(a, t * BN + row); return RowAt{min(r.pos, doc.qn - 1), r.head}; };
+    copy_tile<T, DP, BN, THREADS, kFrugal<T, DP, BIAS, WAVES>>(b.q, [&](int row) { const RowAt r = row_of(row); return q0 + (long long)r.pos * a.qp + (long long)r.head * a.qh; }, whole, a.dim);
+    copy_tile<T, DP, BN, THREADS, kFrugal<T, DP, BIAS, WAVES>>(b.g, [&](int row) { const RowAt r = row_of(row); return (const T *)a.gy + (o0 + (long long)r.pos * a.H + r.head) * a.ldy; }, whole, a.dim);
 #pragma unroll
     for (int e = 0; e < ROW; e++)
       if (WAVES == 1 || (int)threadIdx.x / 64 == e % 4)
@@ -954,54 +961,50 @@ __device__ __forceinline__ void attention_keys_head(const AttnArgs &a, const Att
           for (int s = 0; s < QS; s++) p[u][s] = Tile::product(fq, fk[s][k], p[u][s]), ds[u][s] = Tile::product(fg, fv[s][k], ds[u][s]);
         }
       }
-      // what rows are: the second 16 have the positions of the first where SHARE
-      f32x4 nlse[2], slope[2], point[SHARE ? 1 : 2][3];
-#pragma unroll
-      for (int u = 0; u < 2; u++) {
-        nlse[u] = kHalfUp<T> - *(const f32x4 *)&b.r[0][(j0 + u) * 16 + q4];   // (weights times 2^kHalfUp from here on)
-        if constexpr (BIAS != kBiasNone) {
-          slope[u] = *(const f32x4 *)&b.r[2][(j0 + u) * 16 + q4];
-          if (!SHARE || u == 0)
-#pragma unroll
-            for (int e = 0; e < 3; e++) point[u][e] = *(const f32x4 *)&b.r[3 + e][(j0 + u) * 16 + q4];
-        }
-      }
-      if (j0 * 16 + 32 > whole - t * BN) {   // (zeros of rows that do not exist, times a key or value of infinity)
-#pragma unroll
-        for (int u = 0; u < 2; u++)
-#pragma unroll
-          for (int i = 0; i < 4; i++)
-            if (nlse[u][i] == -INFINITY)
-#pragma unroll
-              for (int s = 0; s < QS; s++) p[u][s][i] = 0.f, ds[u][s][i] = 0.f;
-      }
       float part[QS][3] = {};
+      // 16 rows after the other, or, where SHARE, all: the second 16 have the positions of the first
 #pragma unroll
-      for (int s = 0; s < QS; s++)
+      for (int u0 = 0; u0 < (SHARE ? 1 : 2); u0++) {
+        in_turn<kFrugal<T, DP, BIAS, WAVES>>();
+        constexpr int U = SHARE ? 2 : 1;
+        f32x4 nlse[U], slope[U], point[3];   // what rows are
 #pragma unroll
-        for (int i = 0; i < 4; i++) {
-          Distance<BIAS> far;
-          float both = 0.f;   // gradients of rows of one position, times their slopes
-#pragma unroll
-          for (int u = 0; u < 2; u++) {
-            if (!SHARE || u == 0) far.form(x[s], point[u], i);   // (from the key: the sign that its gradient takes)
-            float v = nlse[u][i];
-            if constexpr (BIAS != kBiasNone) v = __builtin_fmaf(far.far, slope[u][i] * -1.44269504088896341f, v);
-            const float prob = __builtin_amdgcn_exp2f(__builtin_fmaf(p[u][s][i], a.scale2, v)), g = prob * ds[u][s][i];
-            p[u][s][i] = prob, ds[u][s][i] = g;
-            if constexpr (BIAS == kBiasGradients) {
-              both = SHARE && u == 1 ? __builtin_fmaf(g, slope[u][i], both) : g * slope[u][i];
-              if (!SHARE || u == 1) far.add(part[s], both);
-            }
-          }
+        for (int v = 0; v < U; v++) {
+          nlse[v] = kHalfUp<T> - *(const f32x4 *)&b.r[0][(j0 + u0 + v) * 16 + q4];   // (weights times 2^kHalfUp from here on)
+          if constexpr (BIAS != kBiasNone) slope[v] = *(const f32x4 *)&b.r[2][(j0 + u0 + v) * 16 + q4];
         }
+        if constexpr (BIAS != kBiasNone)
+#pragma unroll
+          for (int e = 0; e < 3; e++) point[e] = *(const f32x4 *)&b.r[3 + e][(j0 + u0) * 16 + q4];
+#pragma unroll
+        for (int s = 0; s < QS; s++)
+#pragma unroll
+          for (int i = 0; i < 4; i++) {
+            Distance<BIAS> far;
+            far.form(x[s], point, i);   // (from the key: the sign that its gradient takes)
+            float both = 0.f;           // gradients of rows of one position, times their slopes
+#pragma unroll
+            for (int v = 0; v < U; v++) {
+              const int u = u0 + v;
+              float less = nlse[v][i];
+              if constexpr (BIAS != kBiasNone) less = __builtin_fmaf(far.far, slope[v][i] * -1.44269504088896341f, less);
+              const float prob = __builtin_amdgcn_exp2f(__builtin_fmaf(p[u][s][i], a.scale2, less)), g = prob * ds[u][s][i];
+              p[u][s][i] = prob, ds[u][s][i] = g;
+              if constexpr (BIAS == kBiasGradients) both = __builtin_fmaf(g, slope[v][i], both);
+            }
+            if constexpr (BIAS == kBiasGradients) far.add(part[s], both);
+          }
+      }
       if constexpr (BIAS == kBiasGradients)
 #pragma unroll
         for (int s = 0; s < QS; s++)
 #pragma unroll
           for (int e = 0; e < 3; e++) geo[s][e] -= part[s][e];
-      lift.apply(ds, ak);
+      in_turn<kFrugal<T, DP, BIAS, WAVES>>();
       Tile::template transposed<QS>(av, b.g, j0 * 16, p[0], p[1]);
+      in_turn<kFrugal<T, DP, BIAS, WAVES>>();
+      lift.apply(ds, ak);
+      in_turn<kFrugal<T, DP, BIAS, WAVES>>();
       Tile::template transposed<QS>(ak, b.q, j0 * 16, ds[0], ds[1]);
     }
   });
