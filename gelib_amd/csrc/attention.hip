@@ -207,29 +207,34 @@ __global__ void __launch_bounds__(256) attention_sum_kernel(T *out, const float 
   out[at] = from_f<T>(v);
 }
 
-// gradients of points: sums over heads and pieces, of queries (geo_q), keys (geo_k) or, where they are the same points, both.  16 lanes a row,
-// neighbouring heads side by side: one query of 128 heads on 65536 keys in 64 pieces, both directions of the call: 609 us,
-// with a thread a row 1411; 16 heads on 4: 371 / 471.
-__global__ void __launch_bounds__(256) attention_points_kernel(float *out, const float4 *gq, int splits_q, int H, const float4 *gk, int splits_k, int KV,
+// gradients of points: sums over heads and pieces, of queries (geo_q), keys (geo_k) or, where they are the same points, both.  2^shift lanes a row
+// (up to 16), neighbouring heads side by side: one query of 128 heads on 65536 keys in 64 pieces, both directions of the call:
+// 609 us, with a thread a row 1411; 16 heads on 4: 371 / 471.  No more lanes than terms (4 heads on 2, 65536 points: 16
+// lanes 5.9 us, four 3.8; one head of 2048 points: 3.5 with one as with 16).
+__global__ void __launch_bounds__(256) attention_points_kernel(float *out, const float4 *gq, int splits_q, int H, const float4 *gk, int splits_k, int KV, int shift,
                                                                long long first, long long rows) {
-  const long long row = (first + (long long)blockIdx.x * 256 + threadIdx.x) / 16;
-  const int lane = threadIdx.x % 16;
-  float x = 0.f, y = 0.f, z = 0.f;
+  const long long row = (first + (long long)blockIdx.x * 256 + threadIdx.x) >> shift;
+  const int lanes = 1 << shift, lane = threadIdx.x & (lanes - 1);
+  float sum[3] = {0.f, 0.f, 0.f};
   auto add = [&](const float4 *g, int splits, int heads) {
 #pragma unroll 4
-    for (int i = lane; i < splits * heads; i += 16) {
+    for (int i = lane; i < splits * heads; i += lanes) {
       const int s = splits == 1 ? 0 : i / heads;
       const float4 v = g[(s * rows + row) * heads + (i - s * heads)];
-      x += v.x, y += v.y, z += v.z;
+      sum[0] += v.x, sum[1] += v.y, sum[2] += v.z;
     }
   };
   if (row < rows) {
     if (gq) add(gq, splits_q, H);
     if (gk) add(gk, splits_k, KV);
   }
+  for (int d = 1; d < lanes; d *= 2)
 #pragma unroll
-  for (int d = 1; d < 16; d *= 2) x += __shfl_xor(x, d), y += __shfl_xor(y, d), z += __shfl_xor(z, d);
-  if (row < rows && lane < 3) out[row * 3 + lane] = lane == 0 ? x : lane == 1 ? y : z;
+    for (int e = 0; e < 3; e++) sum[e] += __shfl_xor(sum[e], d);
+  if (row < rows)
+#pragma unroll
+    for (int e = 0; e < 3; e++)
+      if ((e & (lanes - 1)) == lane) out[row * 3 + e] = sum[e];
 }
 
 // gradients of slopes: of kSlopeRows rows and up to 64 heads, a block (side: threads side by side on heads, a power of two); then of all blocks
@@ -393,8 +398,11 @@ int backward(const AttnCall &c, const AttnGrads &g, void *ws, hipStream_t s) {
   }
   if (!geometry) return 0;
   auto points = [&](float *out, bool of_q, bool of_k, long long rows) {
-    return in_launches(rows * 16, [&](long long first, dim3 grid) {
-      hipLaunchKernelGGL(attention_points_kernel, grid, dim3(256), 0, s, out, of_q ? a.geo_q : nullptr, pr.splits, a.H, of_k ? a.geo_k : nullptr, pk.splits, a.KV, first, rows);
+    const int terms = std::max(of_q ? pr.splits * a.H : 0, of_k ? pk.splits * a.KV : 0);
+    int shift = 0;
+    while (shift < 4 && 1 << shift < terms) shift++;
+    return in_launches(rows << shift, [&](long long first, dim3 grid) {
+      hipLaunchKernelGGL(attention_points_kernel, grid, dim3(256), 0, s, out, of_q ? a.geo_q : nullptr, pr.splits, a.H, of_k ? a.geo_k : nullptr, pk.splits, a.KV, shift, first, rows);
     });
   };
   if (g.gx)

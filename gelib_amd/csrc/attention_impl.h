@@ -366,7 +366,8 @@ typedef __attribute__((address_space(3))) char *AttnLds;
 
 // 16 (or 4) bytes of every lane to LDS, lane after lane from `to` (the same for the whole wave) on.  Written out because the compiler, which
 // cannot tell two buffers apart, would wait for the builtin's copy before the next read of either; the wave waits by itself (arrive()).  No
-// register is written.
+// register is written but m0, which is reserved: the compiler keeps nothing there, and cannot be told of it as clobbered (nothing but these
+// copies names it in the kernels).
 __device__ __forceinline__ void attn_copy16(const void *from, char *to) {
   const unsigned at = __builtin_amdgcn_readfirstlane((unsigned)(uintptr_t)(AttnLds)to);
   asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" : : "s"(at), "v"(from) : "memory");
