@@ -83,18 +83,14 @@ constexpr float kLowest = -3.0e38f;
 // float16's least normal value is 2^-14, and what the second products take as float16 values may lie anywhere below: weights, one over the number
 // of keys, and their scores' gradients, which are as small or large as the loss's.  Powers of two bring them into its range, and the float32
 // results are scaled back.
-//   Forward: weights less the maximum stand at 2^7, and at 2^15 before the maximum is moved (kHalfTop).
-//   Backward: weights, at most one, stand at 2^12 (kHalfUp: 2^4 to spare for scores so large that exp(s - lse) is off by that).
+//   Forward: the largest weight of the first keys stands at 2^7 (kHalfTop), and the largest at 2^15 before the maximum is moved.
+//   Gradients of values: weights, at most one, stand at 2^12 (kHalfUp: 2^4 to spare for scores so large that exp(s - lse) is off by that).
+//   Both are multiplied after the exponential: 12 more in front of it would round s - lse, and gradients of points, three times as coarsely.
 //   ds: each own row has a power of two of its own, which is chosen when its first ds come so that the largest is 2^11 to 2^12, and again when
 //   one is beyond 2^15 (Lift).
 template <typename T>
 constexpr bool kIsHalf = std::is_same<T, half_t>::value;
-template <typename T>
-constexpr float kHalfTop = kIsHalf<T> ? 7.f : 0.f;
-template <typename T>
-constexpr float kHalfUp = kIsHalf<T> ? 12.f : 0.f;       // log2
-template <typename T>
-constexpr float kHalfDown = kIsHalf<T> ? 0x1p-12f : 1.f;
+constexpr float kHalfTop = 0x1p7f, kHalfUp = 0x1p12f;
 
 // A document as a block sees it: where its rows begin in the strided operands and in packed results, how many exist, and how many there
 // are to write (rows that do not exist get zeros).
@@ -347,9 +343,9 @@ struct Lift {
       for (int u = 0; u < 2; u++) d[u][s] *= by[s];
     }
   }
-  // the sums as they are, but for a factor
+  // the sums as they are
   template <int NF>
-  __device__ __forceinline__ void down(f32x4 (*acc)[NF], float besides) const {
+  __device__ __forceinline__ void down(f32x4 (*acc)[NF]) const {
     if constexpr (!kIsHalf<T>) return;
 #pragma unroll
     for (int s = 0; s < QS; s++) {
@@ -357,7 +353,7 @@ struct Lift {
 #pragma unroll
       for (int f = 0; f < NF; f++)
 #pragma unroll
-        for (int i = 0; i < 4; i++) acc[s][f][i] = ldexpf(acc[s][f][i], less) * besides;
+        for (int i = 0; i < 4; i++) acc[s][f][i] = ldexpf(acc[s][f][i], less);
     }
   }
 };
@@ -568,8 +564,7 @@ __device__ __forceinline__ void attention_fwd_head(const AttnArgs &a, const Attn
 
   // Exponentials are formed less the maximum so far, m (log2), which is that of the first tile with a score above -infinity (begun: a row
   // has had one).  It moves only when a score is more than 8 above it: values are then at most 2^8 times what they would be, and
-  // rescaling is rare.  (float16: m is 7 below the maximum, see kHalfTop.)  Scores themselves are kept whole until then: less a maximum
-  // far below them they would lose digits.
+  // rescaling is rare.  Scores themselves are kept whole until then: less a maximum far below them they would lose digits.
   // Without distances what is kept are products that the scale, which is above zero then, has not met yet (q takes its sign): it and the
   // maximum are one instruction in front of the exponential.  8192 x 8192, 16 heads of 64, bfloat16: 411 us, with scores scaled at once 423, less the
   // maximum from the start 397; with points (8192, 16 heads on 4) an instruction more than that, 540 and 506.
@@ -640,13 +635,13 @@ __device__ __forceinline__ void attention_fwd_head(const AttnArgs &a, const Attn
 #pragma unroll
       for (int j = 0; j < SUB; j++) v = fmaxf(v, fmaxf(fmaxf(sc[s][j][0], sc[s][j][1]), fmaxf(sc[s][j][2], sc[s][j][3])));
       top[s] = over_row_max(v);
-      grown |= begun[s] ? top[s] * unit > m[s] + (kHalfTop<T> + 8.f) : top[s] > kLowest;
+      grown |= begun[s] ? top[s] * unit > m[s] + 8.f : top[s] > kLowest;
     }
     if (__any(grown)) {
 #pragma unroll
       for (int s = 0; s < QS; s++) {
         const bool first = !begun[s] && top[s] > kLowest;
-        const float to = first || (begun[s] && top[s] * unit > m[s] + kHalfTop<T>) ? top[s] * unit - kHalfTop<T> : m[s], by = first ? 0.f : __builtin_amdgcn_exp2f(m[s] - to);
+        const float to = first || (begun[s] && top[s] * unit > m[s]) ? top[s] * unit : m[s], by = first ? 0.f : __builtin_amdgcn_exp2f(m[s] - to);
         m[s] = to, l[s] *= by, begun[s] |= first;
 #pragma unroll
         for (int f = 0; f < Tile::NF; f++) acc[s][f] *= by;
@@ -660,6 +655,7 @@ __device__ __forceinline__ void attention_fwd_head(const AttnArgs &a, const Attn
       for (int s = 0; s < QS; s++) {
 #pragma unroll
         for (int i = 0; i < 4; i++) p0[s][i] = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[s][j][i], unit, -m[s])), p1[s][i] = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[s][j + 1][i], unit, -m[s]));
+        if constexpr (kIsHalf<T>) p0[s] *= kHalfTop, p1[s] *= kHalfTop;
         const f32x4 both = p0[s] + p1[s];
         l[s] += (both[0] + both[1]) + (both[2] + both[3]);
       }
@@ -669,7 +665,10 @@ __device__ __forceinline__ void attention_fwd_head(const AttnArgs &a, const Attn
 
 #pragma unroll
   for (int s = 0; s < QS; s++) {
-    const float all = over_row_sum(l[s]), sum = own.there[s] ? all : 0.f;
+    if constexpr (kIsHalf<T>)
+#pragma unroll
+      for (int f = 0; f < Tile::NF; f++) acc[s][f] *= 1.f / kHalfTop;
+    const float all = over_row_sum(l[s]) * (kIsHalf<T> ? 1.f / kHalfTop : 1.f), sum = own.there[s] ? all : 0.f;
     if (!own.mine[s]) continue;
     const long long at = own.out(a, doc, w.kv, row0, s);
     if (a.part_q) {
@@ -740,7 +739,7 @@ __device__ __forceinline__ void attention_rows_head(const AttnArgs &a, const Att
       for (int e = 0; e < Tile::EP; e++) delta[s] += to_f(gv[e]) * to_f(yv[e]);
     }
     delta[s] = over_row_sum(delta[s]);
-    nlse[s] = own.there[s] ? kHalfUp<T> - a.lse[at] : -INFINITY;   // (weights times 2^kHalfUp from here on)
+    nlse[s] = own.there[s] ? -a.lse[at] : -INFINITY;
   }
   Lift<T, QS> lift;
   f32x4 acc[SETS][Tile::NF];
@@ -820,20 +819,17 @@ __device__ __forceinline__ void attention_rows_head(const AttnArgs &a, const Att
     }
   });
 
-  lift.down(acc, kHalfDown<T>);
+  lift.down(acc);
 #pragma unroll
   for (int s = 0; s < QS; s++) {
-    if constexpr (kIsHalf<T>)
-#pragma unroll
-      for (int f = 0; f < Tile::NF; f++) acc[QS + s][f] *= kHalfDown<T>;
     const bool pieces = MEND && a.part_d;   // (what is lacking is known when all pieces are there)
-    const float lacks = MEND ? over_row_sum(rest[s]) * kHalfDown<T> : 0.f;
+    const float lacks = MEND ? over_row_sum(rest[s]) : 0.f;
     const long long at = own.out(a, doc, w.kv, row0, s), in_part = w.split * a.rows_q * a.H + at;
     if (BIAS == kBiasGradients) {
 #pragma unroll
       for (int e = 0; e < 4; e++) {
-        geo[s][e] = over_row_sum(geo[s][e]) * (kHalfDown<T> * (e < 3 ? 0.69314718055994531f : -1.f));
-        if (MEND) geo[QS * MEND + s][e] = over_row_sum(geo[QS * MEND + s][e]) * (kHalfDown<T> * (e < 3 ? own.slope[s] * 0.69314718055994531f : -1.f));
+        geo[s][e] = over_row_sum(geo[s][e]) * (e < 3 ? 0.69314718055994531f : -1.f);
+        if (MEND) geo[QS * MEND + s][e] = over_row_sum(geo[QS * MEND + s][e]) * (e < 3 ? own.slope[s] * 0.69314718055994531f : -1.f);
         if (MEND && !pieces) geo[s][e] -= lacks * geo[QS * MEND + s][e];
       }
       if (own.mine[s] && q4 == 0) {
@@ -971,7 +967,7 @@ __device__ __forceinline__ void attention_keys_head(const AttnArgs &a, const Att
         f32x4 nlse[U], slope[U], point[3];   // what rows are
 #pragma unroll
         for (int v = 0; v < U; v++) {
-          nlse[v] = kHalfUp<T> - *(const f32x4 *)&b.r[0][(j0 + u0 + v) * 16 + q4];   // (weights times 2^kHalfUp from here on)
+          nlse[v] = -*(const f32x4 *)&b.r[0][(j0 + u0 + v) * 16 + q4];
           if constexpr (BIAS != kBiasNone) slope[v] = *(const f32x4 *)&b.r[2][(j0 + u0 + v) * 16 + q4];
         }
         if constexpr (BIAS != kBiasNone)
@@ -990,7 +986,7 @@ __device__ __forceinline__ void attention_keys_head(const AttnArgs &a, const Att
               float less = nlse[v][i];
               if constexpr (BIAS != kBiasNone) less = __builtin_fmaf(far.far, slope[v][i] * -1.44269504088896341f, less);
               const float prob = __builtin_amdgcn_exp2f(__builtin_fmaf(p[u][s][i], a.scale2, less)), g = prob * ds[u][s][i];
-              p[u][s][i] = prob, ds[u][s][i] = g;
+              p[u][s][i] = kIsHalf<T> ? prob * kHalfUp : prob, ds[u][s][i] = g;
               if constexpr (BIAS == kBiasGradients) both = __builtin_fmaf(g, slope[v][i], both);
             }
             if constexpr (BIAS == kBiasGradients) far.add(part[s], both);
@@ -1010,13 +1006,13 @@ __device__ __forceinline__ void attention_keys_head(const AttnArgs &a, const Att
     }
   });
 
-  lift.down(ak, kHalfDown<T>);
+  lift.down(ak);
 #pragma unroll
   for (int s = 0; s < QS; s++) {
     const long long out = (doc.out_k + key0 + 16 * s + c) * a.KV + w.kv, at = w.split * a.rows_k * a.KV + out;
     if constexpr (kIsHalf<T>)
 #pragma unroll
-      for (int f = 0; f < Tile::NF; f++) av[s][f] *= kHalfDown<T>;
+      for (int f = 0; f < Tile::NF; f++) av[s][f] *= 1.f / kHalfUp;
     if (!exists[s]) {   // (its score is no -infinity above: its values and gradients are zeros here)
 #pragma unroll
       for (int f = 0; f < Tile::NF; f++) ak[s][f] = f32x4{0.f, 0.f, 0.f, 0.f}, av[s][f] = ak[s][f];
@@ -1025,7 +1021,7 @@ __device__ __forceinline__ void attention_keys_head(const AttnArgs &a, const Att
 #pragma unroll
       for (int e = 0; e < 3; e++) {
         const float all = over_row_sum(geo[s][e]);
-        geo[s][e] = exists[s] ? all * kHalfDown<T> : 0.f;
+        geo[s][e] = exists[s] ? all : 0.f;
       }
       if (mine[s] && q4 == 0) a.geo_k[at] = make_float4(geo[s][0], geo[s][1], geo[s][2], 0.f);
     }

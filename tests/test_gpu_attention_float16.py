@@ -147,3 +147,29 @@ def test_many_small_weights_beside_a_large_one(gelib):
     y = gelib.attention(*(t.expand(n, *t.shape) for t in (q, k, v)), scale=1.0)
     want = reference(q.double(), k.double(), v.double(), torch.zeros_like(q).double(), 1.0)["y"]
     check(y, *(t.expand(n, *t.shape) for t in want), "y")
+
+
+@pytest.mark.parametrize("size", [(300, 3, 8, 8, 32), (100, 7, 8, 4, 16), (64, 24, 8, 8, 32)], ids=lambda s: "x".join(map(str, s)))
+def test_gradients_of_points_are_float32(gelib, size):
+    """What float16 operands do not round: relative errors of the whole gradients of points and slopes.  An exponent, below 4 in log2 units, is
+    rounded by at most 2^-23 (1.4 u of a weight), hardware's exponential by 2 u, distance, gy . v - D and the product by 2 u each at the
+    most, independently: 4 u is more than the root of the sum of their squares.  Gradients of slopes: a row's ds sum to zero, so the sum of ds
+    times distances that are nearly alike is small beside its terms; it is off by 4 u of their moduli, and so are the rows, independently."""
+    n, m, heads, kv, dim = size
+    gen = torch.Generator(device="cuda").manual_seed(n)
+    q, k, v, g = ((torch.randn(n, m, h, dim, device="cuda", generator=gen)).half() for h in (heads, kv, kv, heads))
+    x, s = (torch.rand(n, m, 3, device="cuda", generator=gen) * 6).requires_grad_(), (torch.rand(heads, device="cuda", generator=gen) + 0.1).requires_grad_()
+    got = torch.autograd.grad(gelib.attention(q, k, v, x, s), (x, s), g)
+    X, S = (t.detach().double().requires_grad_() for t in (x, s))
+    kk, vv = (t.double().repeat_interleave(heads // kv, 2).transpose(1, 2).contiguous() for t in (k, v))
+    sq = (X[:, :, None] - X[:, None]).square().sum(3)
+    same = torch.eye(m, dtype=torch.bool, device="cuda")
+    far = sq.masked_fill(same, 1.).sqrt().masked_fill(same, 0.)
+    p = torch.softmax(q.double().transpose(1, 2).contiguous() @ kk.transpose(2, 3).contiguous() * dim ** -0.5 - S.view(1, -1, 1, 1) * far[:, None], 3)
+    want = torch.autograd.grad((p @ vv).transpose(1, 2), (X, S), g.double(), retain_graph=True)
+    with torch.no_grad():
+        dp = g.double().transpose(1, 2).contiguous() @ vv.transpose(2, 3).contiguous()
+        ds = p * (dp - (p * dp).sum(3, keepdim=True))
+        rows = (ds.abs() * far[:, None]).sum(3).square().sum((0, 2)).sqrt()
+    assert (got[0].double() - want[0]).norm() <= 4 * u * want[0].norm()
+    assert ((got[1].double() - want[1]).abs() <= 4 * u * rows + u * want[1].abs()).all()
