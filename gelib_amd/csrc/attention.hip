@@ -207,14 +207,16 @@ __global__ void __launch_bounds__(256) attention_sum_kernel(T *out, const float 
   out[at] = from_f<T>(v);
 }
 
-// gradients of points: sums over heads and pieces, of queries (geo_q), keys (geo_k) or, where they are the same points, both.  2^shift lanes a row
-// (up to 16), neighbouring heads side by side: one query of 128 heads on 65536 keys in 64 pieces, both directions of the call:
+// gradients of points: sums over heads and pieces, of queries (geo_q), keys (geo_k) or, where they are the same points, both.  2^SHIFT lanes a row
+// (up to 16; known to the compiler, which has four loads under way then: with a number that it does not know 732 instead of 609 us), neighbouring heads side by side: one query of 128 heads on 65536 keys in 64 pieces, both directions of the call:
 // 609 us, with a thread a row 1411; 16 heads on 4: 371 / 471.  No more lanes than terms (4 heads on 2, 65536 points: 16
 // lanes 5.9 us, four 3.8; one head of 2048 points: 3.5 with one as with 16).
-__global__ void __launch_bounds__(256) attention_points_kernel(float *out, const float4 *gq, int splits_q, int H, const float4 *gk, int splits_k, int KV, int shift,
+template <int SHIFT>
+__global__ void __launch_bounds__(256) attention_points_kernel(float *out, const float4 *gq, int splits_q, int H, const float4 *gk, int splits_k, int KV,
                                                                long long first, long long rows) {
-  const long long row = (first + (long long)blockIdx.x * 256 + threadIdx.x) >> shift;
-  const int lanes = 1 << shift, lane = threadIdx.x & (lanes - 1);
+  const long long row = (first + (long long)blockIdx.x * 256 + threadIdx.x) >> SHIFT;
+  constexpr int lanes = 1 << SHIFT;
+  const int lane = threadIdx.x & (lanes - 1);
   float sum[3] = {0.f, 0.f, 0.f};
   auto add = [&](const float4 *g, int splits, int heads) {
 #pragma unroll 4
@@ -228,6 +230,7 @@ __global__ void __launch_bounds__(256) attention_points_kernel(float *out, const
     if (gq) add(gq, splits_q, H);
     if (gk) add(gk, splits_k, KV);
   }
+#pragma unroll
   for (int d = 1; d < lanes; d *= 2)
 #pragma unroll
     for (int e = 0; e < 3; e++) sum[e] += __shfl_xor(sum[e], d);
@@ -401,9 +404,19 @@ int backward(const AttnCall &c, const AttnGrads &g, void *ws, hipStream_t s) {
     const int terms = std::max(of_q ? pr.splits * a.H : 0, of_k ? pk.splits * a.KV : 0);
     int shift = 0;
     while (shift < 4 && 1 << shift < terms) shift++;
-    return in_launches(rows << shift, [&](long long first, dim3 grid) {
-      hipLaunchKernelGGL(attention_points_kernel, grid, dim3(256), 0, s, out, of_q ? a.geo_q : nullptr, pr.splits, a.H, of_k ? a.geo_k : nullptr, pk.splits, a.KV, shift, first, rows);
-    });
+    auto launch = [&](auto lanes_log2) {
+      constexpr int S = decltype(lanes_log2)::value;
+      return in_launches(rows << S, [&](long long first, dim3 grid) {
+        hipLaunchKernelGGL(attention_points_kernel<S>, grid, dim3(256), 0, s, out, of_q ? a.geo_q : nullptr, pr.splits, a.H, of_k ? a.geo_k : nullptr, pk.splits, a.KV, first, rows);
+      });
+    };
+    switch (shift) {
+      case 0: return launch(std::integral_constant<int, 0>());
+      case 1: return launch(std::integral_constant<int, 1>());
+      case 2: return launch(std::integral_constant<int, 2>());
+      case 3: return launch(std::integral_constant<int, 3>());
+      default: return launch(std::integral_constant<int, 4>());
+    }
   };
   if (g.gx)
     if (int rc = points(g.gx, true, g.same_points, a.rows_q)) return rc;
