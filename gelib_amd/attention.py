@@ -15,10 +15,13 @@ def attention(q, k, v, points=None, slopes=None, key_points=None, lengths=None, 
 
     Heads h of q stand on heads h / (heads / kv_heads) of k and v.  dim is at most 128; a head's channels are contiguous, other strides
     as they come.  points and key_points (rows of q and of k, three coordinates each; key_points None: points) and slopes (heads) are float32.
-    Points are finite numbers below 1e38; a distance above 1.8e19, whose square float32 does not hold, counts as that.  scale None: dim ** -0.5.  One query a sample (n_q = 1) reads a sample out.
+    Points are finite numbers below 1e38; a distance above 1.8e19, whose square float32 does not hold, counts as that.  scale None: dim ** -0.5.
+    One query a sample (n_q = 1) reads a sample out.
 
-    Scores, softmax and sums are float32; 16-bit types round its values to their own for the second product, and results once.  Differentiable
+    Scores, softmax and sums are float32; 16-bit types round its values to their own for the second product, and results once, so that errors are
+    those of rounding the result times 1.4.  Differentiable
     in q, k, v, points, slopes and key_points (points in one place have no direction and add nothing to each other's gradient), twice by torch's
-    own operations, which forward-mode derivatives, function transforms, tracing and dispatch modes get from the start.  float16 gradients
-    are float16 values: losses are scaled up as usual with that type."""
+    own operations, which forward-mode derivatives, function transforms, tracing and dispatch modes get from the start.  Those form the
+    scores of all rows with all rows of packed documents, and what is no number in one document reaches the others there.  float16
+    gradients are float16 values: losses are scaled up as usual with that type (what leads to them is kept in range, whatever their size)."""
     return backend().attention(q, k, v, points, slopes, key_points, lengths, query_lengths, starts, query_starts, scale)

@@ -14,9 +14,10 @@
 // A document's query rows are its (position, head of the group) pairs: heads that share keys stand in one tile.
 //
 // What bounds it: the vector unit, 70 to 75 % busy with the distances, exponentials and sums between the products.  8192 points, 16 heads of 64
-// on 4, bfloat16, with points: forward 520 us (530 TFLOP/s), by rows 940, by keys 920; 16 on 16, without points: forward 408 us (675), both
-// directions 1645 (585); 2 x 8192, 8 heads of 128 on 2, without points: forward 599 (918).  Short documents: the instructions around the
-// products (addresses, rows, results): 2048 packed documents of up to 60 rows, 8 heads of 32, bfloat16: 66, 97 and 103 us.
+// on 4, bfloat16, with points: forward 556 us (495 TFLOP/s), by rows 931, by keys 915; 16 on 16, without points: forward 411 us (669), both
+// directions 1630 (590); 2 x 8192, 8 heads of 128 on 2, without points: forward 618 (890).  float16 scales its weights and their gradients
+// (kHalfTop): forward 577, both directions 2693 where bfloat16 has 556 and 2430.  Short documents: the instructions around the
+// products (addresses, rows, results): 2048 packed documents of up to 60 rows, 8 heads of 32, bfloat16: 63, 96 and 101 us.
 #pragma once
 
 #include <type_traits>
