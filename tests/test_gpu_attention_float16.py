@@ -173,3 +173,52 @@ def test_gradients_of_points_are_float32(gelib, size):
         rows = (ds.abs() * far[:, None]).sum(3).square().sum((0, 2)).sqrt()
     assert (got[0].double() - want[0]).norm() <= 4 * u * want[0].norm()
     assert ((got[1].double() - want[1]).abs() <= 4 * u * rows + u * want[1].abs()).all()
+
+
+@pytest.mark.parametrize("size", [(40, 100, 2, 2, 32), (150, 200, 4, 2, 64), (150, 700, 8, 2, 64)], ids=lambda s: "x".join(map(str, s)))
+def test_gradients_of_infinity_stay_where_they_are(gelib, size):
+    """A gradient that overflowed (what a scaled loss is watched for): gq of the other queries and heads has the bits that it has without it."""
+    nq, nk, heads, kv, dim = size
+    gen = torch.Generator(device="cuda").manual_seed(nq)
+    q, k, v, g = (torch.randn(1, n, h, dim, device="cuda", generator=gen).half() for n, h in ((nq, heads), (nk, kv), (nk, kv), (nq, heads)))
+    x, xk, s = torch.randn(1, nq, 3, device="cuda", generator=gen), torch.randn(1, nk, 3, device="cuda", generator=gen), torch.rand(heads, device="cuda", generator=gen).requires_grad_()
+    leaves = [t.requires_grad_() for t in (q, k, v)]
+
+    def grads(g):
+        return torch.autograd.grad(gelib.attention(q, k, v, x, s, key_points=xk), [*leaves, s], g)
+    want = grads(g)
+    bad = g.clone()
+    bad[0, 7, 1, 3] = float("inf")
+    got = grads(bad)
+    other = torch.ones(1, nq, heads, dtype=torch.bool, device="cuda")
+    other[0, 7, 1] = False
+    assert torch.equal(got[0][other], want[0][other]) and not torch.isfinite(got[0][~other]).all()
+    rest = [h for h in range(kv) if h != 1 // (heads // kv)]
+    assert torch.equal(got[1][:, :, rest], want[1][:, :, rest]) and torch.equal(got[2][:, :, rest], want[2][:, :, rest])
+    assert torch.equal(got[3][torch.arange(heads) != 1], want[3][torch.arange(heads) != 1])
+
+
+def test_recorded(gelib):
+    """Powers of two are chosen anew at every replay: gradients that grow and shrink by 2^8 between them."""
+    gen = torch.Generator(device="cuda").manual_seed(4)
+    q, k, v = (torch.randn(2, 90, h, 32, device="cuda", generator=gen).half().requires_grad_() for h in (4, 2, 2))
+    g = torch.randn(2, 90, 4, 32, device="cuda", generator=gen).half()
+
+    def step():
+        y = gelib.attention(q, k, v)
+        return (y.detach(), *torch.autograd.grad(y, (q, k, v), g))   # (no graph outlives a step)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step()
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = step()
+    for e in (0, -8, 8, 0):
+        g.copy_(torch.randn(2, 90, 4, 32, device="cuda", generator=gen) * 2.0 ** e)
+        graph.replay()
+        torch.cuda.synchronize()
+        kept = [t.clone() for t in out]
+        for a, b in zip(kept, step()):
+            assert torch.equal(a, b)
